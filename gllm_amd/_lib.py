@@ -15,7 +15,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libgllm_attn.so")
 
 OK, EINVAL, EUNSUPPORTED, EHIP = 0, 1, 2, 3
-DTYPE_F32, DTYPE_BF16, DTYPE_FP8_E4M3, DTYPE_F16 = 0, 1, 2, 3
+DTYPE_F32, DTYPE_BF16, DTYPE_FP8_E4M3, DTYPE_F16, DTYPE_MXFP4 = 0, 1, 2, 3, 4
 ROPE_NONE, ROPE_BY_POSITION, ROPE_BY_ROW = 0, 1, 2
 
 _p = ctypes.c_void_p
@@ -28,10 +28,13 @@ _sz = ctypes.c_size_t
 SIGNATURES = {
     "gllm_attn_last_error": (ctypes.c_char_p, []),
     "gllm_attn_version": (ctypes.c_int, []),
+    "gllm_kv4_record_bytes": (_sz, [_i32, _i32]),
     "gllm_rope_kv_write": (ctypes.c_int, [_p, _p, _p, _p, _p, _p, _p, _p, _i64, _p, _p, _p, _i64, _i64,
                                           _i32, _i32, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _p]),
     "gllm_attn_plan_create": (ctypes.c_int, [ctypes.POINTER(_p), _p, _p, _i32, _i64, _i32, _i32, _i32,
                                              _i32, _i32, _i32, _i32]),
+    "gllm_attn_plan_create_window": (ctypes.c_int, [ctypes.POINTER(_p), _p, _p, _i32, _i64, _i32, _i32, _i32,
+                                                    _i32, _i32, _i32, _i32, _i32, _i32]),
     "gllm_attn_plan_workspace_bytes": (_sz, [_p]),
     "gllm_attn_plan_upload": (ctypes.c_int, [_p, _p, _sz, _p]),
     "gllm_attn_plan_info": (ctypes.c_int, [_p, ctypes.POINTER(_i64), _i32]),

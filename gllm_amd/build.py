@@ -20,12 +20,14 @@ LIB = os.path.join(LIBDIR, "libgllm_attn.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
 
-SOURCES = ["paged_attention.hip", "paged_attention_f16.hip", "api.hip", "rope_kv_write.hip", "generic_attention.hip",
-           "generic_attention_bf16.hip", "generic_attention_f16.hip", "metadata.hip", "qkv_proj.hip"]
-GENERIC = {"generic_attention.hip", "generic_attention_bf16.hip", "generic_attention_f16.hip"}
-NO_CONTRACT = {"rope_kv_write.hip", "qkv_proj.hip"} | GENERIC
+PAGED = ["paged_attention.hip", "paged_attention_f16.hip", "paged_attention_kv4.hip", "paged_attention_kv4_f16.hip",
+         "paged_attention_window.hip", "paged_attention_window_f16.hip"]
+GENERIC = ["generic_attention.hip", "generic_attention_bf16.hip", "generic_attention_f16.hip", "generic_window_f32.hip",
+           "generic_window_bf16.hip", "generic_window_f16.hip"]
+SOURCES = [*PAGED, *GENERIC, "api.hip", "rope_kv_write.hip", "metadata.hip", "qkv_proj.hip"]
+NO_CONTRACT = {"rope_kv_write.hip", "qkv_proj.hip", *GENERIC}
 # MFMA accumulators stay in VGPRs (no per-tile AGPR<->VGPR copies)
-EXTRA = {f: ["-mllvm", "--amdgpu-mfma-vgpr-form"] for f in {"paged_attention.hip", "paged_attention_f16.hip", "qkv_proj.hip"} | GENERIC}
+EXTRA = {f: ["-mllvm", "--amdgpu-mfma-vgpr-form"] for f in [*PAGED, *GENERIC, "qkv_proj.hip"]}
 COMMON = [
     f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC",
     # packed fp32 VALU ops are disabled on purpose for every HIP unit

@@ -77,6 +77,7 @@ constexpr int32_t kMaxFusedRows = 16;
 
 // Model dtypes (the reference's model_dtype, model.py:64): f32, bf16, f16;
 // cache dtypes (kv_dtype, model.py:75): those and fp8 e4m3fn, any pairing.
+// The 4-bit cache (GLLM_DTYPE_MXFP4) is laid out and taken differently.
 bool model_dtype_ok(int32_t d) { return d == GLLM_DTYPE_F32 || d == GLLM_DTYPE_BF16 || d == GLLM_DTYPE_F16; }
 bool kv_dtype_ok(int32_t d) { return model_dtype_ok(d) || d == GLLM_DTYPE_FP8_E4M3; }
 // 16-bit model dtypes run the MFMA kernels (head dim 64 / 128)
@@ -178,6 +179,7 @@ PinnedPool& pinned_pool() {
 struct gllm_attn_plan {
   int32_t num_seqs = 0, Hq = 0, Hkv = 0, D = 0, bs = 0, dtype = 0;
   int32_t split_len = 0, max_q = 0;
+  int32_t window = 0, sinks = 0;   // sliding window (0: none reaches a sequence's first keys)
   int32_t n_decode_seqs = 0, n_prefill_seqs = 0, heads_per_wg = 8, decode_waves = 8, prefill_waves = 8;
   bool prefill_pairs = false;  // prefill-only launches at D = 64: two workgroups per CU
   bool mfma = false;      // bf16 head dim 64 / 128: the MFMA kernels; otherwise the generic kernel
@@ -204,6 +206,13 @@ struct gllm_attn_plan {
 };
 
 namespace {
+
+// Keys that a decode task list counts through: the sequence's without the run
+// that its window leaves out (the kernels take the same key_skip).
+int32_t counted_keys(const gllm_attn_plan* p, const SeqInfo& s) {
+  const int32_t L = s.ctx_len + s.q_len;
+  return p->window > 0 ? L - key_skip(s.ctx_len, p->window, p->sinks, 16).by : L;
+}
 
 // Resident 8-wave decode workgroups per CU (register-bound: 2 at D = 64,
 // 1 at D = 128).
@@ -238,7 +247,7 @@ BalancedShape balanced_shape(const gllm_attn_plan* p, int cus, int heads_req) {
   b.hgroups = (p->Hkv + b.hw - 1) / b.hw;
   const int G = p->Hq / p->Hkv;
   for (const SeqInfo& si : p->seqs)
-    if (si.q_len * G <= 16) b.units += (int64_t)b.hgroups * ((si.ctx_len + si.q_len + 15) / 16);
+    if (si.q_len * G <= 16) b.units += (int64_t)b.hgroups * ((counted_keys(p, si) + 15) / 16);
   b.wgs = std::max<int64_t>(1, std::min<int64_t>(b.units, (int64_t)cus * GLLM_DECODE_WG_PER_CU(p->D)));
   return b;
 }
@@ -260,8 +269,9 @@ void plan_balanced_decode(gllm_attn_plan* p, int cus, int heads_req, int64_t wgs
   const int64_t bs = p->bs;
   const int G = p->Hq / p->Hkv;
   // a segment's keys start on a 16-key unit, so a block size that is not a
-  // power of two <= 16 can add one partial block at the front: stay <= 511
-  const int64_t ucap = std::max<int64_t>(1, (is_pow2(bs) && bs <= 16 ? 512 * bs : 510 * bs) / 16);
+  // power of two <= 16 can add one partial block at the front: stay <= 511 (a
+  // window's two runs of blocks add three more)
+  const int64_t ucap = std::max<int64_t>(1, (is_pow2(bs) && bs <= 16 ? 512 * bs : (p->window > 0 ? 507 : 510) * bs) / 16);
   const int64_t U = shape.units;
   const int64_t W = wgs > 0 ? std::max<int64_t>(1, std::min(wgs, U)) : shape.wgs;
   p->heads_per_wg = hw;
@@ -279,7 +289,7 @@ void plan_balanced_decode(gllm_attn_plan* p, int cus, int heads_req, int64_t wgs
     if (si.q_len * G > 16) continue;   // a prefill item of the mixed launch
     ++p->n_decode_seqs;
     si.nsplits = 1;
-    const int L = si.ctx_len + si.q_len;
+    const int L = counted_keys(p, si);
     const int64_t nu = (L + 15) / 16;
     for (int hg = 0; hg < hgroups; ++hg) {
       const size_t first = p->segs.size();
@@ -318,16 +328,22 @@ struct PrefillPiece {
   int64_t kend;
   int64_t pairs;
 };
-void prefill_pieces(const SeqInfo& s, int i, int G, int Hkv, std::vector<PrefillPiece>& out, int pw = 8) {
+void prefill_pieces(const gllm_attn_plan* p, const SeqInfo& s, int i, int G, int Hkv, std::vector<PrefillPiece>& out,
+                    int pw = 8) {
   const int nrb = (s.q_len + 31) / 32;
   const int nwg = (G * nrb + pw - 1) / pw;
   for (int h = 0; h < Hkv; ++h)
     for (int w = 0; w < nwg; ++w) {
       const int c0 = w * pw, c1 = std::min(w * pw + pw - 1, G * nrb - 1);
-      const int64_t kend = s.ctx_len + std::min(s.q_len - 1, (c1 / G) * 32 + 31) + 1;
+      int64_t kend = s.ctx_len + std::min(s.q_len - 1, (c1 / G) * 32 + 31) + 1;
       int64_t pairs = 0;
+      if (p->window > 0) kend -= key_skip(s.ctx_len + c0 / G * 32, p->window, p->sinks, 64).by;   // keys passed over
       for (int c = c0; c <= c1; ++c) {
         const int64_t r0 = (int64_t)(c / G) * 32, r1 = std::min<int64_t>(s.q_len, r0 + 32);
+        if (p->window > 0) {                       // the first row's keys for each: the item's work within a tile's
+          pairs += (r1 - r0) * (s.ctx_len + r0 + 1 - key_skip((int32_t)(s.ctx_len + r0), p->window, p->sinks, 1).by);
+          continue;
+        }
         pairs += (r1 - r0) * (s.ctx_len + 1) + (r0 + r1 - 1) * (r1 - r0) / 2;   // row r sees ctx + r + 1 keys
       }
       out.push_back({WorkItem{kItemPrefill | (w << 8), i, h, s.q_row_start, s.ctx_len, s.q_len, 0, 0}, kend, pairs});
@@ -417,6 +433,11 @@ extern "C" {
 
 const char* gllm_attn_last_error(void) { return g_last_error.c_str(); }
 int gllm_attn_version(void) { return 1; }
+
+size_t gllm_kv4_record_bytes(int32_t block_size, int32_t head_dim) {
+  if (block_size <= 0 || block_size > kMaxBlockSize || head_dim <= 0 || head_dim % 32) return 0;
+  return (size_t)kv4_record_bytes(block_size, head_dim);
+}
 
 int gllm_build_metadata(const int32_t* block_table, int64_t block_table_stride, int64_t block_table_width,
                         const int32_t* seq_lens, const int32_t* query_lens, int32_t num_seqs,
@@ -619,6 +640,15 @@ int gllm_attn_plan_create(gllm_attn_plan** out, const int32_t* query_lens, const
                           int32_t num_seqs, int64_t q_seq_stride, int32_t num_q_heads,
                           int32_t num_kv_heads, int32_t head_dim, int32_t block_size, int32_t dtype,
                           int32_t split_tokens, int32_t decode_heads_per_wg) {
+  return gllm_attn_plan_create_window(out, query_lens, seq_lens, num_seqs, q_seq_stride, num_q_heads, num_kv_heads,
+                                      head_dim, block_size, dtype, split_tokens, decode_heads_per_wg, 0, 0);
+}
+
+int gllm_attn_plan_create_window(gllm_attn_plan** out, const int32_t* query_lens, const int32_t* seq_lens,
+                                 int32_t num_seqs, int64_t q_seq_stride, int32_t num_q_heads,
+                                 int32_t num_kv_heads, int32_t head_dim, int32_t block_size, int32_t dtype,
+                                 int32_t split_tokens, int32_t decode_heads_per_wg, int32_t window,
+                                 int32_t sinks) {
   if (!out) return fail(GLLM_ATTN_EINVAL, "plan out-pointer is null");
   *out = nullptr;
   if (num_seqs < 0 || (num_seqs > 0 && (!query_lens || !seq_lens)))
@@ -638,12 +668,26 @@ int gllm_attn_plan_create(gllm_attn_plan** out, const int32_t* query_lens, const
       decode_heads_per_wg != 4 && decode_heads_per_wg != 8)
     return fail(GLLM_ATTN_EINVAL, "decode_heads_per_wg must be 0 (auto), 1, 2, 4 or 8");
   if (q_seq_stride < 0) return fail(GLLM_ATTN_EINVAL, "q_seq_stride < 0");
+  if (window < 0 || sinks < 0) return fail(GLLM_ATTN_EINVAL, "window %d and sinks %d must be >= 0", window, sinks);
+  if (window == 0 && sinks > 0) return fail(GLLM_ATTN_EINVAL, "sinks go with a window (every key is visible without one)");
   const int G = num_q_heads / num_kv_heads;
+  // A window that hides no key of the batch is none (the last row of a sequence
+  // sees back furthest from its end): the plain kernels are the same or faster.
+  bool hides = false;
+  for (int i = 0; i < num_seqs; ++i) {
+    hides = hides || (window > 0 && seq_lens[i] > window && (int64_t)seq_lens[i] - window > sinks);
+    if (window > 0 && seq_lens[i] > INT32_MAX - 64)
+      return fail(GLLM_ATTN_EINVAL, "sequence %d: seq_len %d too long for a window", i, seq_lens[i]);
+  }
 
   gllm_attn_plan* p = new (std::nothrow) gllm_attn_plan();
   if (!p) return fail(GLLM_ATTN_EINVAL, "out of host memory");
   p->num_seqs = num_seqs; p->Hq = num_q_heads; p->Hkv = num_kv_heads; p->D = head_dim;
   p->bs = block_size; p->dtype = dtype; p->mfma = mfma;
+  if (hides) {
+    p->window = window;
+    p->sinks = sinks;
+  }
   p->seqs.resize(num_seqs);
   int64_t row = 0, all_rows = 0, tile_wgs = 0;
   for (int i = 0; i < num_seqs; ++i) {
@@ -675,7 +719,7 @@ int gllm_attn_plan_create(gllm_attn_plan** out, const int32_t* query_lens, const
     return fail(GLLM_ATTN_EINVAL, "too many query rows");
   }
 
-  if (tile_wgs >= kTileMinWgs) p->tile_min_q = kTileMinRows;
+  if (tile_wgs >= kTileMinWgs && !hides) p->tile_min_q = kTileMinRows;
   else {
     p->max_stream_q = p->max_q;
     p->stream_rows = all_rows;
@@ -695,7 +739,7 @@ int gllm_attn_plan_create(gllm_attn_plan** out, const int32_t* query_lens, const
       // below; 291 vs 299 µs with 128 decodes and 4 prefills).
       if (n_pf < num_seqs && split_tokens == GLLM_SPLIT_BALANCED) {
         for (int i = 0; i < num_seqs; ++i)
-          if (p->seqs[i].q_len * G > 16) prefill_pieces(p->seqs[i], i, G, num_kv_heads, pcs);
+          if (p->seqs[i].q_len * G > 16) prefill_pieces(p, p->seqs[i], i, G, num_kv_heads, pcs);
         mixed_wgs = mixed_decode_wgs(p, cus, decode_heads_per_wg, pcs);
         balanced = true;
       }
@@ -724,7 +768,7 @@ int gllm_attn_plan_create(gllm_attn_plan** out, const int32_t* query_lens, const
     // spreads one sequence over several CUs.  If none fills the GPU, HW=2 and
     // sequences are split into equal key ranges.  A split caches at most 511
     // block ids.
-    int64_t cap = (int64_t)511 * block_size / 32 * 32;
+    int64_t cap = (int64_t)(hides ? 507 : 511) * block_size / 32 * 32;
     cap = std::max<int64_t>(32, std::min<int64_t>(cap, 8192));
     int64_t ndec = 0;
     for (int i = 0; i < num_seqs; ++i)
@@ -749,7 +793,7 @@ int gllm_attn_plan_create(gllm_attn_plan** out, const int32_t* query_lens, const
       const auto items = [&](int64_t S) {
         int64_t k = 0;
         for (const SeqInfo& s : p->seqs)
-          if (s.q_len * G <= 16) k += (s.ctx_len + s.q_len + S - 1) / S * hg_n;
+          if (s.q_len * G <= 16) k += (counted_keys(p, s) + S - 1) / S * hg_n;
         return k;
       };
       int64_t lo = min_S / 32, hi = cap / 32;     // items(S) falls as S grows
@@ -774,7 +818,7 @@ int gllm_attn_plan_create(gllm_attn_plan** out, const int32_t* query_lens, const
         if (n_pf > 0) {
           int64_t decode_tokens = 0;
           for (const SeqInfo& s : p->seqs)
-            if (s.q_len * G <= 16) decode_tokens += s.ctx_len + s.q_len;
+            if (s.q_len * G <= 16) decode_tokens += counted_keys(p, s);
           best_S = std::max<int64_t>(((2 * decode_tokens * hg_n + target - 1) / target + 31) / 32 * 32, 256);
         } else {
           best_S = shortest_split(128, cus);
@@ -783,7 +827,7 @@ int gllm_attn_plan_create(gllm_attn_plan** out, const int32_t* query_lens, const
           // 448 keys: 1B heads 8.5 / 10.3, 9.6 / 10.3, 11.5 / 10.6; 8B heads 13.5 /
           // 13.9, 15.8 / 13.8, 19.6 / 14.0).
           int64_t longest = 0;
-          for (const SeqInfo& s : p->seqs) longest = std::max<int64_t>(longest, s.ctx_len + s.q_len);
+          for (const SeqInfo& s : p->seqs) longest = std::max<int64_t>(longest, counted_keys(p, s));
           const int64_t n = (longest + best_S - 1) / best_S;
           if ((longest - (longest + n - 1) / n) * best_hw * head_dim * 4 < 128 << 10) best_S = cap;
         }
@@ -813,7 +857,7 @@ int gllm_attn_plan_create(gllm_attn_plan** out, const int32_t* query_lens, const
       dc.clear();
       for (int i = 0; i < num_seqs; ++i) {
         SeqInfo& s = p->seqs[i];
-        const int L = s.ctx_len + s.q_len;
+        const int L = counted_keys(p, s);
         if (s.q_len * G > 16) continue;
         ++p->n_decode_seqs;
         // equal splits of 16-key multiples (a remainder split after full
@@ -841,7 +885,7 @@ int gllm_attn_plan_create(gllm_attn_plan** out, const int32_t* query_lens, const
       if (p->seqs[i].q_len * G <= 16) continue;
       ++p->n_prefill_seqs;
       pcs.clear();
-      prefill_pieces(p->seqs[i], i, G, num_kv_heads, pcs, pw);
+      prefill_pieces(p, p->seqs[i], i, G, num_kv_heads, pcs, pw);
       for (const PrefillPiece& pc : pcs) pf.push_back({pc.kend, pc.it});
     }
     longest_first(pf);
@@ -854,7 +898,7 @@ int gllm_attn_plan_create(gllm_attn_plan** out, const int32_t* query_lens, const
     // the other side: 1 x 2,048 44.5 / 52.0 (256), 4 x 1,024 33.1 / 37.9 (512, 528), 2 x 4,096
     // 173 / 177 (1,024), 64 x 64 on 1,000 65.7 / 64.8, 109 x 132 on 1,024 279 / 303 (2,616, 1,132),
     // 32 x 1,024 256 / 258.  fp16 and an fp8 cache lose 2-45% everywhere and stay at one.
-    if (!pf.empty() && head_dim == 64) {
+    if (!pf.empty() && head_dim == 64 && !hides) {
       int64_t keys = 0;
       bool context = false;
       for (const Keyed& k : pf) {
@@ -1080,6 +1124,18 @@ static int fill_common(AttnArgs& a, int32_t Hq, int32_t Hkv, int32_t D, float sc
   return ok();
 }
 
+// The layout of a 4-bit cache: 16-byte rows of codes, blocks at 32-bit byte strides.
+static int kv4_check(const void* k_cache, const void* v_cache, int64_t block_stride, int32_t Hkv, int32_t D,
+                     int64_t bs) {
+  if (D % 32) return fail(GLLM_ATTN_EUNSUPPORTED, "4-bit cache: head_dim %d must be a multiple of 32", D);
+  if (((uintptr_t)k_cache | (uintptr_t)v_cache) & 15) return fail(GLLM_ATTN_EINVAL, "4-bit caches must be 16-byte aligned");
+  const int64_t rec = kv4_record_bytes(bs, D);
+  if (block_stride < Hkv * rec || block_stride % 16 || block_stride >= (int64_t(1) << 32))
+    return fail(GLLM_ATTN_EINVAL, "4-bit cache: %lld bytes between blocks; a multiple of 16 and at least %lld needed "
+                                  "(%d kv heads x %lld)", (long long)block_stride, (long long)(Hkv * rec), Hkv, (long long)rec);
+  return ok();
+}
+
 // gllm_paged_attention and, with k_new / v_new, gllm_paged_attention_write_kv.
 static int paged_attention_impl(const gllm_attn_plan* p, const void* q, int64_t q_row_stride, void* out,
                                 int64_t out_row_stride, const void* k_cache, const void* v_cache,
@@ -1094,7 +1150,15 @@ static int paged_attention_impl(const gllm_attn_plan* p, const void* q, int64_t 
   if (!q || !out || !k_cache || !v_cache || !block_table) return fail(GLLM_ATTN_EINVAL, "null pointer argument");
   const int64_t hd = (int64_t)p->Hq * p->D;
   if (q_row_stride < hd || out_row_stride < hd) return fail(GLLM_ATTN_EINVAL, "q/out row stride < num_q_heads * head_dim");
-  if (cache_slot_stride < (int64_t)p->Hkv * p->D) return fail(GLLM_ATTN_EINVAL, "cache_slot_stride too small");
+  const bool kv4 = kv_dtype == GLLM_DTYPE_MXFP4;
+  if (kv4) {
+    if (!p->mfma) return fail(GLLM_ATTN_EUNSUPPORTED, "4-bit cache: bf16 or f16 model, head_dim 64 or 128 (model dtype %d, "
+                                                      "head_dim %d)", p->dtype, p->D);
+    if (int rc = kv4_check(k_cache, v_cache, cache_slot_stride, p->Hkv, p->D, p->bs)) return rc;
+    if (k_new || v_new) return fail(GLLM_ATTN_EUNSUPPORTED, "4-bit cache: the KV write is a call of its own");
+  } else if (cache_slot_stride < (int64_t)p->Hkv * p->D) {
+    return fail(GLLM_ATTN_EINVAL, "cache_slot_stride too small");
+  }
   if (num_blocks <= 0) return fail(GLLM_ATTN_EINVAL, "num_blocks must be > 0");
   if ((uint64_t)num_blocks * (uint64_t)p->bs >= (1ull << 32))
     return fail(GLLM_ATTN_EUNSUPPORTED, "pool of %lld blocks x %d slots exceeds 2^32 slots", (long long)num_blocks, p->bs);
@@ -1103,7 +1167,8 @@ static int paged_attention_impl(const gllm_attn_plan* p, const void* q, int64_t 
     return fail(GLLM_ATTN_EINVAL, "rope_mode %d", rope_mode);
   if (rope_mode != GLLM_ROPE_NONE && (!rope_cos || !rope_sin || rope_row_stride < p->D / 2))
     return fail(GLLM_ATTN_EINVAL, "rope tables missing or row stride < head_dim / 2");
-  if (!kv_dtype_ok(kv_dtype)) return fail(GLLM_ATTN_EUNSUPPORTED, "kv_dtype %d (f32, bf16, f16 or fp8 e4m3fn)", kv_dtype);
+  if (!kv4 && !kv_dtype_ok(kv_dtype))
+    return fail(GLLM_ATTN_EUNSUPPORTED, "kv_dtype %d (f32, bf16, f16, fp8 e4m3fn or mxfp4)", kv_dtype);
   AttnArgs a{};
   if (int rc = fill_common(a, p->Hq, p->Hkv, p->D, scale, dtype, kv_dtype)) return rc;
   a.q = q; a.q_row_stride = q_row_stride; a.out = out; a.out_row_stride = out_row_stride;
@@ -1112,6 +1177,8 @@ static int paged_attention_impl(const gllm_attn_plan* p, const void* q, int64_t 
   a.block_size = p->bs;
   block_div(p->bs, &a.block_magic, &a.block_shift);
   a.rope_cos = rope_cos; a.rope_sin = rope_sin; a.rope_row_stride = rope_row_stride; a.rope_mode = rope_mode;
+  a.window = p->window; a.sinks = p->sinks;
+  if (kv4) a.kv4_record = (int32_t)kv4_record_bytes(p->bs, p->D);
   a.seqs = (const SeqInfo*)(p->ws + p->off_seqs);
   a.items = (const WorkItem*)(p->ws + p->off_items);
   a.n_items = (int32_t)p->items.size();
@@ -1136,7 +1203,7 @@ static int paged_attention_impl(const gllm_attn_plan* p, const void* q, int64_t 
   // the MFMA kernels read a cache in the model dtype or fp8; a 16-bit model
   // over an f32 (or the other 16-bit) cache takes the generic kernel, which
   // rounds each cached value to the model dtype as the reference's gather does
-  const bool use_mfma = p->mfma && (kv_dtype == dtype || kv_dtype == GLLM_DTYPE_FP8_E4M3);
+  const bool use_mfma = p->mfma && (kv_dtype == dtype || kv_dtype == GLLM_DTYPE_FP8_E4M3 || kv4);
   if (k_new || v_new) {
     if (!k_new || !v_new) return fail(GLLM_ATTN_EINVAL, "k_new and v_new go together");
     const int64_t kvd = (int64_t)p->Hkv * p->D;
@@ -1144,6 +1211,8 @@ static int paged_attention_impl(const gllm_attn_plan* p, const void* q, int64_t 
       return fail(GLLM_ATTN_EINVAL, "k_new / v_new row stride < num_kv_heads * head_dim");
     // every sequence on the decode path: its new keys are read only by the
     // task that writes them (prefill items read other items' new keys)
+    if (!use_mfma && p->window > 0)
+      return fail(GLLM_ATTN_EUNSUPPORTED, "sliding window on the generic kernel: the KV write is a call of its own");
     if (use_mfma ? p->n_prefill_seqs > 0 : p->max_q > kMaxFusedRows)
       return fail(GLLM_ATTN_EINVAL, "the fused KV write needs a decode-path plan (query_len x G <= 16 on the MFMA "
                                     "kernels, query_len <= %d on the generic one)", kMaxFusedRows);

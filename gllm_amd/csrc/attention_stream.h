@@ -131,6 +131,9 @@ __device__ __forceinline__ u32x2 pack4(const Raw4<KV>& r) {
 // [0, ctx), and one wave takes the new ones from LDS as a last sub-tile.  The
 // workgroup of the first column stores them at their slots (block table); no
 // workgroup of the launch reads those slots.
+// WIN (sliding window): the sub-tiles count through the keys that the first of
+// the workgroup's rows leaves (key_skip); a sub-tile at the edge of a row's
+// window is masked.
 constexpr int kFusedRows = 16;
 template <typename KV, typename QT, int DP, int V>
 struct StreamCfg {
@@ -145,7 +148,7 @@ struct StreamCfg {
   // 4 are rare)
   static constexpr int kPF = V < 4 || DP == 256 ? 0 : (kBytes <= 256 ? 2 : 1);
 };
-template <bool DENSE, typename KV, typename QT, int DP, bool FUSED, int V>
+template <bool DENSE, typename KV, typename QT, int DP, bool FUSED, int V, bool WIN>
 __global__ void __launch_bounds__((64 * StreamCfg<KV, QT, DP, V>::kNW)) attn_stream_kernel(AttnArgs a) {
   using Cfg = StreamCfg<KV, QT, DP, V>;
   constexpr int NW = Cfg::kNW, PF = Cfg::kPF;
@@ -187,7 +190,10 @@ __global__ void __launch_bounds__((64 * StreamCfg<KV, QT, DP, V>::kNW)) attn_str
   const int col = min(c0 + n, ncol - 1);
   const int r = col / G, g = col - r * G;
   const int r_last = (min(c0 + 16, ncol) - 1) / G;
-  const int nkeys = DENSE ? L : (FUSED ? ctx : ctx + r_last + 1);
+  static_assert(!WIN || (!DENSE && !FUSED), "a window is the paged kernel's, its KV write a call of its own");
+  const KeySkip sk = WIN ? key_skip(ctx + c0 / G, a.window, a.sinks, 16) : KeySkip{0, 0, 0};
+  const auto key_of = [&](int v) { return WIN && v >= sk.from ? v + sk.by : v; };
+  const int nkeys = DENSE ? L : (FUSED ? ctx : ctx + r_last + 1 - (WIN ? sk.by : 0));
   const int vis = DENSE ? L - 1 : ctx + r;       // last visible key of the lane's column
   const int32_t* bt = DENSE ? nullptr : a.block_table + (int64_t)b * a.block_table_stride;
   const KV* kbase = DENSE ? (const KV*)a.k + (int64_t)b * a.k_batch_stride + (int64_t)kvh * D
@@ -206,7 +212,8 @@ __global__ void __launch_bounds__((64 * StreamCfg<KV, QT, DP, V>::kNW)) attn_str
   // its K/V); lanes of grp share it
   auto block_of = [&](int t) -> uint32_t {
     if (DENSE) return 0;
-    const int key = min(16 * (wave + NW * t) + n, nkeys - 1);
+    const int v = min(16 * (wave + NW * t) + n, nkeys - 1);
+    const int key = WIN ? seen_key(key_of(v), sk, a.sinks) : v;
     return (uint32_t)bt[div_bs((uint32_t)key, a.block_magic, a.block_shift)];
   };
   struct Tile {
@@ -216,7 +223,8 @@ __global__ void __launch_bounds__((64 * StreamCfg<KV, QT, DP, V>::kNW)) attn_str
   };
   auto issue = [&](int t, uint32_t blk, Tile& x) {
     const int p0 = 16 * (wave + NW * t);
-    const int key = min(p0 + n, nkeys - 1);      // keys past the end: masked, re-read the last
+    const int v = min(p0 + n, nkeys - 1);        // keys past the end: masked, re-read the last
+    const int key = WIN ? seen_key(key_of(v), sk, a.sinks) : v;
     int64_t row = key;
     if (!DENSE) {
       const uint32_t bi = div_bs((uint32_t)key, a.block_magic, a.block_shift);
@@ -344,8 +352,8 @@ __global__ void __launch_bounds__((64 * StreamCfg<KV, QT, DP, V>::kNW)) attn_str
 
   // One sub-tile: kf(u) = K dims 16u + 4grp .. + 3 of key n, vf(j, u) = V dims
   // 64u + 4n .. + 3 of key 4grp + j (fp32 values, or packed words of a 16-bit
-  // model); lim: keys 4grp + j <= lim are visible
-  auto tile = [&](auto kf, auto vf, int lim, bool mask, const float* bias) {
+  // model); lim: keys 4grp + j <= lim are visible (WIN: except those <= lo and >= sink)
+  auto tile = [&](auto kf, auto vf, int lim, int lo, int sink, bool mask, const float* bias) {
     // two chains: half the length of the fp32 sums; from 128 dims on, the fp32
     // products' in two halves of the dims
     f32x4 s = {0.f, 0.f, 0.f, 0.f}, s1 = s, sh = s;
@@ -377,7 +385,7 @@ __global__ void __launch_bounds__((64 * StreamCfg<KV, QT, DP, V>::kNW)) attn_str
     for (int j = 0; j < 4; ++j) {
       s[j] *= a.scale;
       if constexpr (DENSE) s[j] += bias[j];
-      if (mask && 4 * grp + j > lim) s[j] = kNegInf;
+      if (mask && (4 * grp + j > lim || (WIN && 4 * grp + j <= lo && 4 * grp + j >= sink))) s[j] = kNegInf;
     }
     float tm = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
     tm = max_xor32(max_xor16(tm));
@@ -423,8 +431,11 @@ __global__ void __launch_bounds__((64 * StreamCfg<KV, QT, DP, V>::kNW)) attn_str
 #pragma unroll
         for (int u = 0; u < NU; ++u) last2(x.v[j][u], 64 * u + 4 * n + 2 == D);
     }
-    const int lim = min(vis, nkeys - 1) - p0;
-    const bool mask = p0 + 16 > nkeys || (!DENSE && p0 + 15 > ctx);
+    const int pr = key_of(p0);
+    const int lim = min(vis, nkeys - 1 + (WIN ? sk.by : 0)) - pr;
+    const int lo = WIN ? vis - a.window - pr : 0, sink = WIN ? a.sinks - pr : 0;
+    const bool mask = p0 + 16 > nkeys || (!DENSE && pr + 15 > ctx) ||
+                      (WIN && pr <= ctx + r_last - a.window && pr + 16 > a.sinks);
     if constexpr (k16) {
       tile(
           [&](int u) {
@@ -435,7 +446,7 @@ __global__ void __launch_bounds__((64 * StreamCfg<KV, QT, DP, V>::kNW)) attn_str
             }
             return kk;
           },
-          [&](int j, int u) { return pack4<KV, QT>(x.v[j][u]); }, lim, mask, x.bias);
+          [&](int j, int u) { return pack4<KV, QT>(x.v[j][u]); }, lim, lo, sink, mask, x.bias);
     } else {
       tile(
           [&](int u) {
@@ -446,7 +457,7 @@ __global__ void __launch_bounds__((64 * StreamCfg<KV, QT, DP, V>::kNW)) attn_str
             }
             return kk;
           },
-          [&](int j, int u) { return widen4<KV, QT>(x.v[j][u]); }, lim, mask, x.bias);
+          [&](int j, int u) { return widen4<KV, QT>(x.v[j][u]); }, lim, lo, sink, mask, x.bias);
     }
   };
   // Loads are issued unconditionally in whole groups of PF + 1 sub-tiles (past
@@ -477,7 +488,7 @@ __global__ void __launch_bounds__((64 * StreamCfg<KV, QT, DP, V>::kNW)) attn_str
         else return x;
       };
       tile([&](int u) { return get(&nk[min(n, qlen - 1)][16 * u + 4 * grp]); },
-           [&](int j, int u) { return get(&nv[4 * grp + j][64 * u + 4 * n]); }, r, true, nullptr);
+           [&](int j, int u) { return get(&nv[4 * grp + j][64 * u + 4 * n]); }, r, 0, 0, true, nullptr);
     }
   }
   l = sum_xor32(sum_xor16(l));
@@ -527,12 +538,12 @@ __global__ void __launch_bounds__((64 * StreamCfg<KV, QT, DP, V>::kNW)) attn_str
   }
 }
 
-template <bool DENSE, typename KV, typename QT, bool FUSED>
+template <bool DENSE, typename KV, typename QT, bool FUSED, bool WIN>
 static hipError_t launch_stream_d(const AttnArgs& a, dim3 grid, hipStream_t st) {
   auto go = [&](auto dp, auto v) {
     constexpr int DP = decltype(dp)::value, V = decltype(v)::value;
     const dim3 block(64 * StreamCfg<KV, QT, DP, V>::kNW);
-    hipLaunchKernelGGL((attn_stream_kernel<DENSE, KV, QT, DP, FUSED, V>), grid, block, 0, st, a);
+    hipLaunchKernelGGL((attn_stream_kernel<DENSE, KV, QT, DP, FUSED, V, WIN>), grid, block, 0, st, a);
   };
   auto by_dim = [&](auto v) {
     if (a.head_dim <= 64) go(std::integral_constant<int, 64>(), v);
@@ -545,13 +556,19 @@ static hipError_t launch_stream_d(const AttnArgs& a, dim3 grid, hipStream_t st) 
   return hipGetLastError();
 }
 
-// Cache dtype KV under model dtype QT (paged), or QT throughout (dense).
-template <typename QT>
+// Cache dtype KV under model dtype QT (paged), or QT throughout (dense); WIN:
+// with a sliding window (paged, no fused KV write).
+template <typename QT, bool WIN>
 static hipError_t launch_stream_t(const AttnArgs& a, bool dense, dim3 grid, hipStream_t st) {
-  if (dense) return launch_stream_d<true, QT, QT, false>(a, grid, st);
+  if constexpr (!WIN) {
+    if (dense) return launch_stream_d<true, QT, QT, false, false>(a, grid, st);
+  }
   auto go = [&](auto kv) {
     using KV = decltype(kv);
-    return a.k_new ? launch_stream_d<false, KV, QT, true>(a, grid, st) : launch_stream_d<false, KV, QT, false>(a, grid, st);
+    if constexpr (!WIN) {
+      if (a.k_new) return launch_stream_d<false, KV, QT, true, false>(a, grid, st);
+    }
+    return launch_stream_d<false, KV, QT, false, WIN>(a, grid, st);
   };
   switch (a.kv_dtype) {
     case kF32: return go(float{});

@@ -163,6 +163,10 @@ template <> struct E16<__bf16> {
   template <bool HI> __device__ static uint32_t fp8x2(uint32_t w) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, 1.0f, HI));
   }
+  // 2 fp4 e2m1 codes (byte SEL of w, low half first) times scale (a power of two) -> 2 elements
+  template <int SEL> __device__ static uint32_t fp4x2(uint32_t w, float scale) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, SEL));
+  }
   // c + lo + hi (one v_dot2c against 1.0)
   __device__ static float add2(uint32_t w, float c) {
     const bf16x2 one = {(__bf16)1.0f, (__bf16)1.0f};
@@ -194,6 +198,9 @@ template <> struct E16<_Float16> {
   // every e4m3 value is an fp16 value: exact
   template <bool HI> __device__ static uint32_t fp8x2(uint32_t w) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.0f, HI));
+  }
+  template <int SEL> __device__ static uint32_t fp4x2(uint32_t w, float scale) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, SEL));
   }
   __device__ static float add2(uint32_t w, float c) {
     const f16x2 one = {(_Float16)1.0f, (_Float16)1.0f};
@@ -246,6 +253,27 @@ template <typename T>
 __device__ __forceinline__ u32x4 fp8x8_to(uint32_t w0, uint32_t w1) {
   return u32x4{E16<T>::template fp8x2<false>(w0), E16<T>::template fp8x2<true>(w0),
                E16<T>::template fp8x2<false>(w1), E16<T>::template fp8x2<true>(w1)};
+}
+
+// ---------------------------------------------------------------- 4-bit cache (MXFP4)
+// A 4-bit KV cache holds, of each (block, kv head), a record of block_size rows
+// of D / 2 code bytes (OCP fp4 e2m1, the even dim in the low half), then
+// block_size rows of D / 32 scale bytes, padded to 16 bytes.  A block of 32
+// dims stands for code x 2^(byte - 127); byte 255 makes its values NaN.  The
+// scale is the least 2^e at which the block's largest magnitude rounds to at
+// most 6, the largest code: amax < 7 x 2^e (7 would round to 8), so no value is
+// off by more than half a step.  The hardware's converts agree with that (low
+// half first, ties to even, scale byte 255 -> NaN), checked on gfx950.
+enum : int { kKV16 = 0, kKV8 = 1, kKV4 = 2 };   // cache format of the MFMA kernels
+
+__host__ __device__ inline int64_t kv4_record_bytes(int64_t block_size, int64_t head_dim) {
+  return (block_size * (head_dim / 32 * 17) + 15) / 16 * 16;
+}
+// 8 codes of one block -> 8 elements of T (bf16: exact; fp16: rounded to nearest even)
+template <typename T>
+__device__ __forceinline__ u32x4 fp4x8_to(uint32_t w, float scale) {
+  return u32x4{E16<T>::template fp4x2<0>(w, scale), E16<T>::template fp4x2<1>(w, scale),
+               E16<T>::template fp4x2<2>(w, scale), E16<T>::template fp4x2<3>(w, scale)};
 }
 
 // ---------------------------------------------------------------- memory
@@ -323,6 +351,29 @@ __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_ex
 // magic = 2^31, i.e. p >> k.
 __device__ __forceinline__ uint32_t div_bs(uint32_t p, uint32_t magic, int shift) {
   return __umulhi(p << 1, magic) >> shift;
+}
+
+// Sliding window: key t is visible to the row at position p iff t <= p and
+// (t > p - window or t < sinks).  Rows from position p0 on leave out the keys
+// [from, from + by): whole units (of `unit` keys) past the last sink and before
+// p0's window, which starts at `first`.
+struct KeySkip { int32_t from, by, first; };
+__host__ __device__ inline KeySkip key_skip(int32_t p0, int32_t window, int32_t sinks, int32_t unit) {
+  KeySkip s;
+  const int32_t f = p0 - window + 1;          // no overflow: p0 >= 0, window >= 1
+  s.first = f > 0 ? f : 0;
+  const int32_t n = sinks < s.first ? sinks : s.first;
+  s.from = (n + unit - 1) / unit * unit;
+  const int32_t lo = s.first / unit * unit;
+  s.by = lo > s.from ? lo - s.from : 0;
+  return s;
+}
+// A key that may be read in place of `key`: itself where some row sees it, else
+// (between the sinks and the first row's window, where a caller may have given
+// the block back) a visible key of the same unit: the last sink or the window's
+// first key.
+__device__ __forceinline__ int seen_key(int key, const KeySkip& s, int sinks) {
+  return key >= sinks && key < s.first ? (key < s.from ? sinks - 1 : s.first) : key;
 }
 
 // Sequence / work descriptors shared by host planner and kernels.

@@ -1,7 +1,8 @@
 // Generic attention (any model dtype over any cache dtype, even head dims up to
 // 256): the fp32 model's kernels and the dispatch between them.  The 16-bit
 // models' instantiations are units of their own (generic_attention_bf16.hip,
-// generic_attention_f16.hip).
+// generic_attention_f16.hip), and so are those with a sliding window
+// (generic_window_*.hip).
 #ifndef GLLM_GENERIC_QT
 #define GLLM_GENERIC_QT float
 #define GLLM_GENERIC_LAUNCH launch_generic_f32
@@ -9,17 +10,29 @@
 #endif
 
 #include "attention_stream.h"
+#ifndef GLLM_GENERIC_WINDOW
 #include "attention_tile.h"
+#endif
 
 namespace gllm {
 
-hipError_t GLLM_GENERIC_LAUNCH(const AttnArgs& a, bool tile, bool dense, dim3 grid, hipStream_t st) {
-  return tile ? launch_tile_t<GLLM_GENERIC_QT>(a, dense, grid, st) : launch_stream_t<GLLM_GENERIC_QT>(a, dense, grid, st);
+#ifdef GLLM_GENERIC_WINDOW
+hipError_t GLLM_GENERIC_LAUNCH(const AttnArgs& a, dim3 grid, hipStream_t st) {
+  return launch_stream_t<GLLM_GENERIC_QT, true>(a, false, grid, st);
 }
+#else
+hipError_t GLLM_GENERIC_LAUNCH(const AttnArgs& a, bool tile, bool dense, dim3 grid, hipStream_t st) {
+  return tile ? launch_tile_t<GLLM_GENERIC_QT>(a, dense, grid, st)
+              : launch_stream_t<GLLM_GENERIC_QT, false>(a, dense, grid, st);
+}
+#endif
 
 #ifdef GLLM_GENERIC_DISPATCH
 hipError_t launch_generic_bf16(const AttnArgs& a, bool tile, bool dense, dim3 grid, hipStream_t st);
 hipError_t launch_generic_f16(const AttnArgs& a, bool tile, bool dense, dim3 grid, hipStream_t st);
+hipError_t launch_window_f32(const AttnArgs& a, dim3 grid, hipStream_t st);
+hipError_t launch_window_bf16(const AttnArgs& a, dim3 grid, hipStream_t st);
+hipError_t launch_window_f16(const AttnArgs& a, dim3 grid, hipStream_t st);
 
 static hipError_t launch_kind(AttnArgs a, bool tile, bool dense, dim3 grid, hipStream_t st) {
   const size_t eq = a.dtype == kF32 ? 4 : 2;
@@ -33,6 +46,14 @@ static hipError_t launch_kind(AttnArgs a, bool tile, bool dense, dim3 grid, hipS
                         : rows(a.k_cache, a.cache_slot_stride, 0) && rows(a.v_cache, a.cache_slot_stride, 0));
   }
   a.vec_out = a.head_dim % 4 == 0 && a.out_row_stride % 4 == 0 && ((uintptr_t)a.out & (4 * eq - 1)) == 0;
+  if (!dense && a.window > 0) {
+    switch (a.dtype) {
+      case kF32: return launch_window_f32(a, grid, st);
+      case kBF16: return launch_window_bf16(a, grid, st);
+      case kF16: return launch_window_f16(a, grid, st);
+      default: return hipErrorInvalidValue;
+    }
+  }
   switch (a.dtype) {
     case kF32: return launch_generic_f32(a, tile, dense, grid, st);
     case kBF16: return launch_generic_bf16(a, tile, dense, grid, st);

@@ -10,7 +10,8 @@ namespace gllm {
 // Scratch of the no-alloc QKV entry point (split-K partials)
 constexpr size_t kQkvScratchBytes = size_t(24) << 20;
 
-enum : int32_t { kF32 = 0, kBF16 = 1, kFP8 = 2, kF16 = 3 };   // kFP8: OCP e4m3fn (KV cache only)
+// kFP8: OCP e4m3fn, kMXFP4: 4-bit records (common.h); KV cache only
+enum : int32_t { kF32 = 0, kBF16 = 1, kFP8 = 2, kF16 = 3, kMXFP4 = 4 };
 
 struct RopeKVWriteArgs {
   const void* q;            // [N, q_row_stride] model dtype, heads at h*D
@@ -70,7 +71,7 @@ struct AttnArgs {
   // paged source
   const void* k_cache;
   const void* v_cache;
-  int64_t cache_slot_stride;  // elements between slots (Hkv * D)
+  int64_t cache_slot_stride;  // elements between slots (Hkv * D); 4-bit cache: bytes between blocks
   int64_t num_blocks;
   const int32_t* block_table;
   int64_t block_table_stride;
@@ -129,6 +130,10 @@ struct AttnArgs {
   int32_t tile_min_q;
   int32_t vec_rows;            // tiled kernel: K/V rows in whole aligned 16-byte chunks (set by the launcher)
   int32_t vec_out;             // output rows aligned for stores of 4 elements (set by the launcher)
+  // sliding window (0: none): keys that a row sees back from its own on, and first
+  // keys that stay visible
+  int32_t window, sinks;
+  int32_t kv4_record;          // 4-bit cache: bytes of one (block, kv head)
 };
 
 struct MetadataArgs {

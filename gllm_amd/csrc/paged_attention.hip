@@ -20,6 +20,8 @@
 //   K/V tiles of 64 keys staged in LDS, S^T = K Q^T and O^T += V^T P^T on
 //   v_mfma_f32_32x32x16_bf16, flash-style running max/sum, causal tile skip.
 //   The G query heads of one kv head share every K/V tile.
+#include <type_traits>
+
 #include "common.h"
 #include "launch.h"
 
@@ -37,8 +39,8 @@ __device__ __forceinline__ void rope8(float* x1, float* x2, const float* c, cons
 // ============================================================== decode
 constexpr int kWaves = 8;   // waves per workgroup (both paths; one block size)
 
-template <int D, int NW> struct DecodeCfg {
-  static constexpr int kPF = 2;                         // sub-tiles in flight per wave (2 beat 3 at D = 64)
+template <int D, int NW, int KF> struct DecodeCfg {
+  static constexpr int kPF = KF == kKV4 ? 4 : 2;        // sub-tiles in flight per wave (16-bit: 2 beat 3 at D = 64)
   static constexpr int kRowBytes = D * 2 + 32;         // V staging row stride (bytes)
   static constexpr int kVBytes = 16 * kRowBytes;       // per-wave V staging: 16 keys
   static constexpr int kMaxBlocks = 512;               // block ids of one split, cached in LDS
@@ -61,19 +63,25 @@ template <int D, int NW> struct DecodeCfg {
 // LDS; a split sequence writes (max, sum, acc) partials that merge_splits
 // combines in a second, tiny launch (no cross-workgroup fences here).
 // Cached K/V come in 16-byte loads per lane: 8 bf16 dims, or 16 fp8 dims
-// that are widened (exactly) to bf16 on use and feed two MFMA K-chunks.
+// that are widened (exactly) to bf16 on use and feed two MFMA K-chunks; of a
+// 4-bit cache a quarter of the head (D = 128: a whole block of 32 dims with its
+// scale byte, 16 bytes; D = 64: half a block, 8 bytes).
 // Head dim of element i of MFMA chunk kk in lane group grp:
-//   bf16: 32 kk + 8 grp + i
-//   fp8:  64 (kk / 2) + 16 grp + 8 (kk % 2) + i
+//   bf16:  32 kk + 8 grp + i
+//   fp8:   64 (kk / 2) + 16 grp + 8 (kk % 2) + i
+//   4-bit: D / 4 grp + 8 kk + i
 // S = K Q^T sums over dims, so any order serves as long as K and Q agree;
 // V is staged to LDS in natural dim order, so the output is too.
-template <bool KV8>
+template <int D, int KF>
 __device__ __forceinline__ int chunk_dim(int kk, int grp) {
-  return KV8 ? 64 * (kk >> 1) + 16 * grp + 8 * (kk & 1) : 32 * kk + 8 * grp;
+  if constexpr (KF == kKV4) return D / 4 * grp + 8 * kk;
+  return KF == kKV8 ? 64 * (kk >> 1) + 16 * grp + 8 * (kk & 1) : 32 * kk + 8 * grp;
 }
-template <typename T, bool KV8>
-__device__ __forceinline__ u32x4 chunk_elems(const u32x4* raw, int kk) {
-  if constexpr (KV8) {
+template <typename T, int KF>
+__device__ __forceinline__ u32x4 chunk_elems(const u32x4* raw, float scale, int kk) {
+  if constexpr (KF == kKV4) {
+    return fp4x8_to<T>(raw[0][kk], scale);
+  } else if constexpr (KF == kKV8) {
     const u32x4 w = raw[kk >> 1];
     return (kk & 1) ? fp8x8_to<T>(w[2], w[3]) : fp8x8_to<T>(w[0], w[1]);
   } else {
@@ -96,10 +104,12 @@ struct DecodeTask {
 // this launch (each key of each head belongs to one task); the workgroup
 // barrier after the prologue orders the stores before this task's own loads
 // of the key.  Element-wise stores: at most 16 tokens x HW heads x D.
-template <typename T, int D, int HW, bool KV8>
+template <typename T, int D, int HW, int KF, bool WIN>
 __device__ __forceinline__ void write_new_keys(const AttnArgs& a, const DecodeTask& tk, int tid, int nthreads) {
+  // the range in keys of the sequence: a window's left-out keys lie before every new one
+  const int by = WIN ? key_skip(tk.ctx_len, a.window, a.sinks, 16).by : 0;
   const int L = tk.ctx_len + tk.q_len;
-  const int p0 = max(tk.ctx_len, tk.kbeg), p1 = min(L, tk.kend);
+  const int p0 = max(tk.ctx_len, tk.kbeg + by), p1 = min(L, tk.kend + by);
   if (p0 >= p1) return;
   constexpr int H2 = D / 2;
   const int per_tok = HW * H2;
@@ -126,7 +136,7 @@ __device__ __forceinline__ void write_new_keys(const AttnArgs& a, const DecodeTa
     if (blk >= (uint64_t)a.num_blocks) continue;   // never address outside the pool
     const int64_t off = ((int64_t)blk * a.block_size + (p - (int64_t)bi * a.block_size)) * a.cache_slot_stride +
                         (int64_t)kvh * D + j;
-    if constexpr (KV8) {
+    if constexpr (KF == kKV8) {
       uint8_t* kc = (uint8_t*)a.k_cache + off;
       uint8_t* vc = (uint8_t*)a.v_cache + off;
       kc[0] = fp8_byte(x1); kc[H2] = fp8_byte(x2);
@@ -142,18 +152,21 @@ __device__ __forceinline__ void write_new_keys(const AttnArgs& a, const DecodeTa
 
 // Runs one task with every wave of the workgroup; returns with the workgroup
 // converged (no early exit), so a workgroup can run several tasks in a row.
-template <typename T, int D, int HW, int KW, bool KV8>
+// WIN: the keys are those of the sequence without the run that its window
+// leaves out (key_skip): tk's range counts them through, key v at v >= from
+// being key v + by.
+template <typename T, int D, int HW, int KW, int KF, bool WIN>
 __device__ __forceinline__ void decode_task(const AttnArgs& a, const DecodeTask& tk, char* lds) {
   constexpr int NW = HW * KW;
-  constexpr int E = KV8 ? 1 : 2;   // bytes per cached element
-  using Cfg = DecodeCfg<D, NW>;
+  constexpr int E = KF == kKV16 ? 2 : 1;   // bytes per cached element (4-bit: strides in bytes)
+  using Cfg = DecodeCfg<D, NW, KF>;
   constexpr int NK = D / 32;   // 32-dim K chunks per key
-  constexpr int NL = KV8 ? NK / 2 : NK;   // 16-byte loads per key (K and V each)
+  constexpr int NL = KF == kKV4 ? 1 : (KF == kKV8 ? NK / 2 : NK);   // 16-byte loads per key (K and V each)
   constexpr int ND = D / 16;   // 16-dim output blocks
   constexpr int RB = Cfg::kRowBytes;
   // RoPE partners d, d + D/2 in the same lane (chunks kk, kk + NK/2), except
-  // for fp8 at D = 64, where a lane's 16 dims lie in one half
-  constexpr bool kPairInLane = !KV8 || D >= 128;
+  // for fp8 at D = 64 and 4-bit caches, where a lane's dims lie in one half
+  constexpr bool kPairInLane = KF == kKV16 || (KF == kKV8 && D >= 128);
   constexpr int NC = kPairInLane ? NK / 2 : NK;   // cos/sin loads
   constexpr int PF = Cfg::kPF;
   // the thread id through an opaque move: nothing derived from it is hoisted
@@ -185,14 +198,22 @@ __device__ __forceinline__ void decode_task(const AttnArgs& a, const DecodeTask&
   // store does not wait for the others).
   static_assert(Cfg::kMaxBlocks <= 64 * NW, "one block id per thread");
   int32_t* lbid = reinterpret_cast<int32_t*>(lds + NW * Cfg::kVBytes);
-  const int blk0 = (int)div_bs((uint32_t)kbeg, a.block_magic, a.block_shift);
-  const int nblk = (int)div_bs((uint32_t)(kend - 1), a.block_magic, a.block_shift) - blk0 + 1;
+  // WIN: two runs of blocks where the range has keys on both sides of the
+  // left-out ones; entry e of the cache is block blk0 + e, or from nblk_s on
+  // blk0 + bgap + e
+  const KeySkip sk = WIN ? key_skip(tk.ctx_len, a.window, a.sinks, 16) : KeySkip{0, 0, 0};
+  const bool both = WIN && kbeg < sk.from && kend > sk.from && sk.by > 0;
+  const auto key_of = [&](int v) { return WIN && v >= sk.from ? v + sk.by : v; };
+  const int blk0 = (int)div_bs((uint32_t)key_of(kbeg), a.block_magic, a.block_shift);
+  const int nblk_s = both ? (int)div_bs((uint32_t)(sk.from - 1), a.block_magic, a.block_shift) - blk0 + 1 : 0;
+  const int bgap = both ? (int)div_bs((uint32_t)(sk.from + sk.by), a.block_magic, a.block_shift) - blk0 - nblk_s : 0;
+  const int nblk = (int)div_bs((uint32_t)key_of(kend - 1), a.block_magic, a.block_shift) - (WIN ? blk0 + bgap : blk0) + 1;
   const int32_t* bt = a.block_table + (int64_t)seq * a.block_table_stride + blk0;
-  const uint32_t bid = tid < nblk ? (uint32_t)bt[tid] : 0u;
+  const uint32_t bid = tid < nblk ? (uint32_t)bt[WIN && tid >= nblk_s ? tid + bgap : tid] : 0u;
   const T* qp = (const T*)a.q + qrow * a.q_row_stride + (int64_t)qh * D;
   u32x4 qraw[NK], praw[kPairInLane ? 1 : NK], craw[NC], sraw[NC];
 #pragma unroll
-  for (int kk = 0; kk < NK; ++kk) qraw[kk] = ld16(qp + chunk_dim<KV8>(kk, grp));
+  for (int kk = 0; kk < NK; ++kk) qraw[kk] = ld16(qp + chunk_dim<D, KF>(kk, grp));
   const bool rope = a.rope_mode != kRopeNone;
   if (rope) {
     const int64_t crow = a.rope_mode == kRopeByPosition ? (int64_t)vis : qrow;
@@ -200,17 +221,19 @@ __device__ __forceinline__ void decode_task(const AttnArgs& a, const DecodeTask&
     const T* sp = (const T*)a.rope_sin + crow * a.rope_row_stride;
 #pragma unroll
     for (int kk = 0; kk < NC; ++kk) {
-      const int d = chunk_dim<KV8>(kk, grp) & (D / 2 - 1);
+      const int d = chunk_dim<D, KF>(kk, grp) & (D / 2 - 1);
       craw[kk] = ld16(cp + d);
       sraw[kk] = ld16(sp + d);
     }
     if constexpr (!kPairInLane) {
 #pragma unroll
-      for (int kk = 0; kk < NK; ++kk) praw[kk] = ld16(qp + (chunk_dim<KV8>(kk, grp) ^ (D / 2)));
+      for (int kk = 0; kk < NK; ++kk) praw[kk] = ld16(qp + (chunk_dim<D, KF>(kk, grp) ^ (D / 2)));
     }
   }
   if (tid < nblk) lbid[tid] = bid < (uint64_t)a.num_blocks ? (int32_t)bid : 0;  // never address outside the pool
-  if (a.k_new) write_new_keys<T, D, HW, KV8>(a, tk, tid, 64 * NW);
+  if constexpr (KF != kKV4) {
+    if (a.k_new) write_new_keys<T, D, HW, KF, WIN>(a, tk, tid, 64 * NW);
+  }
 
   // Q as the B operand of S^T = K Q^T: lane holds Q[row n][chunk_dim(kk) + i].
   u32x4 qB[NK];
@@ -229,7 +252,7 @@ __device__ __forceinline__ void decode_task(const AttnArgs& a, const DecodeTask&
         }
       } else {
         // the same roundings as rope8, one half of the pair per lane
-        const bool first = chunk_dim<KV8>(0, grp) < D / 2;
+        const bool first = chunk_dim<D, KF>(0, grp) < D / 2;
 #pragma unroll
         for (int kk = 0; kk < NK; ++kk) {
           float c[8], s[8], xp[8];
@@ -262,9 +285,14 @@ __device__ __forceinline__ void decode_task(const AttnArgs& a, const DecodeTask&
   __syncthreads();
 
   // byte addressing: slot (< 2^32) x slot bytes (< 2^32) is one 32x32->64 mad
+  // (4-bit: block x block bytes, the head's record inside the block)
   const uint32_t sbytes = (uint32_t)(a.cache_slot_stride * E);
-  const char* kc = (const char*)a.k_cache + (int64_t)(head_ok ? kvh : 0) * D * E + 16 * grp;
-  const char* vc = (const char*)a.v_cache + (int64_t)(head_ok ? kvh : 0) * D * E + 16 * grp;
+  const int64_t head_off = KF == kKV4 ? (int64_t)(head_ok ? kvh : 0) * a.kv4_record + D / 8 * grp
+                                      : (int64_t)(head_ok ? kvh : 0) * D * E + 16 * grp;
+  const char* kc = (const char*)a.k_cache + head_off;
+  const char* vc = (const char*)a.v_cache + head_off;
+  // from a key's codes to the scale byte of its row 0: the scales follow the record's codes
+  const int64_t sc_off = KF == kKV4 ? (int64_t)a.block_size * (D / 2) - D / 8 * grp + D / 4 * grp / 32 : 0;
   const float sl2 = a.scale * kLog2e;
   char* ldsV = lds + wave * Cfg::kVBytes;
 
@@ -276,33 +304,67 @@ __device__ __forceinline__ void decode_task(const AttnArgs& a, const DecodeTask&
   // this wave's sub-tiles: j = ki + KW * t, t < ntw
   const int ntw = head_ok && nsub > ki ? (nsub - ki + KW - 1) / KW : 0;
   u32x4 kr[PF + 1][NL], vr[PF + 1][NL];
-  auto issue = [&](int t, u32x4 (&kd)[NL], u32x4 (&vd)[NL]) {
+  uint32_t ksr[KF == kKV4 ? PF + 1 : 1], vsr[KF == kKV4 ? PF + 1 : 1];   // 4-bit: the scale bytes
+  auto issue = [&](int t, u32x4 (&kd)[NL], u32x4 (&vd)[NL], int slot_i) {
     // ring padding (t >= ntw): every lane reads the task's last slot, one
     // cache line per load instead of a whole 16-key tile
-    const int key = t < ntw ? min(kbeg + 16 * (ki + KW * t) + n, kend - 1) : kend - 1;
+    const int v = t < ntw ? min(kbeg + 16 * (ki + KW * t) + n, kend - 1) : kend - 1;
+    const int key = WIN ? seen_key(key_of(v), sk, a.sinks) : v;
+    const int blk = WIN && both && v >= sk.from ? blk0 + bgap : blk0;
     const uint32_t bi = div_bs((uint32_t)key, a.block_magic, a.block_shift);
-    const uint32_t slot = (uint32_t)lbid[bi - blk0] * (uint32_t)a.block_size + ((uint32_t)key - bi * (uint32_t)a.block_size);
-    const uint64_t off = (uint64_t)slot * sbytes;
+    if constexpr (KF == kKV4) {
+      const uint32_t o = (uint32_t)key - bi * (uint32_t)a.block_size;
+      const uint64_t off = (uint64_t)(uint32_t)lbid[bi - blk] * sbytes;
+      const uint64_t code = off + o * (D / 2), sc = off + sc_off + o * (D / 32);
+      if constexpr (D == 128) {
+        kd[0] = ld16(kc + code);
+        vd[0] = ld16(vc + code);
+      } else {
+        const u32x2 k2 = *reinterpret_cast<const u32x2*>(kc + code), v2 = *reinterpret_cast<const u32x2*>(vc + code);
+        kd[0] = u32x4{k2[0], k2[1], 0u, 0u};
+        vd[0] = u32x4{v2[0], v2[1], 0u, 0u};
+      }
+      ksr[slot_i] = (uint8_t)kc[sc];
+      vsr[slot_i] = (uint8_t)vc[sc];
+    } else {
+      const uint32_t slot = (uint32_t)lbid[bi - blk] * (uint32_t)a.block_size + ((uint32_t)key - bi * (uint32_t)a.block_size);
+      const uint64_t off = (uint64_t)slot * sbytes;
 #pragma unroll
-    for (int l = 0; l < NL; ++l) {
-      kd[l] = ld16(kc + off + 64 * l);
-      vd[l] = ld16(vc + off + 64 * l);
+      for (int l = 0; l < NL; ++l) {
+        kd[l] = ld16(kc + off + 64 * l);
+        vd[l] = ld16(vc + off + 64 * l);
+      }
     }
   };
-  auto compute = [&](int t, const u32x4 (&kd)[NL], const u32x4 (&vd)[NL]) {
+  auto compute = [&](int t, const u32x4 (&kd)[NL], const u32x4 (&vd)[NL], int slot_i) {
     // tiles past the last one (ring padding) are fully masked
     const int kb = t < ntw ? kbeg + 16 * (ki + KW * t) : kend;
+    float ks = 1.f, vs = 1.f;
+    if constexpr (KF == kKV4) {
+      ks = __uint_as_float(ksr[slot_i] << 23);
+      vs = __uint_as_float(vsr[slot_i] << 23);
+    }
     f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int kk = 0; kk < NK; ++kk) s = E16<T>::mfma16(chunk_elems<T, KV8>(kd, kk), qB[kk], s);
+    for (int kk = 0; kk < NK; ++kk) s = E16<T>::mfma16(chunk_elems<T, KF>(kd, ks, kk), qB[kk], s);
 #pragma unroll
     for (int kk = 0; kk < NK; ++kk)
-      *reinterpret_cast<u32x4*>(ldsV + n * RB + chunk_dim<KV8>(kk, grp) * 2) = chunk_elems<T, KV8>(vd, kk);
+      *reinterpret_cast<u32x4*>(ldsV + n * RB + chunk_dim<D, KF>(kk, grp) * 2) = chunk_elems<T, KF>(vd, vs, kk);
     // lane holds S[key kb + 4grp + j][row n]
     float p[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) p[j] = s[j] * sl2;
-    if (kb + 16 > kend || kb + 15 > tk.ctx_len) {
+    if constexpr (WIN) {
+      const int kr = key_of(kb);            // a sub-tile lies on one side of the left-out keys
+      // past the range, past the first row, or before the last row's window
+      if (kb + 16 > kend || kr + 15 > tk.ctx_len || (kr <= tk.ctx_len + tk.q_len - 1 - a.window && kr + 16 > a.sinks)) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int key = kr + 4 * grp + j;
+          if (kb + 4 * grp + j >= kend || key > vis || (key <= vis - a.window && key >= a.sinks)) p[j] = kNegInf;
+        }
+      }
+    } else if (kb + 16 > kend || kb + 15 > tk.ctx_len) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int key = kb + 4 * grp + j;
@@ -341,7 +403,7 @@ __device__ __forceinline__ void decode_task(const AttnArgs& a, const DecodeTask&
   if (ntw > 0) {
 #pragma unroll
     for (int u = 0; u < PF; ++u) {
-      issue(u, kr[u], vr[u]);
+      issue(u, kr[u], vr[u], u);
       __builtin_amdgcn_sched_barrier(0);
     }
     int t0 = 0;
@@ -349,16 +411,17 @@ __device__ __forceinline__ void decode_task(const AttnArgs& a, const DecodeTask&
 #pragma unroll
       for (int u = 0; u <= PF; ++u) {
         const int t = t0 + u;
-        issue(t + PF, kr[(u + PF) % (PF + 1)], vr[(u + PF) % (PF + 1)]);
+        constexpr int R = PF + 1;
+        issue(t + PF, kr[(u + PF) % R], vr[(u + PF) % R], (u + PF) % R);
         __builtin_amdgcn_sched_barrier(0);
-        compute(t, kr[u], vr[u]);
+        compute(t, kr[u], vr[u], u);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
     // last ntw - t0 (<= PF) tiles: already in flight, nothing more to issue
 #pragma unroll
     for (int u = 0; u < PF; ++u)
-      if (t0 + u < ntw) compute(t0 + u, kr[u], vr[u]);
+      if (t0 + u < ntw) compute(t0 + u, kr[u], vr[u], u);
   }
   float lt = sum_xor32(sum_xor16(lsum));
 
@@ -424,12 +487,13 @@ __device__ __forceinline__ void decode_task(const AttnArgs& a, const DecodeTask&
 // One decode work item of the split-launch planner (split it.a of the
 // sequence's it.nsplits equal key ranges; split partials merged by
 // merge_splits_kernel).
-template <typename T, int D, int HW, int KW, bool KV8>
+template <typename T, int D, int HW, int KW, int KF, bool WIN>
 __device__ __forceinline__ void decode_wg(const AttnArgs& a, const WorkItem& it, char* lds) {
   DecodeTask tk;
   tk.seq = it.seq;
   tk.hg = it.kind_b >> 8;
-  const int L = it.ctx_len + it.q_len;
+  int L = it.ctx_len + it.q_len;
+  if constexpr (WIN) L -= key_skip(it.ctx_len, a.window, a.sinks, 16).by;
   const int len = split_len_of(L, it.nsplits);   // equal splits (the planner's split_len bounds them)
   tk.kbeg = it.a * len;
   tk.kend = min(L, tk.kbeg + len);
@@ -439,7 +503,7 @@ __device__ __forceinline__ void decode_wg(const AttnArgs& a, const WorkItem& it,
   tk.nseg = it.nsplits;
   tk.pbase = it.partial_base + tk.hg * HW * it.nsplits;
   tk.ord = it.a;
-  decode_task<T, D, HW, KW, KV8>(a, tk, lds);
+  decode_task<T, D, HW, KW, KF, WIN>(a, tk, lds);
 }
 
 // Combines the split partials of every (sequence, kv head) whose sequence
@@ -560,9 +624,14 @@ __device__ __forceinline__ int pf_swz(int r) {
 // Paged mode: keys through the block table, causal mask on diagonal tiles
 // only.  Dense mode (DENSE): keys from k/v [B, T, Hkv, D], additive bias
 // [B, T_q, T] on every tile.
-template <typename T, int D, bool DENSE, int NW, int NS, bool KV8>
+// WIN: the tiles that every row of the workgroup is past with its window, and
+// that hold no sink, are left out (key_skip); tiles at either edge of a row's
+// window are masked, and a row's reference is chosen at its first tile with a
+// visible key.
+template <typename T, int D, bool DENSE, int NW, int NS, int KF, bool WIN>
 __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it, int seq, int kvh, int wgrp, char* lds) {
-  static_assert(!(DENSE && KV8), "the dense op has no cache");
+  static_assert(!(DENSE && (KF != kKV16 || WIN)), "the dense op has no cache");
+  constexpr bool KREG = KF != kKV16;       // K/V pass through registers (widened) on the way to LDS
   using Cfg = PrefillCfg<D, NS>;
   constexpr int NQ = D / 16;               // Q operand chunks (16 dims)
   constexpr int NO = D / 32;               // output blocks (32 dims)
@@ -612,15 +681,26 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
   const int64_t qrow = qstart + rr;
   const int qh = kvh * G + g;
 
+  // WIN: the workgroup's tiles start on 64 keys, so a tile lies on one side of
+  // the left-out run; its blocks are cached in two runs (nblk_s of the sinks').
+  const KeySkip sk = WIN ? key_skip(ctx + wgrp * NW / G * 32, a.window, a.sinks, BN) : KeySkip{0, 0, 0};
+  const bool both = WIN && sk.by > 0;
+  const int nblk_s = both && sk.from > 0 ? (int)div_bs((uint32_t)(sk.from - 1), a.block_magic, a.block_shift) + 1 : 0;
+  const int bgap = both ? (int)div_bs((uint32_t)(sk.from + sk.by), a.block_magic, a.block_shift) - nblk_s : 0;
+  const int lo_w = WIN ? max(0, ctx + r0 + 1 - a.window) : 0;              // first key in the wave's windows
+  const int hid_w = WIN ? ctx + min(qlen - 1, r0 + 31) - a.window : 0;     // last key before its last row's
+  const auto tile_key = [&](int t) { return WIN && t * BN >= sk.from ? t * BN + sk.by : t * BN; };
+
   // Block ids of keys [0, kend_wg), loaded into registers now and cached in
   // LDS (first kBidCache blocks; any beyond are read from the table
   // directly) after the first tiles' copies are issued.
   const int32_t* bt = DENSE ? nullptr : a.block_table + (int64_t)seq * a.block_table_stride;
   constexpr int KB = (Cfg::kBidCache + NT - 1) / NT;
-  const int nbc = DENSE ? 0 : min((int)div_bs((uint32_t)(kend_wg - 1), a.block_magic, a.block_shift) + 1, Cfg::kBidCache);
+  const int nbc = DENSE ? 0 : min((int)div_bs((uint32_t)(kend_wg - 1), a.block_magic, a.block_shift) + (WIN ? 1 - bgap : 1), Cfg::kBidCache);
   uint32_t lb[KB];
 #pragma unroll
-  for (int k = 0; k < KB; ++k) lb[k] = tid + k * NT < nbc ? (uint32_t)bt[tid + k * NT] : 0u;
+  for (int k = 0; k < KB; ++k)
+    lb[k] = tid + k * NT < nbc ? (uint32_t)bt[WIN && tid + k * NT >= nblk_s ? tid + k * NT + bgap : tid + k * NT] : 0u;
 
   // Q rows (and their cos/sin rows): loads issued now, used after the first
   // K/V copies are on their way.
@@ -674,36 +754,45 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
   constexpr int NSEG = BN / RPS;
   constexpr int CHD = NSEG / NW;          // copies per wave per K (or V) tile
   static_assert(CHD >= 1 && NSEG % NW == 0, "tile / workgroup mismatch");
-  constexpr int E = KV8 ? 1 : 2;           // bytes per cached element
+  constexpr int E = KF == kKV16 ? 2 : 1;   // bytes per cached element (4-bit: strides in bytes)
   const uint32_t sbytes = (uint32_t)(a.cache_slot_stride * E);
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
   // Slots of the DMA rows of the tile starting at key ts: block id from the
   // LDS cache (or the table past it) times the block size plus the offset in
   // the block.  Fetched one tile before the copy is issued, so the copy never
   // waits on LDS.
-  auto dma_bids = [&](int ts, uint32_t (&slot)[CHD]) {
+  // (4-bit cache: the block, and the row in it beside).
+  struct Row4 { uint32_t blk, off; };
+  using Row = std::conditional_t<KF == kKV4, Row4, uint32_t>;
+  auto copy_key = [&](int ts, int i) {
+    const int p = min(ts + (i * NW + wave) * RPS + lane / CPR, kend_wg - 1);
+    return WIN ? seen_key(p, sk, a.sinks) : p;
+  };
+  auto dma_bids = [&](int ts, Row (&slot)[CHD]) {
 #pragma unroll
     for (int i = 0; i < CHD; ++i) {
       if (DENSE) {
-        slot[i] = 0;
+        slot[i] = Row{};
       } else {
-        const int p = min(ts + (i * NW + wave) * RPS + lane / CPR, kend_wg - 1);
+        const int p = copy_key(ts, i);
         const uint32_t bi = div_bs((uint32_t)p, a.block_magic, a.block_shift);
+        const uint32_t ci = WIN && both && p >= sk.from + sk.by ? bi - (uint32_t)bgap : bi;
         uint32_t blk;
-        if (bi < (uint32_t)Cfg::kBidCache) {
-          blk = (uint32_t)lbid[bi];
+        if (ci < (uint32_t)Cfg::kBidCache) {
+          blk = (uint32_t)lbid[ci];
         } else {
           blk = (uint32_t)bt[bi];
           if (blk >= (uint64_t)a.num_blocks) blk = 0;
         }
-        slot[i] = blk * (uint32_t)a.block_size + ((uint32_t)p - bi * (uint32_t)a.block_size);
+        if constexpr (KF == kKV4) slot[i] = Row{blk, (uint32_t)p - bi * (uint32_t)a.block_size};
+        else slot[i] = blk * (uint32_t)a.block_size + ((uint32_t)p - bi * (uint32_t)a.block_size);
       }
     }
   };
   // Source of one lane's 8 elements (logical chunk lc of its row) for copy
   // instruction i, K (v = 0) or V (v = 1), of the tile at key ts (paged: the
   // row's slot from dma_bids).
-  auto copy_src = [&](int ts, const uint32_t (&slot)[CHD], int i, int v) -> const char* {
+  auto copy_src = [&](int ts, const Row (&slot)[CHD], int i, int v) -> const char* {
     const int sg = i * NW + wave;
     const int row = sg * RPS + lane / CPR;
     const int lc = (lane % CPR) ^ pf_swz<D>(row);
@@ -713,37 +802,57 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
                 : (const char*)a.k + ((int64_t)seq * a.k_batch_stride + (int64_t)p * a.k_row_stride + (int64_t)kvh * D) * 2) +
              lc * 16;
     }
-    const uint64_t off = (uint64_t)slot[i] * sbytes + (uint64_t)kvh * D * E;
-    return (const char*)(v ? a.v_cache : a.k_cache) + off + lc * 8 * E;
+    if constexpr (KF == kKV4) {
+      return (const char*)(v ? a.v_cache : a.k_cache) + ((uint64_t)slot[i].blk * sbytes + (uint64_t)kvh * a.kv4_record) +
+             (slot[i].off * (D / 2) + lc * 4);
+    } else {
+      const uint64_t off = (uint64_t)slot[i] * sbytes + (uint64_t)kvh * D * E;
+      return (const char*)(v ? a.v_cache : a.k_cache) + off + lc * 8 * E;
+    }
+  };
+  // 4-bit cache: the scale byte of the same eight elements
+  auto scale_src = [&](const Row (&slot)[CHD], int i, int v) -> const uint8_t* {
+    const int lc = (lane % CPR) ^ pf_swz<D>((i * NW + wave) * RPS + lane / CPR);
+    if constexpr (KF == kKV4)
+      return (const uint8_t*)(v ? a.v_cache : a.k_cache) + ((uint64_t)slot[i].blk * sbytes + (uint64_t)kvh * a.kv4_record) +
+             ((uint32_t)a.block_size * (D / 2) + slot[i].off * (D / 32) + lc / 4);
+    return nullptr;
   };
   // One copy instruction into `stage`: bf16 caches go HBM -> LDS directly;
-  // fp8 caches are fetched into registers (`fp8_fetch`, a tile ahead) and
-  // widened to bf16 when written (`fp8_put`), so LDS always holds bf16.
-  auto dma_one = [&](int ts, int stage, const uint32_t (&blk)[CHD], int i, int v) {
+  // fp8 and 4-bit caches are fetched into registers (`reg_fetch`, a tile ahead)
+  // and widened to bf16 when written (`reg_put`), so LDS always holds bf16.
+  auto dma_one = [&](int ts, int stage, const Row (&blk)[CHD], int i, int v) {
     const int sg = i * NW + wave;
     const uint32_t dst = __builtin_amdgcn_readfirstlane(lds0 + v * Cfg::kVBase + stage * Cfg::kTile + sg * 1024);
     lds_dma16(copy_src(ts, blk, i, v), dst);
   };
-  u32x2 f8st[CHD][2];                      // fp8 cache: fetched chunks of the tile being copied
-  auto fp8_fetch = [&](int ts, const uint32_t (&blk)[CHD]) {
-#pragma unroll
-    for (int i = 0; i < CHD; ++i)
-#pragma unroll
-      for (int v = 0; v < 2; ++v) f8st[i][v] = *reinterpret_cast<const u32x2*>(copy_src(ts, blk, i, v));
-  };
-  auto fp8_put = [&](int stage, int i, int v) {
-    const int sg = i * NW + wave;
-    *reinterpret_cast<u32x4*>(lds + v * Cfg::kVBase + stage * Cfg::kTile + sg * 1024 + lane * 16) =
-        fp8x8_to<T>(f8st[i][v][0], f8st[i][v][1]);
-  };
-  auto dma_issue = [&](int ts, int stage, const uint32_t (&blk)[CHD]) {
-    if (KV8) fp8_fetch(ts, blk);
+  u32x2 rst[CHD][2];                       // fetched chunks of the tile being copied (4-bit: codes, scale)
+  auto reg_fetch = [&](int ts, const Row (&blk)[CHD]) {
 #pragma unroll
     for (int i = 0; i < CHD; ++i)
 #pragma unroll
       for (int v = 0; v < 2; ++v) {
-        if (KV8)
-          fp8_put(stage, i, v);
+        if constexpr (KF == kKV4)
+          rst[i][v] = u32x2{*reinterpret_cast<const uint32_t*>(copy_src(ts, blk, i, v)), *scale_src(blk, i, v)};
+        else
+          rst[i][v] = *reinterpret_cast<const u32x2*>(copy_src(ts, blk, i, v));
+      }
+  };
+  auto reg_put = [&](int stage, int i, int v) {
+    const int sg = i * NW + wave;
+    u32x4 w;
+    if constexpr (KF == kKV4) w = fp4x8_to<T>(rst[i][v][0], __uint_as_float(rst[i][v][1] << 23));
+    else w = fp8x8_to<T>(rst[i][v][0], rst[i][v][1]);
+    *reinterpret_cast<u32x4*>(lds + v * Cfg::kVBase + stage * Cfg::kTile + sg * 1024 + lane * 16) = w;
+  };
+  auto dma_issue = [&](int ts, int stage, const Row (&blk)[CHD]) {
+    if (KREG) reg_fetch(ts, blk);
+#pragma unroll
+    for (int i = 0; i < CHD; ++i)
+#pragma unroll
+      for (int v = 0; v < 2; ++v) {
+        if (KREG)
+          reg_put(stage, i, v);
         else
           dma_one(ts, stage, blk, i, v);
       }
@@ -791,6 +900,7 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
   constexpr float kT = kF16 ? 15.f : 64.f;
   constexpr float kTwoT = kF16 ? 32768.f : 18446744073709551616.f;   // 2^T
   float rref = 0.f;              // paged mode: the row's reference r (log2 units)
+  bool rset = false;             // WIN: chosen
   struct Soft { float alpha, dlt, psum; };
   auto row_max = [&](const f32x16& s) {
     float tmax = kNegInf;
@@ -805,8 +915,17 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
   // common path)
   auto apply_mask = [&](f32x16& s, int k0) {
     const int lim = vis - k0 - 4 * h;
+    if constexpr (WIN) {               // nor at or before vis - window, unless a sink
+      const int lo = lim - a.window, sink = a.sinks - k0 - 4 * h;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) s[j] = 8 * (j >> 2) + (j & 3) > lim ? kNegInf : s[j];
+      for (int j = 0; j < 16; ++j) {
+        const int c = 8 * (j >> 2) + (j & 3);
+        s[j] = c > lim || (c <= lo && c >= sink) ? kNegInf : s[j];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) s[j] = 8 * (j >> 2) + (j & 3) > lim ? kNegInf : s[j];
+    }
   };
   // paged mode, piece 0: scale and reference (one FMA), the causal mask, and
   // on the row's first half-tile the choice of r
@@ -815,7 +934,19 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
 #pragma unroll
     for (int j = 0; j < 16; ++j) s[j] = __builtin_fmaf(s[j], sl2, nr);
     if (mask) apply_mask(s, k0);
-    if (first) {
+    if constexpr (WIN) {
+      // rows that have met no visible key yet (l and O are 0 there)
+      if (__builtin_amdgcn_ballot_w64(!rset)) {
+        const float m1 = row_max(s);
+        const float d = rset || (!kF16 && m1 >= -kT && m1 <= kT) || m1 == kNegInf ? 0.f : m1;
+        rset = rset || m1 != kNegInf;
+        rref += d;
+        if (__builtin_amdgcn_ballot_w64(d != 0.f)) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) s[j] -= d;
+        }
+      }
+    } else if (first) {
       const float m1 = row_max(s);
       rref = (!kF16 && m1 >= -kT && m1 <= kT) || m1 == kNegInf ? 0.f : m1;
       if (__builtin_amdgcn_ballot_w64(rref != 0.f)) {
@@ -981,7 +1112,7 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
   // One wave thus keeps the matrix core busy while its own VALU work runs;
   // the two commits (rare wave-uniform branches inside) split the regions.
   // `first`: the row's first tile (key 0).
-  auto compute = [&](const char* st, int ts, bool mask, bool dma, int dts, int dstage, const uint32_t (&blk)[CHD],
+  auto compute = [&](const char* st, int ts, bool mask, bool dma, int dts, int dstage, const Row (&blk)[CHD],
                      bool first) {
     f32x16 s0, s1;
     u32x4 va0[2][NO], va1[2][NO];
@@ -1047,8 +1178,8 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
         const int tp = i / NO, db = i % NO;
         o[db] = E16<T>::mfma32(va1[tp][db], pb1[tp], o[db]);
         if (i < 2 * CHD) {
-          if (KV8)
-            fp8_put(dstage, i / 2, i % 2);     // fetched at the start of the tile
+          if (KREG)
+            reg_put(dstage, i / 2, i % 2);     // fetched at the start of the tile
           else
             dma_one(dts, dstage, blk, i / 2, i % 2);
         }
@@ -1073,7 +1204,7 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
   // MFMAs of tile t - TPB, into that tile's stage.
   constexpr int TPB = NS / 2;
   static_assert(NS % 2 == 0 && TPB >= 1, "stage ring must hold two tile groups");
-  const int ntiles = (kend_wg + BN - 1) / BN;
+  const int ntiles = (kend_wg + (WIN ? BN - 1 - sk.by : BN - 1)) / BN;
   const int full_end = ctx + r0;           // tiles ending at or before key ctx + r0 need no mask
   // The first TPB tiles' copies are addressed with block ids read straight
   // from the table (issued together with the loads above), so they need no
@@ -1087,7 +1218,7 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
       fbid[t][i] = 0u;
       foff[t][i] = 0u;
       if (!DENSE) {
-        const int p = min(t * BN + (i * NW + wave) * RPS + lane / CPR, kend_wg - 1);
+        const int p = copy_key(tile_key(t), i);
         const uint32_t bi = div_bs((uint32_t)p, a.block_magic, a.block_shift);
         fbid[t][i] = (uint32_t)bt[bi];
         foff[t][i] = (uint32_t)p - bi * (uint32_t)a.block_size;
@@ -1097,19 +1228,21 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
 #pragma unroll
   for (int t = 0; t < TPB; ++t)
     if (t < ntiles) {
+      Row row[CHD];
 #pragma unroll
       for (int i = 0; i < CHD; ++i) {
         if (fbid[t][i] >= (uint64_t)a.num_blocks) fbid[t][i] = 0u;  // never address outside the pool
-        fbid[t][i] = fbid[t][i] * (uint32_t)a.block_size + foff[t][i];   // the row's slot
+        if constexpr (KF == kKV4) row[i] = Row{fbid[t][i], foff[t][i]};
+        else row[i] = fbid[t][i] * (uint32_t)a.block_size + foff[t][i];   // the row's slot
       }
-      dma_issue(t * BN, t, fbid[t]);
+      dma_issue(tile_key(t), t, row);
     }
   if (!DENSE) {
 #pragma unroll
     for (int k = 0; k < KB; ++k)
       if (tid + k * NT < nbc) lbid[tid + k * NT] = lb[k] < (uint64_t)a.num_blocks ? (int32_t)lb[k] : 0;
   }
-  uint32_t nbid[CHD];
+  Row nbid[CHD];
   if (DENSE && kBiasAhead && wact) bias_load(0);
 
   // Q as the B operand of S^T = K Q^T: lane holds Q[row n][16kk + 8h + i].
@@ -1130,7 +1263,7 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
     for (int kk = 0; kk < NQ; ++kk) qB[kk] = pack8<T>(x[kk]);   // exact: q and its rotation are in T
   }
   if (!DENSE) __syncthreads();  // block ids in LDS visible
-  if (TPB < ntiles) dma_bids(TPB * BN, nbid);
+  if (TPB < ntiles) dma_bids(tile_key(TPB), nbid);
 
   // The loop walks the ring NS tiles at a time so that every stage index is a
   // compile-time constant (operand reads then carry it as an immediate); a
@@ -1147,15 +1280,19 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
           const int t = tg + u;
           const int stage = gi * TPB + u;    // == t % NS
           if (t < ntiles) {
-            const int ts = t * BN;
+            const int ts = tile_key(t);
             const bool dma = t + TPB < ntiles;
-            const int dts = (t + TPB) * BN, dstage = (stage + TPB) % NS;
-            if (KV8 && dma && wact && ts < kend_w) fp8_fetch(dts, nbid);   // written in the tile's last region
-            if (wact && ts < kend_w)
-              compute(lds + stage * Cfg::kTile, ts, DENSE || ts + BN - 1 > full_end, dma, dts, dstage, nbid, t == 0);
+            const int dts = tile_key(t + TPB), dstage = (stage + TPB) % NS;
+            // keys of the wave's rows in the tile (WIN: not all before its windows and past the sinks)
+            const bool live = wact && ts < kend_w && !(WIN && ts + BN <= lo_w && ts >= a.sinks);
+            if (KREG && dma && live) reg_fetch(dts, nbid);   // written in the tile's last region
+            if (live)
+              compute(lds + stage * Cfg::kTile, ts,
+                      DENSE || ts + BN - 1 > full_end || (WIN && ts <= hid_w && ts + BN > a.sinks), dma, dts, dstage, nbid,
+                      t == 0);
             else if (dma)
               dma_issue(dts, dstage, nbid);
-            if (t + TPB + 1 < ntiles) dma_bids((t + TPB + 1) * BN, nbid);
+            if (t + TPB + 1 < ntiles) dma_bids(tile_key(t + TPB + 1), nbid);
           }
         }
       }
@@ -1179,9 +1316,9 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
 // ============================================================== kernels
 constexpr int kPrefillStages = 4;     // prefill LDS ring: two groups of two 64-key tiles
 
-template <int D, bool PF, bool DC, int NW> struct MixedLds {
+template <int D, bool PF, bool DC, int NW, int KF> struct MixedLds {
   static constexpr int a = PF ? PrefillCfg<D, kPrefillStages>::kLdsBytes : 0;
-  static constexpr int b = DC ? DecodeCfg<D, NW>::kLdsBytes : 0;
+  static constexpr int b = DC ? DecodeCfg<D, NW, KF>::kLdsBytes : 0;
   static constexpr int kBytes = a > b ? a : b;
 };
 
@@ -1204,31 +1341,31 @@ __device__ __forceinline__ int xcd_item(int b, int n) {
 // Work items of both kinds in one launch (mixed continuous batch; 8-wave
 // workgroups), or decode items only (HW x KW waves).  T: the model dtype
 // (__bf16 or _Float16), also the cache's unless KV8 (fp8 e4m3fn cache).
-template <typename T, int D, bool PF, bool DC, int HW, int KW, bool KV8>
+template <typename T, int D, bool PF, bool DC, int HW, int KW, int KF, bool WIN>
 __global__ void __launch_bounds__(64 * HW * KW) paged_attn_kernel(AttnArgs a) {
-  __shared__ __attribute__((aligned(16))) char lds[MixedLds<D, PF, DC, HW * KW>::kBytes];
-  const WorkItem it = a.items[xcd_item<!PF && KV8 && HW * D < 128>(blockIdx.x, a.n_items)];
+  __shared__ __attribute__((aligned(16))) char lds[MixedLds<D, PF, DC, HW * KW, KF>::kBytes];
+  const WorkItem it = a.items[xcd_item<!PF && KF == kKV8 && HW * D < 128>(blockIdx.x, a.n_items)];
   if (PF && (!DC || (it.kind_b & 0xff) == kItemPrefill)) {
     if constexpr (HW * KW == kWaves)
-      prefill_wg<T, D, false, kWaves, kPrefillStages, KV8>(a, it, it.seq, it.a, it.kind_b >> 8, lds);
+      prefill_wg<T, D, false, kWaves, kPrefillStages, KF, WIN>(a, it, it.seq, it.a, it.kind_b >> 8, lds);
     return;
   }
-  if constexpr (DC) decode_wg<T, D, HW, KW, KV8>(a, it, lds);
+  if constexpr (DC) decode_wg<T, D, HW, KW, KF, WIN>(a, it, lds);
 }
 
 // Page-balanced decode: workgroup w runs its key segments in order (all
 // waves converge between segments; the LDS staging is reused).
-template <typename T, int D, int HW, int KW, bool KV8>
+template <typename T, int D, int HW, int KW, int KF, bool WIN>
 __global__ void __launch_bounds__(64 * HW * KW) __attribute__((amdgpu_waves_per_eu(D == 64 ? 4 : 2)))
 decode_balanced_kernel(AttnArgs a) {
-  __shared__ __attribute__((aligned(16))) char lds[DecodeCfg<D, HW * KW>::kLdsBytes];
+  __shared__ __attribute__((aligned(16))) char lds[DecodeCfg<D, HW * KW, KF>::kLdsBytes];
   const int s0 = a.seg_ptr[blockIdx.x], s1 = a.seg_ptr[blockIdx.x + 1];
   for (int s = s0; s < s1; ++s) {
     if (s > s0) __syncthreads();
     const DecodeSeg sg = a.segs[s];
     const DecodeTask tk{sg.seq, sg.hg, sg.k0, sg.k1, sg.q_row_start, sg.ctx_len, sg.q_len,
                         sg.nseg, sg.pbase, sg.ord};
-    decode_task<T, D, HW, KW, KV8>(a, tk, lds);
+    decode_task<T, D, HW, KW, KF, WIN>(a, tk, lds);
   }
 }
 
@@ -1236,13 +1373,13 @@ decode_balanced_kernel(AttnArgs a) {
 // key shares of the decode sequences (segments, as decode_balanced_kernel);
 // each later workgroup runs one prefill item.  One 8-wave workgroup per CU
 // (the prefill path's LDS ring and registers).
-template <typename T, int D, int HW, bool KV8>
+template <typename T, int D, int HW, int KF, bool WIN>
 __global__ void __launch_bounds__(64 * kWaves) mixed_balanced_kernel(AttnArgs a) {
-  __shared__ __attribute__((aligned(16))) char lds[MixedLds<D, true, true, kWaves>::kBytes];
+  __shared__ __attribute__((aligned(16))) char lds[MixedLds<D, true, true, kWaves, KF>::kBytes];
   const int b = blockIdx.x;
   if (b >= a.n_seg_wgs) {
     const WorkItem it = a.items[b - a.n_seg_wgs];
-    prefill_wg<T, D, false, kWaves, kPrefillStages, KV8>(a, it, it.seq, it.a, it.kind_b >> 8, lds);
+    prefill_wg<T, D, false, kWaves, kPrefillStages, KF, WIN>(a, it, it.seq, it.a, it.kind_b >> 8, lds);
     return;
   }
   const int s0 = a.seg_ptr[b], s1 = a.seg_ptr[b + 1];
@@ -1251,7 +1388,7 @@ __global__ void __launch_bounds__(64 * kWaves) mixed_balanced_kernel(AttnArgs a)
     const DecodeSeg sg = a.segs[s];
     const DecodeTask tk{sg.seq, sg.hg, sg.k0, sg.k1, sg.q_row_start, sg.ctx_len, sg.q_len,
                         sg.nseg, sg.pbase, sg.ord};
-    decode_task<T, D, HW, kWaves / HW, KV8>(a, tk, lds);
+    decode_task<T, D, HW, kWaves / HW, KF, WIN>(a, tk, lds);
   }
 }
 
@@ -1259,12 +1396,12 @@ __global__ void __launch_bounds__(64 * kWaves) mixed_balanced_kernel(AttnArgs a)
 // kPrefillOnlyStages-stage ring.  PAIR (bf16, D = 64, 16-bit cache): two
 // workgroups per CU (128 registers, some of them in scratch, 69 KB of LDS each),
 // so one's start and barriers run under the other; the plan says when that pays.
-template <typename T, int D, bool KV8, bool PAIR = false>
+template <typename T, int D, int KF, bool WIN, bool PAIR = false>
 __global__ void __launch_bounds__(64 * kPrefillOnlyWaves) __attribute__((amdgpu_waves_per_eu(PAIR ? 4 : 2)))
 prefill_kernel(AttnArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[PrefillCfg<D, kPrefillOnlyStages>::kLdsBytes];
   const WorkItem it = a.items[blockIdx.x];
-  prefill_wg<T, D, false, kPrefillOnlyWaves, kPrefillOnlyStages, KV8>(a, it, it.seq, it.a, it.kind_b >> 8, lds);
+  prefill_wg<T, D, false, kPrefillOnlyWaves, kPrefillOnlyStages, KF, WIN>(a, it, it.seq, it.a, it.kind_b >> 8, lds);
 }
 
 template <typename T, int D>
@@ -1275,55 +1412,55 @@ __global__ void __launch_bounds__(64 * kWaves) dense_attn_kernel(AttnArgs a, int
   const int kvh = rest % a.num_kv_heads;
   const int b = rest / a.num_kv_heads;
   const WorkItem none{};
-  prefill_wg<T, D, true, kWaves, kPrefillStages, false>(a, none, b, kvh, w, lds);
+  prefill_wg<T, D, true, kWaves, kPrefillStages, kKV16, false>(a, none, b, kvh, w, lds);
 }
 
-template <typename T, int D, int HW, int KW, bool KV8>
+template <typename T, int D, int HW, int KW, int KF, bool WIN>
 static void launch_paged_hk(const AttnArgs& a, bool pf, bool dc, hipStream_t st) {
   dim3 grid(a.n_items);
   if (pf && dc) {
     if constexpr (HW * KW == kWaves)
-      hipLaunchKernelGGL((paged_attn_kernel<T, D, true, true, HW, KW, KV8>), grid, dim3(64 * kWaves), 0, st, a);
+      hipLaunchKernelGGL((paged_attn_kernel<T, D, true, true, HW, KW, KF, WIN>), grid, dim3(64 * kWaves), 0, st, a);
   } else if (pf) {
-    if constexpr (std::is_same_v<T, __bf16> && D == 64 && !KV8) {
+    if constexpr (std::is_same_v<T, __bf16> && D == 64 && KF == kKV16 && !WIN) {
       if (a.prefill_pairs) {
-        hipLaunchKernelGGL((prefill_kernel<T, D, KV8, true>), grid, dim3(64 * kPrefillOnlyWaves), 0, st, a);
+        hipLaunchKernelGGL((prefill_kernel<T, D, KF, WIN, true>), grid, dim3(64 * kPrefillOnlyWaves), 0, st, a);
         return;
       }
     }
-    hipLaunchKernelGGL((prefill_kernel<T, D, KV8>), grid, dim3(64 * kPrefillOnlyWaves), 0, st, a);
+    hipLaunchKernelGGL((prefill_kernel<T, D, KF, WIN>), grid, dim3(64 * kPrefillOnlyWaves), 0, st, a);
   } else {
-    hipLaunchKernelGGL((paged_attn_kernel<T, D, false, true, HW, KW, KV8>), grid, dim3(64 * HW * KW), 0, st, a);
+    hipLaunchKernelGGL((paged_attn_kernel<T, D, false, true, HW, KW, KF, WIN>), grid, dim3(64 * HW * KW), 0, st, a);
   }
 }
 
-template <typename T, int D, bool KV8>
+template <typename T, int D, int KF, bool WIN>
 static hipError_t launch_decode_balanced(const AttnArgs& a, hipStream_t st) {
   const dim3 grid(a.n_items);
   switch (a.heads_per_wg) {
-    case 1: hipLaunchKernelGGL((decode_balanced_kernel<T, D, 1, 8, KV8>), grid, dim3(512), 0, st, a); break;
-    case 2: hipLaunchKernelGGL((decode_balanced_kernel<T, D, 2, 4, KV8>), grid, dim3(512), 0, st, a); break;
-    case 4: hipLaunchKernelGGL((decode_balanced_kernel<T, D, 4, 2, KV8>), grid, dim3(512), 0, st, a); break;
-    case 8: hipLaunchKernelGGL((decode_balanced_kernel<T, D, 8, 1, KV8>), grid, dim3(512), 0, st, a); break;
+    case 1: hipLaunchKernelGGL((decode_balanced_kernel<T, D, 1, 8, KF, WIN>), grid, dim3(512), 0, st, a); break;
+    case 2: hipLaunchKernelGGL((decode_balanced_kernel<T, D, 2, 4, KF, WIN>), grid, dim3(512), 0, st, a); break;
+    case 4: hipLaunchKernelGGL((decode_balanced_kernel<T, D, 4, 2, KF, WIN>), grid, dim3(512), 0, st, a); break;
+    case 8: hipLaunchKernelGGL((decode_balanced_kernel<T, D, 8, 1, KF, WIN>), grid, dim3(512), 0, st, a); break;
     default: return hipErrorInvalidValue;
   }
   return hipGetLastError();
 }
 
-template <typename T, int D, bool KV8>
+template <typename T, int D, int KF, bool WIN>
 static hipError_t launch_mixed_balanced(const AttnArgs& a, hipStream_t st) {
   const dim3 grid(a.n_items);
   switch (a.heads_per_wg) {
-    case 1: hipLaunchKernelGGL((mixed_balanced_kernel<T, D, 1, KV8>), grid, dim3(64 * kWaves), 0, st, a); break;
-    case 2: hipLaunchKernelGGL((mixed_balanced_kernel<T, D, 2, KV8>), grid, dim3(64 * kWaves), 0, st, a); break;
-    case 4: hipLaunchKernelGGL((mixed_balanced_kernel<T, D, 4, KV8>), grid, dim3(64 * kWaves), 0, st, a); break;
-    case 8: hipLaunchKernelGGL((mixed_balanced_kernel<T, D, 8, KV8>), grid, dim3(64 * kWaves), 0, st, a); break;
+    case 1: hipLaunchKernelGGL((mixed_balanced_kernel<T, D, 1, KF, WIN>), grid, dim3(64 * kWaves), 0, st, a); break;
+    case 2: hipLaunchKernelGGL((mixed_balanced_kernel<T, D, 2, KF, WIN>), grid, dim3(64 * kWaves), 0, st, a); break;
+    case 4: hipLaunchKernelGGL((mixed_balanced_kernel<T, D, 4, KF, WIN>), grid, dim3(64 * kWaves), 0, st, a); break;
+    case 8: hipLaunchKernelGGL((mixed_balanced_kernel<T, D, 8, KF, WIN>), grid, dim3(64 * kWaves), 0, st, a); break;
     default: return hipErrorInvalidValue;
   }
   return hipGetLastError();
 }
 
-template <typename T, int D, bool KV8>
+template <typename T, int D, int KF, bool WIN>
 static hipError_t launch_paged_d(const AttnArgs& a, bool pf, bool dc, hipStream_t st) {
   const int hw = a.heads_per_wg, nw = a.decode_waves;
   hipError_t e;
@@ -1331,14 +1468,14 @@ static hipError_t launch_paged_d(const AttnArgs& a, bool pf, bool dc, hipStream_
     if (nw != kWaves || (pf && a.prefill_waves != kWaves) || a.n_seg_wgs <= 0 || a.n_seg_wgs > a.n_items)
       return hipErrorInvalidValue;
     if (pf && !dc) return hipErrorInvalidValue;
-    e = pf ? launch_mixed_balanced<T, D, KV8>(a, st) : launch_decode_balanced<T, D, KV8>(a, st);
+    e = pf ? launch_mixed_balanced<T, D, KF, WIN>(a, st) : launch_decode_balanced<T, D, KF, WIN>(a, st);
   } else {
     if (nw != kWaves || (pf && a.prefill_waves != (dc ? kWaves : kPrefillOnlyWaves))) return hipErrorInvalidValue;
     switch (hw) {
-      case 1: launch_paged_hk<T, D, 1, 8, KV8>(a, pf, dc, st); break;
-      case 2: launch_paged_hk<T, D, 2, 4, KV8>(a, pf, dc, st); break;
-      case 4: launch_paged_hk<T, D, 4, 2, KV8>(a, pf, dc, st); break;
-      case 8: launch_paged_hk<T, D, 8, 1, KV8>(a, pf, dc, st); break;
+      case 1: launch_paged_hk<T, D, 1, 8, KF, WIN>(a, pf, dc, st); break;
+      case 2: launch_paged_hk<T, D, 2, 4, KF, WIN>(a, pf, dc, st); break;
+      case 4: launch_paged_hk<T, D, 4, 2, KF, WIN>(a, pf, dc, st); break;
+      case 8: launch_paged_hk<T, D, 8, 1, KF, WIN>(a, pf, dc, st); break;
       default: return hipErrorInvalidValue;
     }
     e = hipGetLastError();
@@ -1348,13 +1485,17 @@ static hipError_t launch_paged_d(const AttnArgs& a, bool pf, bool dc, hipStream_
   return hipGetLastError();
 }
 
-template <typename T>
-static hipError_t launch_paged_t(const AttnArgs& a, bool pf, bool dc, hipStream_t st) {
-  const bool kv8 = a.kv_dtype == kFP8;
-  if (a.head_dim == 64) return kv8 ? launch_paged_d<T, 64, true>(a, pf, dc, st) : launch_paged_d<T, 64, false>(a, pf, dc, st);
-  if (a.head_dim == 128)
-    return kv8 ? launch_paged_d<T, 128, true>(a, pf, dc, st) : launch_paged_d<T, 128, false>(a, pf, dc, st);
+template <typename T, int KF, bool WIN>
+static hipError_t launch_paged_f(const AttnArgs& a, bool pf, bool dc, hipStream_t st) {
+  if (a.head_dim == 64) return launch_paged_d<T, 64, KF, WIN>(a, pf, dc, st);
+  if (a.head_dim == 128) return launch_paged_d<T, 128, KF, WIN>(a, pf, dc, st);
   return hipErrorInvalidValue;
+}
+
+// Cache of the model dtype or fp8
+template <typename T, bool WIN>
+static hipError_t launch_paged_t(const AttnArgs& a, bool pf, bool dc, hipStream_t st) {
+  return a.kv_dtype == kFP8 ? launch_paged_f<T, kKV8, WIN>(a, pf, dc, st) : launch_paged_f<T, kKV16, WIN>(a, pf, dc, st);
 }
 
 template <typename T>
@@ -1369,26 +1510,53 @@ static hipError_t launch_dense_t(const AttnArgs& a, dim3 grid, int nwg, hipStrea
   return hipGetLastError();
 }
 
+// This file is compiled once per element type and kind, so that they build as
+// separate units in parallel: plain (the dense op and the dispatch beside the
+// bf16 one), GLLM_PAGED_WINDOW (sliding windows) and GLLM_PAGED_KV4 (4-bit
+// cache, with or without a window).
 #ifdef GLLM_PAGED_F16
-// fp16 models: this file compiled a second time (paged_attention_f16.hip), so
-// the two element types build as separate units in parallel.
-hipError_t launch_paged_f16(const AttnArgs& a, bool pf, bool dc, hipStream_t st) {
-  return launch_paged_t<_Float16>(a, pf, dc, st);
+using UnitT = _Float16;
+#define GLLM_UNIT(name) name##_f16
+#else
+using UnitT = __bf16;
+#define GLLM_UNIT(name) name##_bf16
+#endif
+
+#if defined(GLLM_PAGED_KV4)
+hipError_t GLLM_UNIT(launch_paged_kv4)(const AttnArgs& a, bool pf, bool dc, hipStream_t st) {
+  return launch_paged_f<UnitT, kKV4, true>(a, pf, dc, st);
 }
-hipError_t launch_dense_f16(const AttnArgs& a, dim3 grid, int nwg, hipStream_t st) {
-  return launch_dense_t<_Float16>(a, grid, nwg, st);
+#elif defined(GLLM_PAGED_WINDOW)
+hipError_t GLLM_UNIT(launch_paged_window)(const AttnArgs& a, bool pf, bool dc, hipStream_t st) {
+  return launch_paged_t<UnitT, true>(a, pf, dc, st);
 }
 #else
-hipError_t launch_paged_f16(const AttnArgs& a, bool pf, bool dc, hipStream_t st);
+hipError_t GLLM_UNIT(launch_paged)(const AttnArgs& a, bool pf, bool dc, hipStream_t st) {
+  return launch_paged_t<UnitT, false>(a, pf, dc, st);
+}
+hipError_t GLLM_UNIT(launch_dense)(const AttnArgs& a, dim3 grid, int nwg, hipStream_t st) {
+  return launch_dense_t<UnitT>(a, grid, nwg, st);
+}
+#ifndef GLLM_PAGED_F16
+using PagedLaunch = hipError_t(const AttnArgs&, bool, bool, hipStream_t);
+PagedLaunch launch_paged_f16, launch_paged_window_bf16, launch_paged_window_f16, launch_paged_kv4_bf16, launch_paged_kv4_f16;
 hipError_t launch_dense_f16(const AttnArgs& a, dim3 grid, int nwg, hipStream_t st);
 
 hipError_t launch_paged_attention_mfma(const AttnArgs& a, bool has_prefill, bool has_decode, hipStream_t st) {
   if (a.n_items == 0) return hipSuccess;
-  // the cache holds the model dtype or fp8 e4m3fn
-  if (a.kv_dtype != kFP8 && a.kv_dtype != a.dtype) return hipErrorInvalidValue;
-  if (a.dtype == kBF16) return launch_paged_t<__bf16>(a, has_prefill, has_decode, st);
-  if (a.dtype == kF16) return launch_paged_f16(a, has_prefill, has_decode, st);
-  return hipErrorInvalidValue;
+  // the cache holds the model dtype, fp8 e4m3fn or 4-bit records
+  if (a.kv_dtype != kFP8 && a.kv_dtype != kMXFP4 && a.kv_dtype != a.dtype) return hipErrorInvalidValue;
+  if (a.dtype != kBF16 && a.dtype != kF16) return hipErrorInvalidValue;
+  const bool f16 = a.dtype == kF16;
+  PagedLaunch* go = f16 ? launch_paged_f16 : launch_paged_bf16;
+  if (a.kv_dtype == kMXFP4) go = f16 ? launch_paged_kv4_f16 : launch_paged_kv4_bf16;
+  else if (a.window > 0) go = f16 ? launch_paged_window_f16 : launch_paged_window_bf16;
+  if (a.kv_dtype == kMXFP4 && a.window == 0) {   // the 4-bit kernels always take one
+    AttnArgs w = a;
+    w.window = INT32_MAX;
+    return go(w, has_prefill, has_decode, st);
+  }
+  return go(a, has_prefill, has_decode, st);
 }
 
 hipError_t launch_dense_attention_mfma(const AttnArgs& a, int B, int Tq, hipStream_t st) {
@@ -1398,11 +1566,11 @@ hipError_t launch_dense_attention_mfma(const AttnArgs& a, int B, int Tq, hipStre
   if (blocks == 0) return hipSuccess;
   if (blocks > 0x7fffffff) return hipErrorInvalidValue;
   const dim3 grid((unsigned)blocks);
-  if (a.dtype == kBF16) return launch_dense_t<__bf16>(a, grid, nwg, st);
+  if (a.dtype == kBF16) return launch_dense_bf16(a, grid, nwg, st);
   if (a.dtype == kF16) return launch_dense_f16(a, grid, nwg, st);
   return hipErrorInvalidValue;
 }
-
 #endif  // GLLM_PAGED_F16
+#endif
 
 }  // namespace gllm

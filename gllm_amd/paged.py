@@ -57,6 +57,37 @@ def _cache_rows(k_cache: torch.Tensor, v_cache: torch.Tensor, Hkv: int, D: int) 
             raise ValueError(f"{nm}: expected [num_slots, {Hkv}, {D}] with contiguous rows")
 
 
+# Storage type of a 4-bit KV cache (OCP MXFP4): uint8 ``[num_blocks, Hkv,
+# kv4_record_bytes(block_size, D)]``.  A record holds, of one block and KV head,
+# block_size rows of D / 2 code bytes (fp4 e2m1, the even dim in the low half),
+# then block_size rows of D / 32 scale bytes (a block of 32 dims stands for code x
+# 2^(byte - 127)), padded to 16 bytes.
+KV4 = torch.uint8
+
+
+def kv4_record_bytes(block_size: int, head_dim: int) -> int:
+    """Bytes of one (block, KV head) of a 4-bit cache."""
+    if head_dim <= 0 or head_dim % 32 or block_size <= 0:
+        raise ValueError(f"4-bit cache: head_dim {head_dim} must be a multiple of 32, block_size {block_size} positive")
+    return -(-block_size * (head_dim // 32 * 17) // 16) * 16
+
+
+def _kv4_blocks(k_cache: torch.Tensor, v_cache: torch.Tensor, Hkv: int, D: int, block_size: int) -> int:
+    """Blocks of a 4-bit cache pair, after a check of its layout."""
+    rec = kv4_record_bytes(block_size, D)
+    for t, nm in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+        if t.dtype != KV4 or t.dim() != 3 or t.shape[1:] != (Hkv, rec) or t.stride()[1:] != (rec, 1):
+            raise ValueError(f"{nm}: expected a 4-bit cache, uint8 [num_blocks, {Hkv}, {rec}] with contiguous blocks "
+                             f"(block_size {block_size}, head_dim {D}), got {t.dtype} {tuple(t.shape)}")
+    if k_cache.shape[0] != v_cache.shape[0] or k_cache.stride(0) != v_cache.stride(0):
+        raise ValueError("k_cache and v_cache must have the same shape and block stride")
+    return k_cache.shape[0]
+
+
+def _kv_code(cache: torch.Tensor) -> int:
+    return _lib.DTYPE_MXFP4 if cache.dtype == KV4 else _lib.dtype_code(cache.dtype)
+
+
 def rope_kv_write(k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
                   k_cache: torch.Tensor, v_cache: torch.Tensor, slot_mapping: torch.Tensor,
                   query_lens: torch.Tensor | None = None, q: torch.Tensor | None = None,
@@ -322,23 +353,34 @@ class AttentionPlan:
     0 lets the planner choose, a multiple of 32 fixes the decode split length,
     ``BALANCED`` deals the decode sequences' keys evenly to the workgroups (in
     a mixed batch: to part of the CUs, the prefill items run on the rest).
+
+    ``window``: sliding window; the row at position p sees the ``window`` keys
+    up to its own (t > p - window) and the sequence's first ``sinks`` keys
+    (None: every earlier key).  Keys that no row of the batch sees are never
+    read, so blocks that hold only such keys may have been given back.
     """
 
     def __init__(self, query_lens, seq_lens, *, num_q_heads: int, num_kv_heads: int, head_dim: int,
                  block_size: int, dtype: torch.dtype, device, q_seq_stride: int = 0,
-                 split_tokens: int = 0, heads_per_wg: int = 0):
+                 split_tokens: int = 0, heads_per_wg: int = 0, window: int | None = None, sinks: int = 0):
         ql = [int(x) for x in query_lens]
         sl = [int(x) for x in seq_lens]
         if len(ql) != len(sl):
             raise ValueError("query_lens and seq_lens differ in length")
+        if window is not None and not 1 <= window < 1 << 31:
+            raise ValueError(f"window {window} must be at least 1 (None: no window)")
+        if not 0 <= sinks < 1 << 31 or (sinks and window is None):
+            raise ValueError(f"sinks {sinks} must be >= 0 and go with a window")
         lib = _lib.load()
         self._lib = lib
         self._h = ctypes.c_void_p()
         qa = (ctypes.c_int32 * max(len(ql), 1))(*ql)
         sa = (ctypes.c_int32 * max(len(sl), 1))(*sl)
-        _lib.check(lib.gllm_attn_plan_create(ctypes.byref(self._h), qa, sa, len(ql), q_seq_stride,
-                                             num_q_heads, num_kv_heads, head_dim, block_size,
-                                             _lib.dtype_code(dtype), split_tokens, heads_per_wg))
+        _lib.check(lib.gllm_attn_plan_create_window(ctypes.byref(self._h), qa, sa, len(ql), q_seq_stride,
+                                                    num_q_heads, num_kv_heads, head_dim, block_size,
+                                                    _lib.dtype_code(dtype), split_tokens, heads_per_wg,
+                                                    window or 0, sinks))
+        self.window, self.sinks = window, sinks
         self.num_q_heads, self.num_kv_heads, self.head_dim = num_q_heads, num_kv_heads, head_dim
         self.block_size, self.dtype = block_size, dtype
         self.query_lens, self.seq_lens = ql, sl
@@ -377,15 +419,16 @@ class AttentionPlan:
 def fused_kv_write_ok(plan: AttentionPlan, kv_dtype: torch.dtype) -> bool:
     """Whether :func:`paged_attention` can take ``kv_new`` for this plan and
     cache dtype: every sequence on the decode path of the kernel that runs
-    (MFMA kernels: query_len x G <= 16; generic kernel: query_len <= 16)."""
-    if not plan.max_query_len:             # no sequences
+    (MFMA kernels: query_len x G <= 16; generic kernel: query_len <= 16, no
+    sliding window), and no 4-bit cache."""
+    if not plan.max_query_len or kv_dtype == KV4:   # no sequences; a 4-bit cache is written by a call of its own
         return False
     mfma = (plan.dtype in (torch.bfloat16, torch.float16) and plan.head_dim in (64, 128)
             and kv_dtype in (plan.dtype, torch.float8_e4m3fn))
     G = plan.num_q_heads // plan.num_kv_heads
     if mfma:
         return plan.max_query_len * G <= 16
-    return plan.max_query_len <= 16
+    return plan.max_query_len <= 16 and plan.window is None
 
 
 def paged_attention(plan: AttentionPlan, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -395,7 +438,7 @@ def paged_attention(plan: AttentionPlan, q: torch.Tensor, k_cache: torch.Tensor,
     """Attention over the paged cache for every query row in ``plan``.
 
     q ``[rows, Hq, D]`` or ``[B, T_q, Hq, D]`` (rows flattened), caches
-    ``[num_slots, Hkv, D]``, block_table int32 ``[B, W]``.  ``rope`` =
+    ``[num_slots, Hkv, D]`` or 4-bit ones (:data:`KV4`), block_table int32 ``[B, W]``.  ``rope`` =
     ``(cos, sin, mode)`` with mode ``"position"`` (table rows ``c_i + r``) or
     ``"row"`` (one cos/sin row per query row, the reference's gathered
     ``cos_pos``) rotates q on load.  ``kv_new`` = ``(k, v)``, one row per
@@ -413,7 +456,11 @@ def paged_attention(plan: AttentionPlan, q: torch.Tensor, k_cache: torch.Tensor,
         os_ = _rows(out, Hq, D, "out")
     if q.dtype != plan.dtype or out.dtype != plan.dtype:
         raise ValueError("q/out dtype differs from the plan's")
-    _cache_rows(k_cache, v_cache, Hkv, D)
+    if k_cache.dtype == KV4:
+        num_blocks = _kv4_blocks(k_cache, v_cache, Hkv, D, plan.block_size)
+    else:
+        _cache_rows(k_cache, v_cache, Hkv, D)
+        num_blocks = k_cache.shape[0] // plan.block_size
     if k_cache.stride(0) != v_cache.stride(0):
         raise ValueError("k_cache and v_cache slot strides differ")
     bt_shape = block_table.shape
@@ -443,7 +490,6 @@ def paged_attention(plan: AttentionPlan, q: torch.Tensor, k_cache: torch.Tensor,
             raise ValueError(f"cos/sin have {cos.shape[0]} rows, {need_rows} needed")
         cos_p, sin_p, rs = cos.data_ptr(), sin.data_ptr(), cos.stride(0)
     sc = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    num_blocks = k_cache.shape[0] // plan.block_size
     lib = plan._lib
     if kv_new is not None:
         kn, vn = kv_new
@@ -456,11 +502,11 @@ def paged_attention(plan: AttentionPlan, q: torch.Tensor, k_cache: torch.Tensor,
         _lib.check(lib.gllm_paged_attention_write_kv(
             plan._h, q.data_ptr(), qs, out.data_ptr(), os_, k_cache.data_ptr(), v_cache.data_ptr(),
             k_cache.stride(0), num_blocks, block_table.data_ptr(), block_table.stride(0), kn.data_ptr(), ks,
-            vn.data_ptr(), vs, cos_p, sin_p, rs, mode, sc, _lib.dtype_code(q.dtype), _lib.dtype_code(k_cache.dtype),
+            vn.data_ptr(), vs, cos_p, sin_p, rs, mode, sc, _lib.dtype_code(q.dtype), _kv_code(k_cache),
             _lib.stream_ptr(q.device)))
         return out
     _lib.check(lib.gllm_paged_attention(
         plan._h, q.data_ptr(), qs, out.data_ptr(), os_, k_cache.data_ptr(), v_cache.data_ptr(),
         k_cache.stride(0), num_blocks, block_table.data_ptr(), block_table.stride(0), cos_p, sin_p, rs, mode,
-        sc, _lib.dtype_code(q.dtype), _lib.dtype_code(k_cache.dtype), _lib.stream_ptr(q.device)))
+        sc, _lib.dtype_code(q.dtype), _kv_code(k_cache), _lib.stream_ptr(q.device)))
     return out

@@ -54,7 +54,8 @@ enum {
   GLLM_DTYPE_F32 = 0,
   GLLM_DTYPE_BF16 = 1,
   GLLM_DTYPE_FP8_E4M3 = 2, /* torch.float8_e4m3fn, KV cache only */
-  GLLM_DTYPE_F16 = 3
+  GLLM_DTYPE_F16 = 3,
+  GLLM_DTYPE_MXFP4 = 4     /* 4-bit KV cache (records, see gllm_kv4_record_bytes), KV cache only */
 };
 
 enum {
@@ -71,6 +72,23 @@ typedef struct gllm_attn_plan gllm_attn_plan;
 /* Thread-local message of the last failing call ("" if none). */
 const char* gllm_attn_last_error(void);
 int gllm_attn_version(void);
+
+/*
+ * The 4-bit KV cache (GLLM_DTYPE_MXFP4, OCP MXFP4; no counterpart in the
+ * reference).  K and V are [num_blocks][num_kv_heads][record bytes]; a record
+ * holds, of one (block, kv head), block_size rows of head_dim / 2 code bytes
+ * (fp4 e2m1: 0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign bit; the even dim in the low
+ * half), then block_size rows of head_dim / 32 scale bytes, padded to 16 bytes.
+ * A block of 32 dims stands for code x 2^(byte - 127).  Writers take the least
+ * scale 2^e (-126 <= e <= 127) at which the block's largest magnitude rounds to
+ * 6 or less, |x| < 7 x 2^e, and round each value to the nearest code, ties to
+ * the even one; a block with an infinity or NaN gets byte 255 and stands for
+ * NaN.  head_dim a multiple of 32.  Wherever an entry point takes such a cache,
+ * `cache_slot_stride` is the bytes between blocks (a multiple of 16), the heads
+ * of a block follow each other, and the caches are 16-byte aligned.
+ * Returns the bytes of one record (0 for sizes that no 4-bit cache has).
+ */
+size_t gllm_kv4_record_bytes(int32_t block_size, int32_t head_dim);
 
 /*
  * Query-row metadata on the device (gllm/llm/llm.py:245-281).  For query row
@@ -218,6 +236,20 @@ int gllm_attn_plan_create(gllm_attn_plan** plan, const int32_t* query_lens,
                           int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
                           int32_t block_size, int32_t dtype, int32_t split_tokens,
                           int32_t decode_heads_per_wg);
+/*
+ * gllm_attn_plan_create with a sliding window: key t is visible to the query
+ * row at position p iff t <= p and (t > p - window or t < sinks), i.e. the
+ * `window` keys up to the row's own and the first `sinks` keys.  window 0: no
+ * window (sinks must be 0).  gllm_paged_attention with such a plan never reads
+ * a key that no row of the call sees, nor the block-table values of blocks
+ * without a visible key as addresses: those blocks may have been given back.
+ * No counterpart in the reference.
+ */
+int gllm_attn_plan_create_window(gllm_attn_plan** plan, const int32_t* query_lens,
+                                 const int32_t* seq_lens, int32_t num_seqs, int64_t q_seq_stride,
+                                 int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                                 int32_t block_size, int32_t dtype, int32_t split_tokens,
+                                 int32_t decode_heads_per_wg, int32_t window, int32_t sinks);
 /* Device bytes the plan needs (work list, split partials). */
 size_t gllm_attn_plan_workspace_bytes(const gllm_attn_plan* plan);
 /* Stream-ordered upload of the plan into `workspace` (>= workspace_bytes).
@@ -245,7 +277,10 @@ int gllm_attn_plan_destroy(gllm_attn_plan* plan);
  * a cache in the model dtype or fp8 e4m3fn; every other pairing (f32 model;
  * a 16-bit model over an f32 or the other 16-bit cache; other even head dims
  * up to 256) runs a generic kernel (fp32 arithmetic, model dtype in and
- * out).  Cached values are read as the reference reads them: cast to the
+ * out).  A 4-bit cache (GLLM_DTYPE_MXFP4) takes a bf16 or f16 model of
+ * head_dim 64 or 128.  A plan with a sliding window (gllm_attn_plan_create_window)
+ * limits the visible keys.  Every key that some row of a sequence sees has to hold
+ * finite values: rows that do not see it may give it weight 0.  Cached values are read as the reference reads them: cast to the
  * model dtype (attention.py:169-170's .to(q.dtype); exact for fp8, rounded
  * to nearest even where the cache is wider).
  * Returns after enqueueing on `stream`.
@@ -262,7 +297,8 @@ int gllm_paged_attention(const gllm_attn_plan* plan, const void* q, int64_t q_ro
  * gllm_rope_kv_write followed by gllm_paged_attention in one launch, for
  * plans whose sequences are all on the decode path (query_len x G <= 16 on
  * the MFMA kernels; query_len <= 16 on the generic kernel; other plans give
- * GLLM_ATTN_EINVAL).  Replaces gllm/model/layers/attention.py:151-178 for a
+ * GLLM_ATTN_EINVAL).  A 4-bit cache, and a sliding window on the generic kernel,
+ * give GLLM_ATTN_EUNSUPPORTED: their KV write is a call of its own.  Replaces gllm/model/layers/attention.py:151-178 for a
  * decode step (the reference's RoPE of k, its index_put_ into the cache and
  * the attention), i.e. model.py:202-222's per-layer write + attention pair.
  * k_new / v_new: one row per query row of q (same row layout, row strides in

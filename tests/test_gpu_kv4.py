@@ -1,0 +1,115 @@
+"""Paged attention over a 4-bit KV cache against the 64-bit oracle on the values
+that the cache stands for."""
+import pytest
+import torch
+
+from gllm_amd import paged
+from oracle import kv4
+from oracle import rope as orope
+from tests.window_helpers import BF, F16, F32, Batch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+DECODE = dict(ctx=[0, 3, 15, 16, 40, 299, 1000, 2500], ql=[1] * 8)
+
+
+def _plan(b, window=None, sinks=0, **kw):
+    return paged.AttentionPlan(b.ql, b.L, num_q_heads=b.Hq, num_kv_heads=b.Hkv, head_dim=b.D, block_size=b.bs,
+                               dtype=b.dtype, device=DEV, q_seq_stride=b.stride, window=window, sinks=sinks, **kw)
+
+
+def _run(b, window=None, sinks=0, bt=None, kc=None, vc=None, rope=None, **kw):
+    bt, kc, vc = (x.to(DEV) for x in (b.bt if bt is None else bt, b.kc if kc is None else kc, b.vc if vc is None else vc))
+    out = paged.paged_attention(_plan(b, window, sinks, **kw), b.q.to(DEV), kc, vc, bt, rope=rope)
+    torch.cuda.synchronize()
+    return out
+
+
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("split", [0, 64, paged.BALANCED])
+def test_decode(dtype, D, split):
+    for bs in (16, 1, 24, 7):
+        print(f"kv4 decode {dtype} D={D} split={split} bs={bs}", flush=True)
+        b = Batch(**DECODE, D=D, dtype=dtype, kv="4", bs=bs, seed=D + bs)
+        b.check(_run(b, split_tokens=split), None, 0, "kv4 decode")
+
+
+@pytest.mark.parametrize("Hq,Hkv", [(4, 4), (8, 1), (6, 3), (32, 8)])
+def test_rows_and_heads(Hq, Hkv):
+    n = min(4, 16 // (Hq // Hkv))
+    for D in (64, 128):
+        b = Batch([0, 14, 130, 777, 1500], [1, n, 1, n, n], Hq=Hq, Hkv=Hkv, D=D, kv="4", stride=5, seed=Hq)
+        b.check(_run(b), None, 0, "kv4 rows")
+
+
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("D,bs", [(64, 16), (128, 16), (128, 24), (64, 5)])
+def test_prefill_and_mixed(dtype, D, bs):
+    for ctx, ql in (([0, 0, 37, 1000], [33, 200, 77, 130]), ([300, 0, 57, 1000, 5, 2500], [1, 120, 64, 1, 1, 1])):
+        print(f"kv4 prefill / mixed {dtype} D={D} bs={bs}", flush=True)
+        b = Batch(ctx, ql, D=D, dtype=dtype, kv="4", bs=bs, seed=D + bs)
+        b.check(_run(b), None, 0, "kv4 prefill")
+        if dtype == BF:
+            b.check(_run(b, split_tokens=paged.BALANCED), None, 0, "kv4 mixed, balanced")
+
+
+@pytest.mark.parametrize("window,sinks", [(1, 0), (17, 4), (129, 20), (600, 64)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_windows(D, window, sinks):
+    for ctx, ql in ((DECODE["ctx"], DECODE["ql"]), ([0, 37, 1000, 700], [150, 77, 64, 1])):
+        print(f"kv4 window={window} sinks={sinks} D={D}", flush=True)
+        b = Batch(ctx, ql, D=D, kv="4", seed=window + D)
+        want = _run(b, window, sinks)
+        b.check(want, window, sinks, "kv4 window")
+        assert torch.equal(_run(b, window, sinks, *b.evict(window, sinks)), want)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_rope_on_load(D):
+    b = Batch([0, 300, 20], [1, 1, 50], D=D, kv="4", seed=D)
+    cos, sin = orope.rope_cache(512, D, 500000.0, BF)
+    pos = torch.cat([torch.arange(c, c + n) for c, n in zip(b.ctx, b.ql)])
+    out = _run(b, rope=(cos.to(DEV), sin.to(DEV), "position"))
+    b.q = orope.apply_rope(b.q[None], cos[pos][None], sin[pos][None])[0]
+    b.check(out, None, 0, "kv4 rope")
+
+
+def test_scales_from_end_to_end():
+    """Scale bytes across their range of finite scores; a NaN block reaches its
+    own head's rows only."""
+    b = Batch([100, 40], [1, 1], D=128, kv="4", seed=4)
+    codes, scales = kv4.views(b.vc, b.bs, 128)
+    g = torch.Generator().manual_seed(1)
+    scales[:] = torch.randint(1, 230, scales.shape, generator=g, dtype=torch.uint8)
+    b.check(_run(b), None, 0, "kv4 scales")
+    slot = int(b.bt[0, 2])
+    scales[slot, 1, 5, 2] = 255                       # dims 64..95 of key 37, KV head 1
+    out = _run(b).float().cpu()
+    nan = torch.zeros(2, 8, 128, dtype=torch.bool)
+    nan[0, 4:, 64:96] = True
+    assert torch.equal(out.isnan(), nan)
+
+
+def test_strided_blocks_and_view():
+    """K and V as the halves of one pool, as an engine keeps them."""
+    b = Batch(**DECODE, D=64, kv="4", seed=6)
+    pool = torch.stack([b.kc, b.vc], 1).to(DEV)       # [NB, 2, Hkv, record]
+    plan = _plan(b)
+    out = paged.paged_attention(plan, b.q.to(DEV), pool[:, 0], pool[:, 1], b.bt.to(DEV))
+    torch.cuda.synchronize()
+    b.check(out, None, 0, "strided")
+
+
+def test_refusals():
+    b = Batch([10], [1], D=64, kv="4")
+    q, kc, vc, bt = (x.to(DEV) for x in (b.q, b.kc, b.vc, b.bt))
+    plan = _plan(b)
+    with pytest.raises(ValueError):
+        paged.paged_attention(plan, q, kc[..., :-16], vc[..., :-16], bt)
+    with pytest.raises(NotImplementedError):
+        paged.paged_attention(plan, q, kc, vc, bt, kv_new=(q[:, :2], q[:, :2]))
+    for D, dtype in ((96, BF), (64, F32)):
+        c = Batch([10], [1], D=D, dtype=dtype, kv="4")
+        with pytest.raises(NotImplementedError):
+            paged.paged_attention(_plan(c), c.q.to(DEV), c.kc.to(DEV), c.vc.to(DEV), c.bt.to(DEV))
