@@ -8,9 +8,12 @@ call site (``attention.Attention`` / ``AttentionMetadata``) and paged pool
 from .attention import Attention, AttentionMetadata, plan_for
 from .attention_op import flash_attention, reference_attention
 from .kv_cache import PagedKVCache
-from .paged import AttentionPlan, paged_attention, rope_kv_write, rope_rotate
+from .paged import (AttentionPlan, kv4_values, paged_attention, rope_kv_write, rope_rotate, rotary_kv_write,
+                    rotary_rotate)
+from .rotary import Rotary
 
 __all__ = [
-    "Attention", "AttentionMetadata", "AttentionPlan", "PagedKVCache", "flash_attention",
-    "paged_attention", "plan_for", "reference_attention", "rope_kv_write", "rope_rotate",
+    "Attention", "AttentionMetadata", "AttentionPlan", "PagedKVCache", "Rotary", "flash_attention", "kv4_values",
+    "paged_attention", "plan_for", "reference_attention", "rope_kv_write", "rope_rotate", "rotary_kv_write",
+    "rotary_rotate",
 ]

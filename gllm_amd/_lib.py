@@ -22,6 +22,7 @@ _p = ctypes.c_void_p
 _i32 = ctypes.c_int32
 _i64 = ctypes.c_int64
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
 _sz = ctypes.c_size_t
 
 # name -> (restype, argtypes); mirrors include/gllm_attn.h
@@ -29,6 +30,11 @@ SIGNATURES = {
     "gllm_attn_last_error": (ctypes.c_char_p, []),
     "gllm_attn_version": (ctypes.c_int, []),
     "gllm_kv4_record_bytes": (_sz, [_i32, _i32]),
+    "gllm_rotary_kv_write": (ctypes.c_int, [_p, _p, _p, _p, _p, _p, _p, _p, _i64, _p, _f64, _p, _i32, _i32, _i64, _i32,
+                                            _i32, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _p]),
+    "gllm_rope_kv_write_kv4": (ctypes.c_int, [_p, _p, _p, _p, _p, _p, _p, _p, _i64, _p, _p, _p, _i64, _i64, _i32, _i32,
+                                              _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _p]),
+    "gllm_kv4_values": (ctypes.c_int, [_p, _i64, _i64, _i32, _p, _i64, _i32, _i32, _p, _i64, _i32, _p]),
     "gllm_rope_kv_write": (ctypes.c_int, [_p, _p, _p, _p, _p, _p, _p, _p, _i64, _p, _p, _p, _i64, _i64,
                                           _i32, _i32, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _p]),
     "gllm_attn_plan_create": (ctypes.c_int, [ctypes.POINTER(_p), _p, _p, _i32, _i64, _i32, _i32, _i32,

@@ -24,8 +24,8 @@ PAGED = ["paged_attention.hip", "paged_attention_f16.hip", "paged_attention_kv4.
          "paged_attention_window.hip", "paged_attention_window_f16.hip"]
 GENERIC = ["generic_attention.hip", "generic_attention_bf16.hip", "generic_attention_f16.hip", "generic_window_f32.hip",
            "generic_window_bf16.hip", "generic_window_f16.hip"]
-SOURCES = [*PAGED, *GENERIC, "api.hip", "rope_kv_write.hip", "metadata.hip", "qkv_proj.hip"]
-NO_CONTRACT = {"rope_kv_write.hip", "qkv_proj.hip", *GENERIC}
+SOURCES = [*PAGED, *GENERIC, "api.hip", "rope_kv_write.hip", "rotary_write.hip", "metadata.hip", "qkv_proj.hip"]
+NO_CONTRACT = {"rope_kv_write.hip", "rotary_write.hip", "qkv_proj.hip", *GENERIC}
 # MFMA accumulators stay in VGPRs (no per-tile AGPR<->VGPR copies)
 EXTRA = {f: ["-mllvm", "--amdgpu-mfma-vgpr-form"] for f in [*PAGED, *GENERIC, "qkv_proj.hip"]}
 COMMON = [

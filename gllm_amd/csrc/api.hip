@@ -174,6 +174,19 @@ PinnedPool& pinned_pool() {
   return *pool;
 }
 
+// The layout of a 4-bit cache: 16-byte rows of codes, blocks at 32-bit byte strides.
+int kv4_check(const void* k_cache, const void* v_cache, int64_t block_stride, int32_t Hkv, int32_t D, int64_t bs) {
+  if (D % 32) return fail(GLLM_ATTN_EUNSUPPORTED, "4-bit cache: head_dim %d must be a multiple of 32", D);
+  if (bs <= 0 || bs > kMaxBlockSize)
+    return fail(GLLM_ATTN_EINVAL, "4-bit cache: block_size %lld must be in [1, %d]", (long long)bs, kMaxBlockSize);
+  if (((uintptr_t)k_cache | (uintptr_t)v_cache) & 15) return fail(GLLM_ATTN_EINVAL, "4-bit caches must be 16-byte aligned");
+  const int64_t rec = kv4_record_bytes(bs, D);
+  if (block_stride < Hkv * rec || block_stride % 16 || block_stride >= (int64_t(1) << 32))
+    return fail(GLLM_ATTN_EINVAL, "4-bit cache: %lld bytes between blocks; a multiple of 16, at least %lld (%d kv heads x "
+                                  "%lld) and less than 2^32 needed", (long long)block_stride, (long long)(Hkv * rec), Hkv, (long long)rec);
+  return ok();
+}
+
 }  // namespace
 
 struct gllm_attn_plan {
@@ -505,6 +518,101 @@ int gllm_rope_kv_write(const void* q, void* q_out, const void* k, const void* v,
   a.q_out_row_stride = q_out_row_stride; a.cache_slot_stride = cache_slot_stride; a.num_slots = num_slots;
   a.dtype = dtype; a.kv_dtype = kv_dtype;
   return hip_check(launch_rope_kv_write(a, (hipStream_t)stream), "rope_kv_write launch");
+}
+
+// The checks that gllm_rotary_kv_write and gllm_rope_kv_write_kv4 share.
+static int rotary_write_impl(RotaryWriteArgs& a, void* stream, const char* what) {
+  if (a.num_tokens < 0) return fail(GLLM_ATTN_EINVAL, "num_tokens < 0");
+  const bool kv = a.k || a.v;
+  if (kv && (!a.k || !a.v || !a.k_cache || !a.v_cache || !a.slot_mapping))
+    return fail(GLLM_ATTN_EINVAL, "k, v, k_cache, v_cache and slot_mapping go together");
+  if (!kv && !a.q_out) return fail(GLLM_ATTN_EINVAL, "nothing to do: neither k/v nor q_out given");
+  if (a.q_out && !a.q) return fail(GLLM_ATTN_EINVAL, "q_out given without q");
+  if (a.num_kv_heads <= 0 || a.num_q_heads <= 0) return fail(GLLM_ATTN_EINVAL, "head counts must be > 0");
+  if (!model_dtype_ok(a.dtype)) return fail(GLLM_ATTN_EUNSUPPORTED, "model dtype %d (f32, bf16 or f16)", a.dtype);
+  if (a.head_dim <= 0 || a.head_dim > 256 || a.head_dim % 8)
+    return fail(GLLM_ATTN_EUNSUPPORTED, "head_dim %d must be a multiple of 8, at most 256", a.head_dim);
+  const int64_t qd = (int64_t)a.num_q_heads * a.head_dim, kd = (int64_t)a.num_kv_heads * a.head_dim;
+  if (kv && (a.k_row_stride < kd || a.v_row_stride < kd))
+    return fail(GLLM_ATTN_EINVAL, "k/v row stride smaller than num_kv_heads * head_dim");
+  if (a.q_out && (a.q_row_stride < qd || a.q_out_row_stride < qd))
+    return fail(GLLM_ATTN_EINVAL, "q row stride smaller than num_q_heads * head_dim");
+  if (a.query_lens && a.tokens_per_seq <= 0) return fail(GLLM_ATTN_EINVAL, "tokens_per_seq must be > 0 with query_lens");
+  if (kv) {
+    if (a.num_slots <= 0) return fail(GLLM_ATTN_EINVAL, "num_slots must be > 0");
+    if (a.kv_dtype == GLLM_DTYPE_MXFP4) {
+      if (int rc = kv4_check(a.k_cache, a.v_cache, a.cache_slot_stride, a.num_kv_heads, a.head_dim, a.block_size)) return rc;
+      a.kv4_record = (int32_t)kv4_record_bytes(a.block_size, a.head_dim);
+    } else if (!kv_dtype_ok(a.kv_dtype)) {
+      return fail(GLLM_ATTN_EUNSUPPORTED, "kv_dtype %d (f32, bf16, f16, fp8 e4m3fn or mxfp4)", a.kv_dtype);
+    } else if (a.cache_slot_stride < kd) {
+      return fail(GLLM_ATTN_EINVAL, "cache_slot_stride too small");
+    }
+  }
+  return hip_check(launch_rotary_write(a, device_cus(), (hipStream_t)stream), what);
+}
+
+int gllm_rotary_kv_write(const void* q, void* q_out, const void* k, const void* v, void* k_cache, void* v_cache,
+                         const int64_t* slot_mapping, const int32_t* query_lens, int64_t tokens_per_seq,
+                         const double* freq, double factor, const int64_t* positions, int32_t rotary_dim,
+                         int32_t interleaved, int64_t num_tokens, int32_t num_q_heads, int32_t num_kv_heads,
+                         int32_t head_dim, int64_t q_row_stride, int64_t k_row_stride, int64_t v_row_stride,
+                         int64_t q_out_row_stride, int64_t cache_slot_stride, int64_t num_slots,
+                         int32_t block_size, int32_t dtype, int32_t kv_dtype, void* stream) {
+  Range range("gllm_rotary_kv_write");
+  if (rotary_dim < 0 || rotary_dim % 2 || rotary_dim > head_dim)
+    return fail(GLLM_ATTN_EINVAL, "rotary_dim %d must be even and at most head_dim %d", rotary_dim, head_dim);
+  if (!positions || (rotary_dim > 0 && !freq)) return fail(GLLM_ATTN_EINVAL, "null positions or freq");
+  if (!std::isfinite(factor)) return fail(GLLM_ATTN_EINVAL, "factor must be finite");
+  RotaryWriteArgs a{};
+  a.q = q; a.q_out = q_out; a.k = k; a.v = v; a.k_cache = k_cache; a.v_cache = v_cache;
+  a.slot_mapping = slot_mapping; a.query_lens = query_lens; a.tokens_per_seq = tokens_per_seq;
+  a.freq = freq; a.factor = factor; a.positions = positions; a.rotary_dim = rotary_dim; a.interleaved = interleaved ? 1 : 0;
+  a.num_tokens = num_tokens; a.num_q_heads = num_q_heads; a.num_kv_heads = num_kv_heads; a.head_dim = head_dim;
+  a.q_row_stride = q_row_stride; a.k_row_stride = k_row_stride; a.v_row_stride = v_row_stride;
+  a.q_out_row_stride = q_out_row_stride; a.cache_slot_stride = cache_slot_stride; a.num_slots = num_slots;
+  a.block_size = block_size; a.dtype = dtype; a.kv_dtype = kv_dtype;
+  return rotary_write_impl(a, stream, "rotary_kv_write launch");
+}
+
+int gllm_rope_kv_write_kv4(const void* q, void* q_out, const void* k, const void* v, void* k_cache, void* v_cache,
+                           const int64_t* slot_mapping, const int32_t* query_lens, int64_t tokens_per_seq,
+                           const void* cos, const void* sin, const int64_t* rope_rows, int64_t rope_row_stride,
+                           int64_t num_tokens, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                           int64_t q_row_stride, int64_t k_row_stride, int64_t v_row_stride,
+                           int64_t q_out_row_stride, int64_t block_stride, int64_t num_slots, int32_t block_size,
+                           int32_t dtype, void* stream) {
+  Range range("gllm_rope_kv_write_kv4");
+  if (!k || !v) return fail(GLLM_ATTN_EINVAL, "null k / v");
+  if (!cos || !sin) return fail(GLLM_ATTN_EINVAL, "null cos/sin");
+  if (rope_row_stride < head_dim / 2) return fail(GLLM_ATTN_EINVAL, "rope_row_stride < head_dim / 2");
+  RotaryWriteArgs a{};
+  a.q = q; a.q_out = q_out; a.k = k; a.v = v; a.k_cache = k_cache; a.v_cache = v_cache;
+  a.slot_mapping = slot_mapping; a.query_lens = query_lens; a.tokens_per_seq = tokens_per_seq;
+  a.cos = cos; a.sin = sin; a.rope_rows = rope_rows; a.rope_row_stride = rope_row_stride; a.rotary_dim = head_dim;
+  a.num_tokens = num_tokens; a.num_q_heads = num_q_heads; a.num_kv_heads = num_kv_heads; a.head_dim = head_dim;
+  a.q_row_stride = q_row_stride; a.k_row_stride = k_row_stride; a.v_row_stride = v_row_stride;
+  a.q_out_row_stride = q_out_row_stride; a.cache_slot_stride = block_stride; a.num_slots = num_slots;
+  a.block_size = block_size; a.dtype = dtype; a.kv_dtype = GLLM_DTYPE_MXFP4;
+  return rotary_write_impl(a, stream, "rope_kv_write_kv4 launch");
+}
+
+int gllm_kv4_values(const void* cache, int64_t block_stride, int64_t num_slots, int32_t block_size,
+                    const int64_t* slots, int64_t num_rows, int32_t num_kv_heads, int32_t head_dim, void* out,
+                    int64_t out_row_stride, int32_t dtype, void* stream) {
+  Range range("gllm_kv4_values");
+  if (num_rows < 0) return fail(GLLM_ATTN_EINVAL, "num_rows < 0");
+  if (!cache || !slots || !out) return fail(GLLM_ATTN_EINVAL, "null pointer argument");
+  if (num_kv_heads <= 0 || head_dim <= 0 || num_slots <= 0) return fail(GLLM_ATTN_EINVAL, "sizes must be > 0");
+  if (!model_dtype_ok(dtype)) return fail(GLLM_ATTN_EUNSUPPORTED, "dtype %d (f32, bf16 or f16)", dtype);
+  if (int rc = kv4_check(cache, cache, block_stride, num_kv_heads, head_dim, block_size)) return rc;
+  if (out_row_stride < (int64_t)num_kv_heads * head_dim) return fail(GLLM_ATTN_EINVAL, "out row stride too small");
+  Kv4ValuesArgs a{};
+  a.cache = cache; a.block_stride = block_stride; a.block_size = block_size;
+  a.kv4_record = (int32_t)kv4_record_bytes(block_size, head_dim);
+  a.num_slots = num_slots; a.slots = slots; a.num_rows = num_rows; a.out = out; a.out_row_stride = out_row_stride;
+  a.num_kv_heads = num_kv_heads; a.head_dim = head_dim; a.dtype = dtype;
+  return hip_check(launch_kv4_values(a, (hipStream_t)stream), "kv4_values launch");
 }
 
 int gllm_qkv_rope_kv_write(const void* x, int64_t x_row_stride, int64_t num_tokens, int32_t hidden,
@@ -1121,18 +1229,6 @@ static int fill_common(AttnArgs& a, int32_t Hq, int32_t Hkv, int32_t D, float sc
   a.num_q_heads = Hq; a.num_kv_heads = Hkv; a.head_dim = D;
   a.scale = scale; a.dtype = dtype; a.kv_dtype = kv_dtype;
   if (!(scale > 0.f) || !std::isfinite(scale)) return fail(GLLM_ATTN_EINVAL, "scale must be finite and > 0");
-  return ok();
-}
-
-// The layout of a 4-bit cache: 16-byte rows of codes, blocks at 32-bit byte strides.
-static int kv4_check(const void* k_cache, const void* v_cache, int64_t block_stride, int32_t Hkv, int32_t D,
-                     int64_t bs) {
-  if (D % 32) return fail(GLLM_ATTN_EUNSUPPORTED, "4-bit cache: head_dim %d must be a multiple of 32", D);
-  if (((uintptr_t)k_cache | (uintptr_t)v_cache) & 15) return fail(GLLM_ATTN_EINVAL, "4-bit caches must be 16-byte aligned");
-  const int64_t rec = kv4_record_bytes(bs, D);
-  if (block_stride < Hkv * rec || block_stride % 16 || block_stride >= (int64_t(1) << 32))
-    return fail(GLLM_ATTN_EINVAL, "4-bit cache: %lld bytes between blocks; a multiple of 16 and at least %lld needed "
-                                  "(%d kv heads x %lld)", (long long)block_stride, (long long)(Hkv * rec), Hkv, (long long)rec);
   return ok();
 }
 

@@ -187,11 +187,53 @@ struct QKVArgs {
   int32_t full_tiles, full_wgs, half_tiles;
 };
 
+// Rotary positions (or, with `cos`, table rows) + KV write; rows of a 4-bit cache.
+struct RotaryWriteArgs {
+  const void* q;                 // as in RopeKVWriteArgs
+  void* q_out;                   // nullable: no q
+  const void* k;                 // nullable: no cache
+  const void* v;
+  void* k_cache;
+  void* v_cache;
+  const int64_t* slot_mapping;
+  const int32_t* query_lens;
+  int64_t tokens_per_seq;
+  const double* freq;            // [rotary_dim / 2] radians per position
+  double factor;                 // of cos and sin
+  const int64_t* positions;      // [N]
+  const void* cos;               // not null: table rows, each op rounded to the model dtype
+  const void* sin;
+  const int64_t* rope_rows;
+  int64_t rope_row_stride;
+  int32_t rotary_dim, interleaved;
+  int64_t num_tokens;
+  int32_t num_q_heads, num_kv_heads, head_dim;
+  int64_t q_row_stride, k_row_stride, v_row_stride, q_out_row_stride;
+  int64_t cache_slot_stride;     // 4-bit cache: bytes between blocks
+  int64_t num_slots;
+  int32_t block_size, kv4_record;   // 4-bit cache
+  int32_t dtype, kv_dtype;
+  int32_t parts;                 // waves per token (set by the launcher)
+};
+struct Kv4ValuesArgs {
+  const void* cache;
+  int64_t block_stride;          // bytes
+  int32_t block_size, kv4_record;
+  int64_t num_slots;
+  const int64_t* slots;          // [num_rows]
+  int64_t num_rows;
+  void* out;                     // [num_rows, out_row_stride] of dtype
+  int64_t out_row_stride;
+  int32_t num_kv_heads, head_dim, dtype;
+};
+
 size_t qkv_workspace_bytes(int64_t num_tokens, int hidden, int heads, int head_dim, int cus);
 bool qkv_tiles_ahead(int64_t num_tokens, int q_cols, int kv_cols, int cus);
 
 hipError_t launch_rope_kv_write(const RopeKVWriteArgs& a, hipStream_t stream);
 hipError_t launch_qkv_rope_write(const QKVArgs& a, hipStream_t stream);
+hipError_t launch_rotary_write(RotaryWriteArgs a, int cus, hipStream_t stream);
+hipError_t launch_kv4_values(const Kv4ValuesArgs& a, hipStream_t stream);
 hipError_t launch_build_metadata(const MetadataArgs& a, hipStream_t stream);
 // MFMA kernels: bf16 or fp16 model (a.dtype), head dim 64 or 128, cache in
 // the model dtype or fp8 e4m3fn

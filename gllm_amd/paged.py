@@ -72,6 +72,15 @@ def kv4_record_bytes(block_size: int, head_dim: int) -> int:
     return -(-block_size * (head_dim // 32 * 17) // 16) * 16
 
 
+def _kv4_block_size(cache: torch.Tensor, D: int) -> int:
+    """The block size whose records a 4-bit cache of head dim D holds (the
+    padding is shorter than a key's bytes)."""
+    if cache.dtype != KV4 or cache.dim() != 3 or D <= 0 or D % 32 or cache.shape[2] < D // 32 * 17:
+        raise ValueError(f"expected a 4-bit cache of head_dim {D}, uint8 [num_blocks, Hkv, record bytes] (head_dim a "
+                         f"multiple of 32), got {cache.dtype} {tuple(cache.shape)}")
+    return cache.shape[2] // (D // 32 * 17)
+
+
 def _kv4_blocks(k_cache: torch.Tensor, v_cache: torch.Tensor, Hkv: int, D: int, block_size: int) -> int:
     """Blocks of a 4-bit cache pair, after a check of its layout."""
     rec = kv4_record_bytes(block_size, D)
@@ -99,7 +108,7 @@ def rope_kv_write(k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torc
     token (or ``rope_rows`` indexing a table), caches ``[num_slots, Hkv, D]``,
     ``slot_mapping`` int64 with one slot per token.  With ``query_lens``
     (padded ``[B, T_q]`` token layout) rows past each sequence's length are not
-    written.
+    written.  The caches may be 4-bit ones (:data:`KV4`; slots must differ there).
     """
     Hkv, D = k.shape[-2], k.shape[-1]
     if k.shape != v.shape:
@@ -107,7 +116,12 @@ def rope_kv_write(k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torc
     ks = _rows(k, Hkv, D, "k")
     vs = _rows(v, Hkv, D, "v")
     n = k.numel() // (Hkv * D)
-    _cache_rows(k_cache, v_cache, Hkv, D)
+    if k_cache.dtype == KV4:
+        bs = _kv4_block_size(k_cache, D)
+        num_slots = _kv4_blocks(k_cache, v_cache, Hkv, D, bs) * bs
+    else:
+        _cache_rows(k_cache, v_cache, Hkv, D)
+        num_slots = k_cache.shape[0]
     if k_cache.stride(0) != v_cache.stride(0) or k_cache.shape[0] != v_cache.shape[0]:
         raise ValueError("k_cache and v_cache must have the same shape and slot stride")
     sm = slot_mapping if slot_mapping.dim() == 1 else slot_mapping.reshape(-1)
@@ -136,11 +150,126 @@ def rope_kv_write(k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torc
         rr = _index_rows(rope_rows)
     dev = k.device
     lib = _lib.load()
+    if k_cache.dtype == KV4:
+        _lib.check(lib.gllm_rope_kv_write_kv4(
+            _lib.ptr(q), _lib.ptr(q_out), k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+            sm.data_ptr(), _lib.ptr(ql), tps, cs.data_ptr(), sn.data_ptr(), _lib.ptr(rr), cs.stride(0), n,
+            Hq, Hkv, D, qs, ks, vs, qos, k_cache.stride(0), num_slots, bs, _lib.dtype_code(k.dtype),
+            _lib.stream_ptr(dev)))
+        return
     _lib.check(lib.gllm_rope_kv_write(
         _lib.ptr(q), _lib.ptr(q_out), k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
         sm.data_ptr(), _lib.ptr(ql), tps, cs.data_ptr(), sn.data_ptr(), _lib.ptr(rr), cs.stride(0), n,
         Hq, Hkv, D, qs, ks, vs, qos, k_cache.stride(0), k_cache.shape[0],
         _lib.dtype_code(k.dtype), _lib.dtype_code(k_cache.dtype), _lib.stream_ptr(dev)))
+
+
+def _same_device(dev: torch.device, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, the call on {dev}")
+
+
+def rotary_kv_write(k: torch.Tensor | None, v: torch.Tensor | None, positions: torch.Tensor, rotary,
+                    k_cache: torch.Tensor | None, v_cache: torch.Tensor | None, slot_mapping: torch.Tensor | None,
+                    query_lens: torch.Tensor | None = None, q: torch.Tensor | None = None,
+                    q_out: torch.Tensor | None = None) -> None:
+    """Rotary positions on k (and q -> q_out) plus the KV-cache write, in one
+    launch and without a cos/sin table.
+
+    ``rotary``: a :class:`gllm_amd.Rotary`; ``positions`` int64, one per token.
+    k/v ``[..., Hkv, D]`` (token rows), caches ``[num_slots, Hkv, D]`` of any
+    cache dtype or 4-bit ones (:data:`KV4`), ``slot_mapping`` int64 with one slot
+    per token (outside the cache: not written; 4-bit: slots must differ),
+    ``query_lens`` as in :func:`rope_kv_write`.  ``q_out`` may be q itself.  k is
+    rounded once, to the cache dtype; q once, to the model dtype.
+    """
+    x = q if k is None else k
+    if x is None or (k is None) != (v is None) or (q is None) != (q_out is None):
+        raise ValueError("k and v, and q and q_out, go together; at least one pair is needed")
+    D, dev = x.shape[-1], x.device
+    if D != rotary.head_dim:
+        raise ValueError(f"head_dim {D}, the rotary positions are for {rotary.head_dim}")
+    _same_device(dev, v=v, q=q, q_out=q_out, positions=positions, freq=rotary.freq, k_cache=k_cache, v_cache=v_cache,
+                 slot_mapping=slot_mapping, query_lens=query_lens)
+    H = x.shape[-2]
+    n = x.numel() // (H * D)
+    pos = _index_rows(positions)
+    if positions.dtype.is_floating_point or pos.numel() != n:
+        raise ValueError("positions must be integers, one per token")
+    ks = vs = qs = qos = stride = num_slots = bs = 0
+    Hq = Hkv = 1
+    kv_code, sm = _lib.DTYPE_F32, None
+    if k is not None:
+        if k_cache is None or v_cache is None or slot_mapping is None:
+            raise ValueError("k and v need caches and a slot mapping")
+        Hkv = H
+        if v.shape != k.shape or v.dtype != k.dtype:
+            raise ValueError("k and v shapes or dtypes differ")
+        ks, vs = _rows(k, Hkv, D, "k"), _rows(v, Hkv, D, "v")
+        if k_cache.dtype == KV4:
+            bs = _kv4_block_size(k_cache, D)
+            num_slots = _kv4_blocks(k_cache, v_cache, Hkv, D, bs) * bs
+        else:
+            _cache_rows(k_cache, v_cache, Hkv, D)
+            num_slots = k_cache.shape[0]
+        if k_cache.shape != v_cache.shape or k_cache.stride(0) != v_cache.stride(0) or k_cache.dtype != v_cache.dtype:
+            raise ValueError("k_cache and v_cache must have the same shape, dtype and slot stride")
+        sm = slot_mapping if slot_mapping.dim() == 1 else slot_mapping.reshape(-1)
+        if sm.dtype != torch.int64 or sm.numel() != n or not sm.is_contiguous():
+            raise ValueError("slot_mapping must be contiguous int64 with one entry per token")
+        stride, kv_code = k_cache.stride(0), _kv_code(k_cache)
+    if q is not None:
+        Hq = q.shape[-2]
+        if q.dtype != x.dtype or q_out.dtype != x.dtype or q.numel() != n * Hq * D or q_out.numel() != q.numel():
+            raise ValueError("q and q_out need the model dtype and one row per token")
+        qs, qos = _rows(q, Hq, D, "q"), _rows(q_out, Hq, D, "q_out")
+    tps, ql = 0, None
+    if query_lens is not None:
+        ql = query_lens.to(torch.int32).contiguous()
+        if ql.numel() == 0 or n % ql.numel():
+            raise ValueError("query_lens: the tokens must be as many rows for each sequence")
+        tps = n // ql.numel()
+    if n == 0:
+        return
+    lib = _lib.load()
+    _lib.check(lib.gllm_rotary_kv_write(
+        _lib.ptr(q), _lib.ptr(q_out), _lib.ptr(k), _lib.ptr(v), _lib.ptr(k_cache), _lib.ptr(v_cache), _lib.ptr(sm),
+        _lib.ptr(ql), tps, rotary.freq.data_ptr(), rotary.factor, pos.data_ptr(), rotary.rotary_dim,
+        int(rotary.interleaved), n, Hq, Hkv, D, qs, ks, vs, qos, stride, num_slots, bs, _lib.dtype_code(x.dtype),
+        kv_code, _lib.stream_ptr(dev)))
+
+
+def rotary_rotate(x: torch.Tensor, positions: torch.Tensor, rotary, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotary positions of ``x [..., H, D]``, one position per row of heads;
+    returns ``out`` (a new tensor by default, x itself rotates in place)."""
+    if out is None:
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    rotary_kv_write(None, None, positions, rotary, None, None, None, q=x, q_out=out)
+    return out
+
+
+def kv4_values(cache: torch.Tensor, slots: torch.Tensor, head_dim: int, dtype: torch.dtype,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rows of a 4-bit cache (:data:`KV4`) as the values they stand for, in
+    ``dtype``: ``[N, Hkv, head_dim]`` for int64 ``slots [N]`` (zeros for a slot
+    outside the cache).  For moving rows to another cache or looking at them."""
+    bs = _kv4_block_size(cache, head_dim)
+    Hkv = cache.shape[1]
+    nb = _kv4_blocks(cache, cache, Hkv, head_dim, bs)
+    sl = _index_rows(slots)
+    _same_device(cache.device, slots=slots, out=out)
+    if out is None:
+        out = torch.empty(sl.numel(), Hkv, head_dim, dtype=dtype, device=cache.device)
+    elif out.dtype != dtype or out.numel() != sl.numel() * Hkv * head_dim:
+        raise ValueError(f"out must be {dtype} with one row per slot")
+    stride = _rows(out, Hkv, head_dim, "out")
+    if sl.numel() == 0:
+        return out
+    _lib.check(_lib.load().gllm_kv4_values(cache.data_ptr(), cache.stride(0), nb * bs, bs, sl.data_ptr(), sl.numel(), Hkv,
+                                           head_dim, out.data_ptr(), stride, _lib.dtype_code(dtype),
+                                           _lib.stream_ptr(cache.device)))
+    return out
 
 
 # Token count from which qkv_rope_kv_write projects with hipBLASLt (three

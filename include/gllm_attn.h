@@ -211,6 +211,55 @@ int gllm_rope_kv_write(const void* q, void* q_out, const void* k, const void* v,
                        int32_t kv_dtype, void* stream);
 
 /*
+ * Rotary positions and the paged KV write without a cos/sin table.  The token
+ * at positions[t] turns pair i (0 <= i < rotary_dim / 2) of q and k by the angle
+ * a = positions[t] * freq[i] (one fp64 product): [x1 c - x2 s, x1 s + x2 c] with
+ * c = factor cos a, s = factor sin a, over dims (i, i + rotary_dim / 2), or
+ * (2i, 2i + 1) if `interleaved`; dims from rotary_dim on pass unchanged.  freq is a
+ * device array of radians per position, so any scaling of the positions is a
+ * matter of its values.  q is rotated in fp32 and rounded once to the model
+ * dtype; k in fp64 and rounded once to the cache dtype (as .to(kv_dtype) rounds;
+ * GLLM_DTYPE_MXFP4 as at gllm_kv4_record_bytes); v is rounded to the cache dtype.
+ * k == v == NULL: q only.  q_out == NULL: no q; q_out may be q.  query_lens /
+ * tokens_per_seq, slots and strides as in gllm_rope_kv_write; block_size is
+ * read for a 4-bit cache only, whose num_slots counts blocks x block_size and
+ * whose slots have to differ (equal ones leave a mixture of their rows).
+ * head_dim a multiple of 8, at most 256.  No counterpart in the reference.
+ */
+int gllm_rotary_kv_write(const void* q, void* q_out, const void* k, const void* v, void* k_cache,
+                         void* v_cache, const int64_t* slot_mapping, const int32_t* query_lens,
+                         int64_t tokens_per_seq, const double* freq, double factor,
+                         const int64_t* positions, int32_t rotary_dim, int32_t interleaved,
+                         int64_t num_tokens, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                         int64_t q_row_stride, int64_t k_row_stride, int64_t v_row_stride,
+                         int64_t q_out_row_stride, int64_t cache_slot_stride, int64_t num_slots,
+                         int32_t block_size, int32_t dtype, int32_t kv_dtype, void* stream);
+
+/*
+ * gllm_rope_kv_write into a 4-bit cache: the same rotation from cos/sin rows
+ * (each op rounded to the model dtype), k and v then rounded as at
+ * gllm_kv4_record_bytes.  block_stride: bytes between blocks; num_slots: blocks x
+ * block_size.
+ */
+int gllm_rope_kv_write_kv4(const void* q, void* q_out, const void* k, const void* v, void* k_cache,
+                           void* v_cache, const int64_t* slot_mapping, const int32_t* query_lens,
+                           int64_t tokens_per_seq, const void* cos, const void* sin,
+                           const int64_t* rope_rows, int64_t rope_row_stride, int64_t num_tokens,
+                           int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                           int64_t q_row_stride, int64_t k_row_stride, int64_t v_row_stride,
+                           int64_t q_out_row_stride, int64_t block_stride, int64_t num_slots,
+                           int32_t block_size, int32_t dtype, void* stream);
+
+/*
+ * Rows of a 4-bit cache as the values they stand for, in dtype (f32, bf16:
+ * exact; f16: rounded to nearest even): out[r] = the num_kv_heads x head_dim
+ * values at slots[r] (zeros for a slot outside [0, num_slots)).
+ */
+int gllm_kv4_values(const void* cache, int64_t block_stride, int64_t num_slots, int32_t block_size,
+                    const int64_t* slots, int64_t num_rows, int32_t num_kv_heads, int32_t head_dim,
+                    void* out, int64_t out_row_stride, int32_t dtype, void* stream);
+
+/*
  * Plan the work for one batch from HOST lengths.  Sequence i has
  * query_lens[i] query rows starting at row i * q_seq_stride of q/out
  * (q_seq_stride = the padded T_q of the reference's [B, T_q, ...] layout), or,
