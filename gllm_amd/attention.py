@@ -77,23 +77,38 @@ def _block_size(meta, ql: list[int], sl: list[int], hint: int | None = None) -> 
     return cands[0]
 
 
+def _kept_plan(meta, window: int | None, sinks: int):
+    """The plan that an earlier layer of the step left on the metadata, or None."""
+    if window is None:
+        return getattr(meta, "_gllm_plan", None)
+    return (getattr(meta, "_gllm_window_plans", None) or {}).get((window, sinks))
+
+
 def plan_for(meta, *, num_q_heads: int, num_kv_heads: int, head_dim: int,
-             dtype: torch.dtype, device, block_size_hint: int | None = None) -> paged.AttentionPlan:
+             dtype: torch.dtype, device, block_size_hint: int | None = None,
+             window: int | None = None, sinks: int = 0) -> paged.AttentionPlan:
     """The batch plan, built once per metadata object (one engine step) and
-    reused by every layer.  Reads the lengths back once, like the reference's
+    reused by every layer (of each sliding window: a model may have layers with
+    and without).  Reads the lengths back once, like the reference's
     own ``.tolist()`` / ``.item()`` calls in ``llm.py:166,176``.  ``meta`` is
     this module's :class:`AttentionMetadata` or the reference's (no
     ``block_size``: derived from the slot mapping, or ``block_size_hint``
     checked against it)."""
-    plan = getattr(meta, "_gllm_plan", None)
+    plan = _kept_plan(meta, window, sinks)
     if plan is None:
         ql = meta.query_lens.tolist()
         sl = meta.seq_lens.tolist()
         bs = _block_size(meta, ql, sl, block_size_hint)
         plan = paged.AttentionPlan(ql, sl, num_q_heads=num_q_heads, num_kv_heads=num_kv_heads,
                                    head_dim=head_dim, block_size=bs, dtype=dtype,
-                                   device=device, q_seq_stride=meta.query_slot_mapping.shape[1])
-        object.__setattr__(meta, "_gllm_plan", plan)
+                                   device=device, q_seq_stride=meta.query_slot_mapping.shape[1], window=window,
+                                   sinks=sinks)
+        if window is None:
+            object.__setattr__(meta, "_gllm_plan", plan)
+        else:
+            plans = getattr(meta, "_gllm_window_plans", None) or {}
+            plans[window, sinks] = plan
+            object.__setattr__(meta, "_gllm_window_plans", plans)
     return plan
 
 
@@ -116,10 +131,12 @@ class Attention:
     """``attention.py:30-182``.  ``weights`` maps the reference's safetensors
     names (``model.layers.{i}.self_attn.{q,k,v,o}_proj.weight``) to tensors;
     ``model_config`` needs ``dtype, hidden_size, head_dim, num_attn_heads,
-    num_kv_heads``."""
+    num_kv_heads``.  ``window`` / ``sinks``: the layer's sliding window
+    (:class:`paged.AttentionPlan`).  The cache may be a 4-bit one."""
 
-    def __init__(self, layer_idx: int, model_config, safetensors):
+    def __init__(self, layer_idx: int, model_config, safetensors, *, window: int | None = None, sinks: int = 0):
         self.layer_idx = layer_idx
+        self.window, self.sinks = window, sinks
         self.num_q_heads = model_config.num_attn_heads
         self.num_kv_heads = model_config.num_kv_heads
         self.hidden_size = model_config.hidden_size
@@ -158,12 +175,13 @@ class Attention:
 
     def _plan(self, meta, dtype, device) -> paged.AttentionPlan:
         """The step's plan: built by the step's first layer, kept on ``meta``."""
-        plan = getattr(meta, "_gllm_plan", None)
+        plan = _kept_plan(meta, self.window, self.sinks)
         if plan is not None:
             self._block_size = plan.block_size
             return plan
         plan = plan_for(meta, num_q_heads=self.num_q_heads, num_kv_heads=self.num_kv_heads, head_dim=self.head_dim,
-                        dtype=dtype, device=device, block_size_hint=self._block_size)
+                        dtype=dtype, device=device, block_size_hint=self._block_size, window=self.window,
+                        sinks=self.sinks)
         self._block_size = plan.block_size
         return plan
 

@@ -7,10 +7,15 @@ with the per-layer view ``[2, NB * block_size, Hkv, D]``; slot
 allocation (``reserve_blocks`` / ``release_blocks``, ``paged_kv_cache.py:
 81-110``) stays with the reference's own host allocator: the kernels only
 read the block table it fills.
+
+``kv_dtype=paged.KV4`` makes a 4-bit pool instead, ``[2 (K/V), L, NB, Hkv,
+record bytes]`` with the per-layer view ``[2, NB, Hkv, record bytes]``.
 """
 from __future__ import annotations
 
 import torch
+
+from . import paged
 
 
 class PagedKVCache:
@@ -19,12 +24,18 @@ class PagedKVCache:
         self.block_size = block_size
         nb = self.num_required_blocks(max_batch_size * max_seq_len)
         self.num_blocks = nb
+        if kv_dtype == paged.KV4:
+            rec = paged.kv4_record_bytes(block_size, head_dim)
+            self.physical_kv_cache = torch.zeros((2, num_layers, nb, num_kv_heads, rec), dtype=kv_dtype, device=device)
+            self.flattened_kv_cache = self.physical_kv_cache
+            return
         self.physical_kv_cache = torch.zeros((2, num_layers, nb, block_size, num_kv_heads, head_dim),
                                              dtype=kv_dtype, device=device)
         self.flattened_kv_cache = self.physical_kv_cache.view(2, num_layers, -1, num_kv_heads, head_dim)
 
     def get_layer_kv_cache(self, layer: int) -> torch.Tensor:
-        """``[2, NB * block_size, Hkv, D]`` view of one layer."""
+        """``[2, NB * block_size, Hkv, D]`` view of one layer (4-bit: ``[2, NB,
+        Hkv, record bytes]``)."""
         return self.flattened_kv_cache[:, layer]
 
     def num_required_blocks(self, num_tokens: int) -> int:
