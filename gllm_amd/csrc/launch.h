@@ -213,7 +213,6 @@ struct RotaryWriteArgs {
   int64_t num_slots;
   int32_t block_size, kv4_record;   // 4-bit cache
   int32_t dtype, kv_dtype;
-  int32_t parts;                 // waves per token (set by the launcher)
 };
 struct Kv4ValuesArgs {
   const void* cache;
@@ -232,7 +231,7 @@ bool qkv_tiles_ahead(int64_t num_tokens, int q_cols, int kv_cols, int cus);
 
 hipError_t launch_rope_kv_write(const RopeKVWriteArgs& a, hipStream_t stream);
 hipError_t launch_qkv_rope_write(const QKVArgs& a, hipStream_t stream);
-hipError_t launch_rotary_write(RotaryWriteArgs a, int cus, hipStream_t stream);
+hipError_t launch_rotary_write(const RotaryWriteArgs& a, int cus, hipStream_t stream);
 hipError_t launch_kv4_values(const Kv4ValuesArgs& a, hipStream_t stream);
 hipError_t launch_build_metadata(const MetadataArgs& a, hipStream_t stream);
 // MFMA kernels: bf16 or fp16 model (a.dtype), head dim 64 or 128, cache in

@@ -126,7 +126,10 @@ __device__ __forceinline__ uint32_t encode4(const float* v, uint32_t* byte) {
 }
 
 constexpr int kRotWaves = 4;        // waves per workgroup
-constexpr int kRotPairs = 128;      // most pairs of a head (head_dim 256)
+// LDS place of a pair's (cos, sin): a gap after every eight, so that lanes
+// eight pairs apart read different banks
+__device__ __forceinline__ int pair_at(int i) { return i + (i >> 3); }
+constexpr int kRotPairs = 128 + 16;  // places of the most pairs of a head (head_dim 256)
 
 // TABLE: cos / sin rows in the model dtype and every op rounded to it, half
 // pairs over the whole head: rope_kv_write's arithmetic
@@ -142,128 +145,134 @@ __global__ void __launch_bounds__(64 * kRotWaves) rotary_write_kernel(RotaryWrit
   const int ch = lane % cpd, hl = lane / cpd;     // the lane's chunk and head of the pass
   const int d0 = 8 * ch;
   const int nq = a.q_out ? (a.num_q_heads + hpi - 1) / hpi : 0;
+  // the pair that dim d belongs to (-1: it passes), and the sign of its partner's product
+  auto pair_of = [&](int d) { return d >= R ? -1 : (a.interleaved ? d / 2 : (d < half ? d : d - half)); };
+  auto flip = [&](int d) { return (a.interleaved ? !(d & 1) : d < half) ? -1.f : 1.f; };
   const int nk = a.k ? (a.num_kv_heads + hpi - 1) / hpi : 0;
-  const int64_t units = a.num_tokens * a.parts;
-  for (int64_t u = (int64_t)blockIdx.x * kRotWaves + wave; u < units; u += (int64_t)gridDim.x * kRotWaves) {
-    const int64_t tok = u / a.parts;
-    const int part = (int)(u - tok * a.parts);
-    if (a.query_lens) {                           // padded rows are skipped whole
-      const int64_t b = tok / a.tokens_per_seq;
-      if (tok - b * a.tokens_per_seq >= a.query_lens[b]) continue;
-    }
-    int64_t slot = -1;
-    if (a.k) slot = a.slot_mapping[tok];
-    const bool kv_ok = slot >= 0 && slot < a.num_slots;   // never address outside the pool
+  const int part = blockIdx.y;
+  const int64_t tok = (int64_t)blockIdx.x * kRotWaves + wave;   // no loop over tokens: its invariants would fill the registers
+  if (tok >= a.num_tokens) return;
+  if (a.query_lens) {                           // padded rows are skipped whole
+    const int64_t b = tok / a.tokens_per_seq;
+    if (tok - b * a.tokens_per_seq >= a.query_lens[b]) return;
+  }
+  int64_t slot = -1;
+  if (a.k) slot = a.slot_mapping[tok];
+  const bool kv_ok = slot >= 0 && slot < a.num_slots;   // never address outside the pool
+  int64_t at = slot * a.cache_slot_stride;              // the row's place in the caches
+  int64_t sc_at = 0;                                    // 4-bit: its scales'
+  if constexpr (std::is_same<KV, kv4>::value) {
+    const int64_t blk = kv_ok ? slot / a.block_size : 0, off = slot - blk * a.block_size;
+    at = blk * a.cache_slot_stride + off * (D / 2);
+    sc_at = blk * a.cache_slot_stride + (int64_t)a.block_size * (D / 2) + off * (D / 32);
+  }
 
-    // the lane's (cos, sin): of its 8 dims (half pairs) or 4 pairs (interleaved)
-    double c[8], s[8];
-    float c32[8], s32[8];
-    if constexpr (TABLE) {
-      const int64_t row = a.rope_rows ? a.rope_rows[tok] : tok;
-      const int j = d0 < half ? d0 : d0 - half;
-      load8<T>((const T*)a.cos + row * a.rope_row_stride + j, c32);
-      load8<T>((const T*)a.sin + row * a.rope_row_stride + j, s32);
+  // cos and sin of the lane's 8 dims: q's in registers, k's (fp64) stay in LDS
+  float c32[8], s32[8];
+  if constexpr (TABLE) {
+    const int64_t row = a.rope_rows ? a.rope_rows[tok] : tok;
+    const int j = d0 < half ? d0 : d0 - half;
+    load8<T>((const T*)a.cos + row * a.rope_row_stride + j, c32);
+    load8<T>((const T*)a.sin + row * a.rope_row_stride + j, s32);
+  } else {
+    const double p = (double)a.positions[tok];
+    __builtin_amdgcn_wave_barrier();
+    for (int i = lane; i < half; i += 64) {
+      double ci, si;
+      sincos64(p * a.freq[i], a.factor, &ci, &si);
+      cs[wave][pair_at(i)][0] = ci;
+      cs[wave][pair_at(i)][1] = si;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // the wave's own LDS, in order
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int pr = pair_of(d0 + i);
+      c32[i] = pr < 0 ? 1.f : (float)cs[wave][pair_at(pr)][0];
+      s32[i] = pr < 0 ? 0.f : flip(d0 + i) * (float)cs[wave][pair_at(pr)][1];
+    }
+  }
+
+  // the row's 8 dims and their partners
+  auto pair8 = [&](const T* row, float* x, float* y) {
+    load8<T>(row + d0, x);
+    if (!TABLE && a.interleaved) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = x[i ^ 1];
+    } else if (TABLE || half % 8 == 0) {         // a chunk lies in one half
+      const int dp = d0 < half ? d0 + half : (d0 < R ? d0 - half : d0);
+      load8<T>(row + dp, y);
     } else {
-      const double p = (double)a.positions[tok];
-      for (int i = lane; i < half; i += 64) {
-        double ci, si;
-        sincos64(p * a.freq[i], a.factor, &ci, &si);
-        cs[wave][i][0] = ci;
-        cs[wave][i][1] = si;
-      }
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // the wave's own LDS, in order
-      __builtin_amdgcn_wave_barrier();
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int d = d0 + i;
-        const bool turned = d < R;
-        const int pr = !turned ? 0 : (a.interleaved ? d / 2 : (d < half ? d : d - half));
-        c[i] = turned ? cs[wave][pr][0] : 1.0;
-        s[i] = turned ? cs[wave][pr][1] : 0.0;
-        // the sign of the partner's product goes into s
-        if (a.interleaved ? !(d & 1) : d < half) s[i] = -s[i];
-        c32[i] = (float)c[i];
-        s32[i] = (float)s[i];
+        y[i] = (float)row[d < half ? d + half : (d < R ? d - half : d)];
       }
-      __builtin_amdgcn_wave_barrier();
     }
-
-    // the row's 8 dims and their partners
-    auto pair8 = [&](const T* row, float* x, float* y) {
-      load8<T>(row + d0, x);
-      if (!TABLE && a.interleaved) {
+  };
+  auto turn_ops = [&](const float* x, const float* y, float* o) {     // each op rounded to T
+    const bool first = d0 < half;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = x[i ^ 1];
-      } else if (TABLE || half % 8 == 0) {         // a chunk lies in one half
-        const int dp = d0 < half ? d0 + half : (d0 < R ? d0 - half : d0);
-        load8<T>(row + dp, y);
+    for (int i = 0; i < 8; i += 2) {
+      float u0 = rnd<T>(__fmul_rn(x[i], c32[i])), v0 = rnd<T>(__fmul_rn(y[i], s32[i]));
+      float u1 = rnd<T>(__fmul_rn(x[i + 1], c32[i + 1])), v1 = rnd<T>(__fmul_rn(y[i + 1], s32[i + 1]));
+      if constexpr (std::is_same<T, _Float16>::value) opaque4(u0, v0, u1, v1);
+      o[i] = rnd<T>(first ? __fsub_rn(u0, v0) : __fadd_rn(u0, v0));
+      o[i + 1] = rnd<T>(first ? __fsub_rn(u1, v1) : __fadd_rn(u1, v1));
+    }
+  };
+
+  for (int g = part; g < nq; g += gridDim.y) {
+    const int h = g * hpi + hl;
+    if (hl >= hpi || h >= a.num_q_heads) continue;
+    float x[8], y[8];
+    pair8((const T*)a.q + tok * a.q_row_stride + (int64_t)h * D, x, y);
+    if constexpr (TABLE) {
+      float o[8];
+      turn_ops(x, y, o);
+      store8<T>((T*)a.q_out + tok * a.q_out_row_stride + (int64_t)h * D + d0, o);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = d0 + i < R ? __builtin_fmaf(y[i], s32[i], x[i] * c32[i]) : x[i];
+      store8<T>((T*)a.q_out + tok * a.q_out_row_stride + (int64_t)h * D + d0, x);
+    }
+  }
+  if (!kv_ok) return;
+  // the first of k's passes goes to the part after q's last, so that few parts have more than one
+  for (int g = (part + gridDim.y - nq % gridDim.y) % gridDim.y; g < 2 * nk; g += gridDim.y) {
+    const bool is_v = g >= nk;
+    const int h = (is_v ? g - nk : g) * hpi + hl;
+    if (hl >= hpi || h >= a.num_kv_heads) continue;
+    float x[8], y[8];
+    if (is_v) {
+      load8<T>((const T*)a.v + tok * a.v_row_stride + (int64_t)h * D + d0, x);
+    } else {
+      pair8((const T*)a.k + tok * a.k_row_stride + (int64_t)h * D, x, y);
+      if constexpr (TABLE) {
+        float o[8];
+        turn_ops(x, y, o);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = o[i];
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const int d = d0 + i;
-          y[i] = (float)row[d < half ? d + half : (d < R ? d - half : d)];
+          const int pr = pair_of(d0 + i);
+          if (pr < 0) continue;
+          const double c = cs[wave][pair_at(pr)][0], sn = cs[wave][pair_at(pr)][1] * (double)flip(d0 + i);
+          const double d = __builtin_fma((double)y[i], sn, (double)x[i] * c);
+          x[i] = std::is_same<KV, float>::value ? (float)d : to_odd(d);
         }
       }
-    };
-    auto turn_ops = [&](const float* x, const float* y, float* o) {     // each op rounded to T
-      const bool first = d0 < half;
-#pragma unroll
-      for (int i = 0; i < 8; i += 2) {
-        float u0 = rnd<T>(__fmul_rn(x[i], c32[i])), v0 = rnd<T>(__fmul_rn(y[i], s32[i]));
-        float u1 = rnd<T>(__fmul_rn(x[i + 1], c32[i + 1])), v1 = rnd<T>(__fmul_rn(y[i + 1], s32[i + 1]));
-        if constexpr (std::is_same<T, _Float16>::value) opaque4(u0, v0, u1, v1);
-        o[i] = rnd<T>(first ? __fsub_rn(u0, v0) : __fadd_rn(u0, v0));
-        o[i + 1] = rnd<T>(first ? __fsub_rn(u1, v1) : __fadd_rn(u1, v1));
-      }
-    };
-
-    for (int g = part; g < nq + 2 * nk; g += a.parts) {
-      const bool is_q = g < nq, is_v = g >= nq + nk;
-      const int h = (is_q ? g : (is_v ? g - nq - nk : g - nq)) * hpi + hl;
-      if (hl >= hpi || h >= (is_q ? a.num_q_heads : a.num_kv_heads)) continue;
-      float x[8], y[8];
-      if (is_q) {
-        pair8((const T*)a.q + tok * a.q_row_stride + (int64_t)h * D, x, y);
-        if constexpr (TABLE) {
-          float o[8];
-          turn_ops(x, y, o);
-          store8<T>((T*)a.q_out + tok * a.q_out_row_stride + (int64_t)h * D + d0, o);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = d0 + i < R ? __builtin_fmaf(y[i], s32[i], x[i] * c32[i]) : x[i];
-          store8<T>((T*)a.q_out + tok * a.q_out_row_stride + (int64_t)h * D + d0, x);
-        }
-        continue;
-      }
-      if (!kv_ok) continue;
-      if (is_v) {
-        load8<T>((const T*)a.v + tok * a.v_row_stride + (int64_t)h * D + d0, x);
-      } else {
-        pair8((const T*)a.k + tok * a.k_row_stride + (int64_t)h * D, x, y);
-        if constexpr (TABLE) {
-          float o[8];
-          turn_ops(x, y, o);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = o[i];
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const double d = __builtin_fma((double)y[i], s[i], (double)x[i] * c[i]);
-            x[i] = d0 + i >= R ? x[i] : (std::is_same<KV, float>::value ? (float)d : to_odd(d));
-          }
-        }
-      }
-      void* const cache = is_v ? a.v_cache : a.k_cache;
-      if constexpr (std::is_same<KV, kv4>::value) {
-        const int64_t blk = slot / a.block_size, off = slot - blk * a.block_size;
-        uint8_t* const rec = (uint8_t*)cache + blk * a.cache_slot_stride + (int64_t)h * a.kv4_record;
-        uint32_t byte;
-        const uint32_t w = encode4(x, &byte);
-        *reinterpret_cast<uint32_t*>(rec + off * (D / 2) + 4 * ch) = w;
-        if ((ch & 3) == 0) rec[(int64_t)a.block_size * (D / 2) + off * (D / 32) + ch / 4] = (uint8_t)byte;
-      } else {
-        store8<KV>((KV*)cache + slot * a.cache_slot_stride + (int64_t)h * D + d0, x);
-      }
+    }
+    void* const cache = is_v ? a.v_cache : a.k_cache;
+    if constexpr (std::is_same<KV, kv4>::value) {
+      uint8_t* const rec = (uint8_t*)cache + (int64_t)h * a.kv4_record;
+      uint32_t byte;
+      const uint32_t w = encode4(x, &byte);
+      *reinterpret_cast<uint32_t*>(rec + at + 4 * ch) = w;
+      if ((ch & 3) == 0) rec[sc_at + ch / 4] = (uint8_t)byte;
+    } else {
+      store8<KV>((KV*)cache + at + (int64_t)h * D + d0, x);
     }
   }
 }
@@ -315,16 +324,16 @@ static hipError_t launch_rotary_t(const RotaryWriteArgs& a, dim3 grid, hipStream
   return hipGetLastError();
 }
 
-hipError_t launch_rotary_write(RotaryWriteArgs a, int cus, hipStream_t st) {
+hipError_t launch_rotary_write(const RotaryWriteArgs& a, int cus, hipStream_t st) {
   const int hpi = 64 / (a.head_dim / 8);
   const int passes = (a.q_out ? (a.num_q_heads + hpi - 1) / hpi : 0) + (a.k ? 2 * ((a.num_kv_heads + hpi - 1) / hpi) : 0);
   if (a.num_tokens == 0 || passes == 0) return hipSuccess;
   // few tokens: their passes go to several waves, up to two per SIMD
   const int64_t want = (int64_t)cus * 8 / a.num_tokens;
-  a.parts = (int)(want < 1 ? 1 : (want > passes ? passes : want));
-  int64_t blocks = (a.num_tokens * a.parts + kRotWaves - 1) / kRotWaves;
-  if (blocks > 65536) blocks = 65536;
-  const dim3 grid((unsigned)blocks);
+  const int parts = (int)(want < 1 ? 1 : (want > passes ? passes : want));
+  const int64_t blocks = (a.num_tokens + kRotWaves - 1) / kRotWaves;
+  if (blocks > 0x7fffffff / kRotWaves / 64) return hipErrorInvalidValue;   // the grid's threads
+  const dim3 grid((unsigned)blocks, (unsigned)parts);
   switch (a.dtype) {
     case kF32: return launch_rotary_t<float>(a, grid, st);
     case kBF16: return launch_rotary_t<__bf16>(a, grid, st);

@@ -72,24 +72,25 @@ def kv4_record_bytes(block_size: int, head_dim: int) -> int:
     return -(-block_size * (head_dim // 32 * 17) // 16) * 16
 
 
-def _kv4_block_size(cache: torch.Tensor, D: int) -> int:
-    """The block size whose records a 4-bit cache of head dim D holds (the
-    padding is shorter than a key's bytes)."""
-    if cache.dtype != KV4 or cache.dim() != 3 or D <= 0 or D % 32 or cache.shape[2] < D // 32 * 17:
-        raise ValueError(f"expected a 4-bit cache of head_dim {D}, uint8 [num_blocks, Hkv, record bytes] (head_dim a "
-                         f"multiple of 32), got {cache.dtype} {tuple(cache.shape)}")
-    return cache.shape[2] // (D // 32 * 17)
+def _kv4_block_size(cache: torch.Tensor, Hkv: int, D: int, name: str = "cache") -> int:
+    """The block size of a 4-bit cache of Hkv heads of D, after a check of its
+    layout (a record's padding is shorter than a key's bytes)."""
+    shape, unit = cache.shape, D // 32 * 17
+    if cache.dtype == KV4 and len(shape) == 3 and shape[1] == Hkv and D > 0 and D % 32 == 0 and shape[2] >= unit:
+        bs, rec = shape[2] // unit, shape[2]
+        if -(-bs * unit // 16) * 16 == rec and cache.stride()[1:] == (rec, 1):
+            return bs
+    raise ValueError(f"{name}: expected a 4-bit cache of head_dim {D} (a multiple of 32), uint8 [num_blocks, {Hkv}, record "
+                     f"bytes] with contiguous blocks, got {cache.dtype} {tuple(shape)}")
 
 
 def _kv4_blocks(k_cache: torch.Tensor, v_cache: torch.Tensor, Hkv: int, D: int, block_size: int) -> int:
-    """Blocks of a 4-bit cache pair, after a check of its layout."""
-    rec = kv4_record_bytes(block_size, D)
+    """Blocks of a 4-bit cache pair of a plan's block size."""
     for t, nm in ((k_cache, "k_cache"), (v_cache, "v_cache")):
-        if t.dtype != KV4 or t.dim() != 3 or t.shape[1:] != (Hkv, rec) or t.stride()[1:] != (rec, 1):
-            raise ValueError(f"{nm}: expected a 4-bit cache, uint8 [num_blocks, {Hkv}, {rec}] with contiguous blocks "
-                             f"(block_size {block_size}, head_dim {D}), got {t.dtype} {tuple(t.shape)}")
-    if k_cache.shape[0] != v_cache.shape[0] or k_cache.stride(0) != v_cache.stride(0):
-        raise ValueError("k_cache and v_cache must have the same shape and block stride")
+        if _kv4_block_size(t, Hkv, D, nm) != block_size:
+            raise ValueError(f"{nm}: blocks of {t.shape[2] // (D // 32 * 17)} rows, the plan's have {block_size}")
+    if k_cache.shape[0] != v_cache.shape[0]:
+        raise ValueError("k_cache and v_cache must have the same shape")
     return k_cache.shape[0]
 
 
@@ -117,7 +118,7 @@ def rope_kv_write(k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torc
     vs = _rows(v, Hkv, D, "v")
     n = k.numel() // (Hkv * D)
     if k_cache.dtype == KV4:
-        bs = _kv4_block_size(k_cache, D)
+        bs = _kv4_block_size(k_cache, Hkv, D, "k_cache")
         num_slots = _kv4_blocks(k_cache, v_cache, Hkv, D, bs) * bs
     else:
         _cache_rows(k_cache, v_cache, Hkv, D)
@@ -164,10 +165,17 @@ def rope_kv_write(k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torc
         _lib.dtype_code(k.dtype), _lib.dtype_code(k_cache.dtype), _lib.stream_ptr(dev)))
 
 
-def _same_device(dev: torch.device, **tensors) -> None:
+def _same_device(index: int, **tensors) -> None:
     for name, t in tensors.items():
-        if t is not None and t.device != dev:
-            raise ValueError(f"{name} is on {t.device}, the call on {dev}")
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"{name} is on {t.device}, the call on device {index}")
+
+
+def _row_stride(t: torch.Tensor, shape, heads: int, head_dim: int, name: str) -> int:
+    """:func:`_rows`, without its look at the strides of contiguous rows."""
+    if len(shape) >= 3 and shape[-1] == head_dim and shape[-2] == heads and t.is_contiguous():
+        return heads * head_dim
+    return _rows(t, heads, head_dim, name)
 
 
 def rotary_kv_write(k: torch.Tensor | None, v: torch.Tensor | None, positions: torch.Tensor, rotary,
@@ -187,57 +195,70 @@ def rotary_kv_write(k: torch.Tensor | None, v: torch.Tensor | None, positions: t
     x = q if k is None else k
     if x is None or (k is None) != (v is None) or (q is None) != (q_out is None):
         raise ValueError("k and v, and q and q_out, go together; at least one pair is needed")
-    D, dev = x.shape[-1], x.device
+    shape, dtype, dev = x.shape, x.dtype, x.get_device()
+    D, H = shape[-1], shape[-2]
     if D != rotary.head_dim:
         raise ValueError(f"head_dim {D}, the rotary positions are for {rotary.head_dim}")
-    _same_device(dev, v=v, q=q, q_out=q_out, positions=positions, freq=rotary.freq, k_cache=k_cache, v_cache=v_cache,
-                 slot_mapping=slot_mapping, query_lens=query_lens)
-    H = x.shape[-2]
     n = x.numel() // (H * D)
-    pos = _index_rows(positions)
+    freq = rotary.freq
+    pos = positions if positions.dim() == 1 and positions.dtype == torch.int64 and positions.is_contiguous() \
+        else _index_rows(positions)
     if positions.dtype.is_floating_point or pos.numel() != n:
         raise ValueError("positions must be integers, one per token")
     ks = vs = qs = qos = stride = num_slots = bs = 0
     Hq = Hkv = 1
-    kv_code, sm = _lib.DTYPE_F32, None
+    kp = vp = kcp = vcp = smp = qp = qop = qlp = None
+    kv_code, tps = _lib.DTYPE_F32, 0
+    same = pos.get_device() == dev and freq.get_device() == dev
     if k is not None:
         if k_cache is None or v_cache is None or slot_mapping is None:
             raise ValueError("k and v need caches and a slot mapping")
         Hkv = H
-        if v.shape != k.shape or v.dtype != k.dtype:
+        if v.shape != shape or v.dtype != dtype:
             raise ValueError("k and v shapes or dtypes differ")
-        ks, vs = _rows(k, Hkv, D, "k"), _rows(v, Hkv, D, "v")
-        if k_cache.dtype == KV4:
-            bs = _kv4_block_size(k_cache, D)
-            num_slots = _kv4_blocks(k_cache, v_cache, Hkv, D, bs) * bs
+        ks, vs = _row_stride(k, shape, Hkv, D, "k"), _row_stride(v, shape, Hkv, D, "v")
+        cdtype, cshape, cstride = k_cache.dtype, k_cache.shape, k_cache.stride()
+        if v_cache.shape != cshape or v_cache.stride() != cstride or v_cache.dtype != cdtype:
+            raise ValueError("k_cache and v_cache must have the same shape, dtype and strides")
+        if cdtype == KV4:
+            bs = _kv4_block_size(k_cache, Hkv, D, "k_cache")
+            num_slots = cshape[0] * bs
+            kv_code = _lib.DTYPE_MXFP4
         else:
-            _cache_rows(k_cache, v_cache, Hkv, D)
-            num_slots = k_cache.shape[0]
-        if k_cache.shape != v_cache.shape or k_cache.stride(0) != v_cache.stride(0) or k_cache.dtype != v_cache.dtype:
-            raise ValueError("k_cache and v_cache must have the same shape, dtype and slot stride")
+            if len(cshape) != 3 or cshape[1] != Hkv or cshape[2] != D or cstride[1:] != (D, 1):
+                raise ValueError(f"k_cache and v_cache: expected [num_slots, {Hkv}, {D}] with contiguous rows")
+            num_slots = cshape[0]
+            kv_code = _lib.dtype_code(cdtype)
+        stride = cstride[0]
         sm = slot_mapping if slot_mapping.dim() == 1 else slot_mapping.reshape(-1)
         if sm.dtype != torch.int64 or sm.numel() != n or not sm.is_contiguous():
             raise ValueError("slot_mapping must be contiguous int64 with one entry per token")
-        stride, kv_code = k_cache.stride(0), _kv_code(k_cache)
+        same = same and v.get_device() == dev and k_cache.get_device() == dev and v_cache.get_device() == dev \
+            and sm.get_device() == dev
+        kp, vp, kcp, vcp, smp = k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), sm.data_ptr()
     if q is not None:
-        Hq = q.shape[-2]
-        if q.dtype != x.dtype or q_out.dtype != x.dtype or q.numel() != n * Hq * D or q_out.numel() != q.numel():
+        qshape, oshape = q.shape, q_out.shape
+        Hq = qshape[-2]
+        if q.dtype != dtype or q_out.dtype != dtype or q.numel() != n * Hq * D or q_out.numel() != n * Hq * D:
             raise ValueError("q and q_out need the model dtype and one row per token")
-        qs, qos = _rows(q, Hq, D, "q"), _rows(q_out, Hq, D, "q_out")
-    tps, ql = 0, None
+        qs, qos = _row_stride(q, qshape, Hq, D, "q"), _row_stride(q_out, oshape, Hq, D, "q_out")
+        same = same and q.get_device() == dev and q_out.get_device() == dev
+        qp, qop = q.data_ptr(), q_out.data_ptr()
     if query_lens is not None:
         ql = query_lens.to(torch.int32).contiguous()
         if ql.numel() == 0 or n % ql.numel():
             raise ValueError("query_lens: the tokens must be as many rows for each sequence")
-        tps = n // ql.numel()
+        same = same and ql.get_device() == dev
+        tps, qlp = n // ql.numel(), ql.data_ptr()
+    if not same:
+        _same_device(dev, v=v, q=q, q_out=q_out, positions=positions, freq=freq, k_cache=k_cache, v_cache=v_cache,
+                     slot_mapping=slot_mapping, query_lens=query_lens)
     if n == 0:
         return
-    lib = _lib.load()
-    _lib.check(lib.gllm_rotary_kv_write(
-        _lib.ptr(q), _lib.ptr(q_out), _lib.ptr(k), _lib.ptr(v), _lib.ptr(k_cache), _lib.ptr(v_cache), _lib.ptr(sm),
-        _lib.ptr(ql), tps, rotary.freq.data_ptr(), rotary.factor, pos.data_ptr(), rotary.rotary_dim,
-        int(rotary.interleaved), n, Hq, Hkv, D, qs, ks, vs, qos, stride, num_slots, bs, _lib.dtype_code(x.dtype),
-        kv_code, _lib.stream_ptr(dev)))
+    _lib.check(_lib.load().gllm_rotary_kv_write(
+        qp, qop, kp, vp, kcp, vcp, smp, qlp, tps, freq.data_ptr(), rotary.factor, pos.data_ptr(), rotary.rotary_dim,
+        rotary.interleaved, n, Hq, Hkv, D, qs, ks, vs, qos, stride, num_slots, bs, _lib.dtype_code(dtype), kv_code,
+        _lib.stream_ptr(x.device)))
 
 
 def rotary_rotate(x: torch.Tensor, positions: torch.Tensor, rotary, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -254,16 +275,16 @@ def kv4_values(cache: torch.Tensor, slots: torch.Tensor, head_dim: int, dtype: t
     """Rows of a 4-bit cache (:data:`KV4`) as the values they stand for, in
     ``dtype``: ``[N, Hkv, head_dim]`` for int64 ``slots [N]`` (zeros for a slot
     outside the cache).  For moving rows to another cache or looking at them."""
-    bs = _kv4_block_size(cache, head_dim)
-    Hkv = cache.shape[1]
-    nb = _kv4_blocks(cache, cache, Hkv, head_dim, bs)
+    nb, Hkv = cache.shape[0], cache.shape[1] if cache.dim() == 3 else 0
+    bs = _kv4_block_size(cache, Hkv, head_dim)
     sl = _index_rows(slots)
-    _same_device(cache.device, slots=slots, out=out)
+    if sl.get_device() != cache.get_device() or out is not None and out.get_device() != cache.get_device():
+        raise ValueError(f"slots and out must be on the cache's device {cache.device}")
     if out is None:
         out = torch.empty(sl.numel(), Hkv, head_dim, dtype=dtype, device=cache.device)
     elif out.dtype != dtype or out.numel() != sl.numel() * Hkv * head_dim:
         raise ValueError(f"out must be {dtype} with one row per slot")
-    stride = _rows(out, Hkv, head_dim, "out")
+    stride = _row_stride(out, out.shape, Hkv, head_dim, "out")
     if sl.numel() == 0:
         return out
     _lib.check(_lib.load().gllm_kv4_values(cache.data_ptr(), cache.stride(0), nb * bs, bs, sl.data_ptr(), sl.numel(), Hkv,
