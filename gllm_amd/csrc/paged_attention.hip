@@ -40,9 +40,10 @@ __device__ __forceinline__ void rope8(float* x1, float* x2, const float* c, cons
 constexpr int kWaves = 8;   // waves per workgroup (both paths; one block size)
 
 template <int D, int NW, int KF> struct DecodeCfg {
-  static constexpr int kPF = KF == kKV4 ? 4 : 2;        // sub-tiles in flight per wave (16-bit: 2 beat 3 at D = 64)
+  static constexpr int kPF = 2;                         // steps in flight per wave (16-bit: 2 beat 3 at D = 64)
+  static constexpr int kNS = KF == kKV4 ? 2 : 1;        // 16-key sub-tiles of a step
   static constexpr int kRowBytes = D * 2 + 32;         // V staging row stride (bytes)
-  static constexpr int kVBytes = 16 * kRowBytes;       // per-wave V staging: 16 keys
+  static constexpr int kVBytes = kNS * 16 * kRowBytes; // per-wave V staging: a step's keys
   static constexpr int kMaxBlocks = 512;               // block ids of one split, cached in LDS
   static constexpr int kStage = NW * kVBytes + kMaxBlocks * 4;
   static constexpr int kMerge = NW * 16 * (D + 2) * 4;       // per-wave (acc, m, l), 16 rows
@@ -78,10 +79,8 @@ __device__ __forceinline__ int chunk_dim(int kk, int grp) {
   return KF == kKV8 ? 64 * (kk >> 1) + 16 * grp + 8 * (kk & 1) : 32 * kk + 8 * grp;
 }
 template <typename T, int KF>
-__device__ __forceinline__ u32x4 chunk_elems(const u32x4* raw, float scale, int kk) {
-  if constexpr (KF == kKV4) {
-    return fp4x8_to<T>(raw[0][kk], scale);
-  } else if constexpr (KF == kKV8) {
+__device__ __forceinline__ u32x4 chunk_elems(const u32x4* raw, int kk) {
+  if constexpr (KF == kKV8) {
     const u32x4 w = raw[kk >> 1];
     return (kk & 1) ? fp8x8_to<T>(w[2], w[3]) : fp8x8_to<T>(w[0], w[1]);
   } else {
@@ -301,32 +300,133 @@ __device__ __forceinline__ void decode_task(const AttnArgs& a, const DecodeTask&
 #pragma unroll
   for (int d = 0; d < ND; ++d) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  // this wave's sub-tiles: j = ki + KW * t, t < ntw
-  const int ntw = head_ok && nsub > ki ? (nsub - ki + KW - 1) / KW : 0;
-  u32x4 kr[PF + 1][NL], vr[PF + 1][NL];
-  uint32_t ksr[KF == kKV4 ? PF + 1 : 1], vsr[KF == kKV4 ? PF + 1 : 1];   // 4-bit: the scale bytes
-  auto issue = [&](int t, u32x4 (&kd)[NL], u32x4 (&vd)[NL], int slot_i) {
-    // ring padding (t >= ntw): every lane reads the task's last slot, one
-    // cache line per load instead of a whole 16-key tile
-    const int v = t < ntw ? min(kbeg + 16 * (ki + KW * t) + n, kend - 1) : kend - 1;
-    const int key = WIN ? seen_key(key_of(v), sk, a.sinks) : v;
-    const int blk = WIN && both && v >= sk.from ? blk0 + bgap : blk0;
-    const uint32_t bi = div_bs((uint32_t)key, a.block_magic, a.block_shift);
-    if constexpr (KF == kKV4) {
-      const uint32_t o = (uint32_t)key - bi * (uint32_t)a.block_size;
-      const uint64_t off = (uint64_t)(uint32_t)lbid[bi - blk] * sbytes;
-      const uint64_t code = off + o * (D / 2), sc = off + sc_off + o * (D / 32);
-      if constexpr (D == 128) {
-        kd[0] = ld16(kc + code);
-        vd[0] = ld16(vc + code);
-      } else {
-        const u32x2 k2 = *reinterpret_cast<const u32x2*>(kc + code), v2 = *reinterpret_cast<const u32x2*>(vc + code);
-        kd[0] = u32x4{k2[0], k2[1], 0u, 0u};
-        vd[0] = u32x4{v2[0], v2[1], 0u, 0u};
+  if constexpr (KF == kKV4) {
+    // 4-bit cache: steps of 32 keys (two 16-key sub-tiles), so that one pass of
+    // the softmax and one chain of its latencies serve twice the keys: a step is
+    // 2 x 1088 bytes at D = 128, little to load, and P V takes both sub-tiles in
+    // one 16x16x32 MFMA per 16 dims.  Element i of its k = 8 grp + i is key 4 grp +
+    // i of sub-tile 0 (i < 4) or 4 grp + i - 4 of sub-tile 1, which is how the score
+    // registers already lie.
+    const int ntw = head_ok && nsub > 2 * ki ? ((nsub + 1) / 2 - ki + KW - 1) / KW : 0;
+    struct Step {
+      u32x4 k[2], v[2];
+      uint32_t ks[2], vs[2];
+    } ring[PF + 1];
+    auto issue = [&](int t, Step& x) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int v = t < ntw ? min(kbeg + 32 * (ki + KW * t) + 16 * u + n, kend - 1) : kend - 1;
+        const int key = seen_key(key_of(v), sk, a.sinks);
+        const int blk = both && v >= sk.from ? blk0 + bgap : blk0;
+        const uint32_t bi = div_bs((uint32_t)key, a.block_magic, a.block_shift);
+        const uint32_t o = (uint32_t)key - bi * (uint32_t)a.block_size;
+        const uint64_t off = (uint64_t)(uint32_t)lbid[bi - blk] * sbytes;
+        const uint64_t code = off + o * (D / 2), sc = off + sc_off + o * (D / 32);
+        if constexpr (D == 128) {
+          x.k[u] = ld16(kc + code);
+          x.v[u] = ld16(vc + code);
+        } else {
+          const u32x2 k2 = *reinterpret_cast<const u32x2*>(kc + code), v2 = *reinterpret_cast<const u32x2*>(vc + code);
+          x.k[u] = u32x4{k2[0], k2[1], 0u, 0u};
+          x.v[u] = u32x4{v2[0], v2[1], 0u, 0u};
+        }
+        x.ks[u] = (uint8_t)kc[sc];
+        x.vs[u] = (uint8_t)vc[sc];
       }
-      ksr[slot_i] = (uint8_t)kc[sc];
-      vsr[slot_i] = (uint8_t)vc[sc];
-    } else {
+    };
+    auto compute = [&](int t, const Step& x) {
+      const int kb = t < ntw ? kbeg + 32 * (ki + KW * t) : kend;   // past the last one: fully masked
+      f32x4 s[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kk = 0; kk < NK; ++kk)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          s[u] = E16<T>::mfma16(fp4x8_to<T>(x.k[u][kk], __uint_as_float(x.ks[u] << 23)), qB[kk], s[u]);
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk)
+          *reinterpret_cast<u32x4*>(ldsV + (16 * u + n) * RB + chunk_dim<D, KF>(kk, grp) * 2) =
+              fp4x8_to<T>(x.v[u][kk], __uint_as_float(x.vs[u] << 23));
+      // lane holds S[key kb + 16u + 4grp + j][row n]
+      float p[2][4];
+      float tmax = kNegInf;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int vb = kb + 16 * u, kr = key_of(vb);   // a sub-tile lies on one side of the left-out keys
+#pragma unroll
+        for (int j = 0; j < 4; ++j) p[u][j] = s[u][j] * sl2;
+        // past the range, past the first row, or before the last row's window
+        if (vb + 16 > kend || kr + 15 > tk.ctx_len || (kr <= tk.ctx_len + tk.q_len - 1 - a.window && kr + 16 > a.sinks)) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int key = kr + 4 * grp + j;
+            if (vb + 4 * grp + j >= kend || key > vis || (key <= vis - a.window && key >= a.sinks)) p[u][j] = kNegInf;
+          }
+        }
+        tmax = fmaxf(tmax, fmaxf(fmaxf(p[u][0], p[u][1]), fmaxf(p[u][2], p[u][3])));
+      }
+      tmax = max_xor32(max_xor16(tmax));
+      if (__builtin_amdgcn_ballot_w64(tmax > m + 8.f)) {   // lazy rescale, as above
+        const float mn = tmax > m + 8.f ? tmax : m;
+        const float alpha = fast_exp2(m - (mn == kNegInf ? 0.f : mn));
+        lsum *= alpha;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) acc[d] *= alpha;
+        m = mn;
+      }
+      const float mu = m == kNegInf ? 0.f : m;
+      u32x4 pb;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) p[u][j] = fast_exp2(p[u][j] - mu);
+        pb[2 * u] = E16<T>::pack2(p[u][0], p[u][1]);
+        pb[2 * u + 1] = E16<T>::pack2(p[u][2], p[u][3]);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) lsum = E16<T>::add2(pb[e], lsum);   // the rounded p the MFMA sees
+      const char* vrow = ldsV + (4 * grp + (n >> 2)) * RB + 4 * (n & 3) * 2;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        const u32x2 r0 = lds_read_tr16(vrow + 32 * d), r1 = lds_read_tr16(vrow + 16 * RB + 32 * d);
+        acc[d] = E16<T>::mfma16(u32x4{r0[0], r0[1], r1[0], r1[1]}, pb, acc[d]);
+      }
+    };
+    // the same load order on every path, as below
+    if (ntw > 0) {
+#pragma unroll
+      for (int u = 0; u < PF; ++u) {
+        issue(u, ring[u]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      int t0 = 0;
+      for (; t0 + PF < ntw; t0 += PF + 1) {
+#pragma unroll
+        for (int u = 0; u <= PF; ++u) {
+          issue(t0 + u + PF, ring[(u + PF) % (PF + 1)]);
+          __builtin_amdgcn_sched_barrier(0);
+          compute(t0 + u, ring[u]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < PF; ++u)
+        if (t0 + u < ntw) compute(t0 + u, ring[u]);
+    }
+  } else {
+    // this wave's sub-tiles: j = ki + KW * t, t < ntw
+    const int ntw = head_ok && nsub > ki ? (nsub - ki + KW - 1) / KW : 0;
+    u32x4 kr[PF + 1][NL], vr[PF + 1][NL];
+    auto issue = [&](int t, u32x4 (&kd)[NL], u32x4 (&vd)[NL]) {
+      // ring padding (t >= ntw): every lane reads the task's last slot, one
+      // cache line per load instead of a whole 16-key tile
+      const int v = t < ntw ? min(kbeg + 16 * (ki + KW * t) + n, kend - 1) : kend - 1;
+      const int key = WIN ? seen_key(key_of(v), sk, a.sinks) : v;
+      const int blk = WIN && both && v >= sk.from ? blk0 + bgap : blk0;
+      const uint32_t bi = div_bs((uint32_t)key, a.block_magic, a.block_shift);
       const uint32_t slot = (uint32_t)lbid[bi - blk] * (uint32_t)a.block_size + ((uint32_t)key - bi * (uint32_t)a.block_size);
       const uint64_t off = (uint64_t)slot * sbytes;
 #pragma unroll
@@ -334,94 +434,88 @@ __device__ __forceinline__ void decode_task(const AttnArgs& a, const DecodeTask&
         kd[l] = ld16(kc + off + 64 * l);
         vd[l] = ld16(vc + off + 64 * l);
       }
-    }
-  };
-  auto compute = [&](int t, const u32x4 (&kd)[NL], const u32x4 (&vd)[NL], int slot_i) {
-    // tiles past the last one (ring padding) are fully masked
-    const int kb = t < ntw ? kbeg + 16 * (ki + KW * t) : kend;
-    float ks = 1.f, vs = 1.f;
-    if constexpr (KF == kKV4) {
-      ks = __uint_as_float(ksr[slot_i] << 23);
-      vs = __uint_as_float(vsr[slot_i] << 23);
-    }
-    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+    };
+    auto compute = [&](int t, const u32x4 (&kd)[NL], const u32x4 (&vd)[NL]) {
+      // tiles past the last one (ring padding) are fully masked
+      const int kb = t < ntw ? kbeg + 16 * (ki + KW * t) : kend;
+      f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int kk = 0; kk < NK; ++kk) s = E16<T>::mfma16(chunk_elems<T, KF>(kd, ks, kk), qB[kk], s);
+      for (int kk = 0; kk < NK; ++kk) s = E16<T>::mfma16(chunk_elems<T, KF>(kd, kk), qB[kk], s);
 #pragma unroll
-    for (int kk = 0; kk < NK; ++kk)
-      *reinterpret_cast<u32x4*>(ldsV + n * RB + chunk_dim<D, KF>(kk, grp) * 2) = chunk_elems<T, KF>(vd, vs, kk);
-    // lane holds S[key kb + 4grp + j][row n]
-    float p[4];
+      for (int kk = 0; kk < NK; ++kk)
+        *reinterpret_cast<u32x4*>(ldsV + n * RB + chunk_dim<D, KF>(kk, grp) * 2) = chunk_elems<T, KF>(vd, kk);
+      // lane holds S[key kb + 4grp + j][row n]
+      float p[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) p[j] = s[j] * sl2;
-    if constexpr (WIN) {
-      const int kr = key_of(kb);            // a sub-tile lies on one side of the left-out keys
-      // past the range, past the first row, or before the last row's window
-      if (kb + 16 > kend || kr + 15 > tk.ctx_len || (kr <= tk.ctx_len + tk.q_len - 1 - a.window && kr + 16 > a.sinks)) {
+      for (int j = 0; j < 4; ++j) p[j] = s[j] * sl2;
+      if constexpr (WIN) {
+        const int kr = key_of(kb);            // a sub-tile lies on one side of the left-out keys
+        // past the range, past the first row, or before the last row's window
+        if (kb + 16 > kend || kr + 15 > tk.ctx_len || (kr <= tk.ctx_len + tk.q_len - 1 - a.window && kr + 16 > a.sinks)) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int key = kr + 4 * grp + j;
+            if (kb + 4 * grp + j >= kend || key > vis || (key <= vis - a.window && key >= a.sinks)) p[j] = kNegInf;
+          }
+        }
+      } else if (kb + 16 > kend || kb + 15 > tk.ctx_len) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int key = kr + 4 * grp + j;
-          if (kb + 4 * grp + j >= kend || key > vis || (key <= vis - a.window && key >= a.sinks)) p[j] = kNegInf;
+          const int key = kb + 4 * grp + j;
+          if (key >= kend || key > vis) p[j] = kNegInf;
         }
       }
-    } else if (kb + 16 > kend || kb + 15 > tk.ctx_len) {
+      float tmax = fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3]));
+      tmax = max_xor32(max_xor16(tmax));
+      // Lazy rescale: the running max only moves when a row's tile max exceeds
+      // it by more than 8 (log2 units), so p <= 2^8 and most tiles skip the
+      // acc rescale.  Numerator and denominator share m, so the result is exact.
+      if (__builtin_amdgcn_ballot_w64(tmax > m + 8.f)) {
+        const float mn = tmax > m + 8.f ? tmax : m;
+        const float alpha = fast_exp2(m - (mn == kNegInf ? 0.f : mn));
+        lsum *= alpha;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int key = kb + 4 * grp + j;
-        if (key >= kend || key > vis) p[j] = kNegInf;
+        for (int d = 0; d < ND; ++d) acc[d] *= alpha;
+        m = mn;
       }
-    }
-    float tmax = fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3]));
-    tmax = max_xor32(max_xor16(tmax));
-    // Lazy rescale: the running max only moves when a row's tile max exceeds
-    // it by more than 8 (log2 units), so p <= 2^8 and most tiles skip the
-    // acc rescale.  Numerator and denominator share m, so the result is exact.
-    if (__builtin_amdgcn_ballot_w64(tmax > m + 8.f)) {
-      const float mn = tmax > m + 8.f ? tmax : m;
-      const float alpha = fast_exp2(m - (mn == kNegInf ? 0.f : mn));
-      lsum *= alpha;
+      const float mu = m == kNegInf ? 0.f : m;
 #pragma unroll
-      for (int d = 0; d < ND; ++d) acc[d] *= alpha;
-      m = mn;
-    }
-    const float mu = m == kNegInf ? 0.f : m;
+      for (int j = 0; j < 4; ++j) p[j] = fast_exp2(p[j] - mu);
+      const u32x2 pb = {E16<T>::pack2(p[0], p[1]), E16<T>::pack2(p[2], p[3])};
+      lsum = E16<T>::add2(pb[1], E16<T>::add2(pb[0], lsum));   // the rounded p the MFMA sees
+      const char* vrow = ldsV + (4 * grp + (n >> 2)) * RB + 4 * (n & 3) * 2;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) p[j] = fast_exp2(p[j] - mu);
-    const u32x2 pb = {E16<T>::pack2(p[0], p[1]), E16<T>::pack2(p[2], p[3])};
-    lsum = E16<T>::add2(pb[1], E16<T>::add2(pb[0], lsum));   // the rounded p the MFMA sees
-    const char* vrow = ldsV + (4 * grp + (n >> 2)) * RB + 4 * (n & 3) * 2;
-#pragma unroll
-    for (int d = 0; d < ND; ++d) acc[d] = E16<T>::mfma16k16(lds_read_tr16(vrow + 32 * d), pb, acc[d]);
-  };
+      for (int d = 0; d < ND; ++d) acc[d] = E16<T>::mfma16k16(lds_read_tr16(vrow + 32 * d), pb, acc[d]);
+    };
 
-  // The ring issues loads unconditionally (tiles past the end read one
-  // cached slot and are masked), so the in-flight load order is the same on
-  // every path and the compiler's waits keep PF tiles in flight while the
-  // current one is computed (conditional issues would make it wait for all
-  // of them); the tail after the last whole group issues nothing.
-  // sched_barrier keeps the scheduler from reordering the issues.
-  if (ntw > 0) {
+    // The ring issues loads unconditionally (tiles past the end read one
+    // cached slot and are masked), so the in-flight load order is the same on
+    // every path and the compiler's waits keep PF tiles in flight while the
+    // current one is computed (conditional issues would make it wait for all
+    // of them); the tail after the last whole group issues nothing.
+    // sched_barrier keeps the scheduler from reordering the issues.
+    if (ntw > 0) {
 #pragma unroll
-    for (int u = 0; u < PF; ++u) {
-      issue(u, kr[u], vr[u], u);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    int t0 = 0;
-    for (; t0 + PF < ntw; t0 += PF + 1) {   // whole groups: all PF + 1 computes are real tiles
-#pragma unroll
-      for (int u = 0; u <= PF; ++u) {
-        const int t = t0 + u;
-        constexpr int R = PF + 1;
-        issue(t + PF, kr[(u + PF) % R], vr[(u + PF) % R], (u + PF) % R);
-        __builtin_amdgcn_sched_barrier(0);
-        compute(t, kr[u], vr[u], u);
+      for (int u = 0; u < PF; ++u) {
+        issue(u, kr[u], vr[u]);
         __builtin_amdgcn_sched_barrier(0);
       }
-    }
-    // last ntw - t0 (<= PF) tiles: already in flight, nothing more to issue
+      int t0 = 0;
+      for (; t0 + PF < ntw; t0 += PF + 1) {   // whole groups: all PF + 1 computes are real tiles
 #pragma unroll
-    for (int u = 0; u < PF; ++u)
-      if (t0 + u < ntw) compute(t0 + u, kr[u], vr[u], u);
+        for (int u = 0; u <= PF; ++u) {
+          const int t = t0 + u;
+          issue(t + PF, kr[(u + PF) % (PF + 1)], vr[(u + PF) % (PF + 1)]);
+          __builtin_amdgcn_sched_barrier(0);
+          compute(t, kr[u], vr[u]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      // last ntw - t0 (<= PF) tiles: already in flight, nothing more to issue
+#pragma unroll
+      for (int u = 0; u < PF; ++u)
+        if (t0 + u < ntw) compute(t0 + u, kr[u], vr[u]);
+    }
   }
   float lt = sum_xor32(sum_xor16(lsum));
 
