@@ -363,7 +363,8 @@ __device__ __forceinline__ void decode_task(const AttnArgs& a, const DecodeTask&
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int key = kr + 4 * grp + j;
-            if (vb + 4 * grp + j >= kend || key > vis || (key <= vis - a.window && key >= a.sinks)) p[u][j] = kNegInf;
+            const bool hid = (vb + 4 * grp + j >= kend) | (key > vis) | ((key <= vis - a.window) & (key >= a.sinks));
+            p[u][j] = hid ? kNegInf : p[u][j];
           }
         }
         tmax = fmaxf(tmax, fmaxf(fmaxf(p[u][0], p[u][1]), fmaxf(p[u][2], p[u][3])));
@@ -455,7 +456,8 @@ __device__ __forceinline__ void decode_task(const AttnArgs& a, const DecodeTask&
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int key = kr + 4 * grp + j;
-            if (kb + 4 * grp + j >= kend || key > vis || (key <= vis - a.window && key >= a.sinks)) p[j] = kNegInf;
+            const bool hid = (kb + 4 * grp + j >= kend) | (key > vis) | ((key <= vis - a.window) & (key >= a.sinks));
+          p[j] = hid ? kNegInf : p[j];
           }
         }
       } else if (kb + 16 > kend || kb + 15 > tk.ctx_len) {
@@ -1014,7 +1016,7 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
         const int c = 8 * (j >> 2) + (j & 3);
-        s[j] = c > lim || (c <= lo && c >= sink) ? kNegInf : s[j];
+        s[j] = (c > lim) | ((c <= lo) & (c >= sink)) ? kNegInf : s[j];
       }
     } else {
 #pragma unroll
