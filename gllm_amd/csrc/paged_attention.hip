@@ -307,15 +307,68 @@ __device__ __forceinline__ void decode_task(const AttnArgs& a, const DecodeTask&
     // one 16x16x32 MFMA per 16 dims.  Element i of its k = 8 grp + i is key 4 grp +
     // i of sub-tile 0 (i < 4) or 4 grp + i - 4 of sub-tile 1, which is how the score
     // registers already lie.
-    const int ntw = head_ok && nsub > 2 * ki ? ((nsub + 1) / 2 - ki + KW - 1) / KW : 0;
+    //
+    // In blocks of a multiple of 16 rows a sub-tile lies in one block (ONE): lane i
+    // keeps the place of the wave's i-th sub-tile of the next 64, and a load takes
+    // it as a scalar base plus the lane's fixed offset.  The addresses were a third
+    // of a step's vector instructions (64 x 4,096 keys, 32 / 8 heads of 64:
+    // KV4_ONE us; elsewhere each lane finds its own key's row).
+    const int kis = __builtin_amdgcn_readfirstlane(ki);
+    const int ntw = __builtin_amdgcn_readfirstlane(head_ok && nsub > 2 * ki ? ((nsub + 1) / 2 - ki + KW - 1) / KW : 0);
     struct Step {
       u32x4 k[2], v[2];
       uint32_t ks[2], vs[2];
     } ring[PF + 1];
-    auto issue = [&](int t, Step& x) {
+    uint32_t place_lo = 0, place_hi = 0, place_row = 0;
+    const uint32_t code_l = n * (D / 2) + D / 8 * grp, sc_l = n * (D / 32) + D / 4 * grp / 32;
+    const char* const ks0 = (const char*)a.k_cache;
+    const char* const vs0 = (const char*)a.v_cache;
+    const int64_t head_s = (int64_t)__builtin_amdgcn_readfirstlane(head_ok ? kvh : 0) * a.kv4_record;
+    auto places = [&](int t) {             // of steps t .. t + 31
+      const int v = min(kbeg + 32 * (kis + KW * (t + (lane >> 1))) + 16 * (lane & 1), (kend - 1) & ~15);
+      const int blk = both && v >= sk.from ? blk0 + bgap : blk0;
+      const int key = key_of(v);
+      const uint32_t bi = div_bs((uint32_t)key, a.block_magic, a.block_shift);
+      place_row = (uint32_t)key - bi * (uint32_t)a.block_size;
+      const uint64_t at = (uint64_t)(uint32_t)lbid[bi - blk] * sbytes + head_s + place_row * (D / 2);
+      place_lo = (uint32_t)at;
+      place_hi = (uint32_t)(at >> 32);
+    };
+    auto issue_one = [&](int t, Step& x) {
+      if (t > 0 && (t & 31) == 0) places(t);
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const int v = t < ntw ? min(kbeg + 32 * (ki + KW * t) + 16 * u + n, kend - 1) : kend - 1;
+        const int i = 2 * (t & 31) + u;
+        const uint64_t at = (uint64_t)(uint32_t)__builtin_amdgcn_readlane(place_hi, i) << 32 |
+                            (uint32_t)__builtin_amdgcn_readlane(place_lo, i);
+        const uint32_t row = __builtin_amdgcn_readlane(place_row, i);
+        const uint64_t sc = at + (uint32_t)a.block_size * (D / 2) - row * (D / 2 - D / 32);   // the record's scales
+        const int v = min(kbeg + 32 * (kis + KW * t) + 16 * u, (kend - 1) & ~15), kr = key_of(v);
+        // the rows that may be read: none past the range (steps past the last one
+        // take one line), none between the sinks and the first row's window
+        const int last = t < ntw ? kend - 1 - v : 0;
+        uint32_t cl = code_l, sl = sc_l;
+        if (last < 15 || (kr < sk.first && kr + 15 >= a.sinks)) {
+          const int nn = seen_key(kr + min(n, last), sk, a.sinks) - kr;
+          cl += (nn - n) * (D / 2);
+          sl += (nn - n) * (D / 32);
+        }
+        if constexpr (D == 128) {
+          x.k[u] = ld16(ks0 + at + cl);
+          x.v[u] = ld16(vs0 + at + cl);
+        } else {
+          const u32x2 k2 = *reinterpret_cast<const u32x2*>(ks0 + at + cl), v2 = *reinterpret_cast<const u32x2*>(vs0 + at + cl);
+          x.k[u] = u32x4{k2[0], k2[1], 0u, 0u};
+          x.v[u] = u32x4{v2[0], v2[1], 0u, 0u};
+        }
+        x.ks[u] = (uint8_t)ks0[sc + sl];
+        x.vs[u] = (uint8_t)vs0[sc + sl];
+      }
+    };
+    auto issue_any = [&](int t, Step& x) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int v = t < ntw ? min(kbeg + 32 * (kis + KW * t) + 16 * u + n, kend - 1) : kend - 1;
         const int key = seen_key(key_of(v), sk, a.sinks);
         const int blk = both && v >= sk.from ? blk0 + bgap : blk0;
         const uint32_t bi = div_bs((uint32_t)key, a.block_magic, a.block_shift);
@@ -335,7 +388,7 @@ __device__ __forceinline__ void decode_task(const AttnArgs& a, const DecodeTask&
       }
     };
     auto compute = [&](int t, const Step& x) {
-      const int kb = t < ntw ? kbeg + 32 * (ki + KW * t) : kend;   // past the last one: fully masked
+      const int kb = t < ntw ? kbeg + 32 * (kis + KW * t) : kend;   // past the last one: fully masked
       f32x4 s[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u) s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -351,25 +404,22 @@ __device__ __forceinline__ void decode_task(const AttnArgs& a, const DecodeTask&
           *reinterpret_cast<u32x4*>(ldsV + (16 * u + n) * RB + chunk_dim<D, KF>(kk, grp) * 2) =
               fp4x8_to<T>(x.v[u][kk], __uint_as_float(x.vs[u] << 23));
       // lane holds S[key kb + 16u + 4grp + j][row n]
-      float p[2][4];
       float tmax = kNegInf;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const int vb = kb + 16 * u, kr = key_of(vb);   // a sub-tile lies on one side of the left-out keys
-#pragma unroll
-        for (int j = 0; j < 4; ++j) p[u][j] = s[u][j] * sl2;
         // past the range, past the first row, or before the last row's window
         if (vb + 16 > kend || kr + 15 > tk.ctx_len || (kr <= tk.ctx_len + tk.q_len - 1 - a.window && kr + 16 > a.sinks)) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int key = kr + 4 * grp + j;
             const bool hid = (vb + 4 * grp + j >= kend) | (key > vis) | ((key <= vis - a.window) & (key >= a.sinks));
-            p[u][j] = hid ? kNegInf : p[u][j];
+            s[u][j] = hid ? kNegInf : s[u][j];
           }
         }
-        tmax = fmaxf(tmax, fmaxf(fmaxf(p[u][0], p[u][1]), fmaxf(p[u][2], p[u][3])));
+        tmax = fmaxf(tmax, fmaxf(fmaxf(s[u][0], s[u][1]), fmaxf(s[u][2], s[u][3])));
       }
-      tmax = max_xor32(max_xor16(tmax));
+      tmax = max_xor32(max_xor16(tmax)) * sl2;
       if (__builtin_amdgcn_ballot_w64(tmax > m + 8.f)) {   // lazy rescale, as above
         const float mn = tmax > m + 8.f ? tmax : m;
         const float alpha = fast_exp2(m - (mn == kNegInf ? 0.f : mn));
@@ -383,9 +433,9 @@ __device__ __forceinline__ void decode_task(const AttnArgs& a, const DecodeTask&
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) p[u][j] = fast_exp2(p[u][j] - mu);
-        pb[2 * u] = E16<T>::pack2(p[u][0], p[u][1]);
-        pb[2 * u + 1] = E16<T>::pack2(p[u][2], p[u][3]);
+        for (int j = 0; j < 4; ++j) s[u][j] = fast_exp2(__builtin_fmaf(s[u][j], sl2, -mu));
+        pb[2 * u] = E16<T>::pack2(s[u][0], s[u][1]);
+        pb[2 * u + 1] = E16<T>::pack2(s[u][2], s[u][3]);
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) lsum = E16<T>::add2(pb[e], lsum);   // the rounded p the MFMA sees
@@ -397,7 +447,7 @@ __device__ __forceinline__ void decode_task(const AttnArgs& a, const DecodeTask&
       }
     };
     // the same load order on every path, as below
-    if (ntw > 0) {
+    auto run = [&](auto issue) {
 #pragma unroll
       for (int u = 0; u < PF; ++u) {
         issue(u, ring[u]);
@@ -416,6 +466,14 @@ __device__ __forceinline__ void decode_task(const AttnArgs& a, const DecodeTask&
 #pragma unroll
       for (int u = 0; u < PF; ++u)
         if (t0 + u < ntw) compute(t0 + u, ring[u]);
+    };
+    if (ntw > 0) {
+      if (a.block_size % 16 == 0) {
+        places(0);
+        run(issue_one);
+      } else {
+        run(issue_any);
+      }
     }
   } else {
     // this wave's sub-tiles: j = ki + KW * t, t < ntw
