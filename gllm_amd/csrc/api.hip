@@ -350,7 +350,7 @@ void prefill_pieces(const gllm_attn_plan* p, const SeqInfo& s, int i, int G, int
       const int c0 = w * pw, c1 = std::min(w * pw + pw - 1, G * nrb - 1);
       int64_t kend = s.ctx_len + std::min(s.q_len - 1, (c1 / G) * 32 + 31) + 1;
       int64_t pairs = 0;
-      if (p->window > 0) kend -= key_skip(s.ctx_len + c0 / G * 32, p->window, p->sinks, 64).by;   // keys passed over
+      if (p->window > 0) kend -= key_skip(s.ctx_len + c0 / G * 32, p->window, p->sinks, 1).by;   // keys passed over
       for (int c = c0; c <= c1; ++c) {
         const int64_t r0 = (int64_t)(c / G) * 32, r1 = std::min<int64_t>(s.q_len, r0 + 32);
         if (p->window > 0) {                       // the first row's keys for each: the item's work within a tile's
@@ -1052,6 +1052,20 @@ int gllm_attn_plan_create_window(gllm_attn_plan** out, const int32_t* query_lens
           decode_items(shortest_split(std::min<int64_t>(1024, cap), 3 * (int64_t)cus));
         }
       }
+    }
+    // Windowed sequences are about equally long, so a round of items that does not
+    // fill the CUs costs a whole item's time, and each item its start: at head dim
+    // 128 they go page-balanced from two items per CU on.  Measured (split /
+    // page-balanced us, 32 / 8 heads; sequences x window; 16-bit, fp8, 4-bit cache):
+    // 150 x 1024 138 / 131, 72 / 66, 49 / 41; 200 x 512 104 / 95, 56 / 46, 45 / 35; 300 x
+    // 1024 242 / 243, 133 / 135, 92 / 83; 500 x 256 138 / 123, 78 / 60, 70 / 48; below, 96 x
+    // 128 23 / 20, 16.0 / 16.4, 16.1 / 17.4.  At head dim 64 the items are ahead or level:
+    // 200 x 512 44 / 45, 28 / 31, 26 / 29; 400 x 512 84 / 100, 46 / 49, 42 / 40.
+    if (!balanced && hides && split_tokens == 0 && !decode_heads_per_wg && pf.empty() && head_dim == 128 &&
+        dc.size() >= 2 * (size_t)cus) {
+      p->n_partials = 0;
+      balanced = true;
+      plan_balanced_decode(p, cus, 0, 0);
     }
     if (!balanced) {
     // Workgroups are dispatched slot-major: while every slot is free, item k

@@ -778,10 +778,11 @@ __device__ __forceinline__ int pf_swz(int r) {
 // Paged mode: keys through the block table, causal mask on diagonal tiles
 // only.  Dense mode (DENSE): keys from k/v [B, T, Hkv, D], additive bias
 // [B, T_q, T] on every tile.
-// WIN: the tiles that every row of the workgroup is past with its window, and
-// that hold no sink, are left out (key_skip); tiles at either edge of a row's
-// window are masked, and a row's reference is chosen at its first tile with a
-// visible key.
+// WIN: the keys between the sinks and the first row's window are left out
+// (key_skip, key by key: every row of a tile has its own address), so the tiles
+// count through the sinks and then the window from its first key; tiles at
+// either edge of a row's window are masked, and a row's reference is chosen at
+// its first tile with a visible key.
 template <typename T, int D, bool DENSE, int NW, int NS, int KF, bool WIN>
 __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it, int seq, int kvh, int wgrp, char* lds) {
   static_assert(!(DENSE && (KF != kKV16 || WIN)), "the dense op has no cache");
@@ -835,15 +836,16 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
   const int64_t qrow = qstart + rr;
   const int qh = kvh * G + g;
 
-  // WIN: the workgroup's tiles start on 64 keys, so a tile lies on one side of
-  // the left-out run; its blocks are cached in two runs (nblk_s of the sinks').
-  const KeySkip sk = WIN ? key_skip(ctx + wgrp * NW / G * 32, a.window, a.sinks, BN) : KeySkip{0, 0, 0};
-  const bool both = WIN && sk.by > 0;
-  const int nblk_s = both && sk.from > 0 ? (int)div_bs((uint32_t)(sk.from - 1), a.block_magic, a.block_shift) + 1 : 0;
-  const int bgap = both ? (int)div_bs((uint32_t)(sk.from + sk.by), a.block_magic, a.block_shift) - nblk_s : 0;
-  const int lo_w = WIN ? max(0, ctx + r0 + 1 - a.window) : 0;              // first key in the wave's windows
-  const int hid_w = WIN ? ctx + min(qlen - 1, r0 + 31) - a.window : 0;     // last key before its last row's
-  const auto tile_key = [&](int t) { return WIN && t * BN >= sk.from ? t * BN + sk.by : t * BN; };
+  // WIN: from here on positions count through the keys that are not left out
+  // (v >= from is key v + by); the blocks of the sinks and of the window are
+  // cached as two runs, nblk_s and the rest, bgap apart.
+  const KeySkip sk = WIN ? key_skip(ctx + wgrp * NW / G * 32, a.window, a.sinks, 1) : KeySkip{0, 0, 0};
+  const int by = WIN ? sk.by : 0;
+  const int nblk_s = WIN && by > 0 && sk.from > 0 ? (int)div_bs((uint32_t)(sk.from - 1), a.block_magic, a.block_shift) + 1 : 0;
+  const int bgap = WIN && by > 0 ? (int)div_bs((uint32_t)(sk.from + by), a.block_magic, a.block_shift) - nblk_s : 0;
+  const int nkeys_wg = kend_wg - by, nkeys_w = kend_w - by;
+  const int lo_w = WIN ? max(0, ctx + r0 + 1 - a.window) - by : 0;              // first key in the wave's windows
+  const int hid_w = WIN ? ctx + min(qlen - 1, r0 + 31) - a.window - by : 0;     // last key before its last row's
 
   // Block ids of keys [0, kend_wg), loaded into registers now and cached in
   // LDS (first kBidCache blocks; any beyond are read from the table
@@ -919,8 +921,8 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
   struct Row4 { uint32_t blk, off; };
   using Row = std::conditional_t<KF == kKV4, Row4, uint32_t>;
   auto copy_key = [&](int ts, int i) {
-    const int p = min(ts + (i * NW + wave) * RPS + lane / CPR, kend_wg - 1);
-    return WIN ? seen_key(p, sk, a.sinks) : p;
+    const int v = min(ts + (i * NW + wave) * RPS + lane / CPR, nkeys_wg - 1);
+    return WIN && v >= sk.from ? v + by : v;
   };
   auto dma_bids = [&](int ts, Row (&slot)[CHD]) {
 #pragma unroll
@@ -930,7 +932,7 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
       } else {
         const int p = copy_key(ts, i);
         const uint32_t bi = div_bs((uint32_t)p, a.block_magic, a.block_shift);
-        const uint32_t ci = WIN && both && p >= sk.from + sk.by ? bi - (uint32_t)bgap : bi;
+        const uint32_t ci = WIN && p >= sk.from + by ? bi - (uint32_t)bgap : bi;
         uint32_t blk;
         if (ci < (uint32_t)Cfg::kBidCache) {
           blk = (uint32_t)lbid[ci];
@@ -1068,7 +1070,7 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
   // one per-lane limit against compile-time offsets (nothing to hoist onto the
   // common path)
   auto apply_mask = [&](f32x16& s, int k0) {
-    const int lim = vis - k0 - 4 * h;
+    const int lim = (WIN ? vis - by : vis) - k0 - 4 * h;
     if constexpr (WIN) {               // nor at or before vis - window, unless a sink
       const int lo = lim - a.window, sink = a.sinks - k0 - 4 * h;
 #pragma unroll
@@ -1358,8 +1360,8 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
   // MFMAs of tile t - TPB, into that tile's stage.
   constexpr int TPB = NS / 2;
   static_assert(NS % 2 == 0 && TPB >= 1, "stage ring must hold two tile groups");
-  const int ntiles = (kend_wg + (WIN ? BN - 1 - sk.by : BN - 1)) / BN;
-  const int full_end = ctx + r0;           // tiles ending at or before key ctx + r0 need no mask
+  const int ntiles = (nkeys_wg + BN - 1) / BN;
+  const int full_end = ctx + r0 - by;      // tiles ending at or before key ctx + r0 need no mask
   // The first TPB tiles' copies are addressed with block ids read straight
   // from the table (issued together with the loads above), so they need no
   // trip through LDS and a barrier first; every load so far is waited for
@@ -1372,7 +1374,7 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
       fbid[t][i] = 0u;
       foff[t][i] = 0u;
       if (!DENSE) {
-        const int p = copy_key(tile_key(t), i);
+        const int p = copy_key(t * BN, i);
         const uint32_t bi = div_bs((uint32_t)p, a.block_magic, a.block_shift);
         fbid[t][i] = (uint32_t)bt[bi];
         foff[t][i] = (uint32_t)p - bi * (uint32_t)a.block_size;
@@ -1389,7 +1391,7 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
         if constexpr (KF == kKV4) row[i] = Row{fbid[t][i], foff[t][i]};
         else row[i] = fbid[t][i] * (uint32_t)a.block_size + foff[t][i];   // the row's slot
       }
-      dma_issue(tile_key(t), t, row);
+      dma_issue(t * BN, t, row);
     }
   if (!DENSE) {
 #pragma unroll
@@ -1417,7 +1419,7 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
     for (int kk = 0; kk < NQ; ++kk) qB[kk] = pack8<T>(x[kk]);   // exact: q and its rotation are in T
   }
   if (!DENSE) __syncthreads();  // block ids in LDS visible
-  if (TPB < ntiles) dma_bids(tile_key(TPB), nbid);
+  if (TPB < ntiles) dma_bids(TPB * BN, nbid);
 
   // The loop walks the ring NS tiles at a time so that every stage index is a
   // compile-time constant (operand reads then carry it as an immediate); a
@@ -1434,11 +1436,11 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
           const int t = tg + u;
           const int stage = gi * TPB + u;    // == t % NS
           if (t < ntiles) {
-            const int ts = tile_key(t);
+            const int ts = t * BN;
             const bool dma = t + TPB < ntiles;
-            const int dts = tile_key(t + TPB), dstage = (stage + TPB) % NS;
+            const int dts = (t + TPB) * BN, dstage = (stage + TPB) % NS;
             // keys of the wave's rows in the tile (WIN: not all before its windows and past the sinks)
-            const bool live = wact && ts < kend_w && !(WIN && ts + BN <= lo_w && ts >= a.sinks);
+            const bool live = wact && ts < nkeys_w && !(WIN && ts + BN <= lo_w && ts >= a.sinks);
             if (KREG && dma && live) reg_fetch(dts, nbid);   // written in the tile's last region
             if (live)
               compute(lds + stage * Cfg::kTile, ts,
@@ -1446,7 +1448,7 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
                       t == 0);
             else if (dma)
               dma_issue(dts, dstage, nbid);
-            if (t + TPB + 1 < ntiles) dma_bids(tile_key(t + TPB + 1), nbid);
+            if (t + TPB + 1 < ntiles) dma_bids((t + TPB + 1) * BN, nbid);
           }
         }
       }
