@@ -947,8 +947,7 @@ int gllm_attn_plan_create_window(gllm_attn_plan** out, const int32_t* query_lens
     // Prefill: 8-wave workgroups, one per CU (4-stage K/V ring in LDS).
     // prefill-only launches: kPrefillOnlyWaves-wave workgroups (prefill_kernel);
     // a mixed launch's prefill items run in its 8-wave workgroups
-    const int pw = ndec == 0 ? kPrefillOnlyWaves : 8;
-    p->prefill_waves = pw;
+    int pw = ndec == 0 ? kPrefillOnlyWaves : 8;
     const int hgroups = (num_kv_heads + best_hw - 1) / best_hw;
     p->head_groups = hgroups;
     p->merge.assign((size_t)num_seqs * hgroups, MergeInfo{0, 0});
@@ -989,14 +988,60 @@ int gllm_attn_plan_create_window(gllm_attn_plan** out, const int32_t* query_lens
       longest_first(dc);
     };
     decode_items(best_S);
-    for (int i = 0; i < num_seqs; ++i) {
-      if (p->seqs[i].q_len * G <= 16) continue;
-      ++p->n_prefill_seqs;
-      pcs.clear();
-      prefill_pieces(p, p->seqs[i], i, G, num_kv_heads, pcs, pw);
-      for (const PrefillPiece& pc : pcs) pf.push_back({pc.kend, pc.it});
+    const auto prefill_items = [&](int waves) {
+      p->n_prefill_seqs = 0;
+      pf.clear();
+      for (int i = 0; i < num_seqs; ++i) {
+        if (p->seqs[i].q_len * G <= 16) continue;
+        ++p->n_prefill_seqs;
+        pcs.clear();
+        prefill_pieces(p, p->seqs[i], i, G, num_kv_heads, pcs, waves);
+        for (const PrefillPiece& pc : pcs) pf.push_back({pc.kend, pc.it});
+      }
+    };
+    prefill_items(pw);
+    if (hides && ndec == 0) {
+      // Windowed prompts are many short items, and an item's start (~10 us) is idle
+      // time on its CU: workgroups of half the waves, two or three per CU, run one's
+      // start under the others' keys, at twice the K/V reads.  They pay from two
+      // items per CU on at head dim 64, from three of at most 640 keys at 128.  Measured,
+      // 32 / 8 heads, us whole / half (items; window), bf16, in the order below: head dim
+      // 64, 2 x 2,048 tokens 42 / 37 (512; 512), 4 x 2,048 75 / 60 (1,024; 512), 8 of
+      // 512-8,192 525 / 484 (4,944; 1,024), 1132 / 1116 (4,096), 241 / 209 (256); below,
+      // 1 x 2,048 23.2 / 23.4 (256; 512); head dim 128, 3 x 2,048 87 / 86 (768; 512), 6 x 2,048
+      // 155 / 147, 16 of 300-700 on 4,000 99 / 86 (1,088; 256), 8 of 512-8,192 384 / 365 (256);
+      // the other side, 8 x 2,048 287 / 296 (1,024), 8 of 512-8,192 791 / 818 (1,024), 1737 /
+      // 1891 (4,096).  4-bit and fp8 caches alike.
+      int64_t keys = 0;
+      for (const Keyed& k : pf) keys += k.work;
+      const int64_t n = (int64_t)pf.size();
+      if (head_dim == 64 ? n >= 2 * (int64_t)cus : n >= 3 * (int64_t)cus && keys <= 640 * n) {
+        pw = kPrefillHalfWaves;
+        prefill_items(pw);
+      }
+      // Neighbouring row blocks of a kv head share most of their window: the items,
+      // in the order of their sequences, heads and rows, are cut into eight ranges
+      // of equal work, one per XCD (workgroup b runs on XCD b % 8), which reads its
+      // windows from its own L2; longest first within a range.  Against longest
+      // first over all: 8 of 512-8,192, bf16, 824 -> 791 us (window 1,024), 1793 -> 1737
+      // (4,096), half 570 -> 526 (512); 4-bit within 2% either way.
+      int64_t total = 0, run = 0;
+      for (const Keyed& k : pf) total += k.work;
+      std::vector<Keyed> range[8];
+      for (const Keyed& k : pf) {
+        range[std::min<int64_t>(7, run * 8 / total)].push_back(k);
+        run += k.work;
+      }
+      for (auto& r : range) longest_first(r);
+      const size_t items = pf.size();
+      pf.clear();
+      for (size_t j = 0; pf.size() < items; ++j)
+        for (const auto& r : range)
+          if (j < r.size()) pf.push_back(r[j]);
+    } else {
+      longest_first(pf);
     }
-    longest_first(pf);
+    p->prefill_waves = pw;
     // Two prefill workgroups per CU (D = 64) run a start under the other's keys, but
     // spill: they pay where items are many and short (from two per CU, 320 keys on
     // average), or at eight and more per CU without cached context.  Measured, bf16,

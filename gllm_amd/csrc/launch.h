@@ -42,6 +42,8 @@ enum : int32_t { kRopeNone = 0, kRopeByPosition = 1, kRopeByRow = 2 };
 // overlaps the other's compute) 550-557 us against 516-518 us.
 constexpr int kPrefillOnlyWaves = 8;
 constexpr int kPrefillOnlyStages = 4;
+constexpr int kPrefillHalfWaves = 4;
+constexpr int kPrefillHalfStages = 2;
 
 // Generic attention: (query row, head) columns of one workgroup of the stream
 // kernel (attention_stream.h) and of the tiled kernel (attention_tile.h); the

@@ -1559,6 +1559,14 @@ prefill_kernel(AttnArgs a) {
   const WorkItem it = a.items[blockIdx.x];
   prefill_wg<T, D, false, kPrefillOnlyWaves, kPrefillOnlyStages, KF, WIN>(a, it, it.seq, it.a, it.kind_b >> 8, lds);
 }
+// The same in kPrefillHalfWaves-wave workgroups, two per CU (windowed plans).
+template <typename T, int D, int KF>
+__global__ void __launch_bounds__(64 * kPrefillHalfWaves) __attribute__((amdgpu_waves_per_eu(2)))
+prefill_half_kernel(AttnArgs a) {
+  __shared__ __attribute__((aligned(16))) char lds[PrefillCfg<D, kPrefillHalfStages>::kLdsBytes];
+  const WorkItem it = a.items[blockIdx.x];
+  prefill_wg<T, D, false, kPrefillHalfWaves, kPrefillHalfStages, KF, true>(a, it, it.seq, it.a, it.kind_b >> 8, lds);
+}
 
 template <typename T, int D>
 __global__ void __launch_bounds__(64 * kWaves) dense_attn_kernel(AttnArgs a, int nwg) {
@@ -1581,6 +1589,12 @@ static void launch_paged_hk(const AttnArgs& a, bool pf, bool dc, hipStream_t st)
     if constexpr (std::is_same_v<T, __bf16> && D == 64 && KF == kKV16 && !WIN) {
       if (a.prefill_pairs) {
         hipLaunchKernelGGL((prefill_kernel<T, D, KF, WIN, true>), grid, dim3(64 * kPrefillOnlyWaves), 0, st, a);
+        return;
+      }
+    }
+    if constexpr (WIN) {
+      if (a.prefill_waves == kPrefillHalfWaves) {
+        hipLaunchKernelGGL((prefill_half_kernel<T, D, KF>), grid, dim3(64 * kPrefillHalfWaves), 0, st, a);
         return;
       }
     }
@@ -1626,7 +1640,8 @@ static hipError_t launch_paged_d(const AttnArgs& a, bool pf, bool dc, hipStream_
     if (pf && !dc) return hipErrorInvalidValue;
     e = pf ? launch_mixed_balanced<T, D, KF, WIN>(a, st) : launch_decode_balanced<T, D, KF, WIN>(a, st);
   } else {
-    if (nw != kWaves || (pf && a.prefill_waves != (dc ? kWaves : kPrefillOnlyWaves))) return hipErrorInvalidValue;
+    const bool half = WIN && !dc && a.prefill_waves == kPrefillHalfWaves;
+    if (nw != kWaves || (pf && !half && a.prefill_waves != (dc ? kWaves : kPrefillOnlyWaves))) return hipErrorInvalidValue;
     switch (hw) {
       case 1: launch_paged_hk<T, D, 1, 8, KF, WIN>(a, pf, dc, st); break;
       case 2: launch_paged_hk<T, D, 2, 4, KF, WIN>(a, pf, dc, st); break;
