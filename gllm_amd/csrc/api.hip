@@ -192,6 +192,7 @@ int kv4_check(const void* k_cache, const void* v_cache, int64_t block_stride, in
 struct gllm_attn_plan {
   int32_t num_seqs = 0, Hq = 0, Hkv = 0, D = 0, bs = 0, dtype = 0;
   int32_t split_len = 0, max_q = 0;
+  bool mixed_half = false;         // mixed launches of the windowed and 4-bit kernels: 4-wave workgroups
   int32_t window = 0, sinks = 0;   // sliding window (0: none reaches a sequence's first keys)
   int32_t n_decode_seqs = 0, n_prefill_seqs = 0, heads_per_wg = 8, decode_waves = 8, prefill_waves = 8;
   bool prefill_pairs = false;  // prefill-only launches at D = 64: two workgroups per CU
@@ -1112,6 +1113,32 @@ int gllm_attn_plan_create_window(gllm_attn_plan** out, const int32_t* query_lens
       balanced = true;
       plan_balanced_decode(p, cus, 0, 0);
     }
+    // A mixed launch in half-size workgroups (two a CU; windowed and 4-bit kernels)
+    // runs prefill items beside decode items, but each item takes about 1.6 times as
+    // long: it pays where the longest prefill item, so stretched, still ends well
+    // before the launch (its items' time over the CUs).  An item: ~10 us and 1.75
+    // (head dim 64: 1.0) us per 64 keys for prefill, 5.6 us and its K/V at 29 GB/s for
+    // decode.  At head dim 128, where half workgroups read K/V twice for the same
+    // MFMA rate, only for items of at most 1,100 keys.  Measured, us whole / half, bf16
+    // and 4-bit cache (decodes, chunks, window): head dim 128, 200 + 1 x 256, 512
+    // 96 / 85, 49 / 43; 64 + 16 of 128-256, 512 82 / 78, 82 / 73; 64 + 4 x 512, 1,024 88 / 88, 65 /
+    // 65; the other side, 64 + 2 of 256-1,024, 2,048 173 / 174, 100 / 112; 32 + 4,096, 8,192 292 /
+    // 384, 208 / 248; head dim 64, 200 + 1 x 256, 512 45 / 38, 33 / 31; 16 + 4 of 512-1,024,
+    // 2,048 105 / 96, 116 / 109; 32 + 4,096, 8,192 184 / 190, 160 / 141; the other side, 64 + 2 of
+    // 256-1,024, 2,048 92 / 110, 79 / 95.
+    if (!balanced && !pf.empty() && !dc.empty()) {
+      const double tile = head_dim == 64 ? 1.0 : 1.75;
+      const double key = 4.0 * head_dim * best_hw / 29e3;   // us per key, 16-bit K and V
+      double total = 0;
+      int64_t longest = 0;
+      for (const Keyed& k : pf) {
+        total += 10 + tile * (double)((k.work + 63) / 64);
+        longest = std::max(longest, k.work);
+      }
+      for (const Keyed& k : dc) total += 5.6 + key * (double)k.work;
+      p->mixed_half = 10 + 1.6 * tile * (double)((longest + 63) / 64) < 0.8 * total / cus &&
+                      (head_dim == 64 || longest <= 1100);
+    }
     if (!balanced) {
     // Workgroups are dispatched slot-major: while every slot is free, item k
     // and item k + cus land on the same CU, and the older (first) one wins
@@ -1332,7 +1359,7 @@ static int paged_attention_impl(const gllm_attn_plan* p, const void* q, int64_t 
   a.block_size = p->bs;
   block_div(p->bs, &a.block_magic, &a.block_shift);
   a.rope_cos = rope_cos; a.rope_sin = rope_sin; a.rope_row_stride = rope_row_stride; a.rope_mode = rope_mode;
-  a.window = p->window; a.sinks = p->sinks;
+  a.window = p->window; a.sinks = p->sinks; a.mixed_half = p->mixed_half;
   if (kv4) a.kv4_record = (int32_t)kv4_record_bytes(p->bs, p->D);
   a.seqs = (const SeqInfo*)(p->ws + p->off_seqs);
   a.items = (const WorkItem*)(p->ws + p->off_items);

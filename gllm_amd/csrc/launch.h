@@ -42,6 +42,8 @@ enum : int32_t { kRopeNone = 0, kRopeByPosition = 1, kRopeByRow = 2 };
 // overlaps the other's compute) 550-557 us against 516-518 us.
 constexpr int kPrefillOnlyWaves = 8;
 constexpr int kPrefillOnlyStages = 4;
+// Half of that, two (head dim 64: three) workgroups per CU, for windowed plans
+// of many short items.
 constexpr int kPrefillHalfWaves = 4;
 constexpr int kPrefillHalfStages = 2;
 
@@ -135,6 +137,7 @@ struct AttnArgs {
   // sliding window (0: none): keys that a row sees back from its own on, and first
   // keys that stay visible
   int32_t window, sinks;
+  int32_t mixed_half;          // windows, 4-bit caches: a mixed launch's items by two 4-wave workgroups each
   int32_t kv4_record;          // 4-bit cache: bytes of one (block, kv head)
 };
 

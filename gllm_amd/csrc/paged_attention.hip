@@ -195,7 +195,8 @@ __device__ __forceinline__ void decode_task(const AttnArgs& a, const DecodeTask&
   // cos/sin rows are loaded together, one HBM round trip before the first
   // K/V loads can be addressed (the block-id load is issued first so its LDS
   // store does not wait for the others).
-  static_assert(Cfg::kMaxBlocks <= 64 * NW, "one block id per thread");
+  static_assert(Cfg::kMaxBlocks <= 128 * NW, "at most two block ids per thread");
+  constexpr bool kIds2 = Cfg::kMaxBlocks > 64 * NW;
   int32_t* lbid = reinterpret_cast<int32_t*>(lds + NW * Cfg::kVBytes);
   // WIN: two runs of blocks where the range has keys on both sides of the
   // left-out ones; entry e of the cache is block blk0 + e, or from nblk_s on
@@ -209,6 +210,9 @@ __device__ __forceinline__ void decode_task(const AttnArgs& a, const DecodeTask&
   const int nblk = (int)div_bs((uint32_t)key_of(kend - 1), a.block_magic, a.block_shift) - (WIN ? blk0 + bgap : blk0) + 1;
   const int32_t* bt = a.block_table + (int64_t)seq * a.block_table_stride + blk0;
   const uint32_t bid = tid < nblk ? (uint32_t)bt[WIN && tid >= nblk_s ? tid + bgap : tid] : 0u;
+  const int tid2 = tid + 64 * NW;
+  uint32_t bid2 = 0u;
+  if constexpr (kIds2) bid2 = tid2 < nblk ? (uint32_t)bt[WIN && tid2 >= nblk_s ? tid2 + bgap : tid2] : 0u;
   const T* qp = (const T*)a.q + qrow * a.q_row_stride + (int64_t)qh * D;
   u32x4 qraw[NK], praw[kPairInLane ? 1 : NK], craw[NC], sraw[NC];
 #pragma unroll
@@ -230,6 +234,9 @@ __device__ __forceinline__ void decode_task(const AttnArgs& a, const DecodeTask&
     }
   }
   if (tid < nblk) lbid[tid] = bid < (uint64_t)a.num_blocks ? (int32_t)bid : 0;  // never address outside the pool
+  if constexpr (kIds2) {
+    if (tid2 < nblk) lbid[tid2] = bid2 < (uint64_t)a.num_blocks ? (int32_t)bid2 : 0;
+  }
   if constexpr (KF != kKV4) {
     if (a.k_new) write_new_keys<T, D, HW, KF, WIN>(a, tk, tid, 64 * NW);
   }
@@ -641,8 +648,8 @@ __device__ __forceinline__ void decode_task(const AttnArgs& a, const DecodeTask&
 // One decode work item of the split-launch planner (split it.a of the
 // sequence's it.nsplits equal key ranges; split partials merged by
 // merge_splits_kernel).
-template <typename T, int D, int HW, int KW, int KF, bool WIN>
-__device__ __forceinline__ void decode_wg(const AttnArgs& a, const WorkItem& it, char* lds) {
+template <int HW, bool WIN>
+__device__ __forceinline__ DecodeTask split_task(const AttnArgs& a, const WorkItem& it) {
   DecodeTask tk;
   tk.seq = it.seq;
   tk.hg = it.kind_b >> 8;
@@ -657,7 +664,11 @@ __device__ __forceinline__ void decode_wg(const AttnArgs& a, const WorkItem& it,
   tk.nseg = it.nsplits;
   tk.pbase = it.partial_base + tk.hg * HW * it.nsplits;
   tk.ord = it.a;
-  decode_task<T, D, HW, KW, KF, WIN>(a, tk, lds);
+  return tk;
+}
+template <typename T, int D, int HW, int KW, int KF, bool WIN>
+__device__ __forceinline__ void decode_wg(const AttnArgs& a, const WorkItem& it, char* lds) {
+  decode_task<T, D, HW, KW, KF, WIN>(a, split_task<HW, WIN>(a, it), lds);
 }
 
 // Combines the split partials of every (sequence, kv head) whose sequence
@@ -1509,6 +1520,38 @@ __global__ void __launch_bounds__(64 * HW * KW) paged_attn_kernel(AttnArgs a) {
   if constexpr (DC) decode_wg<T, D, HW, KW, KF, WIN>(a, it, lds);
 }
 
+// The items of a mixed launch by two 4-wave workgroups each (windows, 4-bit
+// caches): a prefill item's wave groups, a decode item's kv heads (its one head
+// at HW = 1: the first workgroup's).  Two workgroups fit a CU (70 KB of LDS), so
+// prefill items compute beside decode items that wait for memory, which in
+// 8-wave workgroups run one after the other; the plan says where that pays.
+// Workgroups b and b + 8, on one XCD, share an item.
+template <typename T, int D, int HW, int KW, int KF>
+__global__ void __launch_bounds__(64 * kPrefillHalfWaves) __attribute__((amdgpu_waves_per_eu(2)))
+mixed_half_kernel(AttnArgs a) {
+  constexpr int H = HW > 1 ? HW / 2 : 1, K = HW > 1 ? KW : KW / 2;
+  static_assert(H * K == kPrefillHalfWaves, "half of a mixed workgroup");
+  constexpr int kDec = DecodeCfg<D, H * K, KF>::kLdsBytes, kPre = PrefillCfg<D, kPrefillHalfStages>::kLdsBytes;
+  __shared__ __attribute__((aligned(16))) char lds[kDec > kPre ? kDec : kPre];
+  const int i = (blockIdx.x >> 4) * 8 + (blockIdx.x & 7), half = (blockIdx.x >> 3) & 1;
+  if (i >= a.n_items) return;
+  WorkItem it = a.items[i];
+  const int hg = it.kind_b >> 8;
+  if ((it.kind_b & 0xff) == kItemPrefill) {
+    const int G = a.num_q_heads / a.num_kv_heads;
+    if ((2 * hg + half) * kPrefillHalfWaves >= G * ((it.q_len + 31) / 32)) return;
+    prefill_wg<T, D, false, kPrefillHalfWaves, kPrefillHalfStages, KF, true>(a, it, it.seq, it.a, 2 * hg + half, lds);
+    return;
+  }
+  if (HW == 1 && half) return;
+  DecodeTask tk = split_task<HW, true>(a, it);
+  if (HW > 1) {
+    tk.hg = 2 * hg + half;
+    tk.pbase += half * H * it.nsplits;
+  }
+  decode_task<T, D, H, K, KF, true>(a, tk, lds);
+}
+
 // Page-balanced decode: workgroup w runs its key segments in order (all
 // waves converge between segments; the LDS staging is reused).
 template <typename T, int D, int HW, int KW, int KF, bool WIN>
@@ -1583,6 +1626,13 @@ template <typename T, int D, int HW, int KW, int KF, bool WIN>
 static void launch_paged_hk(const AttnArgs& a, bool pf, bool dc, hipStream_t st) {
   dim3 grid(a.n_items);
   if (pf && dc) {
+    if constexpr (WIN) {
+      if (a.mixed_half) {
+        const dim3 pairs((a.n_items + 7) / 8 * 16);
+        hipLaunchKernelGGL((mixed_half_kernel<T, D, HW, KW, KF>), pairs, dim3(64 * kPrefillHalfWaves), 0, st, a);
+        return;
+      }
+    }
     if constexpr (HW * KW == kWaves)
       hipLaunchKernelGGL((paged_attn_kernel<T, D, true, true, HW, KW, KF, WIN>), grid, dim3(64 * kWaves), 0, st, a);
   } else if (pf) {
