@@ -1334,8 +1334,6 @@ static int paged_attention_impl(const gllm_attn_plan* p, const void* q, int64_t 
   if (q_row_stride < hd || out_row_stride < hd) return fail(GLLM_ATTN_EINVAL, "q/out row stride < num_q_heads * head_dim");
   const bool kv4 = kv_dtype == GLLM_DTYPE_MXFP4;
   if (kv4) {
-    if (!p->mfma) return fail(GLLM_ATTN_EUNSUPPORTED, "4-bit cache: bf16 or f16 model, head_dim 64 or 128 (model dtype %d, "
-                                                      "head_dim %d)", p->dtype, p->D);
     if (int rc = kv4_check(k_cache, v_cache, cache_slot_stride, p->Hkv, p->D, p->bs)) return rc;
     if (k_new || v_new) return fail(GLLM_ATTN_EUNSUPPORTED, "4-bit cache: the KV write is a call of its own");
   } else if (cache_slot_stride < (int64_t)p->Hkv * p->D) {

@@ -50,6 +50,13 @@ __device__ __forceinline__ Raw4<KV> ld_raw4(const KV* row, int d, int D) {
   }
   return r;
 }
+// Dims d .. d + 3 of a 4-bit row: its codes at `codes`, its scales at `scales`
+// (D a multiple of 32); the scale byte rides above the codes.
+template <> struct Raw4<kv4> { uint32_t w[1]; };
+__device__ __forceinline__ Raw4<kv4> ld_raw4_kv4(const uint8_t* codes, const uint8_t* scales, int d, int D) {
+  const int e = min(d, D - 4);
+  return Raw4<kv4>{{*reinterpret_cast<const uint16_t*>(codes + e / 2) | (uint32_t)scales[e / 32] << 16}};
+}
 // The chunk of dims D - 2, D - 1 (D even), loaded as the row's last four.
 template <typename KV>
 __device__ __forceinline__ void last2(Raw4<KV>& r, bool last) {
@@ -63,7 +70,12 @@ __device__ __forceinline__ void last2(Raw4<KV>& r, bool last) {
 template <typename KV, typename QT>
 __device__ __forceinline__ f32x4 widen4(const Raw4<KV>& r) {
   f32x4 x;
-  if constexpr (std::is_same<KV, float>::value) {
+  if constexpr (std::is_same<KV, kv4>::value) {
+    const float scale = __uint_as_float(r.w[0] >> 16 << 23);
+    const auto lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(r.w[0], scale, 0);
+    const auto hi = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(r.w[0], scale, 1);
+    x = f32x4{lo[0], lo[1], hi[0], hi[1]};
+  } else if constexpr (std::is_same<KV, float>::value) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(r.w[i]);
   } else if constexpr (std::is_same<KV, fp8e4m3>::value) {
@@ -93,6 +105,9 @@ template <typename KV, typename QT>
 __device__ __forceinline__ u32x2 pack4(const Raw4<KV>& r) {
   if constexpr (std::is_same<KV, QT>::value) {
     return u32x2{r.w[0], r.w[1]};
+  } else if constexpr (std::is_same<KV, kv4>::value) {
+    const float scale = __uint_as_float(r.w[0] >> 16 << 23);
+    return u32x2{E16<QT>::template fp4x2<0>(r.w[0], scale), E16<QT>::template fp4x2<1>(r.w[0], scale)};
   } else if constexpr (std::is_same<KV, fp8e4m3>::value) {
     return u32x2{E16<QT>::template fp8x2<false>(r.w[0]), E16<QT>::template fp8x2<true>(r.w[0])};
   } else {
@@ -131,6 +146,9 @@ __device__ __forceinline__ u32x2 pack4(const Raw4<KV>& r) {
 // [0, ctx), and one wave takes the new ones from LDS as a last sub-tile.  The
 // workgroup of the first column stores them at their slots (block table); no
 // workgroup of the launch reads those slots.
+// A 4-bit cache (kv4, with WIN; head dims that are multiples of 32) has rows in
+// two places, codes and scales, so a row is its byte place and its row in the
+// block.
 // WIN (sliding window): the sub-tiles count through the keys that the first of
 // the workgroup's rows leaves (key_skip); a sub-tile at the edge of a row's
 // window is masked.
@@ -196,6 +214,7 @@ __global__ void __launch_bounds__((64 * StreamCfg<KV, QT, DP, V>::kNW)) attn_str
   const int nkeys = DENSE ? L : (FUSED ? ctx : ctx + r_last + 1 - (WIN ? sk.by : 0));
   const int vis = DENSE ? L - 1 : ctx + r;       // last visible key of the lane's column
   const int32_t* bt = DENSE ? nullptr : a.block_table + (int64_t)b * a.block_table_stride;
+  constexpr bool k4 = std::is_same<KV, kv4>::value;
   const KV* kbase = DENSE ? (const KV*)a.k + (int64_t)b * a.k_batch_stride + (int64_t)kvh * D
                           : (const KV*)a.k_cache + (int64_t)kvh * D;
   const KV* vbase = DENSE ? (const KV*)a.v + (int64_t)b * a.v_batch_stride + (int64_t)kvh * D
@@ -226,22 +245,41 @@ __global__ void __launch_bounds__((64 * StreamCfg<KV, QT, DP, V>::kNW)) attn_str
     const int v = min(p0 + n, nkeys - 1);        // keys past the end: masked, re-read the last
     const int key = WIN ? seen_key(key_of(v), sk, a.sinks) : v;
     int64_t row = key;
+    int off4 = 0;
     if (!DENSE) {
       const uint32_t bi = div_bs((uint32_t)key, a.block_magic, a.block_shift);
       if (blk >= (uint64_t)a.num_blocks) blk = 0;   // never address outside the pool
       row = (int64_t)blk * a.block_size + (key - (int)bi * a.block_size);
+      if constexpr (k4) {
+        off4 = key - (int)bi * a.block_size;
+        row = (int64_t)blk * a.cache_slot_stride + (int64_t)kvh * a.kv4_record + off4 * (D / 2);
+      }
     }
-    const KV* kp = kbase + row * kstride;
+    if constexpr (k4) {
+      const uint8_t* kp = (const uint8_t*)a.k_cache + row;
+      const uint8_t* sp = kp + (int64_t)a.block_size * (D / 2) - off4 * (D / 2 - D / 32);
 #pragma unroll
-    for (int u = 0; u < NT; ++u) x.k[u] = ld_raw4<KV, V>(kp, 16 * u + 4 * grp, D);
+      for (int u = 0; u < NT; ++u) x.k[u] = ld_raw4_kv4(kp, sp, 16 * u + 4 * grp, D);
+    } else {
+      const KV* kp = kbase + row * kstride;
+#pragma unroll
+      for (int u = 0; u < NT; ++u) x.k[u] = ld_raw4<KV, V>(kp, 16 * u + 4 * grp, D);
+    }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {                // row of key 4grp + j: lane 4grp + j of the first 16 holds it
       const int src = 4 * grp + j;
       const uint32_t lo = (uint32_t)__shfl((int)(uint32_t)row, src, 64);
       const uint32_t hi = (uint32_t)__shfl((int)((uint64_t)row >> 32), src, 64);
-      const KV* vp = vbase + (int64_t)(((uint64_t)hi << 32) | lo) * vstride;
+      if constexpr (k4) {
+        const uint8_t* vp = (const uint8_t*)a.v_cache + (((uint64_t)hi << 32) | lo);
+        const uint8_t* sp = vp + (int64_t)a.block_size * (D / 2) - __shfl(off4, src, 64) * (D / 2 - D / 32);
 #pragma unroll
-      for (int u = 0; u < NU; ++u) x.v[j][u] = ld_raw4<KV, V>(vp, 64 * u + 4 * n, D);
+        for (int u = 0; u < NU; ++u) x.v[j][u] = ld_raw4_kv4(vp, sp, 64 * u + 4 * n, D);
+      } else {
+        const KV* vp = vbase + (int64_t)(((uint64_t)hi << 32) | lo) * vstride;
+#pragma unroll
+        for (int u = 0; u < NU; ++u) x.v[j][u] = ld_raw4<KV, V>(vp, 64 * u + 4 * n, D);
+      }
     }
     if constexpr (DENSE) {
 #pragma unroll
@@ -556,6 +594,20 @@ static hipError_t launch_stream_d(const AttnArgs& a, dim3 grid, hipStream_t st) 
   return hipGetLastError();
 }
 
+// A 4-bit cache: head dims are multiples of 32.
+template <typename QT>
+static hipError_t launch_stream_kv4(const AttnArgs& a, dim3 grid, hipStream_t st) {
+  auto go = [&](auto dp) {
+    constexpr int DP = decltype(dp)::value;
+    const dim3 block(64 * StreamCfg<kv4, QT, DP, 4>::kNW);
+    hipLaunchKernelGGL((attn_stream_kernel<false, kv4, QT, DP, false, 4, true>), grid, block, 0, st, a);
+  };
+  if (a.head_dim <= 64) go(std::integral_constant<int, 64>());
+  else if (a.head_dim <= 128) go(std::integral_constant<int, 128>());
+  else go(std::integral_constant<int, 256>());
+  return hipGetLastError();
+}
+
 // Cache dtype KV under model dtype QT (paged), or QT throughout (dense); WIN:
 // with a sliding window (paged, no fused KV write).
 template <typename QT, bool WIN>
@@ -575,8 +627,12 @@ static hipError_t launch_stream_t(const AttnArgs& a, bool dense, dim3 grid, hipS
     case kBF16: return go(__bf16{});
     case kF16: return go(_Float16{});
     case kFP8: return go(fp8e4m3{});
-    default: return hipErrorInvalidValue;
+    default: break;
   }
+  if constexpr (WIN) {
+    if (a.kv_dtype == kMXFP4) return launch_stream_kv4<QT>(a, grid, st);
+  }
+  return hipErrorInvalidValue;
 }
 
 }  // namespace gllm

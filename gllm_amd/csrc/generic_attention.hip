@@ -74,7 +74,13 @@ hipError_t launch_attention_generic(AttnArgs a, bool dense, int B, int max_q, in
     const bool tile = max_q >= kTileMinRows && (int64_t)grid(max_q, kTileCols).x * a.num_kv_heads * B >= kTileMinWgs;
     return launch_kind(a, tile, true, grid(max_q, tile ? kTileCols : kStreamCols), st);
   }
-  if (a.k_new) {
+  if (a.kv_dtype == kMXFP4) {
+    // a 4-bit cache: every sequence on the windowed stream kernel
+    if (a.tile_min_q > 0) stream_rows = (int64_t)B * max_q;
+    a.tile_min_q = 0;
+    max_stream_q = max_q;
+    if (a.window == 0) a.window = INT32_MAX;
+  } else if (a.k_new) {
     // the fused KV write (at most kFusedRows rows): every sequence on the
     // stream kernel, which keeps the new keys in LDS
     a.tile_min_q = 0;

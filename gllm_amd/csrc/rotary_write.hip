@@ -26,8 +26,6 @@
 
 namespace gllm {
 
-struct kv4 {};   // the 4-bit cache as a storage type
-
 // 8 elements at p as floats
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, float* v) {

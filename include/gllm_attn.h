@@ -326,8 +326,9 @@ int gllm_attn_plan_destroy(gllm_attn_plan* plan);
  * a cache in the model dtype or fp8 e4m3fn; every other pairing (f32 model;
  * a 16-bit model over an f32 or the other 16-bit cache; other even head dims
  * up to 256) runs a generic kernel (fp32 arithmetic, model dtype in and
- * out).  A 4-bit cache (GLLM_DTYPE_MXFP4) takes a bf16 or f16 model of
- * head_dim 64 or 128.  A plan with a sliding window (gllm_attn_plan_create_window)
+ * out).  A 4-bit cache (GLLM_DTYPE_MXFP4, head_dim a multiple of 32)
+ * runs the MFMA kernels for a bf16 or f16 model of head_dim 64 or 128, else the
+ * generic one.  A plan with a sliding window (gllm_attn_plan_create_window)
  * limits the visible keys.  Every key that some row of a sequence sees has to hold
  * finite values: rows that do not see it may give it weight 0.  Cached values are read as the reference reads them: cast to the
  * model dtype (attention.py:169-170's .to(q.dtype); exact for fp8, rounded

@@ -101,6 +101,25 @@ def test_strided_blocks_and_view():
     b.check(out, None, 0, "strided")
 
 
+@pytest.mark.parametrize("dtype,D", [(F32, 64), (F32, 128), (BF, 32), (F32, 96), (F16, 160), (BF, 256)])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (40, 3), (300, 0)])
+def test_generic(dtype, D, window, sinks):
+    """Model dtypes and head dims of the generic kernel; enough rows for its
+    tiled form in the last batch, which a 4-bit cache does not take."""
+    for ctx, ql, bs in (([0, 20, 500, 0, 130], [1, 3, 1, 60, 40], 16), ([5, 1000], [1, 1], 7)):
+        print(f"kv4 generic {dtype} D={D} window={window} bs={bs}", flush=True)
+        b = Batch(ctx, ql, D=D, dtype=dtype, kv="4", bs=bs, seed=D)
+        out = _run(b, window, sinks)
+        b.check(out, window, sinks, "kv4 generic")
+        if window is not None:
+            assert torch.equal(_run(b, window, sinks, *b.evict(window, sinks)), out)
+
+
+def test_generic_many_rows():
+    b = Batch([0, 64] * 8, [70, 90] * 8, Hq=32, Hkv=8, D=64, dtype=F32, kv="4", seed=1)
+    b.check(_run(b), None, 0, "kv4 generic, many rows")
+
+
 def test_refusals():
     b = Batch([10], [1], D=64, kv="4")
     q, kc, vc, bt = (x.to(DEV) for x in (b.q, b.kc, b.vc, b.bt))
@@ -109,7 +128,6 @@ def test_refusals():
         paged.paged_attention(plan, q, kc[..., :-16], vc[..., :-16], bt)
     with pytest.raises(NotImplementedError):
         paged.paged_attention(plan, q, kc, vc, bt, kv_new=(q[:, :2], q[:, :2]))
-    for D, dtype in ((96, BF), (64, F32)):
-        c = Batch([10], [1], D=D, dtype=dtype, kv="4")
-        with pytest.raises(NotImplementedError):
-            paged.paged_attention(_plan(c), c.q.to(DEV), c.kc.to(DEV), c.vc.to(DEV), c.bt.to(DEV))
+    plan = paged.AttentionPlan([1], [10], num_q_heads=8, num_kv_heads=2, head_dim=80, block_size=16, dtype=BF, device=DEV)
+    with pytest.raises(ValueError):
+        paged.paged_attention(plan, torch.zeros(1, 8, 80, dtype=BF, device=DEV), kc, vc, bt)
