@@ -318,8 +318,8 @@ __device__ __forceinline__ void decode_task(const AttnArgs& a, const DecodeTask&
     // In blocks of a multiple of 16 rows a sub-tile lies in one block (ONE): lane i
     // keeps the place of the wave's i-th sub-tile of the next 64, and a load takes
     // it as a scalar base plus the lane's fixed offset.  The addresses were a third
-    // of a step's vector instructions (64 x 4,096 keys, 32 / 8 heads of 64:
-    // KV4_ONE us; elsewhere each lane finds its own key's row).
+    // of a step's vector instructions (64 x 4,096 keys, 32 / 8 heads of 64: 36.8 ->
+    // 34.3 us).  Elsewhere each lane finds its own key's row.
     const int kis = __builtin_amdgcn_readfirstlane(ki);
     const int ntw = __builtin_amdgcn_readfirstlane(head_ok && nsub > 2 * ki ? ((nsub + 1) / 2 - ki + KW - 1) / KW : 0);
     struct Step {
@@ -921,6 +921,7 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
   constexpr int NSEG = BN / RPS;
   constexpr int CHD = NSEG / NW;          // copies per wave per K (or V) tile
   static_assert(CHD >= 1 && NSEG % NW == 0, "tile / workgroup mismatch");
+  static_assert(KF != kKV4 || (NW * 2 * CHD * 64 == 2 * BN * CPR && (NW == 4 || NW == 8)), "4-bit pieces cover a tile");
   constexpr int E = KF == kKV16 ? 2 : 1;   // bytes per cached element (4-bit: strides in bytes)
   const uint32_t sbytes = (uint32_t)(a.cache_slot_stride * E);
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
@@ -928,16 +929,26 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
   // LDS cache (or the table past it) times the block size plus the offset in
   // the block.  Fetched one tile before the copy is issued, so the copy never
   // waits on LDS.
-  // (4-bit cache: the block, and the row in it beside).
+  //
+  // 4-bit cache: a lane fetches a quarter of a row at once (16 bytes of codes at
+  // D = 128, one block, and its scale byte) and widens it into D / 32 chunks of
+  // LDS: 8 / NW such pieces of a tile, pieces 0 - 3 of 16 K rows each, 4 - 7 of V;
+  // lanes of one quarter write 16 rows' chunk, which pf_swz spreads over the
+  // banks.  Against 4 bytes and a scale byte per chunk, eight prompts of 512-4,096
+  // tokens, 32 / 8 heads of 128: 546 -> 524 us (of 512-8,192, window 1,024 772 -> 728).
+  // A row's place is its block and its row there.
   struct Row4 { uint32_t blk, off; };
   using Row = std::conditional_t<KF == kKV4, Row4, uint32_t>;
+  constexpr int NB = KF == kKV4 ? 1 : CHD;   // rows that a lane copies from
+  constexpr int N4 = 8 / NW;                 // 4-bit: pieces a lane fetches
   auto copy_key = [&](int ts, int i) {
-    const int v = min(ts + (i * NW + wave) * RPS + lane / CPR, nkeys_wg - 1);
+    const int row = KF == kKV4 ? (wave & 3) * 16 + (lane & 15) : (i * NW + wave) * RPS + lane / CPR;
+    const int v = min(ts + row, nkeys_wg - 1);
     return WIN && v >= sk.from ? v + by : v;
   };
-  auto dma_bids = [&](int ts, Row (&slot)[CHD]) {
+  auto dma_bids = [&](int ts, Row (&slot)[NB]) {
 #pragma unroll
-    for (int i = 0; i < CHD; ++i) {
+    for (int i = 0; i < NB; ++i) {
       if (DENSE) {
         slot[i] = Row{};
       } else {
@@ -959,7 +970,7 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
   // Source of one lane's 8 elements (logical chunk lc of its row) for copy
   // instruction i, K (v = 0) or V (v = 1), of the tile at key ts (paged: the
   // row's slot from dma_bids).
-  auto copy_src = [&](int ts, const Row (&slot)[CHD], int i, int v) -> const char* {
+  auto copy_src = [&](int ts, const Row (&slot)[NB], int i, int v) -> const char* {
     const int sg = i * NW + wave;
     const int row = sg * RPS + lane / CPR;
     const int lc = (lane % CPR) ^ pf_swz<D>(row);
@@ -969,50 +980,62 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
                 : (const char*)a.k + ((int64_t)seq * a.k_batch_stride + (int64_t)p * a.k_row_stride + (int64_t)kvh * D) * 2) +
              lc * 16;
     }
-    if constexpr (KF == kKV4) {
-      return (const char*)(v ? a.v_cache : a.k_cache) + ((uint64_t)slot[i].blk * sbytes + (uint64_t)kvh * a.kv4_record) +
-             (slot[i].off * (D / 2) + lc * 4);
-    } else {
+    if constexpr (KF != kKV4) {
       const uint64_t off = (uint64_t)slot[i] * sbytes + (uint64_t)kvh * D * E;
       return (const char*)(v ? a.v_cache : a.k_cache) + off + lc * 8 * E;
     }
-  };
-  // 4-bit cache: the scale byte of the same eight elements
-  auto scale_src = [&](const Row (&slot)[CHD], int i, int v) -> const uint8_t* {
-    const int lc = (lane % CPR) ^ pf_swz<D>((i * NW + wave) * RPS + lane / CPR);
-    if constexpr (KF == kKV4)
-      return (const uint8_t*)(v ? a.v_cache : a.k_cache) + ((uint64_t)slot[i].blk * sbytes + (uint64_t)kvh * a.kv4_record) +
-             ((uint32_t)a.block_size * (D / 2) + slot[i].off * (D / 32) + lc / 4);
     return nullptr;
   };
   // One copy instruction into `stage`: bf16 caches go HBM -> LDS directly;
   // fp8 and 4-bit caches are fetched into registers (`reg_fetch`, a tile ahead)
   // and widened to bf16 when written (`reg_put`), so LDS always holds bf16.
-  auto dma_one = [&](int ts, int stage, const Row (&blk)[CHD], int i, int v) {
+  auto dma_one = [&](int ts, int stage, const Row (&blk)[NB], int i, int v) {
     const int sg = i * NW + wave;
     const uint32_t dst = __builtin_amdgcn_readfirstlane(lds0 + v * Cfg::kVBase + stage * Cfg::kTile + sg * 1024);
     lds_dma16(copy_src(ts, blk, i, v), dst);
   };
-  u32x2 rst[CHD][2];                       // fetched chunks of the tile being copied (4-bit: codes, scale)
-  auto reg_fetch = [&](int ts, const Row (&blk)[CHD]) {
+  u32x2 rst[KF == kKV8 ? CHD : 1][2];      // fp8: fetched chunks of the tile being copied
+  u32x4 code4[KF == kKV4 ? N4 : 1];        // 4-bit: fetched pieces and their scale bytes
+  uint32_t scale4[KF == kKV4 ? N4 : 1];
+  auto reg_fetch = [&](int ts, const Row (&blk)[NB]) {
+    if constexpr (KF == kKV4) {
+      const uint64_t rec = (uint64_t)blk[0].blk * sbytes + (uint64_t)kvh * a.kv4_record;
+      const int q4 = lane >> 4;
+      const uint64_t code = rec + (blk[0].off * (D / 2) + D / 8 * q4);
+      const uint64_t scale = rec + ((uint32_t)a.block_size * (D / 2) + blk[0].off * (D / 32) + D / 4 * q4 / 32);
 #pragma unroll
-    for (int i = 0; i < CHD; ++i)
-#pragma unroll
-      for (int v = 0; v < 2; ++v) {
-        if constexpr (KF == kKV4)
-          rst[i][v] = u32x2{*reinterpret_cast<const uint32_t*>(copy_src(ts, blk, i, v)), *scale_src(blk, i, v)};
-        else
-          rst[i][v] = *reinterpret_cast<const u32x2*>(copy_src(ts, blk, i, v));
+      for (int i = 0; i < N4; ++i) {
+        const char* src = (const char*)(N4 == 2 ? (i ? a.v_cache : a.k_cache) : (wave >> 2 ? a.v_cache : a.k_cache));
+        if constexpr (D == 128) {
+          code4[i] = ld16(src + code);
+        } else {
+          const u32x2 w = *reinterpret_cast<const u32x2*>(src + code);
+          code4[i] = u32x4{w[0], w[1], 0u, 0u};
+        }
+        scale4[i] = (uint8_t)src[scale];
       }
+    } else {
+#pragma unroll
+      for (int i = 0; i < CHD; ++i)
+#pragma unroll
+        for (int v = 0; v < 2; ++v) rst[KF == kKV8 ? i : 0][v] = *reinterpret_cast<const u32x2*>(copy_src(ts, blk, i, v));
+    }
   };
+  // chunk `2 i + v` of the lane's 2 CHD
   auto reg_put = [&](int stage, int i, int v) {
-    const int sg = i * NW + wave;
-    u32x4 w;
-    if constexpr (KF == kKV4) w = fp4x8_to<T>(rst[i][v][0], __uint_as_float(rst[i][v][1] << 23));
-    else w = fp8x8_to<T>(rst[i][v][0], rst[i][v][1]);
-    *reinterpret_cast<u32x4*>(lds + v * Cfg::kVBase + stage * Cfg::kTile + sg * 1024 + lane * 16) = w;
+    if constexpr (KF == kKV4) {
+      const int c = 2 * i + v, e = c / (D / 32), j = c % (D / 32);
+      const int row = (wave & 3) * 16 + (lane & 15), lc = (lane >> 4) * (D / 32) + j;
+      const int vv = N4 == 2 ? e : wave >> 2;
+      *reinterpret_cast<u32x4*>(lds + vv * Cfg::kVBase + stage * Cfg::kTile + row * RW + ((lc ^ pf_swz<D>(row)) << 4)) =
+          fp4x8_to<T>(code4[e][j], __uint_as_float(scale4[e] << 23));
+    } else {
+      const int sg = i * NW + wave;
+      *reinterpret_cast<u32x4*>(lds + v * Cfg::kVBase + stage * Cfg::kTile + sg * 1024 + lane * 16) =
+          fp8x8_to<T>(rst[KF == kKV8 ? i : 0][v][0], rst[KF == kKV8 ? i : 0][v][1]);
+    }
   };
-  auto dma_issue = [&](int ts, int stage, const Row (&blk)[CHD]) {
+  auto dma_issue = [&](int ts, int stage, const Row (&blk)[NB]) {
     if (KREG) reg_fetch(ts, blk);
 #pragma unroll
     for (int i = 0; i < CHD; ++i)
@@ -1279,7 +1302,7 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
   // One wave thus keeps the matrix core busy while its own VALU work runs;
   // the two commits (rare wave-uniform branches inside) split the regions.
   // `first`: the row's first tile (key 0).
-  auto compute = [&](const char* st, int ts, bool mask, bool dma, int dts, int dstage, const Row (&blk)[CHD],
+  auto compute = [&](const char* st, int ts, bool mask, bool dma, int dts, int dstage, const Row (&blk)[NB],
                      bool first) {
     f32x16 s0, s1;
     u32x4 va0[2][NO], va1[2][NO];
@@ -1377,11 +1400,11 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
   // from the table (issued together with the loads above), so they need no
   // trip through LDS and a barrier first; every load so far is waited for
   // here explicitly, so nothing below waits on these copies by accident.
-  uint32_t fbid[TPB][CHD], foff[TPB][CHD];
+  uint32_t fbid[TPB][NB], foff[TPB][NB];
 #pragma unroll
   for (int t = 0; t < TPB; ++t)
 #pragma unroll
-    for (int i = 0; i < CHD; ++i) {
+    for (int i = 0; i < NB; ++i) {
       fbid[t][i] = 0u;
       foff[t][i] = 0u;
       if (!DENSE) {
@@ -1395,9 +1418,9 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
 #pragma unroll
   for (int t = 0; t < TPB; ++t)
     if (t < ntiles) {
-      Row row[CHD];
+      Row row[NB];
 #pragma unroll
-      for (int i = 0; i < CHD; ++i) {
+      for (int i = 0; i < NB; ++i) {
         if (fbid[t][i] >= (uint64_t)a.num_blocks) fbid[t][i] = 0u;  // never address outside the pool
         if constexpr (KF == kKV4) row[i] = Row{fbid[t][i], foff[t][i]};
         else row[i] = fbid[t][i] * (uint32_t)a.block_size + foff[t][i];   // the row's slot
@@ -1409,7 +1432,7 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
     for (int k = 0; k < KB; ++k)
       if (tid + k * NT < nbc) lbid[tid + k * NT] = lb[k] < (uint64_t)a.num_blocks ? (int32_t)lb[k] : 0;
   }
-  Row nbid[CHD];
+  Row nbid[NB];
   if (DENSE && kBiasAhead && wact) bias_load(0);
 
   // Q as the B operand of S^T = K Q^T: lane holds Q[row n][16kk + 8h + i].
