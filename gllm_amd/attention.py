@@ -79,7 +79,7 @@ def _block_size(meta, ql: list[int], sl: list[int], hint: int | None = None) -> 
 
 def _kept_plan(meta, window: int | None, sinks: int):
     """The plan that an earlier layer of the step left on the metadata, or None."""
-    if window is None:
+    if window is None and not sinks:
         return getattr(meta, "_gllm_plan", None)
     return (getattr(meta, "_gllm_window_plans", None) or {}).get((window, sinks))
 

@@ -7,7 +7,9 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <exception>
 #include <functional>
+#include <memory>
 #include <mutex>
 #include <new>
 #include <string>
@@ -753,11 +755,11 @@ int gllm_attn_plan_create(gllm_attn_plan** out, const int32_t* query_lens, const
                                       head_dim, block_size, dtype, split_tokens, decode_heads_per_wg, 0, 0);
 }
 
-int gllm_attn_plan_create_window(gllm_attn_plan** out, const int32_t* query_lens, const int32_t* seq_lens,
-                                 int32_t num_seqs, int64_t q_seq_stride, int32_t num_q_heads,
-                                 int32_t num_kv_heads, int32_t head_dim, int32_t block_size, int32_t dtype,
-                                 int32_t split_tokens, int32_t decode_heads_per_wg, int32_t window,
-                                 int32_t sinks) {
+static int plan_create_impl(gllm_attn_plan** out, const int32_t* query_lens, const int32_t* seq_lens,
+                            int32_t num_seqs, int64_t q_seq_stride, int32_t num_q_heads,
+                            int32_t num_kv_heads, int32_t head_dim, int32_t block_size, int32_t dtype,
+                            int32_t split_tokens, int32_t decode_heads_per_wg, int32_t window,
+                            int32_t sinks) {
   if (!out) return fail(GLLM_ATTN_EINVAL, "plan out-pointer is null");
   *out = nullptr;
   if (num_seqs < 0 || (num_seqs > 0 && (!query_lens || !seq_lens)))
@@ -791,6 +793,7 @@ int gllm_attn_plan_create_window(gllm_attn_plan** out, const int32_t* query_lens
 
   gllm_attn_plan* p = new (std::nothrow) gllm_attn_plan();
   if (!p) return fail(GLLM_ATTN_EINVAL, "out of host memory");
+  std::unique_ptr<gllm_attn_plan> owner(p);   // nothing is staged before the last return: a plain delete frees it all
   p->num_seqs = num_seqs; p->Hq = num_q_heads; p->Hkv = num_kv_heads; p->D = head_dim;
   p->bs = block_size; p->dtype = dtype; p->mfma = mfma;
   if (hides) {
@@ -802,11 +805,9 @@ int gllm_attn_plan_create_window(gllm_attn_plan** out, const int32_t* query_lens
   for (int i = 0; i < num_seqs; ++i) {
     const int32_t ql = query_lens[i], sl = seq_lens[i];
     if (ql < 1 || sl < ql) {
-      delete p;
       return fail(GLLM_ATTN_EINVAL, "sequence %d: query_len %d / seq_len %d invalid", i, ql, sl);
     }
     if (q_seq_stride > 0 && ql > q_seq_stride) {
-      delete p;
       return fail(GLLM_ATTN_EINVAL, "sequence %d: query_len %d exceeds q_seq_stride %lld", i, ql, (long long)q_seq_stride);
     }
     SeqInfo& s = p->seqs[i];
@@ -824,7 +825,6 @@ int gllm_attn_plan_create_window(gllm_attn_plan** out, const int32_t* query_lens
   }
   p->total_rows = q_seq_stride > 0 ? (int64_t)num_seqs * q_seq_stride : row;
   if (p->total_rows > INT32_MAX) {
-    delete p;
     return fail(GLLM_ATTN_EINVAL, "too many query rows");
   }
 
@@ -864,7 +864,6 @@ int gllm_attn_plan_create_window(gllm_attn_plan** out, const int32_t* query_lens
         p->n_prefill_seqs = (int32_t)n_pf;
         plan_mixed_prefill(p, pcs);
         if (p->items.size() + p->seg_ptr.size() > (size_t)INT32_MAX) {
-          delete p;
           return fail(GLLM_ATTN_EINVAL, "too many work items");
         }
       }
@@ -1192,7 +1191,6 @@ int gllm_attn_plan_create_window(gllm_attn_plan** out, const int32_t* query_lens
     p->items.reserve(all.size());
     for (auto& k : all) p->items.push_back(k.it);
     if (p->items.size() > (size_t)INT32_MAX) {
-      delete p;
       return fail(GLLM_ATTN_EINVAL, "too many work items");
     }
     }
@@ -1215,14 +1213,12 @@ int gllm_attn_plan_create_window(gllm_attn_plan** out, const int32_t* query_lens
     }
     std::stable_sort(tiles.begin(), tiles.end(), [](const Keyed& x, const Keyed& y) { return x.kend > y.kend; });
     if (tiles.size() > (size_t)INT32_MAX) {
-      delete p;
       return fail(GLLM_ATTN_EINVAL, "too many work items");
     }
     p->items.reserve(tiles.size());
     for (const Keyed& k : tiles) p->items.push_back(k.it);
   }
   if (p->n_partials > (int64_t)INT32_MAX / 16) {
-    delete p;
     return fail(GLLM_ATTN_EINVAL, "too many split partials");
   }
 
@@ -1246,7 +1242,6 @@ int gllm_attn_plan_create_window(gllm_attn_plan** out, const int32_t* query_lens
       p->pinned = std::malloc(stage);
       p->pinned_is_host_malloc = true;
       if (!p->pinned) {
-        delete p;
         return fail(GLLM_ATTN_EINVAL, "out of host memory for %zu staging bytes", stage);
       }
     }
@@ -1259,8 +1254,21 @@ int gllm_attn_plan_create_window(gllm_attn_plan** out, const int32_t* query_lens
     if (!p->merge.empty())
       std::memcpy((char*)p->pinned + p->off_merge, p->merge.data(), p->merge.size() * sizeof(MergeInfo));
   }
-  *out = p;
+  *out = owner.release();
   return ok();
+}
+
+int gllm_attn_plan_create_window(gllm_attn_plan** out, const int32_t* query_lens, const int32_t* seq_lens,
+                                 int32_t num_seqs, int64_t q_seq_stride, int32_t num_q_heads,
+                                 int32_t num_kv_heads, int32_t head_dim, int32_t block_size, int32_t dtype,
+                                 int32_t split_tokens, int32_t decode_heads_per_wg, int32_t window,
+                                 int32_t sinks) {
+  try {
+    return plan_create_impl(out, query_lens, seq_lens, num_seqs, q_seq_stride, num_q_heads, num_kv_heads, head_dim,
+                            block_size, dtype, split_tokens, decode_heads_per_wg, window, sinks);
+  } catch (const std::exception& e) {              // no exception leaves a C entry
+    return fail(GLLM_ATTN_EINVAL, "plan: %s", e.what());
+  }
 }
 
 size_t gllm_attn_plan_workspace_bytes(const gllm_attn_plan* p) { return p ? p->ws_bytes : 0; }

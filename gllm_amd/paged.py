@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import operator
 
 import torch
 import torch.nn.functional as F
@@ -196,6 +197,11 @@ def rotary_kv_write(k: torch.Tensor | None, v: torch.Tensor | None, positions: t
     if x is None or (k is None) != (v is None) or (q is None) != (q_out is None):
         raise ValueError("k and v, and q and q_out, go together; at least one pair is needed")
     shape, dtype, dev = x.shape, x.dtype, x.get_device()
+    if len(shape) < 2 or q is not None and q.dim() < 2 or not shape[-2]:
+        raise ValueError("expected [..., heads, head_dim] rows")
+    if dev >= 0 and dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return rotary_kv_write(k, v, positions, rotary, k_cache, v_cache, slot_mapping, query_lens, q, q_out)
     D, H = shape[-1], shape[-2]
     if D != rotary.head_dim:
         raise ValueError(f"head_dim {D}, the rotary positions are for {rotary.head_dim}")
@@ -275,6 +281,10 @@ def kv4_values(cache: torch.Tensor, slots: torch.Tensor, head_dim: int, dtype: t
     """Rows of a 4-bit cache (:data:`KV4`) as the values they stand for, in
     ``dtype``: ``[N, Hkv, head_dim]`` for int64 ``slots [N]`` (zeros for a slot
     outside the cache).  For moving rows to another cache or looking at them."""
+    dev = cache.get_device()
+    if dev >= 0 and dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return kv4_values(cache, slots, head_dim, dtype, out)
     nb, Hkv = cache.shape[0], cache.shape[1] if cache.dim() == 3 else 0
     bs = _kv4_block_size(cache, Hkv, head_dim)
     sl = _index_rows(slots)
@@ -363,6 +373,8 @@ def qkv_rope_kv_write(x: torch.Tensor, w_q: torch.Tensor | None, w_k: torch.Tens
         raise ValueError("x rows must be contiguous")
     n = xs.shape[0]
     for t, nm in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+        if t.dtype == KV4:
+            raise ValueError(f"{nm}: 4-bit caches are written by rope_kv_write and rotary_kv_write")
         if t.dim() != 3 or t.stride()[1:] != (t.shape[2], 1):
             raise ValueError(f"{nm}: expected [num_slots, Hkv, D] with contiguous rows")
     if k_cache.shape != v_cache.shape or k_cache.stride(0) != v_cache.stride(0):
@@ -517,6 +529,7 @@ class AttentionPlan:
         sl = [int(x) for x in seq_lens]
         if len(ql) != len(sl):
             raise ValueError("query_lens and seq_lens differ in length")
+        window, sinks = None if window is None else operator.index(window), operator.index(sinks)
         if window is not None and not 1 <= window < 1 << 31:
             raise ValueError(f"window {window} must be at least 1 (None: no window)")
         if not 0 <= sinks < 1 << 31 or (sinks and window is None):

@@ -35,7 +35,8 @@ class Rotary:
       those that make more than ``high_freq_factor`` are kept, in between both
       are blended;
     - ``yarn``: the same by pair index between ``beta_slow`` (1) and ``beta_fast``
-      (32) turns, and cos and sin times ``attention_factor`` (0.1 ln factor + 1).
+      (32) turns, and cos and sin times ``attention_factor`` (0.1 ln factor + 1);
+      ``mscale``, ``mscale_all_dim`` and ``truncate=False`` are refused.
 
     ``freq``: radians per position of each pair, float64 on ``device``;
     ``factor``: of cos and sin.
@@ -59,6 +60,9 @@ class Rotary:
             return base
         if kind not in ("linear", "llama3", "yarn"):
             raise NotImplementedError(f"rope scaling {kind!r} (linear, llama3, yarn)")
+        part = scaling.get("partial_rotary_factor")
+        if scaling.get("rope_theta", theta) != theta or part is not None and int(self.head_dim * part) != self.rotary_dim:
+            raise ValueError(f"rope scaling {scaling!r}: not the theta {theta}, rotary_dim {self.rotary_dim} given")
         f = _need(scaling, "factor")
         if kind == "linear":
             return base / f
@@ -70,7 +74,8 @@ class Rotary:
             keep = ((orig * base / (2 * math.pi) - lo) / (hi - lo)).clamp(0, 1)
         else:
             R = self.rotary_dim
-
+            if scaling.get("mscale") or scaling.get("mscale_all_dim") or scaling.get("truncate") is False:
+                raise NotImplementedError(f"rope scaling {scaling!r}: mscale, mscale_all_dim and truncate=False")
             def index(turns: float) -> float:          # the pair that makes so many turns
                 return R * math.log(orig / (turns * 2 * math.pi)) / (2 * math.log(theta))
             if theta <= 1:
@@ -79,8 +84,8 @@ class Rotary:
                           for k, d in (("beta_fast", 32.0), ("beta_slow", 1.0)))
             lo, hi = max(math.floor(index(fast)), 0), min(math.ceil(index(slow)), R - 1)
             keep = 1 - ((torch.arange(R // 2, dtype=torch.float64) - lo) / max(hi - lo, 0.001)).clamp(0, 1)
-            m = scaling.get("attention_factor")
-            self.factor = (0.1 * math.log(f) + 1.0 if f > 1 else 1.0) if m is None else float(m)
+            self.factor = _need(scaling, "attention_factor") if scaling.get("attention_factor") is not None \
+                else 0.1 * math.log(f) + 1.0 if f > 1 else 1.0
         return base * (keep + (1 - keep) / f)
 
     def tables(self, positions: int, dtype: torch.dtype):

@@ -66,6 +66,26 @@ def test_rotary_refuses_other_schedules():
         gllm_amd.Rotary(128, device="cpu", scaling={"rope_type": "dynamic", "factor": 2.0})
 
 
+def test_rotary_refuses_what_it_would_ignore():
+    """Keys of a configuration that change the rotation are taken or refused."""
+    for kw in (dict(rope_theta=500.0), dict(partial_rotary_factor=0.5), dict(attention_factor=-1.0)):
+        with pytest.raises(ValueError):
+            gllm_amd.Rotary(128, device="cpu", scaling=dict(YARN, **kw))
+    for kw in (dict(mscale=1.0), dict(mscale_all_dim=0.707), dict(truncate=False)):
+        with pytest.raises(NotImplementedError):
+            gllm_amd.Rotary(128, device="cpu", scaling=dict(YARN, **kw))
+    same = gllm_amd.Rotary(128, theta=500.0, rotary_dim=32, device="cpu",
+                           scaling=dict(LLAMA3, rope_theta=500.0, partial_rotary_factor=0.25))
+    assert torch.equal(same.freq, gllm_amd.Rotary(128, theta=500.0, rotary_dim=32, device="cpu", scaling=LLAMA3).freq)
+
+
+@pytest.mark.parametrize("kw", [dict(k=torch.zeros(6, 0, 64), v=torch.zeros(6, 0, 64)), dict(q=torch.zeros(64)),
+                                dict(k=torch.zeros(64), v=torch.zeros(64))])
+def test_rotary_kv_write_refuses_rows_without_heads(kw):
+    with pytest.raises(ValueError):
+        paged.rotary_kv_write(**_args(**kw))
+
+
 def _args(**kw):
     n, Hq, Hkv, D = 6, 4, 2, 64
     a = dict(k=torch.zeros(n, Hkv, D), v=torch.zeros(n, Hkv, D), positions=torch.arange(n),

@@ -156,3 +156,24 @@ def test_fused_kv_write_and_windows():
     assert not paged.fused_kv_write_ok(plan(torch.float32, 10), torch.float32)
     assert paged.fused_kv_write_ok(plan(torch.float32, None), torch.float32)
     assert not paged.fused_kv_write_ok(plan(torch.bfloat16, None), paged.KV4)
+
+
+def test_windows_are_integers():
+    for kw in (dict(window=4.0), dict(window="4"), dict(window=4, sinks=1.5)):
+        with pytest.raises(TypeError):
+            _plan(**kw)
+
+
+def test_sinks_without_a_window_are_refused_with_a_kept_plan():
+    """An earlier layer's plan on the metadata is no answer to other arguments."""
+    from gllm_amd import attention
+    meta = types.SimpleNamespace(_gllm_plan="plan", _gllm_window_plans={(4, 1): "windowed"})
+    assert attention._kept_plan(meta, None, 0) == "plan" and attention._kept_plan(meta, 4, 1) == "windowed"
+    assert attention._kept_plan(meta, None, 2) is None and attention._kept_plan(meta, 4, 0) is None
+
+
+def test_projections_refuse_4_bit_caches():
+    cache = torch.zeros(4, 2, paged.kv4_record_bytes(16, 64), dtype=torch.uint8)
+    w, cs = torch.zeros(128, 64, dtype=torch.bfloat16), torch.zeros(3, 32, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="4-bit"):
+        paged.qkv_rope_kv_write(torch.zeros(3, 64, dtype=torch.bfloat16), w, w, w, cs, cs, cache, cache, torch.arange(3))
