@@ -210,6 +210,62 @@ def test_strided_rows_in_place_and_many_tokens():
     assert torch.equal(vc.cpu(), x0[:, 6:]) and torch.equal(x[:, 4:].cpu(), x0[:, 4:])
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("kv", ["same", "4"])
+def test_rows_at_odd_places(dtype, kv):
+    """Rows that start one element off any vector's alignment, at odd strides."""
+    n, D = 9, 64
+    g = torch.Generator().manual_seed(4)
+    flat = torch.randn(n * (6 * D + 5) + 1, generator=g).to(dtype)
+    def rows(t, first, heads):
+        return t.as_strided((n, heads, D), (6 * D + 5, D, 1), 1 + first * D)
+    q, k, v = (rows(flat, *x) for x in ((0, 2), (2, 2), (4, 2)))
+    rot = gllm_amd.Rotary(D, rotary_dim=32, device=DEV)
+    pos, slots = torch.arange(n) * 31, torch.arange(n) + 7
+    kc, vc = _pool(32, 2, D, dtype if kv == "same" else kv, 16, g), _pool(32, 2, D, dtype if kv == "same" else kv, 16, g)
+    dflat, dk, dv = flat.to(DEV), kc.to(DEV), vc.to(DEV)
+    dq, dkk, dvv = (rows(dflat, *x) for x in ((0, 2), (2, 2), (4, 2)))
+    out_flat = torch.zeros_like(dflat)
+    out = rows(out_flat, 0, 2)
+    paged.rotary_kv_write(dkk, dvv, pos.to(DEV), rot, dk, dv, slots.to(DEV), q=dq, q_out=out)
+    torch.cuda.synchronize()
+    _close(out, _exact(q, pos, rot), _size(q, rot), dtype, 3)
+    keep = torch.ones_like(flat, dtype=torch.bool)
+    rows(keep, 0, 2)[:] = False
+    assert (out_flat.cpu()[keep] == 0).all()
+    if kv == "4":
+        kv4.write(kc, slots, _exact(k, pos, rot), 16)
+        kv4.write(vc, slots, v, 16)
+        assert torch.equal(dk.cpu(), kc) and torch.equal(dv.cpu(), vc)
+    else:
+        _close(dk[slots.to(DEV)], _exact(k, pos, rot), _size(k, rot), dtype, 2.0 ** -20)
+        assert torch.equal(dv.cpu()[slots], v)
+
+
+def test_two_streams():
+    """Calls on streams of their own do not meet."""
+    parts = []
+    for seed in (1, 2):
+        q, k, v, pos, g = _inputs(500, 4, 2, 128, BF, seed)
+        parts.append((q.to(DEV), k.to(DEV), v.to(DEV), pos.to(DEV)))
+    rot = gllm_amd.Rotary(128, device=DEV)
+    slots = torch.arange(500, device=DEV)
+
+    def pools():
+        return [torch.zeros(32, 2, kv4.record_bytes(16, 128), dtype=torch.uint8, device=DEV) for _ in range(4)]
+    want, got = pools(), pools()
+    for i, (q, k, v, pos) in enumerate(parts):
+        paged.rotary_kv_write(k, v, pos, rot, want[2 * i], want[2 * i + 1], slots)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in parts]
+    for _ in range(5):
+        for i, ((q, k, v, pos), st) in enumerate(zip(parts, streams)):
+            with torch.cuda.stream(st):
+                paged.rotary_kv_write(k, v, pos, rot, got[2 * i], got[2 * i + 1], slots)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
 def test_infinities_stay_in_their_block():
     q, k, v, pos, g = _inputs(4, 2, 2, 128, BF, 5)
     k[0, 1, 3], v[1, 0, 40], v[2, 1, 100] = math.inf, math.nan, -math.inf

@@ -80,6 +80,28 @@ def test_mixed(D, split):
         b.check(_run(b, window, sinks, split_tokens=split), window, sinks, "mixed")
 
 
+def _many(kind, D, kv, seed):
+    """Batches large enough for the plans that small ones never get."""
+    if kind == "half prefill":                # 1,024 (head dim 128) / 768 items: half-size workgroups
+        n = 128 if D == 128 else 96
+        return Batch([40 * (i % 5) for i in range(n)], [33 + (7 * i) % 32 for i in range(n)], Hq=32, Hkv=8, D=D, kv=kv, seed=seed)
+    if kind == "half mixed":                  # 200 decodes beside three chunks
+        return Batch([150 + (37 * i) % 200 for i in range(200)] + [0, 70, 200], [1] * 200 + [40, 64, 33], Hq=32, Hkv=8, D=D,
+                     kv=kv, seed=seed)
+    return Batch([100 + (37 * i) % 300 for i in range(140)], [1] * 140, Hq=32, Hkv=8, D=D, kv=kv, seed=seed)
+
+
+@pytest.mark.parametrize("kind", ["half prefill", "half mixed", "balanced"])
+@pytest.mark.parametrize("D,kv", [(64, BF), (128, BF), (128, F8), (128, "4"), (64, "4")])
+def test_plans_of_large_batches(kind, D, kv):
+    print(f"{kind} D={D} kv={kv}", flush=True)
+    b = _many(kind, D, kv, D)
+    plan = _plan(b, 90, 3)
+    assert plan.info["prefill_waves"] == 4 if kind == "half prefill" else plan.info["prefill_waves"] == 8
+    assert (plan.info["decode_segments"] > 0) == (kind == "balanced" and D == 128)
+    b.check(_run(b, 90, 3), 90, 3, kind)
+
+
 @pytest.mark.parametrize("dtype,kv,D", [(F32, F32, 64), (F32, F8, 128), (F32, BF, 50), (BF, BF, 96), (F16, F16, 256),
                                         (BF, F32, 64), (F32, F32, 2)])
 def test_generic(dtype, kv, D):
