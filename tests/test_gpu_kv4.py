@@ -3,10 +3,12 @@ that the cache stands for."""
 import pytest
 import torch
 
+import gllm_amd
 from gllm_amd import paged
 from oracle import kv4
 from oracle import rope as orope
-from tests.window_helpers import BF, F16, F32, Batch
+from oracle import window as ow
+from tests.window_helpers import BF, F8, F16, F32, Batch
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -118,6 +120,85 @@ def test_generic(dtype, D, window, sinks):
 def test_generic_many_rows():
     b = Batch([0, 64] * 8, [70, 90] * 8, Hq=32, Hkv=8, D=64, dtype=F32, kv="4", seed=1)
     b.check(_run(b), None, 0, "kv4 generic, many rows")
+
+
+@pytest.mark.parametrize("kv,D,dtype", [("4", 64, BF), ("4", 128, F16), ("4", 96, F32), (BF, 64, BF), (F8, 128, BF), (F32, 64, F32)])
+@pytest.mark.parametrize("bs", [16, 7])
+def test_nan_in_slots_that_no_row_sees(kv, D, dtype, bs):
+    """Slots behind a sequence's end and beside its window, in blocks that
+    hold visible keys too, may hold anything."""
+    for ctx, ql in (([0, 3, 40, 299, 1000], [1] * 5), ([0, 37, 500, 5], [150, 77, 40, 1]), ([700, 0], [70, 5])):
+        for window, sinks in ((1, 0), (21, 3), (130, 40)) + (((None, 0),) if kv == "4" else ()):
+            print(f"unseen NaN {kv} D={D} bs={bs} window={window} {ctx}", flush=True)
+            b = Batch(ctx, ql, D=D, dtype=dtype, kv=kv, bs=bs, seed=D + bs)
+            want = _run(b, window, sinks)
+            b.check(want, window, sinks, "seen")
+            bad = torch.ones(b.nb * bs, dtype=torch.bool)
+            for i, (c, n) in enumerate(zip(ctx, ql)):
+                t = torch.cat([ow.visible(c + r, window, sinks) for r in range(n)])
+                bad[b.bt[i, t // bs].long() * bs + t % bs] = False
+            bad = bad.nonzero()[:, 0]
+            for c in (b.kc, b.vc):
+                if kv == "4":
+                    kv4.views(c, bs, D)[1][bad // bs, :, bad % bs] = 255
+                else:
+                    c[bad] = float("nan")
+            assert torch.equal(_run(b, window, sinks), want)
+
+
+@pytest.mark.parametrize("D,dtype", [(64, BF), (128, F16), (128, F32)])
+def test_blocks_past_4_gib(D, dtype):
+    """A pool of more than 4 GiB a tensor: blocks at byte 2^31 and behind 2^32,
+    written, read back and attended to."""
+    b = Batch([0, 60, 200], [40, 1, 1], Hq=8, Hkv=8, D=D, dtype=dtype, kv="4", seed=D)
+    rec = kv4.record_bytes(16, D)
+    nb = (1 << 32) // (8 * rec) + b.nb + 7
+    far = torch.tensor([nb - 1 - i if i % 3 else (1 << 31) // (8 * rec) + i for i in range(b.nb)])
+    print(f"far blocks D={D} {dtype}: {nb} blocks", flush=True)
+    kc, vc = (torch.empty(nb, 8, rec, dtype=torch.uint8, device=DEV) for _ in range(2))
+    kc[far.to(DEV)], vc[far.to(DEV)] = b.kc.to(DEV), b.vc.to(DEV)
+    bt = far[b.bt.long().clamp(0, b.nb - 1)].int()
+    for window, sinks in ((None, 0), (50, 2)):
+        b.check(_run(b, window, sinks, bt, kc, vc), window, sinks, "far")
+    g = torch.Generator().manual_seed(1)
+    k, v = (torch.randn(16, 8, D, generator=g).to(dtype) for _ in range(2))
+    slots = (nb - 1) * 16 + torch.arange(16)
+    rot = gllm_amd.Rotary(D, device=DEV)
+    zero = torch.zeros(16, dtype=torch.int64, device=DEV)
+    paged.rotary_kv_write(k.to(DEV), v.to(DEV), zero, rot, kc, vc, slots.to(DEV))
+    small_k, small_v = (torch.zeros(1, 8, rec, dtype=torch.uint8) for _ in range(2))
+    kv4.write(small_k, torch.arange(16), k, 16)
+    kv4.write(small_v, torch.arange(16), v, 16)
+    n = 16 * (D // 32 * 17)                     # a record without its padding
+    assert torch.equal(kc[-1:, :, :n].cpu(), small_k[..., :n]) and torch.equal(vc[-1:, :, :n].cpu(), small_v[..., :n])
+    got = paged.kv4_values(kc, slots.to(DEV), D, torch.float32).cpu()
+    assert torch.equal(got.double(), kv4.read(small_k, torch.arange(16), 16, D))
+
+
+def test_graph_replays():
+    """A mixed batch over a 4-bit cache and a decode with splits, captured on one
+    stream and replayed with eager calls between, on another."""
+    cases = []
+    for ctx, ql in (([0, 37, 1000, 700], [150, 77, 1, 1]), ([2500, 40], [1, 1])):
+        b = Batch(ctx, ql, D=128, kv="4", seed=12)
+        q, kc, vc, bt = (x.to(DEV) for x in (b.q, b.kc, b.vc, b.bt))
+        cases.append((_plan(b), q, kc, vc, bt, torch.empty_like(q)))
+    for plan, q, kc, vc, bt, out in cases:
+        paged.paged_attention(plan, q, kc, vc, bt, out=out)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        for plan, q, kc, vc, bt, out in cases:
+            paged.paged_attention(plan, q, kc, vc, bt, out=out)
+    for i in range(3):
+        want = []
+        for plan, q, kc, vc, bt, out in cases:
+            q.mul_(-0.5)
+            want.append(paged.paged_attention(plan, q, kc, vc, bt))
+            out.fill_(7.0)
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(c[-1], w) for c, w in zip(cases, want))
 
 
 def test_refusals():
