@@ -115,5 +115,10 @@ def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def raw_stream(index: int) -> int:
+    """:func:`stream_ptr` of the device of a tensor's ``get_device()``."""
+    return torch._C._cuda_getCurrentRawStream(index) if index >= 0 else stream_ptr(torch.device("cpu"))
+
+
 def ptr(t) -> int | None:
     return None if t is None else t.data_ptr()

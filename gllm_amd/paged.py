@@ -207,9 +207,10 @@ def rotary_kv_write(k: torch.Tensor | None, v: torch.Tensor | None, positions: t
         raise ValueError(f"head_dim {D}, the rotary positions are for {rotary.head_dim}")
     n = x.numel() // (H * D)
     freq = rotary.freq
-    pos = positions if positions.dim() == 1 and positions.dtype == torch.int64 and positions.is_contiguous() \
-        else _index_rows(positions)
-    if positions.dtype.is_floating_point or pos.numel() != n:
+    pos, kind = positions, positions.dtype
+    if kind != torch.int64 or not pos.is_contiguous():
+        pos = _index_rows(pos)
+    if pos.numel() != n or kind.is_floating_point:
         raise ValueError("positions must be integers, one per token")
     ks = vs = qs = qos = stride = num_slots = bs = 0
     Hq = Hkv = 1
@@ -222,7 +223,8 @@ def rotary_kv_write(k: torch.Tensor | None, v: torch.Tensor | None, positions: t
         Hkv = H
         if v.shape != shape or v.dtype != dtype:
             raise ValueError("k and v shapes or dtypes differ")
-        ks, vs = _row_stride(k, shape, Hkv, D, "k"), _row_stride(v, shape, Hkv, D, "v")
+        ks = Hkv * D if k.is_contiguous() else _rows(k, Hkv, D, "k")     # k's and v's heads and dims are the shape's
+        vs = Hkv * D if v.is_contiguous() else _rows(v, Hkv, D, "v")
         cdtype, cshape, cstride = k_cache.dtype, k_cache.shape, k_cache.stride()
         if v_cache.shape != cshape or v_cache.stride() != cstride or v_cache.dtype != cdtype:
             raise ValueError("k_cache and v_cache must have the same shape, dtype and strides")
@@ -236,7 +238,9 @@ def rotary_kv_write(k: torch.Tensor | None, v: torch.Tensor | None, positions: t
             num_slots = cshape[0]
             kv_code = _lib.dtype_code(cdtype)
         stride = cstride[0]
-        sm = slot_mapping if slot_mapping.dim() == 1 else slot_mapping.reshape(-1)
+        sm = slot_mapping
+        if not sm.is_contiguous() and sm.dim() != 1:
+            sm = sm.reshape(-1)
         if sm.dtype != torch.int64 or sm.numel() != n or not sm.is_contiguous():
             raise ValueError("slot_mapping must be contiguous int64 with one entry per token")
         same = same and v.get_device() == dev and k_cache.get_device() == dev and v_cache.get_device() == dev \
@@ -264,7 +268,7 @@ def rotary_kv_write(k: torch.Tensor | None, v: torch.Tensor | None, positions: t
     _lib.check(_lib.load().gllm_rotary_kv_write(
         qp, qop, kp, vp, kcp, vcp, smp, qlp, tps, freq.data_ptr(), rotary.factor, pos.data_ptr(), rotary.rotary_dim,
         rotary.interleaved, n, Hq, Hkv, D, qs, ks, vs, qos, stride, num_slots, bs, _lib.dtype_code(dtype), kv_code,
-        _lib.stream_ptr(x.device)))
+        _lib.raw_stream(dev)))
 
 
 def rotary_rotate(x: torch.Tensor, positions: torch.Tensor, rotary, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -285,21 +289,23 @@ def kv4_values(cache: torch.Tensor, slots: torch.Tensor, head_dim: int, dtype: t
     if dev >= 0 and dev != torch.cuda.current_device():
         with torch.cuda.device(dev):
             return kv4_values(cache, slots, head_dim, dtype, out)
-    nb, Hkv = cache.shape[0], cache.shape[1] if cache.dim() == 3 else 0
+    shape = cache.shape
+    nb, Hkv = shape[0], shape[1] if len(shape) == 3 else 0
     bs = _kv4_block_size(cache, Hkv, head_dim)
-    sl = _index_rows(slots)
-    if sl.get_device() != cache.get_device() or out is not None and out.get_device() != cache.get_device():
+    sl = slots if slots.dtype == torch.int64 and slots.is_contiguous() else _index_rows(slots)
+    if sl.get_device() != dev or out is not None and out.get_device() != dev:
         raise ValueError(f"slots and out must be on the cache's device {cache.device}")
+    n, stride = sl.numel(), Hkv * head_dim
     if out is None:
-        out = torch.empty(sl.numel(), Hkv, head_dim, dtype=dtype, device=cache.device)
-    elif out.dtype != dtype or out.numel() != sl.numel() * Hkv * head_dim:
+        out = torch.empty((n, Hkv, head_dim), dtype=dtype, device=cache.device)
+    elif out.dtype != dtype or out.numel() != n * stride:
         raise ValueError(f"out must be {dtype} with one row per slot")
-    stride = _row_stride(out, out.shape, Hkv, head_dim, "out")
-    if sl.numel() == 0:
+    else:
+        stride = _row_stride(out, out.shape, Hkv, head_dim, "out")
+    if n == 0:
         return out
-    _lib.check(_lib.load().gllm_kv4_values(cache.data_ptr(), cache.stride(0), nb * bs, bs, sl.data_ptr(), sl.numel(), Hkv,
-                                           head_dim, out.data_ptr(), stride, _lib.dtype_code(dtype),
-                                           _lib.stream_ptr(cache.device)))
+    _lib.check(_lib.load().gllm_kv4_values(cache.data_ptr(), cache.stride(0), nb * bs, bs, sl.data_ptr(), n, Hkv, head_dim,
+                                           out.data_ptr(), stride, _lib.dtype_code(dtype), _lib.raw_stream(dev)))
     return out
 
 
