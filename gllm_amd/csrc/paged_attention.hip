@@ -326,7 +326,7 @@ __device__ __forceinline__ void decode_task(const AttnArgs& a, const DecodeTask&
       u32x4 k[2], v[2];
       uint32_t ks[2], vs[2];
     } ring[PF + 1];
-    uint32_t place_lo = 0, place_hi = 0, place_row = 0;
+    uint32_t place_lo = 0, place_hi = 0, place_sc = 0;   // the sub-tile's codes; from there to its scales
     const uint32_t code_l = n * (D / 2) + D / 8 * grp, sc_l = n * (D / 32) + D / 4 * grp / 32;
     const char* const ks0 = (const char*)a.k_cache;
     const char* const vs0 = (const char*)a.v_cache;
@@ -336,40 +336,54 @@ __device__ __forceinline__ void decode_task(const AttnArgs& a, const DecodeTask&
       const int blk = both && v >= sk.from ? blk0 + bgap : blk0;
       const int key = key_of(v);
       const uint32_t bi = div_bs((uint32_t)key, a.block_magic, a.block_shift);
-      place_row = (uint32_t)key - bi * (uint32_t)a.block_size;
-      const uint64_t at = (uint64_t)(uint32_t)lbid[bi - blk] * sbytes + head_s + place_row * (D / 2);
+      const uint32_t row = (uint32_t)key - bi * (uint32_t)a.block_size;
+      const uint64_t at = (uint64_t)(uint32_t)lbid[bi - blk] * sbytes + head_s + row * (D / 2);
+      place_sc = (uint32_t)a.block_size * (D / 2) - row * (D / 2 - D / 32);
       place_lo = (uint32_t)at;
       place_hi = (uint32_t)(at >> 32);
     };
+    // Most steps need no bounds: their 32 keys lie in the range and every row sees
+    // them.  One scalar test a step, instead of two a sub-tile for its loads and
+    // two for its masks.
+    const int seen_from = tk.ctx_len + tk.q_len - a.window;        // first key that the last row's window holds
+    const int clo = seen_from > 0 ? max(sk.from, seen_from - sk.by) : 0;
+    const uint32_t clean_n = (uint32_t)max(min(kend - 32, tk.ctx_len - 31 - sk.by) - clo + 1, 0);
+    auto clean = [&](int kb) { return (uint32_t)(kb - clo) < clean_n; };
     auto issue_one = [&](int t, Step& x) {
       if (t > 0 && (t & 31) == 0) places(t);
+      const int kb = kbeg + 32 * (kis + KW * t);
+      uint32_t cl[2] = {code_l, code_l}, sl[2] = {sc_l, sc_l};
+      if (!clean(kb)) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int v = min(kb + 16 * u, (kend - 1) & ~15), kr = key_of(v);
+          // the rows that may be read: none past the range (steps past the last one
+          // take one line), none between the sinks and the first row's window
+          const int last = t < ntw ? kend - 1 - v : 0;
+          const int nn = seen_key(kr + min(n, last), sk, a.sinks) - kr;
+          cl[u] += (nn - n) * (D / 2);
+          sl[u] += (nn - n) * (D / 32);
+        }
+      }
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const int i = 2 * (t & 31) + u;
         const uint64_t at = (uint64_t)(uint32_t)__builtin_amdgcn_readlane(place_hi, i) << 32 |
                             (uint32_t)__builtin_amdgcn_readlane(place_lo, i);
-        const uint32_t row = __builtin_amdgcn_readlane(place_row, i);
-        const uint64_t sc = at + (uint32_t)a.block_size * (D / 2) - row * (D / 2 - D / 32);   // the record's scales
-        const int v = min(kbeg + 32 * (kis + KW * t) + 16 * u, (kend - 1) & ~15), kr = key_of(v);
-        // the rows that may be read: none past the range (steps past the last one
-        // take one line), none between the sinks and the first row's window
-        const int last = t < ntw ? kend - 1 - v : 0;
-        uint32_t cl = code_l, sl = sc_l;
-        if (last < 15 || (kr < sk.first && kr + 15 >= a.sinks)) {
-          const int nn = seen_key(kr + min(n, last), sk, a.sinks) - kr;
-          cl += (nn - n) * (D / 2);
-          sl += (nn - n) * (D / 32);
-        }
+        const uint32_t to_sc = __builtin_amdgcn_readlane(place_sc, i);
+        const char *kp = ks0 + at, *vp = vs0 + at;
         if constexpr (D == 128) {
-          x.k[u] = ld16(ks0 + at + cl);
-          x.v[u] = ld16(vs0 + at + cl);
+          x.k[u] = ld16(kp + cl[u]);
+          x.v[u] = ld16(vp + cl[u]);
         } else {
-          const u32x2 k2 = *reinterpret_cast<const u32x2*>(ks0 + at + cl), v2 = *reinterpret_cast<const u32x2*>(vs0 + at + cl);
+          const u32x2 k2 = *reinterpret_cast<const u32x2*>(kp + cl[u]), v2 = *reinterpret_cast<const u32x2*>(vp + cl[u]);
           x.k[u] = u32x4{k2[0], k2[1], 0u, 0u};
           x.v[u] = u32x4{v2[0], v2[1], 0u, 0u};
         }
-        x.ks[u] = (uint8_t)ks0[sc + sl];
-        x.vs[u] = (uint8_t)vs0[sc + sl];
+        kp += to_sc;
+        vp += to_sc;
+        x.ks[u] = (uint8_t)kp[sl[u]];
+        x.vs[u] = (uint8_t)vp[sl[u]];
       }
     };
     auto issue_any = [&](int t, Step& x) {
@@ -394,8 +408,9 @@ __device__ __forceinline__ void decode_task(const AttnArgs& a, const DecodeTask&
         x.vs[u] = (uint8_t)vc[sc];
       }
     };
-    auto compute = [&](int t, const Step& x) {
-      const int kb = t < ntw ? kbeg + 32 * (kis + KW * t) : kend;   // past the last one: fully masked
+    float nmu = 0.f;                       // -m, or 0 before the first visible key
+    auto compute = [&](int t, const Step& x) {           // t < ntw
+      const int kb = kbeg + 32 * (kis + KW * t);
       f32x4 s[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u) s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -411,12 +426,10 @@ __device__ __forceinline__ void decode_task(const AttnArgs& a, const DecodeTask&
           *reinterpret_cast<u32x4*>(ldsV + (16 * u + n) * RB + chunk_dim<D, KF>(kk, grp) * 2) =
               fp4x8_to<T>(x.v[u][kk], __uint_as_float(x.vs[u] << 23));
       // lane holds S[key kb + 16u + 4grp + j][row n]
-      float tmax = kNegInf;
+      if (!clean(kb)) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int vb = kb + 16 * u, kr = key_of(vb);   // a sub-tile lies on one side of the left-out keys
-        // past the range, past the first row, or before the last row's window
-        if (vb + 16 > kend || kr + 15 > tk.ctx_len || (kr <= tk.ctx_len + tk.q_len - 1 - a.window && kr + 16 > a.sinks)) {
+        for (int u = 0; u < 2; ++u) {
+          const int vb = kb + 16 * u, kr = key_of(vb);   // a sub-tile lies on one side of the left-out keys
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int key = kr + 4 * grp + j;
@@ -424,9 +437,17 @@ __device__ __forceinline__ void decode_task(const AttnArgs& a, const DecodeTask&
             s[u][j] = hid ? kNegInf : s[u][j];
           }
         }
-        tmax = fmaxf(tmax, fmaxf(fmaxf(s[u][0], s[u][1]), fmaxf(s[u][2], s[u][3])));
       }
-      tmax = max_xor32(max_xor16(tmax)) * sl2;
+      // maximum, which a NaN passes through (its row is NaN either way), takes no
+      // instruction to quiet its arguments
+      const auto mx = [](float p, float q) { return __builtin_elementwise_maximum(p, q); };
+      float tmax = mx(mx(mx(s[0][0], s[0][1]), mx(s[0][2], s[0][3])), mx(mx(s[1][0], s[1][1]), mx(s[1][2], s[1][3])));
+      {
+        const auto r16 = __builtin_amdgcn_permlane16_swap(__float_as_uint(tmax), __float_as_uint(tmax), false, false);
+        tmax = mx(__uint_as_float(r16[0]), __uint_as_float(r16[1]));
+        const auto r32 = __builtin_amdgcn_permlane32_swap(__float_as_uint(tmax), __float_as_uint(tmax), false, false);
+        tmax = mx(__uint_as_float(r32[0]), __uint_as_float(r32[1])) * sl2;
+      }
       if (__builtin_amdgcn_ballot_w64(tmax > m + 8.f)) {   // lazy rescale, as above
         const float mn = tmax > m + 8.f ? tmax : m;
         const float alpha = fast_exp2(m - (mn == kNegInf ? 0.f : mn));
@@ -434,13 +455,13 @@ __device__ __forceinline__ void decode_task(const AttnArgs& a, const DecodeTask&
 #pragma unroll
         for (int d = 0; d < ND; ++d) acc[d] *= alpha;
         m = mn;
+        nmu = m == kNegInf ? 0.f : -m;
       }
-      const float mu = m == kNegInf ? 0.f : m;
       u32x4 pb;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[u][j] = fast_exp2(__builtin_fmaf(s[u][j], sl2, -mu));
+        for (int j = 0; j < 4; ++j) s[u][j] = fast_exp2(__builtin_fmaf(s[u][j], sl2, nmu));
         pb[2 * u] = E16<T>::pack2(s[u][0], s[u][1]);
         pb[2 * u + 1] = E16<T>::pack2(s[u][2], s[u][3]);
       }
