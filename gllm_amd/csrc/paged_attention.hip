@@ -322,10 +322,18 @@ __device__ __forceinline__ void decode_task(const AttnArgs& a, const DecodeTask&
     // 34.3 us).  Elsewhere each lane finds its own key's row.
     const int kis = __builtin_amdgcn_readfirstlane(ki);
     const int ntw = __builtin_amdgcn_readfirstlane(head_ok && nsub > 2 * ki ? ((nsub + 1) / 2 - ki + KW - 1) / KW : 0);
+    // A scale byte comes as the top one of the four bytes that end with it (the
+    // codes precede the scales): a byte load's value is widened where the loop
+    // ends, and that waits for every load in flight.
     struct Step {
       u32x4 k[2], v[2];
       uint32_t ks[2], vs[2];
     } ring[PF + 1];
+    auto ld_scale = [](const char* p) {
+      typedef uint32_t __attribute__((aligned(1))) bytes4;
+      return *reinterpret_cast<const bytes4*>(p);
+    };
+    auto top_scale = [](uint32_t w) { return __uint_as_float((w >> 1) & 0x7f800000u); };
     uint32_t place_lo = 0, place_hi = 0, place_sc = 0;   // the sub-tile's codes; from there to its scales
     const uint32_t code_l = n * (D / 2) + D / 8 * grp, sc_l = n * (D / 32) + D / 4 * grp / 32;
     const char* const ks0 = (const char*)a.k_cache;
@@ -338,7 +346,7 @@ __device__ __forceinline__ void decode_task(const AttnArgs& a, const DecodeTask&
       const uint32_t bi = div_bs((uint32_t)key, a.block_magic, a.block_shift);
       const uint32_t row = (uint32_t)key - bi * (uint32_t)a.block_size;
       const uint64_t at = (uint64_t)(uint32_t)lbid[bi - blk] * sbytes + head_s + row * (D / 2);
-      place_sc = (uint32_t)a.block_size * (D / 2) - row * (D / 2 - D / 32);
+      place_sc = (uint32_t)a.block_size * (D / 2) - row * (D / 2 - D / 32) - 3;
       place_lo = (uint32_t)at;
       place_hi = (uint32_t)(at >> 32);
     };
@@ -382,8 +390,8 @@ __device__ __forceinline__ void decode_task(const AttnArgs& a, const DecodeTask&
         }
         kp += to_sc;
         vp += to_sc;
-        x.ks[u] = (uint8_t)kp[sl[u]];
-        x.vs[u] = (uint8_t)vp[sl[u]];
+        x.ks[u] = ld_scale(kp + sl[u]);
+        x.vs[u] = ld_scale(vp + sl[u]);
       }
     };
     auto issue_any = [&](int t, Step& x) {
@@ -404,8 +412,8 @@ __device__ __forceinline__ void decode_task(const AttnArgs& a, const DecodeTask&
           x.k[u] = u32x4{k2[0], k2[1], 0u, 0u};
           x.v[u] = u32x4{v2[0], v2[1], 0u, 0u};
         }
-        x.ks[u] = (uint8_t)kc[sc];
-        x.vs[u] = (uint8_t)vc[sc];
+        x.ks[u] = ld_scale(kc + sc - 3);
+        x.vs[u] = ld_scale(vc + sc - 3);
       }
     };
     float nmu = 0.f;                       // -m, or 0 before the first visible key
@@ -418,13 +426,13 @@ __device__ __forceinline__ void decode_task(const AttnArgs& a, const DecodeTask&
       for (int kk = 0; kk < NK; ++kk)
 #pragma unroll
         for (int u = 0; u < 2; ++u)
-          s[u] = E16<T>::mfma16(fp4x8_to<T>(x.k[u][kk], __uint_as_float(x.ks[u] << 23)), qB[kk], s[u]);
+          s[u] = E16<T>::mfma16(fp4x8_to<T>(x.k[u][kk], top_scale(x.ks[u])), qB[kk], s[u]);
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int kk = 0; kk < NK; ++kk)
           *reinterpret_cast<u32x4*>(ldsV + (16 * u + n) * RB + chunk_dim<D, KF>(kk, grp) * 2) =
-              fp4x8_to<T>(x.v[u][kk], __uint_as_float(x.vs[u] << 23));
+              fp4x8_to<T>(x.v[u][kk], top_scale(x.vs[u]));
       // lane holds S[key kb + 16u + 4grp + j][row n]
       if (!clean(kb)) {
 #pragma unroll
