@@ -195,6 +195,7 @@ struct gllm_attn_plan {
   int32_t num_seqs = 0, Hq = 0, Hkv = 0, D = 0, bs = 0, dtype = 0;
   int32_t split_len = 0, max_q = 0;
   bool mixed_half = false;         // mixed launches of the windowed and 4-bit kernels: 4-wave workgroups
+  int32_t longest = 0;             // keys of the longest sequence
   int32_t window = 0, sinks = 0;   // sliding window (0: none reaches a sequence's first keys)
   int32_t n_decode_seqs = 0, n_prefill_seqs = 0, heads_per_wg = 8, decode_waves = 8, prefill_waves = 8;
   bool prefill_pairs = false;  // prefill-only launches at D = 64: two workgroups per CU
@@ -817,6 +818,7 @@ static int plan_create_impl(gllm_attn_plan** out, const int32_t* query_lens, con
     s.q_len = ql;
     row += ql;
     p->max_q = std::max(p->max_q, ql);
+    p->longest = std::max(p->longest, sl);
     all_rows += ql;
     if (ql < kTileMinRows) {
       p->max_stream_q = std::max(p->max_stream_q, ql);
@@ -1335,6 +1337,10 @@ static int paged_attention_impl(const gllm_attn_plan* p, const void* q, int64_t 
                                 const void* rope_sin, int64_t rope_row_stride, int32_t rope_mode, float scale,
                                 int32_t dtype, int32_t kv_dtype, void* stream) {
   if (!p) return fail(GLLM_ATTN_EINVAL, "null plan");
+  // the decode kernel places 32 steps of up to 8 waves ahead, past a range's end: key
+  // indexes up to 8,448 + 32 behind it must still fit
+  if (kv_dtype == GLLM_DTYPE_MXFP4 && p->longest > INT32_MAX - 16383)
+    return fail(GLLM_ATTN_EINVAL, "seq_len %d too long for a 4-bit cache", p->longest);
   if (!p->ws) return fail(GLLM_ATTN_EINVAL, "plan was not uploaded (gllm_attn_plan_upload)");
   if (dtype != p->dtype) return fail(GLLM_ATTN_EINVAL, "dtype %d differs from the plan's %d", dtype, p->dtype);
   if (!q || !out || !k_cache || !v_cache || !block_table) return fail(GLLM_ATTN_EINVAL, "null pointer argument");

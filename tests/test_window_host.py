@@ -177,3 +177,16 @@ def test_projections_refuse_4_bit_caches():
     w, cs = torch.zeros(128, 64, dtype=torch.bfloat16), torch.zeros(3, 32, dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="4-bit"):
         paged.qkv_rope_kv_write(torch.zeros(3, 64, dtype=torch.bfloat16), w, w, w, cs, cs, cache, cache, torch.arange(3))
+
+
+def test_sequences_too_long_for_a_4_bit_cache():
+    import ctypes
+    lib, p = _lib.load(), 1 << 20                    # never dereferenced
+    for keys, why in ((2 ** 31 - 1, b"too long"), (2 ** 31 - 16384, b"not uploaded")):
+        h = ctypes.c_void_p()
+        one, long = (ctypes.c_int32 * 1)(1), (ctypes.c_int32 * 1)(keys)
+        _lib.check(lib.gllm_attn_plan_create(ctypes.byref(h), one, long, 1, 0, 8, 2, 64, 4096, _lib.DTYPE_BF16, 0, 0))
+        rc = lib.gllm_paged_attention(h, p, 512, p, 512, p, p, 1 << 20, 16, p, 8, None, None, 0, 0, 0.1, _lib.DTYPE_BF16,
+                                      _lib.DTYPE_MXFP4, None)
+        assert rc == _lib.EINVAL and why in lib.gllm_attn_last_error()
+        lib.gllm_attn_plan_destroy(h)
