@@ -173,6 +173,41 @@ def test_kv_write_and_rope_in_the_launch(D, kv):
             assert torch.equal(a.cpu().view(torch.uint8), x.view(torch.uint8))
 
 
+@pytest.mark.parametrize("kind,kv", [("balanced", BF), ("balanced", F8), ("split", BF), ("asked", F8)])
+def test_kv_write_in_every_decode_plan(kind, kv):
+    """The new keys are written once and seen, whichever part of a split or
+    page-balanced sequence holds them."""
+    if kind == "balanced":
+        n = 140
+        b = Batch([100 + (37 * i) % 300 for i in range(n)], [1 + i % 4 for i in range(n)], Hq=32, Hkv=8, D=128, kv=kv, seed=3)
+    else:
+        b = Batch([0, 15, 700, 2500, 31, 64], [1, 2, 4, 1, 3, 4], Hq=32, Hkv=8, D=128, kv=kv, seed=4)
+    kw = {"balanced": {}, "split": dict(split_tokens=32), "asked": dict(split_tokens=paged.BALANCED)}[kind]
+    g = torch.Generator().manual_seed(1)
+    k, v = (torch.randn(sum(b.ql), b.Hkv, b.D, generator=g).to(BF) for _ in range(2))
+    at = 0
+    for i, (c, n) in enumerate(zip(b.ctx, b.ql)):
+        t = torch.arange(c, c + n)
+        slots = b.bt[i, t // b.bs].long() * b.bs + t % b.bs
+        b.kc[slots], b.vc[slots] = k[at:at + n].to(kv), v[at:at + n].to(kv)
+        at += n
+    for window, sinks in ((90, 3), (17, 0)):
+        plan = _plan(b, window, sinks, **kw)
+        assert paged.fused_kv_write_ok(plan, kv)
+        assert (plan.info["decode_segments"] > 0) == (kind != "split")
+        kc, vc = b.kc.to(DEV), b.vc.to(DEV)
+        at = 0
+        for i, (c, n) in enumerate(zip(b.ctx, b.ql)):        # what the slots held before
+            t = torch.arange(c, c + n)
+            slots = (b.bt[i, t // b.bs].long() * b.bs + t % b.bs).to(DEV)
+            kc[slots], vc[slots] = float("nan"), float("nan")
+        out = paged.paged_attention(plan, b.q.to(DEV), kc, vc, b.bt.to(DEV), kv_new=(k.to(DEV), v.to(DEV)))
+        torch.cuda.synchronize()
+        for a, x in ((kc, b.kc), (vc, b.vc)):
+            assert torch.equal(a.cpu().view(torch.uint8), x.view(torch.uint8))
+        b.check(out, window, sinks, f"write, {kind}")
+
+
 def test_graph_replays():
     """Captured with one plan, replayed with new values between the replays."""
     b = Batch(**DECODE, D=128, seed=8)
