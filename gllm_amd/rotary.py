@@ -27,8 +27,10 @@ class Rotary:
     """``theta``: the base of the frequencies theta^(-2i / rotary_dim).
     ``rotary_dim``: the first dims of the head that turn (None: all of them).
     ``interleaved``: pairs (2i, 2i + 1) instead of (i, i + rotary_dim / 2).
-    ``scaling``: None or a model configuration's ``rope_scaling``:
+    ``scaling``: None or a model configuration's ``rope_scaling`` (a ``rope_theta``
+    or ``partial_rotary_factor`` in it has to agree with the arguments):
 
+    - ``default``: unscaled;
     - ``linear``: positions divided by ``factor``;
     - ``llama3``: pairs that make fewer than ``low_freq_factor`` turns over
       ``original_max_position_embeddings`` positions are divided by ``factor``,
@@ -53,16 +55,18 @@ class Rotary:
         self.freq = self._scaled(theta ** (-2 * torch.arange(R // 2, dtype=torch.float64) / R), theta, scaling).to(device)
 
     def _scaled(self, base: torch.Tensor, theta: float, scaling: dict | None) -> torch.Tensor:
-        kind = None if scaling is None else scaling.get("rope_type", scaling.get("type"))
-        if kind in (None, "default"):
-            if scaling is not None and kind is None:
-                raise ValueError(f"rope scaling {scaling!r} names no rope_type")
+        if scaling is None:
             return base
-        if kind not in ("linear", "llama3", "yarn"):
-            raise NotImplementedError(f"rope scaling {kind!r} (linear, llama3, yarn)")
+        kind = scaling.get("rope_type", scaling.get("type"))
+        if kind is None:
+            raise ValueError(f"rope scaling {scaling!r} names no rope_type")
+        if kind not in ("default", "linear", "llama3", "yarn"):
+            raise NotImplementedError(f"rope scaling {kind!r} (default, linear, llama3, yarn)")
         part = scaling.get("partial_rotary_factor")
         if scaling.get("rope_theta", theta) != theta or part is not None and int(self.head_dim * part) != self.rotary_dim:
             raise ValueError(f"rope scaling {scaling!r}: not the theta {theta}, rotary_dim {self.rotary_dim} given")
+        if kind == "default":
+            return base
         f = _need(scaling, "factor")
         if kind == "linear":
             return base / f

@@ -151,3 +151,17 @@ def test_kv4_values_refuses():
     with pytest.raises(ValueError):
         paged.kv4_values(cache, slots, 64, torch.float32, out=torch.zeros(2, 2, 64))
     assert paged.kv4_values(cache, slots[:0], 64, torch.float32).shape == (0, 2, 64)
+
+
+@pytest.mark.parametrize("scaling", [{"rope_type": "default"}, {"type": "default"}, {"rope_type": "linear", "factor": 2.0},
+                                     LLAMA3, YARN])
+@pytest.mark.parametrize("kw", [dict(rope_theta=500.0), dict(partial_rotary_factor=0.5)])
+def test_every_schedule_refuses_another_theta_or_part(scaling, kw):
+    """A configuration's dictionary that holds the theta or the part of the head
+    that turns is not overruled in silence."""
+    with pytest.raises(ValueError, match="not the theta"):
+        gllm_amd.Rotary(128, device="cpu", scaling=dict(scaling, **kw))
+    same = gllm_amd.Rotary(128, theta=500.0, rotary_dim=64, device="cpu", scaling=dict(scaling, rope_theta=500.0,
+                                                                                       partial_rotary_factor=0.5))
+    plain = gllm_amd.Rotary(128, theta=500.0, rotary_dim=64, device="cpu", scaling=scaling)
+    assert torch.equal(same.freq, plain.freq) and same.factor == plain.factor
