@@ -263,9 +263,11 @@ __device__ __forceinline__ u32x4 fp8x8_to(uint32_t w0, uint32_t w1) {
 // scale is the least 2^e at which the block's largest magnitude rounds to at
 // most 6, the largest code: amax < 7 x 2^e (7 would round to 8), so no value is
 // off by more than half a step.  The hardware's converts agree with that (low
-// half first, ties to even, scale byte 255 -> NaN), checked on gfx950.
+// half first, ties to even, scale byte 255 -> NaN), checked on gfx950.  An fp16
+// model writes at most +-kKv4MaxF16, the largest value that is finite in fp16.
 enum : int { kKV16 = 0, kKV8 = 1, kKV4 = 2 };   // cache format of the MFMA kernels
 struct kv4 { uint8_t pair; };                    // the 4-bit cache as a storage type
+constexpr float kKv4MaxF16 = 6.f * 8192.f;
 
 __host__ __device__ inline int64_t kv4_record_bytes(int64_t block_size, int64_t head_dim) {
   return (block_size * (head_dim / 32 * 17) + 15) / 16 * 16;

@@ -100,8 +100,11 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t x) {
 }
 
 // 8 of the 32 values of a block (the quad of lanes holds them all) as codes;
-// *byte the block's scale.
-__device__ __forceinline__ uint32_t encode4(const float* v, uint32_t* byte) {
+// *byte the block's scale.  T: the model dtype, which the rows are read in.  An
+// fp16 model's values stop at +-6 x 2^13: the next larger value that a block can
+// stand for, 4 x 2^14, is infinite in fp16 (values round to it from 57,344 on).
+template <typename T>
+__device__ __forceinline__ uint32_t encode4(float* v, uint32_t* byte) {
   uint32_t amax = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) amax = max(amax, __float_as_uint(v[i]) & 0x7fffffffu);
@@ -109,6 +112,12 @@ __device__ __forceinline__ uint32_t encode4(const float* v, uint32_t* byte) {
   if (amax >= 0x7f800000u) {             // an infinity or NaN
     *byte = 255u;
     return 0u;
+  }
+  if constexpr (std::is_same<T, _Float16>::value) {
+    constexpr float top = kKv4MaxF16;
+    amax = min(amax, __float_as_uint(top));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __builtin_amdgcn_fmed3f(v[i], -top, top);
   }
   // the least e with amax < 7 x 2^e: 7 = 1.75 x 4, so a mantissa from 1.75 on
   // carries into the exponent here
@@ -266,7 +275,7 @@ __global__ void __launch_bounds__(64 * kRotWaves) rotary_write_kernel(RotaryWrit
     if constexpr (std::is_same<KV, kv4>::value) {
       uint8_t* const rec = (uint8_t*)cache + (int64_t)h * a.kv4_record;
       uint32_t byte;
-      const uint32_t w = encode4(x, &byte);
+      const uint32_t w = encode4<T>(x, &byte);
       *reinterpret_cast<uint32_t*>(rec + at + 4 * ch) = w;
       if ((ch & 3) == 0) rec[sc_at + ch / 4] = (uint8_t)byte;
     } else {

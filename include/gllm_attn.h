@@ -83,7 +83,9 @@ int gllm_attn_version(void);
  * scale 2^e (-126 <= e <= 127) at which the block's largest magnitude rounds to
  * 6 or less, |x| < 7 x 2^e, and round each value to the nearest code, ties to
  * the even one; a block with an infinity or NaN gets byte 255 and stands for
- * NaN.  head_dim a multiple of 32.  Wherever an entry point takes such a cache,
+ * NaN.  Finite values of an f16 model are limited to +-49,152 = 6 x 2^13 first:
+ * from 57,344 on they would round to 4 x 2^14 = 65,536, an infinity when read in
+ * f16.  head_dim a multiple of 32.  Wherever an entry point takes such a cache,
  * `cache_slot_stride` is the bytes between blocks (a multiple of 16), the heads
  * of a block follow each other, and the caches are 16-byte aligned.
  * Returns the bytes of one record (0 for sizes that no 4-bit cache has).
@@ -252,7 +254,8 @@ int gllm_rope_kv_write_kv4(const void* q, void* q_out, const void* k, const void
 
 /*
  * Rows of a 4-bit cache as the values they stand for, in dtype (f32, bf16:
- * exact; f16: rounded to nearest even): out[r] = the num_kv_heads x head_dim
+ * exact; f16: rounded to nearest even, values past 65,504, which an f16 model
+ * does not write, to infinity): out[r] = the num_kv_heads x head_dim
  * values at slots[r] (zeros for a slot outside [0, num_slots)).
  */
 int gllm_kv4_values(const void* cache, int64_t block_stride, int64_t num_slots, int32_t block_size,

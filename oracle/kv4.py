@@ -1,7 +1,9 @@
 """The 4-bit KV cache's format in plain torch: each block of 32 dims as fp4 e2m1
 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign bit) times 2^e, e the least integer
 with amax < 7 * 2^e (between -126 and 127); a block with an infinity or NaN has
-the scale byte 255 and stands for NaN.  No counterpart in the reference."""
+the scale byte 255 and stands for NaN.  Finite values of an fp16 model stop at
+6 * 2^13: the next larger value that a block can stand for, 4 * 2^14, is past
+fp16's largest.  No counterpart in the reference."""
 from __future__ import annotations
 
 import torch
@@ -14,10 +16,13 @@ def record_bytes(bs: int, D: int) -> int:
     return -(-bs * (D // 2 + D // 32) // 16) * 16
 
 
-def quantize(x: torch.Tensor):
-    """x [..., D] -> (codes uint8 [..., D], scale bytes uint8 [..., D / 32])."""
+def quantize(x: torch.Tensor, model: torch.dtype | None = None):
+    """x [..., D] of a model of dtype `model` -> (codes uint8 [..., D], scale bytes
+    uint8 [..., D / 32])."""
     b = x.double().unflatten(-1, (-1, 32))
     bad = ~torch.isfinite(b).all(-1)
+    if model == torch.float16:
+        b = b.clamp(-6.0 * 2 ** 13, 6.0 * 2 ** 13)
     b = torch.where(bad[..., None], torch.zeros_like(b), b)
     amax = b.abs().amax(-1)
     e = torch.full(amax.shape, -126, dtype=torch.int64)
@@ -46,9 +51,9 @@ def views(cache: torch.Tensor, bs: int, D: int):
     return cache[..., :n].unflatten(-1, (bs, D // 2)), cache[..., n:n + bs * D // 32].unflatten(-1, (bs, D // 32))
 
 
-def write(cache: torch.Tensor, slots: torch.Tensor, x: torch.Tensor, bs: int) -> None:
+def write(cache: torch.Tensor, slots: torch.Tensor, x: torch.Tensor, bs: int, model: torch.dtype | None = None) -> None:
     """Rows x [n, Hkv, D] into their slots of a CPU cache."""
-    code, byte = quantize(x)
+    code, byte = quantize(x, model)
     c, s = views(cache, bs, x.shape[-1])
     c[slots // bs, :, slots % bs] = code[..., 0::2] + 16 * code[..., 1::2]
     s[slots // bs, :, slots % bs] = byte

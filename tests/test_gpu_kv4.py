@@ -212,3 +212,19 @@ def test_refusals():
     plan = paged.AttentionPlan([1], [10], num_q_heads=8, num_kv_heads=2, head_dim=80, block_size=16, dtype=BF, device=DEV)
     with pytest.raises(ValueError):
         paged.paged_attention(plan, torch.zeros(1, 8, 80, dtype=BF, device=DEV), kc, vc, bt)
+
+
+@pytest.mark.parametrize("D", [64, 128, 96])
+@pytest.mark.parametrize("ctx,ql", [([0, 40, 300], [1, 1, 1]), ([0, 200], [70, 40])])
+def test_fp16_rows_up_to_the_largest(D, ctx, ql):
+    """K and V rows of an fp16 model up to 65,504, written and attended to."""
+    print(f"fp16 up to 65504 D={D} {ctx}", flush=True)
+    b = Batch(ctx, ql, D=D, dtype=F16, kv="4", seed=D, scale_q=2.0 ** -13)
+    g = torch.Generator().manual_seed(D)
+    k, v = (((torch.rand(b.nb * b.bs, b.Hkv, D, generator=g) - 0.5) * 2 * 65504).to(F16) for _ in range(2))
+    kc, vc = b.kc.to(DEV), b.vc.to(DEV)
+    slots = torch.arange(b.nb * b.bs, device=DEV)
+    paged.rotary_kv_write(k.to(DEV), v.to(DEV), torch.zeros_like(slots), gllm_amd.Rotary(D, device=DEV), kc, vc, slots)
+    b.kc, b.vc = kc.cpu(), vc.cpu()
+    assert b.rows(b.kc, 0).isfinite().all() and b.rows(b.vc, 0).isfinite().all()
+    b.check(_run(b), None, 0, "fp16, large rows")

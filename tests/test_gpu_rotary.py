@@ -303,3 +303,53 @@ def test_graph_replays(kv):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want) and torch.equal(_bytes(kc), _bytes(k2)) and torch.equal(_bytes(vc), _bytes(v2))
+
+
+@pytest.mark.parametrize("table", [False, True])
+def test_every_fp16_value_in_4_bits(table):
+    """All finite fp16 values, neighbours and mixed: rows read in fp16 are finite,
+    blocks with an infinity or NaN stay NaN."""
+    bits = torch.arange(1 << 16, dtype=torch.int32).to(torch.int16)
+    x = bits.view(F16).view(-1, 1, 64)
+    g = torch.Generator().manual_seed(1)
+    x = torch.cat([x, bits.view(F16)[torch.randperm(1 << 16, generator=g)].view(-1, 1, 64),
+                   bits.view(F16).nan_to_num(1.0, 2.0, 3.0)[torch.randperm(1 << 16, generator=g)].view(-1, 1, 64)])
+    n = x.shape[0]
+    rot = gllm_amd.Rotary(64, device=DEV)
+    kc, vc = (torch.zeros(n // 16, 1, kv4.record_bytes(16, 64), dtype=torch.uint8) for _ in range(2))
+    dk, dv, slots = kc.to(DEV), vc.to(DEV), torch.arange(n)
+    k = x.nan_to_num(1.0, 2.0, 3.0)              # position 0 keeps finite values; NaN would reach its partner
+    if table:
+        cos, sin = torch.ones(n, 32, dtype=F16, device=DEV), torch.zeros(n, 32, dtype=F16, device=DEV)
+        paged.rope_kv_write(k.to(DEV), x.to(DEV), cos, sin, dk, dv, slots.to(DEV))
+    else:
+        paged.rotary_kv_write(k.to(DEV), x.to(DEV), torch.zeros_like(slots).to(DEV), rot, dk, dv, slots.to(DEV))
+    torch.cuda.synchronize()
+    for dev, host, rows in ((dk, kc, k), (dv, vc, x)):
+        kv4.write(host, slots, rows, 16, F16)
+        want = kv4.read(host, slots, 16, 64)
+        assert torch.equal(kv4.views(dev.cpu(), 16, 64)[1], kv4.views(host, 16, 64)[1])
+        got = kv4.read(dev.cpu(), slots, 16, 64)
+        assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(7.0), want.nan_to_num(7.0))
+        half = paged.kv4_values(dev, slots.to(DEV), 64, F16).cpu()
+        assert torch.equal(half.isnan(), want.isnan()) and torch.equal(half.nan_to_num(7.0), want.to(F16).nan_to_num(7.0))
+        assert not half.isinf().any()
+    assert not kv4.read(dk.cpu(), slots, 16, 64).isnan().any()
+
+
+def test_turned_fp16_rows_past_the_largest_value():
+    """k rows that the rotation takes past 65,504 are limited, not infinite."""
+    g = torch.Generator().manual_seed(3)
+    k = ((torch.rand(64, 2, 128, generator=g) - 0.5) * 2 * 65504).to(F16)
+    rot = gllm_amd.Rotary(128, scaling=YARN, device=DEV)
+    pos = torch.randint(0, 100000, (64,), generator=g)
+    kc, vc = (torch.zeros(4, 2, kv4.record_bytes(16, 128), dtype=torch.uint8) for _ in range(2))
+    dk, dv, slots = kc.to(DEV), vc.to(DEV), torch.randperm(64, generator=g)
+    paged.rotary_kv_write(k.to(DEV), k.to(DEV), pos.to(DEV), rot, dk, dv, slots.to(DEV))
+    torch.cuda.synchronize()
+    want = _exact(k, pos, rot)
+    assert want.abs().max() > 65536
+    kv4.write(kc, slots, want, 16, F16)
+    kv4.write(vc, slots, k, 16, F16)
+    assert torch.equal(dk.cpu(), kc) and torch.equal(dv.cpu(), vc)
+    assert paged.kv4_values(dk, slots.to(DEV), 128, F16).isfinite().all()

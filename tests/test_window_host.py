@@ -190,3 +190,16 @@ def test_sequences_too_long_for_a_4_bit_cache():
                                       _lib.DTYPE_MXFP4, None)
         assert rc == _lib.EINVAL and why in lib.gllm_attn_last_error()
         lib.gllm_attn_plan_destroy(h)
+
+
+def test_kv4_of_an_fp16_model_stays_finite():
+    """57,344 and more would round to 65,536, past the largest fp16."""
+    x = torch.zeros(6, 32)
+    x[:, 0] = torch.tensor([49152.0, 57343.0, 57344.0, 65504.0, -65504.0, math.inf])
+    x[:, 1] = 4096.0
+    code, byte = kv4.quantize(x, torch.float16)
+    val = kv4.values(code, byte)
+    assert val[:5, 0].tolist() == [49152.0] * 4 + [-49152.0] and val[5].isnan().all()
+    assert (val[:5, 1] == 4096).all() and byte[:5, 0].tolist() == [127 + 13] * 5
+    assert kv4.values(*kv4.quantize(x))[2:4, 0].tolist() == [65536.0] * 2
+    assert torch.equal(kv4.values(*kv4.quantize(x[:2], torch.float16)), kv4.values(*kv4.quantize(x[:2])))
