@@ -567,6 +567,8 @@ class AttentionPlan:
         # facts every launch checks, computed once (a plan serves every layer of a step)
         self.rows = self._info["rows"]
         self.max_seq_len = max(sl, default=0)
+        # a window that hides no key of the batch is none: the kernels are the plain ones
+        self.hides_keys = window is not None and self.max_seq_len > window + sinks
         self.max_query_len = max(ql, default=0)
         self.table_width = -(-self.max_seq_len // block_size)
 
@@ -589,7 +591,7 @@ def fused_kv_write_ok(plan: AttentionPlan, kv_dtype: torch.dtype) -> bool:
     """Whether :func:`paged_attention` can take ``kv_new`` for this plan and
     cache dtype: every sequence on the decode path of the kernel that runs
     (MFMA kernels: query_len x G <= 16; generic kernel: query_len <= 16, no
-    sliding window), and no 4-bit cache."""
+    sliding window that hides a key), and no 4-bit cache."""
     if not plan.max_query_len or kv_dtype == KV4:   # no sequences; a 4-bit cache is written by a call of its own
         return False
     mfma = (plan.dtype in (torch.bfloat16, torch.float16) and plan.head_dim in (64, 128)
@@ -597,7 +599,7 @@ def fused_kv_write_ok(plan: AttentionPlan, kv_dtype: torch.dtype) -> bool:
     G = plan.num_q_heads // plan.num_kv_heads
     if mfma:
         return plan.max_query_len * G <= 16
-    return plan.max_query_len <= 16 and plan.window is None
+    return plan.max_query_len <= 16 and not getattr(plan, "hides_keys", plan.window is not None)
 
 
 def paged_attention(plan: AttentionPlan, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,

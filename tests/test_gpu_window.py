@@ -238,3 +238,25 @@ def test_rows_of_other_sequences_stay():
     torch.cuda.synchronize()
     b.check(out[:2], 50, 2)
     assert (out[2:] == 7.0).all()
+
+
+@pytest.mark.parametrize("dtype,D", [(F32, 64), (BF, 96)])
+def test_kv_write_in_the_launch_under_a_window_that_hides_nothing(dtype, D):
+    """The generic kernel's write is lost to a window only where keys are hidden."""
+    b = Batch([0, 15, 300], [1, 2, 1], D=D, dtype=dtype, seed=D)
+    g = torch.Generator().manual_seed(1)
+    k, v = (torch.randn(sum(b.ql), b.Hkv, D, generator=g).to(dtype) for _ in range(2))
+    got = []
+    for window, sinks in ((None, 0), (301, 0), (290, 11)):
+        plan = _plan(b, window, sinks)
+        assert paged.fused_kv_write_ok(plan, dtype)
+        kc, vc = b.kc.to(DEV), b.vc.to(DEV)
+        out = paged.paged_attention(plan, b.q.to(DEV), kc, vc, b.bt.to(DEV), kv_new=(k.to(DEV), v.to(DEV)))
+        torch.cuda.synchronize()
+        got.append((out, kc, vc))
+    for x in got[1:]:
+        assert all(torch.equal(s, t) for s, t in zip(x, got[0]))
+    hiding = _plan(b, 290, 10)
+    assert not paged.fused_kv_write_ok(hiding, dtype)
+    with pytest.raises(NotImplementedError):
+        paged.paged_attention(hiding, b.q.to(DEV), kc, vc, b.bt.to(DEV), kv_new=(k.to(DEV), v.to(DEV)))

@@ -203,3 +203,11 @@ def test_kv4_of_an_fp16_model_stays_finite():
     assert (val[:5, 1] == 4096).all() and byte[:5, 0].tolist() == [127 + 13] * 5
     assert kv4.values(*kv4.quantize(x))[2:4, 0].tolist() == [65536.0] * 2
     assert torch.equal(kv4.values(*kv4.quantize(x[:2], torch.float16)), kv4.values(*kv4.quantize(x[:2])))
+
+
+def test_fused_kv_write_under_a_window_that_hides_nothing():
+    plan = types.SimpleNamespace(max_query_len=1, dtype=torch.float32, head_dim=64, num_q_heads=8, num_kv_heads=2, window=10,
+                                 hides_keys=False)
+    assert paged.fused_kv_write_ok(plan, torch.float32) and not paged.fused_kv_write_ok(plan, paged.KV4)
+    plan.hides_keys = True
+    assert not paged.fused_kv_write_ok(plan, torch.float32)
