@@ -1278,10 +1278,10 @@ size_t gllm_attn_plan_workspace_bytes(const gllm_attn_plan* p) { return p ? p->w
 int gllm_attn_plan_info(const gllm_attn_plan* p, int64_t* info, int32_t n) {
   if (!p || !info) return fail(GLLM_ATTN_EINVAL, "null plan or info");
   const int64_t n_wg = (int64_t)p->items.size() + (p->segs.empty() ? 0 : (int64_t)p->seg_ptr.size() - 1);
-  const int64_t v[10] = {n_wg, p->split_len, p->n_decode_seqs, p->n_prefill_seqs, p->n_partials,
+  const int64_t v[11] = {n_wg, p->split_len, p->n_decode_seqs, p->n_prefill_seqs, p->n_partials,
                          p->total_rows, p->heads_per_wg, p->decode_waves, p->prefill_waves,
-                         (int64_t)p->segs.size()};
-  for (int i = 0; i < n && i < 10; ++i) info[i] = v[i];
+                         (int64_t)p->segs.size(), p->mixed_half};
+  for (int i = 0; i < n && i < 11; ++i) info[i] = v[i];
   return ok();
 }
 

@@ -559,10 +559,10 @@ class AttentionPlan:
         self.workspace = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
         _lib.check(lib.gllm_attn_plan_upload(self._h, self.workspace.data_ptr(), nbytes,
                                              _lib.stream_ptr(self.device)))
-        arr = (ctypes.c_int64 * 10)()
-        _lib.check(lib.gllm_attn_plan_info(self._h, arr, 10))
+        arr = (ctypes.c_int64 * 11)()
+        _lib.check(lib.gllm_attn_plan_info(self._h, arr, 11))
         keys = ("work_items", "split_tokens", "decode_seqs", "prefill_seqs", "partials", "rows", "heads_per_wg",
-                "decode_waves", "prefill_waves", "decode_segments")
+                "decode_waves", "prefill_waves", "decode_segments", "mixed_half")
         self._info = dict(zip(keys, list(arr)))
         # facts every launch checks, computed once (a plan serves every layer of a step)
         self.rows = self._info["rows"]

@@ -311,7 +311,10 @@ int gllm_attn_plan_upload(gllm_attn_plan* plan, void* workspace, size_t workspac
  * [3] prefill-path sequences, [4] split partials, [5] total query rows,
  * [6] kv heads per decode workgroup, [7] waves per decode workgroup,
  * [8] waves per prefill workgroup, [9] page-balanced decode segments (0:
- * split planner).  [0] counts workgroups for a page-balanced plan. */
+ * split planner), [10] 1 where a mixed launch over a 4-bit cache or with a window
+ * runs each item in two half-size workgroups ([7] and [8] are those of other
+ * caches).  [0] counts workgroups for a page-balanced plan.  The first n are
+ * written. */
 int gllm_attn_plan_info(const gllm_attn_plan* plan, int64_t* info, int32_t n);
 int gllm_attn_plan_destroy(gllm_attn_plan* plan);
 

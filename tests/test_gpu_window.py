@@ -260,3 +260,39 @@ def test_kv_write_in_the_launch_under_a_window_that_hides_nothing(dtype, D):
     assert not paged.fused_kv_write_ok(hiding, dtype)
     with pytest.raises(NotImplementedError):
         paged.paged_attention(hiding, b.q.to(DEV), kc, vc, b.bt.to(DEV), kv_new=(k.to(DEV), v.to(DEV)))
+
+
+@pytest.mark.parametrize("hw", [0, 1, 4, 8])
+@pytest.mark.parametrize("D,kv", [(64, BF), (128, F8), (64, "4"), (128, "4")])
+def test_half_size_mixed_workgroups(hw, D, kv):
+    """Decodes, split and whole, beside many short chunks, two workgroups an item:
+    each number of KV heads a workgroup, the larger ones with idle heads too."""
+    for Hq, Hkv, window in ((32, 8, 1000), (24, 6, 900))[:1 + (hw > 2)]:
+        ctx = [1000 + (37 * i) % 200 for i in range(16)] + [20 * (i % 5) for i in range(60)]
+        b = Batch(ctx, [1] * 16 + [33] * 60, Hq=Hq, Hkv=Hkv, D=D, kv=kv, seed=D + Hkv)
+        plan = _plan(b, window, 3, heads_per_wg=hw)
+        info = plan.info
+        print(f"half mixed hw={hw} D={D} kv={kv} heads {Hq}/{Hkv} {info}", flush=True)
+        assert info["mixed_half"] == 1 and info["decode_segments"] == 0 and info["heads_per_wg"] == (hw or 2)
+        assert info["partials"] > 0
+        b.check(_run(b, window, 3, heads_per_wg=hw), window, 3, "half mixed")
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_half_size_mixed_workgroups_of_one_head(D):
+    """The planner's own choice of one KV head a workgroup (whole sequences)."""
+    n = 70 if D == 64 else 40
+    b = Batch([150 + (37 * i) % 200 for i in range(n)] + [20 * (i % 5) for i in range(60)], [1] * n + [33] * 60, Hq=32, Hkv=8,
+              D=D, kv="4", seed=D)
+    info = _plan(b, 90, 3).info
+    print(f"half mixed, one head, D={D} {info}", flush=True)
+    assert info["mixed_half"] == 1 and info["heads_per_wg"] == 1 and info["partials"] == 0
+    for window, sinks in ((90, 3), (None, 0)):
+        assert _plan(b, window, sinks).info["mixed_half"] == 1
+        b.check(_run(b, window, sinks), window, sinks, "half mixed, one head")
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("kv", [BF, F8, "4"])
+def test_the_half_mixed_batch_runs_in_half_size_workgroups(D, kv):
+    assert _plan(_many("half mixed", D, kv, D), 90, 3).info["mixed_half"] == 1

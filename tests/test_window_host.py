@@ -211,3 +211,22 @@ def test_fused_kv_write_under_a_window_that_hides_nothing():
     assert paged.fused_kv_write_ok(plan, torch.float32) and not paged.fused_kv_write_ok(plan, paged.KV4)
     plan.hides_keys = True
     assert not paged.fused_kv_write_ok(plan, torch.float32)
+
+
+def test_plan_says_where_mixed_launches_take_half_size_workgroups():
+    import ctypes
+    lib = _lib.load()
+
+    def half(lens, D, window, hw=0):
+        h, info = ctypes.c_void_p(), (ctypes.c_int64 * 11)(*[-1] * 11)
+        arr = [(ctypes.c_int32 * len(lens))(*x) for x in zip(*lens)]
+        _lib.check(lib.gllm_attn_plan_create_window(ctypes.byref(h), arr[0], arr[1], len(lens), 0, 32, 8, D, 16,
+                                                    _lib.DTYPE_BF16, 0, hw, window, 0))
+        _lib.check(lib.gllm_attn_plan_info(h, info, 11))
+        lib.gllm_attn_plan_destroy(h)
+        return info[10]
+    # many short chunks beside the decodes; one long chunk ends last; one kind alone
+    for hw in (0, 1, 2, 4, 8):
+        assert half([(1, 1100)] * 16 + [(33, 33)] * 40, 64, 1000, hw) == 1
+    assert half([(1, 1100)] * 4 + [(1024, 8000)], 128, 5000) == 0
+    assert half([(1, 1100)] * 16, 64, 1000) == 0 and half([(33, 33)] * 40, 64, 20) == 0
