@@ -1275,6 +1275,26 @@ int gllm_attn_plan_create_window(gllm_attn_plan** out, const int32_t* query_lens
 
 size_t gllm_attn_plan_workspace_bytes(const gllm_attn_plan* p) { return p ? p->ws_bytes : 0; }
 
+// The most block ids that a decode task of the plan caches: those of its keys
+// [k0, k1), which count through the sequence without its window's left-out run
+// (decode_task's two runs of blocks).
+static int64_t most_task_blocks(const gllm_attn_plan* p) {
+  int64_t most = 0;
+  const auto task = [&](int32_t ctx, int64_t k0, int64_t k1) {
+    const KeySkip sk = p->window > 0 ? key_skip(ctx, p->window, p->sinks, 16) : KeySkip{0, 0, 0};
+    const auto run = [&](int64_t a, int64_t b) { return a < b ? (b - 1) / p->bs - a / p->bs + 1 : 0; };
+    const int64_t cut = std::max(k0, std::min<int64_t>(k1, sk.from));
+    most = std::max(most, sk.by > 0 ? run(k0, cut) + run(cut + sk.by, k1 + sk.by) : run(k0, k1));
+  };
+  for (const WorkItem& it : p->items) {
+    if (!p->mfma || (it.kind_b & 0xff) != kItemDecode) continue;
+    const int64_t L = counted_keys(p, p->seqs[it.seq]), len = split_len_of(L, it.nsplits);
+    task(it.ctx_len, it.a * len, std::min(L, (it.a + 1) * len));
+  }
+  for (const DecodeSeg& sg : p->segs) task(sg.ctx_len, sg.k0, sg.k1);
+  return most;
+}
+
 int gllm_attn_plan_info(const gllm_attn_plan* p, int64_t* info, int32_t n) {
   if (!p || !info) return fail(GLLM_ATTN_EINVAL, "null plan or info");
   const int64_t n_wg = (int64_t)p->items.size() + (p->segs.empty() ? 0 : (int64_t)p->seg_ptr.size() - 1);
@@ -1282,6 +1302,7 @@ int gllm_attn_plan_info(const gllm_attn_plan* p, int64_t* info, int32_t n) {
                          p->total_rows, p->heads_per_wg, p->decode_waves, p->prefill_waves,
                          (int64_t)p->segs.size(), p->mixed_half};
   for (int i = 0; i < n && i < 11; ++i) info[i] = v[i];
+  if (n > 11) info[11] = most_task_blocks(p);
   return ok();
 }
 

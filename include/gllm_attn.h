@@ -313,8 +313,9 @@ int gllm_attn_plan_upload(gllm_attn_plan* plan, void* workspace, size_t workspac
  * [8] waves per prefill workgroup, [9] page-balanced decode segments (0:
  * split planner), [10] 1 where a mixed launch over a 4-bit cache or with a window
  * runs each item in two half-size workgroups ([7] and [8] are those of other
- * caches).  [0] counts workgroups for a page-balanced plan.  The first n are
- * written. */
+ * caches), [11] the most block ids that one decode task of the MFMA kernels looks
+ * up (they cache 512; counted when asked for).  [0] counts workgroups for a
+ * page-balanced plan.  The first n are written. */
 int gllm_attn_plan_info(const gllm_attn_plan* plan, int64_t* info, int32_t n);
 int gllm_attn_plan_destroy(gllm_attn_plan* plan);
 

@@ -230,3 +230,42 @@ def test_plan_says_where_mixed_launches_take_half_size_workgroups():
         assert half([(1, 1100)] * 16 + [(33, 33)] * 40, 64, 1000, hw) == 1
     assert half([(1, 1100)] * 4 + [(1024, 8000)], 128, 5000) == 0
     assert half([(1, 1100)] * 16, 64, 1000) == 0 and half([(33, 33)] * 40, 64, 20) == 0
+
+
+@pytest.mark.parametrize("bs", [1, 3, 7, 8, 16, 17, 24, 100])
+@pytest.mark.parametrize("split", [0, 32, 8192, -1])
+def test_a_tasks_blocks_fit_its_cache(bs, split):
+    """The decode kernels cache 512 block ids a task, of one or two runs of keys."""
+    import ctypes
+    lib = _lib.load()
+    seen = set()
+    for window, sinks in ((0, 0), (60000, 333), (60001, 1), (400, 70), (8200, 8100), (17, 30000), (30000, 8)):
+        for lens in ([(1, 70000), (1, 9000), (4, 40)], [(1, 70007)] * 33, [(4, 31000 + 13 * i) for i in range(20)],
+                     [(1, 33000), (64, 900)]):
+            for D, hw in ((64, 0), (128, 8)):
+                h, info = ctypes.c_void_p(), (ctypes.c_int64 * 12)()
+                arr = [(ctypes.c_int32 * len(lens))(*x) for x in zip(*lens)]
+                _lib.check(lib.gllm_attn_plan_create_window(ctypes.byref(h), arr[0], arr[1], len(lens), 0, 32, 8, D, bs,
+                                                            _lib.DTYPE_BF16, split, hw, window, sinks))
+                _lib.check(lib.gllm_attn_plan_info(h, info, 12))
+                lib.gllm_attn_plan_destroy(h)
+                assert 0 < info[11] <= 512, (window, sinks, lens[0], D, hw, list(info))
+                seen.add(info[11])
+    assert max(seen) > 400 or bs > 16 or split == 32      # tasks near the limit are among them
+
+
+def test_counted_blocks_of_a_small_plan():
+    """One sequence, whole: the sinks' blocks and the window's."""
+    import ctypes
+    lib = _lib.load()
+
+    def most(keys, bs, window=0, sinks=0):
+        h, info, one, sl = ctypes.c_void_p(), (ctypes.c_int64 * 12)(), (ctypes.c_int32 * 1)(1), (ctypes.c_int32 * 1)(keys)
+        _lib.check(lib.gllm_attn_plan_create_window(ctypes.byref(h), one, sl, 1, 0, 8, 2, 64, bs, _lib.DTYPE_BF16, 8192, 0,
+                                                    window, sinks))
+        _lib.check(lib.gllm_attn_plan_info(h, info, 12))
+        lib.gllm_attn_plan_destroy(h)
+        return info[11]
+    assert most(100, 16) == 7 and most(96, 16) == 6 and most(100, 1) == 100
+    # keys 0..15 hold the sinks' unit, the window's starts at 256 (of 270)
+    assert most(300, 16, 30, 2) == 1 + 3 and most(300, 10, 30, 2) == 2 + 5 and most(300, 16, 30, 0) == 3
