@@ -471,7 +471,7 @@ __global__ void __launch_bounds__((64 * StreamCfg<KV, QT, DP, V>::kNW)) attn_str
     }
     const int pr = key_of(p0);
     const int lim = min(vis, nkeys - 1 + (WIN ? sk.by : 0)) - pr;
-    const int lo = WIN ? vis - a.window - pr : 0, sink = WIN ? a.sinks - pr : 0;
+    const int lo = WIN ? before_window(vis - pr, a.window) : 0, sink = WIN ? a.sinks - pr : 0;
     const bool mask = p0 + 16 > nkeys || (!DENSE && pr + 15 > ctx) ||
                       (WIN && pr <= ctx + r_last - a.window && pr + 16 > a.sinks);
     if constexpr (k16) {

@@ -371,6 +371,12 @@ __host__ __device__ inline KeySkip key_skip(int32_t p0, int32_t window, int32_t 
   s.by = lo > s.from ? lo - s.from : 0;
   return s;
 }
+// lim - window, for the mask "c <= lim - window" of places c >= 0.  It may wrap
+// only where lim is below -1 (the window up to INT32_MAX), and there c > lim hides
+// every place already.
+__device__ __forceinline__ int before_window(int lim, int window) {
+  return (int)((uint32_t)lim - (uint32_t)window);
+}
 // A key that may be read in place of `key`: itself where some row sees it, else
 // (between the sinks and the first row's window, where a caller may have given
 // the block back) a visible key of the same unit: the last sink or the window's

@@ -1135,7 +1135,7 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
   auto apply_mask = [&](f32x16& s, int k0) {
     const int lim = (WIN ? vis - by : vis) - k0 - 4 * h;
     if constexpr (WIN) {               // nor at or before vis - window, unless a sink
-      const int lo = lim - a.window, sink = a.sinks - k0 - 4 * h;
+      const int lo = before_window(lim, a.window), sink = a.sinks - k0 - 4 * h;
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
         const int c = 8 * (j >> 2) + (j & 3);
