@@ -51,11 +51,14 @@ def _index_rows(t: torch.Tensor) -> torch.Tensor:
 
 
 def _cache_rows(k_cache: torch.Tensor, v_cache: torch.Tensor, Hkv: int, D: int) -> None:
-    """Checks that the caches are [num_slots, Hkv, D] with contiguous rows."""
+    """Checks that the caches are [num_slots, Hkv, D] with contiguous rows, of one
+    dtype, and that V has K's slots (a call counts the slots, and reads the dtype, of K)."""
     for t, nm in ((k_cache, "k_cache"), (v_cache, "v_cache")):
         shape = t.shape
         if len(shape) != 3 or shape[1] != Hkv or shape[2] != D or t.stride()[1:] != (D, 1):
             raise ValueError(f"{nm}: expected [num_slots, {Hkv}, {D}] with contiguous rows")
+    if v_cache.dtype != k_cache.dtype or v_cache.shape[0] < k_cache.shape[0]:
+        raise ValueError(f"k_cache {k_cache.dtype} of {k_cache.shape[0]} slots, v_cache {v_cache.dtype} of {v_cache.shape[0]}")
 
 
 # Storage type of a 4-bit KV cache (OCP MXFP4): uint8 ``[num_blocks, Hkv,

@@ -269,3 +269,22 @@ def test_counted_blocks_of_a_small_plan():
     assert most(100, 16) == 7 and most(96, 16) == 6 and most(100, 1) == 100
     # keys 0..15 hold the sinks' unit, the window's starts at 256 (of 270)
     assert most(300, 16, 30, 2) == 1 + 3 and most(300, 10, 30, 2) == 2 + 5 and most(300, 16, 30, 0) == 3
+
+
+def _fake_plan(rows=3, window=None):
+    """What paged_attention reads of a plan before it launches anything."""
+    return types.SimpleNamespace(num_q_heads=4, num_kv_heads=2, head_dim=64, dtype=torch.bfloat16, block_size=16,
+                                 query_lens=[1] * rows, rows=rows, table_width=1, max_seq_len=16, window=window, _h=None, _lib=None)
+
+
+@pytest.mark.parametrize("v", [torch.zeros(64, 2, 64), torch.zeros(64, 2, 64, dtype=torch.uint8),
+                               torch.zeros(63, 2, 64, dtype=torch.bfloat16)])
+def test_a_v_cache_unlike_the_k_cache_is_refused(v):
+    """The kernels address V by K's slots and read it in K's dtype."""
+    k = torch.zeros(64, 2, 64, dtype=torch.bfloat16)
+    q = torch.zeros(3, 4, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="v_cache"):
+        paged.paged_attention(_fake_plan(), q, k, v, torch.zeros(3, 1, dtype=torch.int32))
+    kv, cs = torch.zeros(3, 2, 64, dtype=torch.bfloat16), torch.zeros(3, 32, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="v_cache"):
+        paged.rope_kv_write(kv, kv, cs, cs, k, v, torch.arange(3))
