@@ -646,8 +646,8 @@ def paged_attention(plan: AttentionPlan, q: torch.Tensor, k_cache: torch.Tensor,
         raise ValueError(f"block_table width {bt_shape[1]} < {plan.table_width} blocks the longest "
                          "sequence needs")
     rows = q.numel() // (Hq * D)
-    if rows < plan.rows:
-        raise ValueError(f"q has {rows} rows, the plan addresses {plan.rows}")
+    if rows < plan.rows or out.numel() < plan.rows * Hq * D:
+        raise ValueError(f"q has {rows} rows, out {out.numel() // (Hq * D)}, the plan addresses {plan.rows}")
     cos_p = sin_p = None
     rs = 0
     mode = _lib.ROPE_NONE

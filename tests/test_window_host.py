@@ -288,3 +288,13 @@ def test_a_v_cache_unlike_the_k_cache_is_refused(v):
     kv, cs = torch.zeros(3, 2, 64, dtype=torch.bfloat16), torch.zeros(3, 32, dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="v_cache"):
         paged.rope_kv_write(kv, kv, cs, cs, k, v, torch.arange(3))
+
+
+@pytest.mark.parametrize("window", [None, 8])
+def test_an_out_with_too_few_rows_is_refused(window):
+    k = torch.zeros(64, 2, 64, dtype=torch.bfloat16)
+    q = torch.zeros(3, 4, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="out 2"):
+        paged.paged_attention(_fake_plan(window=window), q, k, k, torch.zeros(3, 1, dtype=torch.int32), out=q[:2].clone())
+    with pytest.raises(ValueError, match="q has 2"):
+        paged.paged_attention(_fake_plan(window=window), q[:2], k, k, torch.zeros(3, 1, dtype=torch.int32), out=q.clone())
