@@ -116,8 +116,8 @@ def rope_kv_write(k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torc
     written.  The caches may be 4-bit ones (:data:`KV4`; slots must differ there).
     """
     Hkv, D = k.shape[-2], k.shape[-1]
-    if k.shape != v.shape:
-        raise ValueError("k and v shapes differ")
+    if k.shape != v.shape or k.dtype != v.dtype:
+        raise ValueError("k and v shapes or dtypes differ")
     ks = _rows(k, Hkv, D, "k")
     vs = _rows(v, Hkv, D, "v")
     n = k.numel() // (Hkv * D)
@@ -137,22 +137,30 @@ def rope_kv_write(k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torc
         raise ValueError("cos/sin must have contiguous rows of equal stride")
     if cs.dtype != k.dtype or sn.dtype != k.dtype:
         raise ValueError("cos/sin must be in the model dtype")
-    if cs.shape[-1] < D // 2 or (rope_rows is None and cs.shape[0] < n):
+    if min(cs.shape[-1], sn.shape[-1]) < D // 2 or (rope_rows is None and min(cs.shape[0], sn.shape[0]) < n):
         raise ValueError("cos/sin need one row of at least D/2 entries per token")
     tps = 0
     ql = None
     if query_lens is not None:
         ql = query_lens.to(torch.int32).contiguous()
+        if ql.numel() == 0 or n % ql.numel():
+            raise ValueError("query_lens: the tokens must be as many rows for each sequence")
         tps = n // ql.numel()
     qs = qos = 0
     Hq = 1
     if q_out is not None:
+        if q is None or q.dtype != k.dtype or q_out.dtype != k.dtype:
+            raise ValueError("q_out needs a q, both in the dtype of k")
         Hq = q.shape[-2]
         qs = _rows(q, Hq, D, "q")
         qos = _rows(q_out, Hq, D, "q_out")
+        if min(q.numel(), q_out.numel()) < n * Hq * D:
+            raise ValueError("q and q_out need one row per token")
     rr = None
     if rope_rows is not None:
         rr = _index_rows(rope_rows)
+        if rr.numel() < n:
+            raise ValueError("rope_rows needs one entry per token")
     dev = k.device
     lib = _lib.load()
     if k_cache.dtype == KV4:

@@ -165,3 +165,19 @@ def test_every_schedule_refuses_another_theta_or_part(scaling, kw):
                                                                                        partial_rotary_factor=0.5))
     plain = gllm_amd.Rotary(128, theta=500.0, rotary_dim=64, device="cpu", scaling=scaling)
     assert torch.equal(same.freq, plain.freq) and same.factor == plain.factor
+
+
+@pytest.mark.parametrize("kv4", [False, True])
+@pytest.mark.parametrize("kw", [
+    dict(v=torch.zeros(6, 2, 64, dtype=torch.bfloat16)), dict(sin=torch.zeros(5, 32)), dict(query_lens=torch.ones(4)),
+    dict(query_lens=torch.zeros(0)), dict(q_out=torch.zeros(6, 4, 64)), dict(q=torch.zeros(6, 4, 64).bfloat16(), q_out=torch.zeros(6, 4, 64)),
+    dict(q=torch.zeros(6, 4, 64), q_out=torch.zeros(5, 4, 64)), dict(q=torch.zeros(5, 4, 64), q_out=torch.zeros(6, 4, 64)),
+    dict(q=torch.zeros(6, 4, 64), q_out=torch.zeros(6, 4, 64).half()), dict(rope_rows=torch.arange(5))])
+def test_rope_kv_write_refuses(kw, kv4):
+    """Tensors that the kernels would read or write past their end, or in another dtype."""
+    cache = torch.zeros(4, 2, paged.kv4_record_bytes(16, 64), dtype=torch.uint8) if kv4 else torch.zeros(64, 2, 64)
+    a = dict(k=torch.zeros(6, 2, 64), v=torch.zeros(6, 2, 64), cos=torch.zeros(6, 32), sin=torch.zeros(6, 32), k_cache=cache,
+             v_cache=cache, slot_mapping=torch.arange(6))
+    a.update(kw)
+    with pytest.raises(ValueError):
+        paged.rope_kv_write(**a)
