@@ -53,6 +53,10 @@ def _index_rows(t: torch.Tensor) -> torch.Tensor:
 def _cache_rows(k_cache: torch.Tensor, v_cache: torch.Tensor, Hkv: int, D: int) -> None:
     """Checks that the caches are [num_slots, Hkv, D] with contiguous rows, of one
     dtype, and that V has K's slots (a call counts the slots, and reads the dtype, of K)."""
+    shape, stride = k_cache.shape, k_cache.stride()
+    if len(shape) == 3 and shape[1] == Hkv and shape[2] == D and stride[1] == D and stride[2] == 1 \
+            and v_cache.shape == shape and v_cache.stride() == stride and v_cache.dtype == k_cache.dtype:
+        return                             # the common case, without a look at each cache
     for t, nm in ((k_cache, "k_cache"), (v_cache, "v_cache")):
         shape = t.shape
         if len(shape) != 3 or shape[1] != Hkv or shape[2] != D or t.stride()[1:] != (D, 1):
@@ -115,8 +119,9 @@ def rope_kv_write(k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torc
     (padded ``[B, T_q]`` token layout) rows past each sequence's length are not
     written.  The caches may be 4-bit ones (:data:`KV4`; slots must differ there).
     """
-    Hkv, D = k.shape[-2], k.shape[-1]
-    if k.shape != v.shape or k.dtype != v.dtype:
+    shape, dtype = k.shape, k.dtype
+    Hkv, D = shape[-2], shape[-1]
+    if v.shape != shape or v.dtype != dtype:
         raise ValueError("k and v shapes or dtypes differ")
     ks = _rows(k, Hkv, D, "k")
     vs = _rows(v, Hkv, D, "v")
@@ -135,10 +140,11 @@ def rope_kv_write(k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torc
     cs, sn = _flat(cos), _flat(sin)
     if cs.stride(-1) != 1 or sn.stride(-1) != 1 or cs.stride(0) != sn.stride(0):
         raise ValueError("cos/sin must have contiguous rows of equal stride")
-    if cs.dtype != k.dtype or sn.dtype != k.dtype:
+    if cs.dtype != dtype or sn.dtype != dtype:
         raise ValueError("cos/sin must be in the model dtype")
-    if min(cs.shape[-1], sn.shape[-1]) < D // 2 or (rope_rows is None and min(cs.shape[0], sn.shape[0]) < n):
-        raise ValueError("cos/sin need one row of at least D/2 entries per token")
+    for rows, width in {cs.shape, sn.shape}:
+        if width < D // 2 or (rope_rows is None and rows < n):
+            raise ValueError("cos/sin need one row of at least D/2 entries per token")
     tps = 0
     ql = None
     if query_lens is not None:
@@ -149,7 +155,7 @@ def rope_kv_write(k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torc
     qs = qos = 0
     Hq = 1
     if q_out is not None:
-        if q is None or q.dtype != k.dtype or q_out.dtype != k.dtype:
+        if q is None or q.dtype != dtype or q_out.dtype != dtype:
             raise ValueError("q_out needs a q, both in the dtype of k")
         Hq = q.shape[-2]
         qs = _rows(q, Hq, D, "q")
@@ -636,6 +642,8 @@ def paged_attention(plan: AttentionPlan, q: torch.Tensor, k_cache: torch.Tensor,
         os_ = Hq * D
     else:
         os_ = _rows(out, Hq, D, "out")
+        if out.numel() < plan.rows * Hq * D:
+            raise ValueError(f"out has {out.numel() // (Hq * D)} rows, the plan addresses {plan.rows}")
     if q.dtype != plan.dtype or out.dtype != plan.dtype:
         raise ValueError("q/out dtype differs from the plan's")
     if k_cache.dtype == KV4:
@@ -654,8 +662,8 @@ def paged_attention(plan: AttentionPlan, q: torch.Tensor, k_cache: torch.Tensor,
         raise ValueError(f"block_table width {bt_shape[1]} < {plan.table_width} blocks the longest "
                          "sequence needs")
     rows = q.numel() // (Hq * D)
-    if rows < plan.rows or out.numel() < plan.rows * Hq * D:
-        raise ValueError(f"q has {rows} rows, out {out.numel() // (Hq * D)}, the plan addresses {plan.rows}")
+    if rows < plan.rows:
+        raise ValueError(f"q has {rows} rows, the plan addresses {plan.rows}")
     cos_p = sin_p = None
     rs = 0
     mode = _lib.ROPE_NONE

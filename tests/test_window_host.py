@@ -294,7 +294,7 @@ def test_a_v_cache_unlike_the_k_cache_is_refused(v):
 def test_an_out_with_too_few_rows_is_refused(window):
     k = torch.zeros(64, 2, 64, dtype=torch.bfloat16)
     q = torch.zeros(3, 4, 64, dtype=torch.bfloat16)
-    with pytest.raises(ValueError, match="out 2"):
+    with pytest.raises(ValueError, match="out has 2"):
         paged.paged_attention(_fake_plan(window=window), q, k, k, torch.zeros(3, 1, dtype=torch.int32), out=q[:2].clone())
     with pytest.raises(ValueError, match="q has 2"):
         paged.paged_attention(_fake_plan(window=window), q[:2], k, k, torch.zeros(3, 1, dtype=torch.int32), out=q.clone())
