@@ -830,6 +830,11 @@ static int plan_create_impl(gllm_attn_plan** out, const int32_t* query_lens, con
     return fail(GLLM_ATTN_EINVAL, "too many query rows");
   }
 
+  // The tiled generic kernel has no window: a batch with a hidden key runs its
+  // prompts on the stream kernel, which leaves the hidden keys out but reads the
+  // others for 16 columns at a time.  8 x 2,048 tokens, 32 / 8 heads, us without a
+  // window / window 512 / 1,900: fp32 head dim 64 1,444 / 1,581 / 2,802, 128 3,028 / 3,081 /
+  // 5,722; bf16 head dim 96 1,925 / - / 4,974.
   if (tile_wgs >= kTileMinWgs && !hides) p->tile_min_q = kTileMinRows;
   else {
     p->max_stream_q = p->max_q;
@@ -876,8 +881,9 @@ static int plan_create_impl(gllm_attn_plan** out, const int32_t* query_lens, con
     // whose unsplit units give every CU its resident workgroups (2 at D=64,
     // 1 at D=128) wins; HW=2 reads 256-byte runs of each slot and still
     // spreads one sequence over several CUs.  If none fills the GPU, HW=2 and
-    // sequences are split into equal key ranges.  A split caches at most 511
-    // block ids.
+    // sequences are split into equal key ranges.  A task caches at most 512
+    // block ids: splits stay at 511 blocks, with a window at 507, since each of its
+    // two runs of keys can start and end inside a block.
     int64_t cap = (int64_t)(hides ? 507 : 511) * block_size / 32 * 32;
     cap = std::max<int64_t>(32, std::min<int64_t>(cap, 8192));
     int64_t ndec = 0;
@@ -1119,7 +1125,8 @@ static int plan_create_impl(gllm_attn_plan** out, const int32_t* query_lens, con
     // long: it pays where the longest prefill item, so stretched, still ends well
     // before the launch (its items' time over the CUs).  An item: ~10 us and 1.75
     // (head dim 64: 1.0) us per 64 keys for prefill, 5.6 us and its K/V at 29 GB/s for
-    // decode.  At head dim 128, where half workgroups read K/V twice for the same
+    // decode, whatever the cache: the plan does not know its type, so beside an 8- or
+    // 4-bit cache the decode items are overestimated.  At head dim 128, where half workgroups read K/V twice for the same
     // MFMA rate, only for items of at most 1,100 keys.  Measured, us whole / half, bf16
     // and 4-bit cache (decodes, chunks, window): head dim 128, 200 + 1 x 256, 512
     // 96 / 85, 49 / 43; 64 + 16 of 128-256, 512 82 / 78, 82 / 73; 64 + 4 x 512, 1,024 88 / 88, 65 /
@@ -1415,7 +1422,7 @@ static int paged_attention_impl(const gllm_attn_plan* p, const void* q, int64_t 
   a.decode_waves = p->decode_waves;
   a.prefill_waves = p->prefill_waves;
   a.prefill_pairs = p->prefill_pairs;
-  // the MFMA kernels read a cache in the model dtype or fp8; a 16-bit model
+  // the MFMA kernels read a cache in the model dtype, fp8 or 4 bits; a 16-bit model
   // over an f32 (or the other 16-bit) cache takes the generic kernel, which
   // rounds each cached value to the model dtype as the reference's gather does
   const bool use_mfma = p->mfma && (kv_dtype == dtype || kv_dtype == GLLM_DTYPE_FP8_E4M3 || kv4);

@@ -551,7 +551,7 @@ __device__ __forceinline__ void decode_task(const AttnArgs& a, const DecodeTask&
           for (int j = 0; j < 4; ++j) {
             const int key = kr + 4 * grp + j;
             const bool hid = (kb + 4 * grp + j >= kend) | (key > vis) | ((key <= vis - a.window) & (key >= a.sinks));
-          p[j] = hid ? kNegInf : p[j];
+            p[j] = hid ? kNegInf : p[j];
           }
         }
       } else if (kb + 16 > kend || kb + 15 > tk.ctx_len) {
@@ -1559,7 +1559,7 @@ __device__ __forceinline__ int xcd_item(int b, int n) {
 
 // Work items of both kinds in one launch (mixed continuous batch; 8-wave
 // workgroups), or decode items only (HW x KW waves).  T: the model dtype
-// (__bf16 or _Float16), also the cache's unless KV8 (fp8 e4m3fn cache).
+// (__bf16 or _Float16), also the cache's unless KF says fp8 e4m3fn or 4-bit.
 template <typename T, int D, bool PF, bool DC, int HW, int KW, int KF, bool WIN>
 __global__ void __launch_bounds__(64 * HW * KW) paged_attn_kernel(AttnArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[MixedLds<D, PF, DC, HW * KW, KF>::kBytes];

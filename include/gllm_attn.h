@@ -85,7 +85,8 @@ int gllm_attn_version(void);
  * the even one; a block with an infinity or NaN gets byte 255 and stands for
  * NaN.  Finite values of an f16 model are limited to +-49,152 = 6 x 2^13 first:
  * from 57,344 on they would round to 4 x 2^14 = 65,536, an infinity when read in
- * f16.  head_dim a multiple of 32.  Wherever an entry point takes such a cache,
+ * f16.  (An f32 or bf16 model's values from 7 x 2^125 = 2.98e38 on do stand for
+ * 2^128, an infinity in every model dtype.)  head_dim a multiple of 32.  Wherever an entry point takes such a cache,
  * `cache_slot_stride` is the bytes between blocks (a multiple of 16), the heads
  * of a block follow each other, and the caches are 16-byte aligned.
  * Returns the bytes of one record (0 for sizes that no 4-bit cache has).
