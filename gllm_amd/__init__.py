@@ -11,9 +11,11 @@ from .kv_cache import PagedKVCache
 from .paged import (AttentionPlan, kv4_values, paged_attention, rope_kv_write, rope_rotate, rotary_kv_write,
                     rotary_rotate)
 from .rotary import Rotary
+from .sparse import SparsePlan, key_bounds_values, new_key_bounds, select_blocks, sparse_attention, write_key_bounds
 
 __all__ = [
-    "Attention", "AttentionMetadata", "AttentionPlan", "PagedKVCache", "Rotary", "flash_attention", "kv4_values",
-    "paged_attention", "plan_for", "reference_attention", "rope_kv_write", "rope_rotate", "rotary_kv_write",
-    "rotary_rotate",
+    "Attention", "AttentionMetadata", "AttentionPlan", "PagedKVCache", "Rotary", "SparsePlan", "flash_attention",
+    "key_bounds_values", "kv4_values", "new_key_bounds", "paged_attention", "plan_for", "reference_attention",
+    "rope_kv_write", "rope_rotate", "rotary_kv_write", "rotary_rotate", "select_blocks", "sparse_attention",
+    "write_key_bounds",
 ]

@@ -57,6 +57,20 @@ SIGNATURES = {
                                                       _i32, _p, _p, _i64, _i64, _p, _p, _i64, _p, _p, _p, _i64, _i32,
                                                       _i32, _i32, _i32, _i32, _p]),
     "gllm_qkv_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32, _i32, _i32]),
+    "gllm_attn_plan_create_shared": (ctypes.c_int, [ctypes.POINTER(_p), _p, _p, _i32, _i64, _i32, _i32, _i32, _i32, _i32,
+                                                    _i32, _i32, _i32, _p, _p, _p]),
+    "gllm_key_bounds_record_bytes": (_sz, [_i32, _i32]),
+    "gllm_sparse_plan_create": (ctypes.c_int, [ctypes.POINTER(_p), _p, _p, _i32, _i64, _i32, _i32, _i32, _i32, _i32, _i32,
+                                               _i32, _i32]),
+    "gllm_sparse_plan_workspace_bytes": (_sz, [_p]),
+    "gllm_sparse_plan_upload": (ctypes.c_int, [_p, _p, _sz, _p]),
+    "gllm_sparse_plan_info": (ctypes.c_int, [_p, ctypes.POINTER(_i64), _i32]),
+    "gllm_sparse_plan_destroy": (ctypes.c_int, [_p]),
+    "gllm_key_bounds_write": (ctypes.c_int, [_p, _p, _i64, _i64, _p, _i64, _p, _i64, _i32, _p]),
+    "gllm_key_bounds_values": (ctypes.c_int, [_p, _i64, _i64, _p, _i64, _i32, _i32, _p, _p]),
+    "gllm_select_blocks": (ctypes.c_int, [_p, _p, _i64, _p, _i64, _i64, _p, _i64, _p, _i32, _p]),
+    "gllm_sparse_attention": (ctypes.c_int, [_p, _p, _i64, _p, _i64, _p, _p, _i64, _i64, _p, _i64, _p, _f32, _i32, _i32,
+                                             _p]),
     "gllm_qkv_tiles_ahead": (ctypes.c_int, [_i64, _i32, _i32, _i32]),
     "gllm_attention_dense": (ctypes.c_int, [_p, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p,
                                             _i64, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _p]),

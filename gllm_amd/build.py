@@ -21,13 +21,16 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
 
 PAGED = ["paged_attention.hip", "paged_attention_f16.hip", "paged_attention_kv4.hip", "paged_attention_kv4_f16.hip",
-         "paged_attention_window.hip", "paged_attention_window_f16.hip"]
+         "paged_attention_window.hip", "paged_attention_window_f16.hip", "paged_attention_sparse.hip",
+         "paged_attention_sparse_f16.hip", "paged_attention_prefix.hip", "paged_attention_prefix_f16.hip"]
 GENERIC = ["generic_attention.hip", "generic_attention_bf16.hip", "generic_attention_f16.hip", "generic_window_f32.hip",
-           "generic_window_bf16.hip", "generic_window_f16.hip"]
-SOURCES = [*PAGED, *GENERIC, "api.hip", "rope_kv_write.hip", "rotary_write.hip", "metadata.hip", "qkv_proj.hip"]
-NO_CONTRACT = {"rope_kv_write.hip", "rotary_write.hip", "qkv_proj.hip", *GENERIC}
+           "generic_window_bf16.hip", "generic_window_f16.hip", "generic_sparse_f32.hip", "generic_sparse_bf16.hip",
+           "generic_sparse_f16.hip"]
+SOURCES = [*PAGED, *GENERIC, "api.hip", "rope_kv_write.hip", "rotary_write.hip", "metadata.hip", "qkv_proj.hip",
+           "sparse_select.hip"]
+NO_CONTRACT = {"rope_kv_write.hip", "rotary_write.hip", "qkv_proj.hip", "sparse_select.hip", *GENERIC}
 # MFMA accumulators stay in VGPRs (no per-tile AGPR<->VGPR copies)
-EXTRA = {f: ["-mllvm", "--amdgpu-mfma-vgpr-form"] for f in [*PAGED, *GENERIC, "qkv_proj.hip"]}
+EXTRA = {f: ["-mllvm", "--amdgpu-mfma-vgpr-form"] for f in [*PAGED, *GENERIC, "qkv_proj.hip", "sparse_select.hip"]}
 COMMON = [
     f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC",
     # packed fp32 VALU ops are disabled on purpose for every HIP unit

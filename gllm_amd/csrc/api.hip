@@ -191,6 +191,29 @@ int kv4_check(const void* k_cache, const void* v_cache, int64_t block_stride, in
 
 }  // namespace
 
+// A batch of sparse attention: its query rows, the blocks that its new tokens touch
+// and the tiles of rows whose blocks are scored together.
+struct gllm_sparse_plan {
+  int32_t num_seqs = 0, Hq = 0, Hkv = 0, D = 0, bs = 0, dtype = 0;
+  int32_t width = 0, first = 0, recent = 0;   // blocks a row selects; of them always the first, the last ones
+  int32_t longest = 0;                        // blocks of the longest sequence
+  int64_t total_rows = 0;                     // rows of q / out / selected that the plan addresses
+  std::vector<SparseRow> rows;
+  std::vector<BoundsBlock> blocks;
+  std::vector<ScoreTile> tiles;
+  // rows are scored and selected a slab at a time, so that the scores' place stays bounded
+  struct Slab { int32_t row0, n_rows, tile0, n_tiles, max_blocks; };
+  std::vector<Slab> slabs;
+  int64_t score_stride = 0;
+  int32_t splits = 1;
+  void* pinned = nullptr;
+  size_t pinned_cap = 0;
+  bool pinned_is_host_malloc = false;
+  size_t off_rows = 0, off_blocks = 0, off_tiles = 0, off_scores = 0, off_ml = 0, off_part = 0, ws_bytes = 0, stage_bytes = 0;
+  char* ws = nullptr;
+  hipEvent_t upload_done = nullptr;
+};
+
 struct gllm_attn_plan {
   int32_t num_seqs = 0, Hq = 0, Hkv = 0, D = 0, bs = 0, dtype = 0;
   int32_t split_len = 0, max_q = 0;
@@ -213,6 +236,13 @@ struct gllm_attn_plan {
   std::vector<int32_t> seg_ptr;
   std::vector<MergeInfo> merge;  // [num_seqs * head_groups], plans with partials
   int32_t head_groups = 1;
+  // shared prefixes: items over the shared keys, the query rows that they serve, and of
+  // each sequence (empty: no sharing) the keys that items cover and their partials
+  std::vector<PrefixItem> prefix_items;
+  std::vector<PrefixRow> prefix_rows;
+  struct Shared { int32_t keys = 0, parts = 0; };
+  std::vector<Shared> shared;
+  size_t off_prefix = 0, off_prefix_rows = 0;
   // staging copy of [items | seqs] in pinned host memory (from the pool), device offsets
   void* pinned = nullptr;
   size_t pinned_cap = 0;
@@ -229,6 +259,61 @@ namespace {
 int32_t counted_keys(const gllm_attn_plan* p, const SeqInfo& s) {
   const int32_t L = s.ctx_len + s.q_len;
   return p->window > 0 ? L - key_skip(s.ctx_len, p->window, p->sinks, 16).by : L;
+}
+// The first of its keys that decode tasks read: those before it are a shared prefix's.
+int32_t first_key(const gllm_attn_plan* p, const SeqInfo& s) {
+  return p->shared.empty() ? 0 : p->shared[&s - p->seqs.data()].keys;
+}
+
+// Pinned staging of a plan's tables, its upload and its release: fields that
+// gllm_attn_plan and gllm_sparse_plan have alike.
+template <typename P>
+int plan_stage(P* p) {
+  p->pinned = pinned_pool().acquire(p->stage_bytes, &p->pinned_cap);
+  if (!p->pinned) {
+    p->pinned = std::malloc(p->stage_bytes);
+    p->pinned_is_host_malloc = true;
+    if (!p->pinned) return fail(GLLM_ATTN_EINVAL, "out of host memory for %zu staging bytes", p->stage_bytes);
+  }
+  std::memset(p->pinned, 0, p->stage_bytes);
+  return ok();
+}
+template <typename P, typename T>
+void plan_put(P* p, size_t off, const std::vector<T>& v) {
+  if (!v.empty()) std::memcpy((char*)p->pinned + off, v.data(), v.size() * sizeof(T));
+}
+template <typename P>
+int plan_upload(P* p, void* workspace, size_t bytes, void* stream) {
+  if (!p) return fail(GLLM_ATTN_EINVAL, "null plan");
+  if (!workspace || bytes < p->ws_bytes)
+    return fail(GLLM_ATTN_EINVAL, "workspace of %zu bytes is smaller than the %zu the plan needs", bytes, p->ws_bytes);
+  if (((uintptr_t)workspace & 255) != 0) return fail(GLLM_ATTN_EINVAL, "workspace must be 256-byte aligned");
+  hipStream_t st = (hipStream_t)stream;
+  p->ws = (char*)workspace;
+  hipError_t e = hipSuccess;
+  if (p->stage_bytes > 0) {
+    e = hipMemcpyAsync(p->ws, p->pinned, p->stage_bytes, hipMemcpyHostToDevice, st);
+    if (e != hipSuccess) return hip_check(e, "plan upload copy");
+  }
+  if (!p->upload_done) {
+    e = hipEventCreateWithFlags(&p->upload_done, hipEventDisableTiming);
+    if (e != hipSuccess) return hip_check(e, "hipEventCreate");
+  }
+  return hip_check(hipEventRecord(p->upload_done, st), "hipEventRecord");
+}
+template <typename P>
+void plan_release(P* p) {
+  if (p->pinned && !p->pinned_is_host_malloc) {
+    // back to the pool with the upload's event: reused once the copy is done
+    pinned_pool().release(p->pinned, p->pinned_cap, p->upload_done);
+  } else {
+    if (p->upload_done) {
+      (void)hipEventSynchronize(p->upload_done);  // the staging copy must finish before the free
+      (void)hipEventDestroy(p->upload_done);
+    }
+    if (p->pinned) std::free(p->pinned);
+  }
+  delete p;
 }
 
 // Resident 8-wave decode workgroups per CU (register-bound: 2 at D = 64,
@@ -264,7 +349,7 @@ BalancedShape balanced_shape(const gllm_attn_plan* p, int cus, int heads_req) {
   b.hgroups = (p->Hkv + b.hw - 1) / b.hw;
   const int G = p->Hq / p->Hkv;
   for (const SeqInfo& si : p->seqs)
-    if (si.q_len * G <= 16) b.units += (int64_t)b.hgroups * ((counted_keys(p, si) + 15) / 16);
+    if (si.q_len * G <= 16) b.units += (int64_t)b.hgroups * ((counted_keys(p, si) - first_key(p, si) + 15) / 16);
   b.wgs = std::max<int64_t>(1, std::min<int64_t>(b.units, (int64_t)cus * GLLM_DECODE_WG_PER_CU(p->D)));
   return b;
 }
@@ -306,8 +391,9 @@ void plan_balanced_decode(gllm_attn_plan* p, int cus, int heads_req, int64_t wgs
     if (si.q_len * G > 16) continue;   // a prefill item of the mixed launch
     ++p->n_decode_seqs;
     si.nsplits = 1;
-    const int L = counted_keys(p, si);
-    const int64_t nu = (L + 15) / 16;
+    const int k0 = first_key(p, si), L = counted_keys(p, si);
+    const int parts = p->shared.empty() ? 0 : p->shared[i].parts;   // partials of the shared keys, before the segments'
+    const int64_t nu = (L - k0 + 15) / 16;
     for (int hg = 0; hg < hgroups; ++hg) {
       const size_t first = p->segs.size();
       for (int64_t u = 0; u < nu;) {
@@ -315,26 +401,113 @@ void plan_balanced_decode(gllm_attn_plan* p, int cus, int heads_req, int64_t wgs
         const int64_t take = std::min(std::min(nu - u, U * (j + 1) / W - (u0 + u)), ucap);
         DecodeSeg sg{};
         sg.seq = i; sg.hg = hg;
-        sg.k0 = (int32_t)(16 * u);
-        sg.k1 = (int32_t)std::min<int64_t>(L, 16 * (u + take));
+        sg.k0 = (int32_t)(k0 + 16 * u);
+        sg.k1 = (int32_t)std::min<int64_t>(L, k0 + 16 * (u + take));
         sg.q_row_start = si.q_row_start; sg.ctx_len = si.ctx_len; sg.q_len = si.q_len;
         p->segs.push_back(sg);
         seg_wg.push_back((int32_t)j);
         u += take;
       }
       u0 += nu;
-      const int nseg = (int)(p->segs.size() - first);
+      const int own = (int)(p->segs.size() - first), nseg = parts + own;
       const int32_t pbase = (int32_t)p->n_partials;
       if (nseg > 1) p->n_partials += (int64_t)hw * nseg;
       p->merge[(size_t)i * hgroups + hg] = MergeInfo{pbase, nseg};
-      for (int k = 0; k < nseg; ++k) {
+      for (int k = 0; k < own; ++k) {
         DecodeSeg& sg = p->segs[first + k];
-        sg.nseg = nseg; sg.ord = k; sg.pbase = nseg > 1 ? pbase : 0;
+        sg.nseg = nseg; sg.ord = parts + k; sg.pbase = nseg > 1 ? pbase : 0;
       }
     }
   }
   for (int32_t w : seg_wg) ++p->seg_ptr[(size_t)w + 1];
   for (int64_t w = 0; w < W; ++w) p->seg_ptr[(size_t)w + 1] += p->seg_ptr[(size_t)w];
+}
+
+// Sequences of a batch that have their first `tokens` keys in common.
+struct PrefixGroups {
+  int32_t n = 0;
+  const int32_t* ptr = nullptr;      // group g: seqs[ptr[g] .. ptr[g + 1])
+  const int32_t* seqs = nullptr;
+  const int32_t* tokens = nullptr;
+};
+int check_groups(const PrefixGroups& g, const int32_t* query_lens, const int32_t* seq_lens, int32_t num_seqs) {
+  if (g.n < 0 || (g.n > 0 && (!g.ptr || !g.seqs || !g.tokens))) return fail(GLLM_ATTN_EINVAL, "bad shared prefix arrays");
+  std::vector<char> seen((size_t)num_seqs, 0);
+  for (int32_t k = 0; k < g.n; ++k) {
+    if (g.ptr[k] < 0 || g.ptr[k + 1] < g.ptr[k]) return fail(GLLM_ATTN_EINVAL, "shared prefix %d: bad member range", k);
+    if (g.tokens[k] < 0) return fail(GLLM_ATTN_EINVAL, "shared prefix %d: %d tokens", k, g.tokens[k]);
+    for (int32_t j = g.ptr[k]; j < g.ptr[k + 1]; ++j) {
+      const int32_t i = g.seqs[j];
+      if (i < 0 || i >= num_seqs) return fail(GLLM_ATTN_EINVAL, "shared prefix %d: sequence %d of %d", k, i, num_seqs);
+      if (seen[(size_t)i]) return fail(GLLM_ATTN_EINVAL, "sequence %d has two shared prefixes", i);
+      seen[(size_t)i] = 1;
+      if (g.tokens[k] > seq_lens[i] - query_lens[i])
+        return fail(GLLM_ATTN_EINVAL, "shared prefix %d: %d tokens, but sequence %d has %d before its query rows", k,
+                    g.tokens[k], i, seq_lens[i] - query_lens[i]);
+    }
+  }
+  return ok();
+}
+
+// Items over the keys that decode sequences share.  All (query row, head) columns of
+// a group, 256 a workgroup, take a range of the shared keys together; the ranges are
+// as long as leaves every CU its resident workgroups (of at least 256 keys), since a
+// range costs every column a partial.  Prompts in a group keep their keys: they read
+// a key for 32 rows a wave already.  Whole sub-tiles of 16 keys are shared, the rest is
+// the sequences' own.
+void plan_prefixes(gllm_attn_plan* p, const PrefixGroups& g, int cus) {
+  const int G = p->Hq / p->Hkv;
+  constexpr int kCols = 32 * kPrefillOnlyWaves;
+  struct Group { int32_t seq, tokens, row0, nrows; };
+  std::vector<Group> groups;
+  p->shared.assign((size_t)p->num_seqs, {});
+  for (int32_t k = 0; k < g.n; ++k) {
+    Group gr{0, g.tokens[k] / 16 * 16, (int32_t)p->prefix_rows.size(), 0};
+    int members = 0;
+    for (int32_t j = g.ptr[k]; j < g.ptr[k + 1]; ++j) members += p->seqs[g.seqs[j]].q_len * G <= 16;
+    if (gr.tokens == 0 || members < 2) continue;
+    for (int32_t j = g.ptr[k]; j < g.ptr[k + 1]; ++j) {
+      const int32_t i = g.seqs[j];
+      const SeqInfo& s = p->seqs[i];
+      if (s.q_len * G > 16) continue;
+      if (gr.nrows == 0) gr.seq = i;
+      for (int r = 0; r < s.q_len; ++r) p->prefix_rows.push_back({s.q_row_start + r, i, r, s.ctx_len + r});
+      gr.nrows += s.q_len;
+      p->shared[i].keys = gr.tokens;
+    }
+    groups.push_back(gr);
+  }
+  if (groups.empty()) {
+    p->shared.clear();
+    return;
+  }
+  const auto tiles = [&](const Group& gr) { return ((int64_t)gr.nrows * G + kCols - 1) / kCols; };
+  const auto items = [&](int64_t len) {
+    int64_t n = 0;
+    for (const Group& gr : groups) n += tiles(gr) * p->Hkv * ((gr.tokens + len - 1) / len);
+    return n;
+  };
+  int64_t lo = 4, hi = 4;                      // in tiles of 64 keys
+  for (const Group& gr : groups) hi = std::max<int64_t>(hi, (gr.tokens + 63) / 64);
+  const int64_t target = (int64_t)cus * (p->D == 64 ? 2 : 1);
+  while (lo < hi) {
+    const int64_t mid = (lo + hi) / 2;
+    if (items(64 * mid) <= target) hi = mid;
+    else lo = mid + 1;
+  }
+  for (const Group& gr : groups) {
+    const int64_t n = (gr.tokens + 64 * lo - 1) / (64 * lo);
+    const int64_t len = ((gr.tokens + n - 1) / n + 63) / 64 * 64;
+    int32_t ord = 0;
+    for (int64_t k0 = 0; k0 < gr.tokens; k0 += len, ++ord)
+      for (int h = 0; h < p->Hkv; ++h)
+        for (int64_t w = 0; w < tiles(gr); ++w)
+          p->prefix_items.push_back({gr.seq, h, (int32_t)w, (int32_t)k0, (int32_t)std::min<int64_t>(gr.tokens, k0 + len),
+                                     gr.row0, gr.nrows, ord});
+    for (int32_t j = 0; j < gr.nrows; ++j) p->shared[p->prefix_rows[(size_t)gr.row0 + j].seq].parts = ord;
+  }
+  std::stable_sort(p->prefix_items.begin(), p->prefix_items.end(),
+                   [](const PrefixItem& x, const PrefixItem& y) { return x.k1 - x.k0 > y.k1 - y.k0; });
 }
 
 // A prefill work item: 8 waves over the (query head, 32-row block) pairs
@@ -760,7 +933,7 @@ static int plan_create_impl(gllm_attn_plan** out, const int32_t* query_lens, con
                             int32_t num_seqs, int64_t q_seq_stride, int32_t num_q_heads,
                             int32_t num_kv_heads, int32_t head_dim, int32_t block_size, int32_t dtype,
                             int32_t split_tokens, int32_t decode_heads_per_wg, int32_t window,
-                            int32_t sinks) {
+                            int32_t sinks, const PrefixGroups& groups) {
   if (!out) return fail(GLLM_ATTN_EINVAL, "plan out-pointer is null");
   *out = nullptr;
   if (num_seqs < 0 || (num_seqs > 0 && (!query_lens || !seq_lens)))
@@ -841,6 +1014,12 @@ static int plan_create_impl(gllm_attn_plan** out, const int32_t* query_lens, con
     p->stream_rows = all_rows;
   }
 
+  if (groups.n > 0) {
+    if (window > 0) return fail(GLLM_ATTN_EUNSUPPORTED, "shared prefixes with a window, which hides them");
+    if (split_tokens > 0) return fail(GLLM_ATTN_EINVAL, "shared prefixes: their plans are page-balanced, split_tokens must be 0 or -1");
+    if (int rc = check_groups(groups, query_lens, seq_lens, num_seqs)) return rc;
+    if (mfma) plan_prefixes(p, groups, device_cus());
+  }
   if (mfma) {
     const int cus = device_cus();
     int64_t n_pf = 0;
@@ -853,13 +1032,13 @@ static int plan_create_impl(gllm_attn_plan** out, const int32_t* query_lens, con
       // Mixed batch, page-balanced decode share plus prefill items: on
       // request only (config (d): 482-487 µs against 455-464 for the item plan
       // below; 291 vs 299 µs with 128 decodes and 4 prefills).
-      if (n_pf < num_seqs && split_tokens == GLLM_SPLIT_BALANCED) {
+      if (n_pf < num_seqs && (split_tokens == GLLM_SPLIT_BALANCED || !p->shared.empty())) {
         for (int i = 0; i < num_seqs; ++i)
           if (p->seqs[i].q_len * G > 16) prefill_pieces(p, p->seqs[i], i, G, num_kv_heads, pcs);
         mixed_wgs = mixed_decode_wgs(p, cus, decode_heads_per_wg, pcs);
         balanced = true;
       }
-    } else if (split_tokens == GLLM_SPLIT_BALANCED) {
+    } else if (split_tokens == GLLM_SPLIT_BALANCED || !p->shared.empty()) {
       balanced = num_seqs > 0;
     } else if (split_tokens == 0 && num_seqs > 0) {
       const BalancedShape bsh = balanced_shape(p, cus, decode_heads_per_wg);
@@ -1240,28 +1419,21 @@ static int plan_create_impl(gllm_attn_plan** out, const int32_t* query_lens, con
   p->off_segs = o; o = align256(o + p->segs.size() * sizeof(DecodeSeg));
   p->off_segptr = o; o = align256(o + p->seg_ptr.size() * sizeof(int32_t));
   p->off_merge = o; o = align256(o + p->merge.size() * sizeof(MergeInfo));
-  const size_t stage = o;                        // uploaded part
-  p->stage_bytes = stage;
+  p->off_prefix = o; o = align256(o + p->prefix_items.size() * sizeof(PrefixItem));
+  p->off_prefix_rows = o; o = align256(o + p->prefix_rows.size() * sizeof(PrefixRow));
+  p->stage_bytes = o;                            // uploaded part
   p->off_ml = o; o = align256(o + (size_t)p->n_partials * 16 * 2 * sizeof(float));
   p->off_part = o; o = align256(o + (size_t)p->n_partials * 16 * head_dim * sizeof(float));
   p->ws_bytes = std::max<size_t>(o, 256);
-  if (stage > 0) {
-    p->pinned = pinned_pool().acquire(stage, &p->pinned_cap);
-    if (!p->pinned) {
-      p->pinned = std::malloc(stage);
-      p->pinned_is_host_malloc = true;
-      if (!p->pinned) {
-        return fail(GLLM_ATTN_EINVAL, "out of host memory for %zu staging bytes", stage);
-      }
-    }
-    std::memset(p->pinned, 0, stage);
-    if (!p->items.empty()) std::memcpy((char*)p->pinned + p->off_items, p->items.data(), p->items.size() * sizeof(WorkItem));
-    if (!p->seqs.empty()) std::memcpy((char*)p->pinned + p->off_seqs, p->seqs.data(), p->seqs.size() * sizeof(SeqInfo));
-    if (!p->segs.empty()) std::memcpy((char*)p->pinned + p->off_segs, p->segs.data(), p->segs.size() * sizeof(DecodeSeg));
-    if (!p->seg_ptr.empty())
-      std::memcpy((char*)p->pinned + p->off_segptr, p->seg_ptr.data(), p->seg_ptr.size() * sizeof(int32_t));
-    if (!p->merge.empty())
-      std::memcpy((char*)p->pinned + p->off_merge, p->merge.data(), p->merge.size() * sizeof(MergeInfo));
+  if (p->stage_bytes > 0) {
+    if (int rc = plan_stage(p)) return rc;
+    plan_put(p, p->off_items, p->items);
+    plan_put(p, p->off_seqs, p->seqs);
+    plan_put(p, p->off_segs, p->segs);
+    plan_put(p, p->off_segptr, p->seg_ptr);
+    plan_put(p, p->off_merge, p->merge);
+    plan_put(p, p->off_prefix, p->prefix_items);
+    plan_put(p, p->off_prefix_rows, p->prefix_rows);
   }
   *out = owner.release();
   return ok();
@@ -1274,8 +1446,22 @@ int gllm_attn_plan_create_window(gllm_attn_plan** out, const int32_t* query_lens
                                  int32_t sinks) {
   try {
     return plan_create_impl(out, query_lens, seq_lens, num_seqs, q_seq_stride, num_q_heads, num_kv_heads, head_dim,
-                            block_size, dtype, split_tokens, decode_heads_per_wg, window, sinks);
+                            block_size, dtype, split_tokens, decode_heads_per_wg, window, sinks, PrefixGroups{});
   } catch (const std::exception& e) {              // no exception leaves a C entry
+    return fail(GLLM_ATTN_EINVAL, "plan: %s", e.what());
+  }
+}
+
+int gllm_attn_plan_create_shared(gllm_attn_plan** out, const int32_t* query_lens, const int32_t* seq_lens,
+                                 int32_t num_seqs, int64_t q_seq_stride, int32_t num_q_heads,
+                                 int32_t num_kv_heads, int32_t head_dim, int32_t block_size, int32_t dtype,
+                                 int32_t split_tokens, int32_t decode_heads_per_wg, int32_t num_groups,
+                                 const int32_t* group_ptr, const int32_t* group_seqs, const int32_t* group_tokens) {
+  try {
+    const PrefixGroups groups{num_groups, group_ptr, group_seqs, group_tokens};
+    return plan_create_impl(out, query_lens, seq_lens, num_seqs, q_seq_stride, num_q_heads, num_kv_heads, head_dim,
+                            block_size, dtype, split_tokens, decode_heads_per_wg, 0, 0, groups);
+  } catch (const std::exception& e) {
     return fail(GLLM_ATTN_EINVAL, "plan: %s", e.what());
   }
 }
@@ -1310,42 +1496,17 @@ int gllm_attn_plan_info(const gllm_attn_plan* p, int64_t* info, int32_t n) {
                          (int64_t)p->segs.size(), p->mixed_half};
   for (int i = 0; i < n && i < 11; ++i) info[i] = v[i];
   if (n > 11) info[11] = most_task_blocks(p);
+  if (n > 12) info[12] = (int64_t)p->prefix_items.size();
   return ok();
 }
 
 int gllm_attn_plan_upload(gllm_attn_plan* p, void* workspace, size_t bytes, void* stream) {
   Range range("gllm_attn_plan_upload");
-  if (!p) return fail(GLLM_ATTN_EINVAL, "null plan");
-  if (!workspace || bytes < p->ws_bytes)
-    return fail(GLLM_ATTN_EINVAL, "workspace of %zu bytes is smaller than the %zu the plan needs", bytes, p->ws_bytes);
-  if (((uintptr_t)workspace & 255) != 0) return fail(GLLM_ATTN_EINVAL, "workspace must be 256-byte aligned");
-  hipStream_t st = (hipStream_t)stream;
-  p->ws = (char*)workspace;
-  hipError_t e = hipSuccess;
-  if (p->stage_bytes > 0) {
-    e = hipMemcpyAsync(p->ws, p->pinned, p->stage_bytes, hipMemcpyHostToDevice, st);
-    if (e != hipSuccess) return hip_check(e, "plan upload copy");
-  }
-  if (!p->upload_done) {
-    e = hipEventCreateWithFlags(&p->upload_done, hipEventDisableTiming);
-    if (e != hipSuccess) return hip_check(e, "hipEventCreate");
-  }
-  return hip_check(hipEventRecord(p->upload_done, st), "hipEventRecord");
+  return plan_upload(p, workspace, bytes, stream);
 }
 
 int gllm_attn_plan_destroy(gllm_attn_plan* p) {
-  if (!p) return ok();
-  if (p->pinned && !p->pinned_is_host_malloc) {
-    // back to the pool with the upload's event: reused once the copy is done
-    pinned_pool().release(p->pinned, p->pinned_cap, p->upload_done);
-  } else {
-    if (p->upload_done) {
-      (void)hipEventSynchronize(p->upload_done);  // the staging copy must finish before the free
-      (void)hipEventDestroy(p->upload_done);
-    }
-    if (p->pinned) std::free(p->pinned);
-  }
-  delete p;
+  if (p) plan_release(p);
   return ok();
 }
 
@@ -1442,6 +1603,11 @@ static int paged_attention_impl(const gllm_attn_plan* p, const void* q, int64_t 
     a.k_new_row_stride = k_new_row_stride; a.v_new_row_stride = v_new_row_stride;
   }
   hipStream_t st = (hipStream_t)stream;
+  if (!p->prefix_items.empty()) {
+    a.prefix_items = (const PrefixItem*)(p->ws + p->off_prefix);
+    a.prefix_rows = (const PrefixRow*)(p->ws + p->off_prefix_rows);
+    a.n_prefix_items = (int32_t)p->prefix_items.size();
+  }
   if (use_mfma)
     return hip_check(launch_paged_attention_mfma(a, p->n_prefill_seqs > 0, p->n_decode_seqs > 0, st),
                      "paged attention launch");
@@ -1513,6 +1679,271 @@ int gllm_attention_dense(const void* q, int64_t q_row_stride, const void* k, int
   if (mfma_dtype(dtype) && (head_dim == 64 || head_dim == 128))
     return hip_check(launch_dense_attention_mfma(a, batch, q_len, st), "dense attention launch");
   return hip_check(launch_attention_generic(a, true, batch, q_len, q_len, (int64_t)batch * q_len, st), "generic dense attention launch");
+}
+
+// ---------------------------------------------------------------- sparse attention
+namespace {
+// Scores of a slab of rows: at most this many bytes (or one tile's).
+constexpr int64_t kScoreBytes = int64_t(256) << 20;
+
+int64_t bounds_record(int64_t Hkv, int64_t D) { return (Hkv * (2 * D + 1) + 15) / 16 * 16; }
+
+int bounds_check(const void* bounds, int64_t stride, int64_t num_blocks, int32_t Hkv, int32_t D) {
+  if (!bounds) return fail(GLLM_ATTN_EINVAL, "null bounds");
+  if (((uintptr_t)bounds & 15) || stride % 16 || stride < bounds_record(Hkv, D))
+    return fail(GLLM_ATTN_EINVAL, "key bounds: 16-byte aligned records, %lld bytes or more apart (a multiple of 16) needed",
+                (long long)bounds_record(Hkv, D));
+  if (num_blocks <= 0) return fail(GLLM_ATTN_EINVAL, "num_blocks must be > 0");
+  return ok();
+}
+
+int sparse_plan_impl(gllm_sparse_plan** out, const int32_t* query_lens, const int32_t* seq_lens, int32_t num_seqs,
+                     int64_t q_seq_stride, int32_t Hq, int32_t Hkv, int32_t D, int32_t bs, int32_t dtype, int32_t blocks,
+                     int32_t first, int32_t recent) {
+  if (!out) return fail(GLLM_ATTN_EINVAL, "plan out-pointer is null");
+  *out = nullptr;
+  if (num_seqs < 0 || (num_seqs > 0 && (!query_lens || !seq_lens))) return fail(GLLM_ATTN_EINVAL, "bad sequence arrays");
+  if (Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0)
+    return fail(GLLM_ATTN_EINVAL, "num_q_heads (%d) must be a positive multiple of num_kv_heads (%d)", Hq, Hkv);
+  if (bs <= 0 || bs > kMaxBlockSize) return fail(GLLM_ATTN_EINVAL, "block_size %d must be in [1, %d]", bs, kMaxBlockSize);
+  if (!model_dtype_ok(dtype)) return fail(GLLM_ATTN_EUNSUPPORTED, "model dtype %d (f32, bf16 or f16)", dtype);
+  if (D <= 0 || D > 256 || D % 8) return fail(GLLM_ATTN_EUNSUPPORTED, "sparse attention: head_dim %d (a multiple of 8, at most 256)", D);
+  if (q_seq_stride < 0) return fail(GLLM_ATTN_EINVAL, "q_seq_stride < 0");
+  if (first < 0 || recent < 1 || blocks < 1 || (int64_t)first + recent > blocks)
+    return fail(GLLM_ATTN_EINVAL, "blocks %d must hold first_blocks %d (>= 0) and recent_blocks %d (>= 1)", blocks, first, recent);
+  if ((int64_t)blocks * bs > INT32_MAX - 16384) return fail(GLLM_ATTN_EINVAL, "%d blocks of %d keys are too many", blocks, bs);
+  std::unique_ptr<gllm_sparse_plan> owner(new gllm_sparse_plan());
+  gllm_sparse_plan* p = owner.get();
+  p->num_seqs = num_seqs; p->Hq = Hq; p->Hkv = Hkv; p->D = D; p->bs = bs; p->dtype = dtype;
+  p->width = blocks; p->first = first; p->recent = recent;
+  const int G = Hq / Hkv;
+  int gp = 1;
+  while (gp < G && gp < 16) gp *= 2;
+  const int tile_rows = 16 / gp;
+  int64_t row = 0, keys = 0, scored = 0;
+  for (int i = 0; i < num_seqs; ++i) {
+    const int32_t ql = query_lens[i], sl = seq_lens[i];
+    if (ql < 1 || sl < ql) return fail(GLLM_ATTN_EINVAL, "sequence %d: query_len %d / seq_len %d invalid", i, ql, sl);
+    if (sl > INT32_MAX - 16384) return fail(GLLM_ATTN_EINVAL, "sequence %d: seq_len %d too long", i, sl);
+    if (q_seq_stride > 0 && ql > q_seq_stride)
+      return fail(GLLM_ATTN_EINVAL, "sequence %d: query_len %d exceeds q_seq_stride %lld", i, ql, (long long)q_seq_stride);
+    const int64_t start = q_seq_stride > 0 ? (int64_t)i * q_seq_stride : row;
+    if (start + ql > INT32_MAX) return fail(GLLM_ATTN_EINVAL, "too many query rows");
+    const int32_t c = sl - ql;
+    for (int32_t r = 0; r < ql; ++r) {
+      p->rows.push_back({(int32_t)(start + r), i, c + r, 0});
+      const int32_t nb = (c + r) / bs + 1;
+      if (nb > blocks) scored = std::max<int64_t>(scored, nb);
+    }
+    for (int32_t b = c / bs; b <= (sl - 1) / bs; ++b)
+      p->blocks.push_back({i, b, (int32_t)std::min<int64_t>(bs, sl - (int64_t)b * bs), 0});
+    p->longest = std::max(p->longest, (sl - 1) / bs + 1);
+    keys = std::max<int64_t>(keys, std::min<int64_t>(sl, (int64_t)blocks * bs));
+    row += ql;
+  }
+  p->total_rows = q_seq_stride > 0 ? (int64_t)num_seqs * q_seq_stride : row;
+  if (p->total_rows > INT32_MAX) return fail(GLLM_ATTN_EINVAL, "too many query rows");
+  if ((int64_t)p->rows.size() * Hq * D > ((int64_t)INT32_MAX - 256) * 4 || p->blocks.size() > (size_t)INT32_MAX)
+    return fail(GLLM_ATTN_EINVAL, "too many query rows");
+  // slabs of rows, their tiles: neighbouring rows of one sequence, of which one is scored
+  p->score_stride = (scored + 3) / 4 * 4;
+  const int64_t per_row = std::max<int64_t>(1, (int64_t)Hkv * p->score_stride * 4);
+  const int64_t slab = std::max<int64_t>(tile_rows, kScoreBytes / per_row);
+  int64_t slab_rows = 0;
+  for (int64_t r0 = 0; r0 < (int64_t)p->rows.size(); r0 += slab) {
+    const int64_t r1 = std::min<int64_t>((int64_t)p->rows.size(), r0 + slab);
+    gllm_sparse_plan::Slab sb{(int32_t)r0, (int32_t)(r1 - r0), (int32_t)p->tiles.size(), 0, 0};
+    for (int64_t r = r0; r < r1;) {
+      int64_t e = r + 1;
+      while (e < r1 && e - r < tile_rows && p->rows[e].seq == p->rows[r].seq) ++e;
+      const int32_t nb = p->rows[e - 1].pos / bs + 1;
+      if (nb > blocks) {
+        p->tiles.push_back({(int32_t)r, (int32_t)(e - r), p->rows[r].seq, nb});
+        sb.max_blocks = std::max(sb.max_blocks, nb);
+      }
+      r = e;
+    }
+    sb.n_tiles = (int32_t)p->tiles.size() - sb.tile0;
+    if (sb.n_tiles > 0) slab_rows = std::max<int64_t>(slab_rows, sb.n_rows);
+    p->slabs.push_back(sb);
+  }
+  // Splits of a row's selected keys (MFMA kernel): as many as leave every CU its
+  // resident workgroups, where the longest sheds enough for the merge's launch, and of
+  // at most 510 blocks (the ids that a task caches).
+  const bool mfma = mfma_dtype(dtype) && (D == 64 || D == 128) && G <= 16;
+  if (mfma && !p->rows.empty()) {
+    const int64_t units = (int64_t)p->rows.size() * Hkv;
+    const int64_t target = (int64_t)device_cus() * (D == 64 ? 2 : 1);
+    int64_t s = std::max<int64_t>(1, std::min(target / units, keys / 128));
+    if ((keys - keys / s) * D * 4 < 128 << 10) s = 1;
+    const int64_t cap = std::max<int64_t>(16, (int64_t)(510 * (int64_t)bs) / 16 * 16 - 16);   // split_len_of rounds up to 16
+    s = std::max<int64_t>(s, (keys + cap - 1) / cap);
+    if (units * s > INT32_MAX / 16) return fail(GLLM_ATTN_EINVAL, "too many splits");
+    p->splits = (int32_t)s;
+  }
+  const size_t parts = p->splits > 1 ? p->rows.size() * Hkv * p->splits : 0;
+  size_t o = 0;
+  p->off_rows = o; o = align256(o + p->rows.size() * sizeof(SparseRow));
+  p->off_blocks = o; o = align256(o + p->blocks.size() * sizeof(BoundsBlock));
+  p->off_tiles = o; o = align256(o + p->tiles.size() * sizeof(ScoreTile));
+  p->stage_bytes = o;
+  p->off_scores = o; o = align256(o + (size_t)(slab_rows * per_row));
+  p->off_ml = o; o = align256(o + parts * 16 * 2 * sizeof(float));
+  p->off_part = o; o = align256(o + parts * 16 * D * sizeof(float));
+  p->ws_bytes = std::max<size_t>(o, 256);
+  if (p->stage_bytes > 0) {
+    if (int rc = plan_stage(p)) return rc;
+    plan_put(p, p->off_rows, p->rows);
+    plan_put(p, p->off_blocks, p->blocks);
+    plan_put(p, p->off_tiles, p->tiles);
+  }
+  *out = owner.release();
+  return ok();
+}
+
+// What every call with a sparse plan takes.
+int sparse_check(const gllm_sparse_plan* p, int64_t num_blocks, const int32_t* block_table, int64_t block_table_stride) {
+  if (!p) return fail(GLLM_ATTN_EINVAL, "null plan");
+  if (!p->ws) return fail(GLLM_ATTN_EINVAL, "plan was not uploaded (gllm_sparse_plan_upload)");
+  if (!block_table || block_table_stride <= 0) return fail(GLLM_ATTN_EINVAL, "null block table, or block_table_stride <= 0");
+  if (num_blocks <= 0) return fail(GLLM_ATTN_EINVAL, "num_blocks must be > 0");
+  if ((uint64_t)num_blocks * (uint64_t)p->bs >= (1ull << 32))
+    return fail(GLLM_ATTN_EUNSUPPORTED, "pool of %lld blocks x %d slots exceeds 2^32 slots", (long long)num_blocks, p->bs);
+  return ok();
+}
+int sparse_cache_check(const gllm_sparse_plan* p, const void* k, const void* v, int64_t stride, int32_t kv_dtype) {
+  if (!k || !v) return fail(GLLM_ATTN_EINVAL, "null cache");
+  if (kv_dtype == GLLM_DTYPE_MXFP4) return kv4_check(k, v, stride, p->Hkv, p->D, p->bs);
+  if (!kv_dtype_ok(kv_dtype))
+    return fail(GLLM_ATTN_EUNSUPPORTED, "kv_dtype %d (f32, bf16, f16, fp8 e4m3fn or mxfp4)", kv_dtype);
+  if (stride < (int64_t)p->Hkv * p->D) return fail(GLLM_ATTN_EINVAL, "cache_slot_stride too small");
+  return ok();
+}
+}  // namespace
+
+size_t gllm_key_bounds_record_bytes(int32_t num_kv_heads, int32_t head_dim) {
+  if (num_kv_heads <= 0 || head_dim <= 0 || head_dim % 8 || head_dim > 256) return 0;
+  return (size_t)bounds_record(num_kv_heads, head_dim);
+}
+
+int gllm_sparse_plan_create(gllm_sparse_plan** out, const int32_t* query_lens, const int32_t* seq_lens, int32_t num_seqs,
+                            int64_t q_seq_stride, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                            int32_t block_size, int32_t dtype, int32_t blocks, int32_t first_blocks, int32_t recent_blocks) {
+  try {
+    return sparse_plan_impl(out, query_lens, seq_lens, num_seqs, q_seq_stride, num_q_heads, num_kv_heads, head_dim,
+                            block_size, dtype, blocks, first_blocks, recent_blocks);
+  } catch (const std::exception& e) {              // no exception leaves a C entry
+    return fail(GLLM_ATTN_EINVAL, "sparse plan: %s", e.what());
+  }
+}
+
+size_t gllm_sparse_plan_workspace_bytes(const gllm_sparse_plan* p) { return p ? p->ws_bytes : 0; }
+
+int gllm_sparse_plan_upload(gllm_sparse_plan* p, void* workspace, size_t bytes, void* stream) {
+  Range range("gllm_sparse_plan_upload");
+  return plan_upload(p, workspace, bytes, stream);
+}
+
+int gllm_sparse_plan_info(const gllm_sparse_plan* p, int64_t* info, int32_t n) {
+  if (!p || !info) return fail(GLLM_ATTN_EINVAL, "null plan or info");
+  const int64_t v[6] = {p->total_rows, (int64_t)p->rows.size(), (int64_t)p->blocks.size(), (int64_t)p->tiles.size(),
+                        (int64_t)p->slabs.size(), p->splits};
+  for (int i = 0; i < n && i < 6; ++i) info[i] = v[i];
+  return ok();
+}
+
+int gllm_sparse_plan_destroy(gllm_sparse_plan* p) {
+  if (p) plan_release(p);
+  return ok();
+}
+
+int gllm_key_bounds_write(const gllm_sparse_plan* p, const void* k_cache, int64_t cache_slot_stride, int64_t num_blocks,
+                          const int32_t* block_table, int64_t block_table_stride, void* bounds, int64_t bounds_stride,
+                          int32_t kv_dtype, void* stream) {
+  Range range("gllm_key_bounds_write");
+  if (int rc = sparse_check(p, num_blocks, block_table, block_table_stride)) return rc;
+  if (int rc = sparse_cache_check(p, k_cache, k_cache, cache_slot_stride, kv_dtype)) return rc;
+  if (int rc = bounds_check(bounds, bounds_stride, num_blocks, p->Hkv, p->D)) return rc;
+  BoundsArgs a{};
+  a.k_cache = k_cache; a.cache_slot_stride = cache_slot_stride; a.num_blocks = num_blocks;
+  a.block_table = block_table; a.block_table_stride = block_table_stride;
+  a.blocks = (const BoundsBlock*)(p->ws + p->off_blocks);
+  a.n_blocks = (int32_t)p->blocks.size();
+  a.bounds = (uint8_t*)bounds; a.bounds_stride = bounds_stride;
+  a.block_size = p->bs; a.num_kv_heads = p->Hkv; a.head_dim = p->D; a.dtype = p->dtype; a.kv_dtype = kv_dtype;
+  if (kv_dtype == GLLM_DTYPE_MXFP4) a.kv4_record = (int32_t)kv4_record_bytes(p->bs, p->D);
+  return hip_check(launch_key_bounds(a, (hipStream_t)stream), "key bounds launch");
+}
+
+int gllm_key_bounds_values(const void* bounds, int64_t bounds_stride, int64_t num_blocks, const int64_t* blocks,
+                           int64_t n, int32_t num_kv_heads, int32_t head_dim, float* out, void* stream) {
+  Range range("gllm_key_bounds_values");
+  if (num_kv_heads <= 0 || head_dim <= 0 || head_dim % 8 || head_dim > 256)
+    return fail(GLLM_ATTN_EUNSUPPORTED, "key bounds: %d kv heads of head_dim %d (a multiple of 8, at most 256)", num_kv_heads, head_dim);
+  if (int rc = bounds_check(bounds, bounds_stride, num_blocks, num_kv_heads, head_dim)) return rc;
+  if (n < 0 || (n > 0 && (!blocks || !out)) || ((uintptr_t)out & 15)) return fail(GLLM_ATTN_EINVAL, "bad blocks or out (16-byte aligned)");
+  const BoundsValuesArgs a{(const uint8_t*)bounds, bounds_stride, num_blocks, blocks, n, out, num_kv_heads, head_dim};
+  return hip_check(launch_key_bounds_values(a, (hipStream_t)stream), "key bounds values launch");
+}
+
+int gllm_select_blocks(const gllm_sparse_plan* p, const void* q, int64_t q_row_stride, const void* bounds,
+                       int64_t bounds_stride, int64_t num_blocks, const int32_t* block_table, int64_t block_table_stride,
+                       int32_t* selected, int32_t dtype, void* stream) {
+  Range range("gllm_select_blocks");
+  if (int rc = sparse_check(p, num_blocks, block_table, block_table_stride)) return rc;
+  if (int rc = bounds_check(bounds, bounds_stride, num_blocks, p->Hkv, p->D)) return rc;
+  if (p->rows.empty()) return ok();                // empty tensors have no address
+  if (!q || !selected) return fail(GLLM_ATTN_EINVAL, "null q or selected");
+  if (dtype != p->dtype) return fail(GLLM_ATTN_EINVAL, "dtype %d differs from the plan's %d", dtype, p->dtype);
+  if (q_row_stride < (int64_t)p->Hq * p->D) return fail(GLLM_ATTN_EINVAL, "q row stride < num_q_heads * head_dim");
+  SelectArgs a{};
+  a.q = q; a.q_row_stride = q_row_stride;
+  a.bounds = (const uint8_t*)bounds; a.bounds_stride = bounds_stride; a.num_blocks = num_blocks;
+  a.block_table = block_table; a.block_table_stride = block_table_stride;
+  a.rows = (const SparseRow*)(p->ws + p->off_rows);
+  a.tiles = (const ScoreTile*)(p->ws + p->off_tiles);
+  a.scores = (float*)(p->ws + p->off_scores); a.score_stride = p->score_stride;
+  a.selected = selected; a.width = p->width; a.first = p->first; a.recent = p->recent;
+  block_div(p->bs, &a.block_magic, &a.block_shift);
+  a.num_q_heads = p->Hq; a.num_kv_heads = p->Hkv; a.head_dim = p->D; a.dtype = dtype;
+  for (const gllm_sparse_plan::Slab& sb : p->slabs) {
+    a.row0 = sb.row0; a.n_rows = sb.n_rows; a.tile0 = sb.tile0; a.n_tiles = sb.n_tiles; a.max_blocks = sb.max_blocks;
+    if (int rc = hip_check(launch_select_blocks(a, (hipStream_t)stream), "block selection launch")) return rc;
+  }
+  return ok();
+}
+
+int gllm_sparse_attention(const gllm_sparse_plan* p, const void* q, int64_t q_row_stride, void* out, int64_t out_row_stride,
+                          const void* k_cache, const void* v_cache, int64_t cache_slot_stride, int64_t num_blocks,
+                          const int32_t* block_table, int64_t block_table_stride, const int32_t* selected, float scale,
+                          int32_t dtype, int32_t kv_dtype, void* stream) {
+  Range range("gllm_sparse_attention");
+  if (int rc = sparse_check(p, num_blocks, block_table, block_table_stride)) return rc;
+  if (int rc = sparse_cache_check(p, k_cache, v_cache, cache_slot_stride, kv_dtype)) return rc;
+  if (p->rows.empty()) return ok();
+  if (!q || !out || !selected) return fail(GLLM_ATTN_EINVAL, "null pointer argument");
+  if (dtype != p->dtype) return fail(GLLM_ATTN_EINVAL, "dtype %d differs from the plan's %d", dtype, p->dtype);
+  const int64_t hd = (int64_t)p->Hq * p->D;
+  if (q_row_stride < hd || out_row_stride < hd) return fail(GLLM_ATTN_EINVAL, "q/out row stride < num_q_heads * head_dim");
+  AttnArgs a{};
+  if (int rc = fill_common(a, p->Hq, p->Hkv, p->D, scale, dtype, kv_dtype)) return rc;
+  const bool kv4 = kv_dtype == GLLM_DTYPE_MXFP4;
+  a.q = q; a.q_row_stride = q_row_stride; a.out = out; a.out_row_stride = out_row_stride;
+  a.k_cache = k_cache; a.v_cache = v_cache; a.cache_slot_stride = cache_slot_stride; a.num_blocks = num_blocks;
+  a.block_table = block_table; a.block_table_stride = block_table_stride;
+  a.block_size = p->bs;
+  block_div(p->bs, &a.block_magic, &a.block_shift);
+  if (kv4) a.kv4_record = (int32_t)kv4_record_bytes(p->bs, p->D);
+  a.selected = selected; a.sel_width = p->width;
+  a.sparse_rows = (const SparseRow*)(p->ws + p->off_rows);
+  a.n_sparse_rows = (int32_t)p->rows.size();
+  a.sparse_splits = p->splits;
+  a.partial_ml = (float*)(p->ws + p->off_ml);
+  a.partials = (float*)(p->ws + p->off_part);
+  const bool mfma = mfma_dtype(dtype) && (p->D == 64 || p->D == 128) && p->Hq / p->Hkv <= 16 &&
+                    (kv_dtype == dtype || kv_dtype == GLLM_DTYPE_FP8_E4M3 || kv4);
+  hipStream_t st = (hipStream_t)stream;
+  return hip_check(mfma ? launch_sparse_attention_mfma(a, st) : launch_sparse_attention_generic(a, st), "sparse attention launch");
 }
 
 }  // extern "C"

@@ -149,6 +149,9 @@ __device__ __forceinline__ u32x2 pack4(const Raw4<KV>& r) {
 // A 4-bit cache (kv4, with WIN; head dims that are multiples of 32) has rows in
 // two places, codes and scales, so a row is its byte place and its row in the
 // block.
+// SEL (sparse attention): one query row a sequence; the keys count through the
+// blocks that the row selected for the kv head (key v is key v % bs of the block that
+// entry v / bs names).
 // WIN (sliding window): the sub-tiles count through the keys that the first of
 // the workgroup's rows leaves (key_skip); a sub-tile at the edge of a row's
 // window is masked.
@@ -166,7 +169,7 @@ struct StreamCfg {
   // 4 are rare)
   static constexpr int kPF = V < 4 || DP == 256 ? 0 : (kBytes <= 256 ? 2 : 1);
 };
-template <bool DENSE, typename KV, typename QT, int DP, bool FUSED, int V, bool WIN>
+template <bool DENSE, typename KV, typename QT, int DP, bool FUSED, int V, bool WIN, bool SEL = false>
 __global__ void __launch_bounds__((64 * StreamCfg<KV, QT, DP, V>::kNW)) attn_stream_kernel(AttnArgs a) {
   using Cfg = StreamCfg<KV, QT, DP, V>;
   constexpr int NW = Cfg::kNW, PF = Cfg::kPF;
@@ -182,19 +185,38 @@ __global__ void __launch_bounds__((64 * StreamCfg<KV, QT, DP, V>::kNW)) attn_str
   float (*const nv)[QS] = reinterpret_cast<float (*)[QS]>(lds + 32 * QS);
   float (*const macc)[16][QS] = reinterpret_cast<float (*)[16][QS]>(lds);
   static_assert(kFusedRows == 16, "LDS layout");
-  const int wgrp = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
+  static_assert(!SEL || (!DENSE && !FUSED), "a selection is the paged kernel's");
+  const int wgrp = SEL ? blockIdx.z : blockIdx.x, kvh = blockIdx.y, b = SEL ? blockIdx.x : blockIdx.z;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, grp = lane >> 4;
   const int D = a.head_dim, half = D / 2;
   const int G = a.num_q_heads / a.num_kv_heads;
-  int ctx, qlen, L;
+  int ctx, qlen, L, seq = b;
   int64_t row0;
+  const int32_t* sel = nullptr;
   if (DENSE) {
     ctx = 0;
     qlen = a.dense_Tq;
     L = a.dense_T;
     row0 = (int64_t)b * a.dense_Tq;
+  } else if constexpr (SEL) {
+    const SparseRow sr = a.sparse_rows[b];
+    sel = a.selected + ((int64_t)sr.row * a.num_kv_heads + kvh) * a.sel_width;
+    const int own = (int)div_bs((uint32_t)sr.pos, a.block_magic, a.block_shift);
+    const int ns = selected_blocks(sel, a.sel_width, own, 64 * NW, reinterpret_cast<int*>(lds));
+    __syncthreads();
+    seq = sr.seq;
+    row0 = sr.row;
+    qlen = 1;
+    L = ns == 0 ? 0 : selected_keys(ns, sel[ns - 1], own, sr.pos, a.block_size);
+    ctx = L - 1;
+    if (L == 0) {                                // no key: zeros
+      const int c1 = min(16 * wgrp + 16, G);
+      for (int e = 16 * wgrp * D + tid; e < c1 * D; e += 64 * NW)
+        stq<QT>((QT*)a.out + row0 * a.out_row_stride + (int64_t)kvh * G * D + e, 0.f);
+      return;
+    }
   } else {
     if (b >= a.num_seqs) return;
     const SeqInfo si = a.seqs[b];
@@ -213,7 +235,7 @@ __global__ void __launch_bounds__((64 * StreamCfg<KV, QT, DP, V>::kNW)) attn_str
   const auto key_of = [&](int v) { return WIN && v >= sk.from ? v + sk.by : v; };
   const int nkeys = DENSE ? L : (FUSED ? ctx : ctx + r_last + 1 - (WIN ? sk.by : 0));
   const int vis = DENSE ? L - 1 : ctx + r;       // last visible key of the lane's column
-  const int32_t* bt = DENSE ? nullptr : a.block_table + (int64_t)b * a.block_table_stride;
+  const int32_t* bt = DENSE ? nullptr : a.block_table + (int64_t)seq * a.block_table_stride;
   constexpr bool k4 = std::is_same<KV, kv4>::value;
   const KV* kbase = DENSE ? (const KV*)a.k + (int64_t)b * a.k_batch_stride + (int64_t)kvh * D
                           : (const KV*)a.k_cache + (int64_t)kvh * D;
@@ -233,7 +255,8 @@ __global__ void __launch_bounds__((64 * StreamCfg<KV, QT, DP, V>::kNW)) attn_str
     if (DENSE) return 0;
     const int v = min(16 * (wave + NW * t) + n, nkeys - 1);
     const int key = WIN ? seen_key(key_of(v), sk, a.sinks) : v;
-    return (uint32_t)bt[div_bs((uint32_t)key, a.block_magic, a.block_shift)];
+    const uint32_t bi = div_bs((uint32_t)key, a.block_magic, a.block_shift);
+    return (uint32_t)bt[SEL ? (uint32_t)sel[bi] : bi];
   };
   struct Tile {
     Raw4<KV> k[NT];
@@ -592,6 +615,32 @@ static hipError_t launch_stream_d(const AttnArgs& a, dim3 grid, hipStream_t st) 
   else if (a.head_dim > 4) by_dim(std::integral_constant<int, 2>());
   else go(std::integral_constant<int, 64>(), std::integral_constant<int, 1>());
   return hipGetLastError();
+}
+
+// Sparse attention: head dims are multiples of 8 (a 4-bit cache's of 32).
+template <typename QT>
+static hipError_t launch_stream_sparse(const AttnArgs& a, dim3 grid, hipStream_t st) {
+  auto go = [&](auto kv, auto dp) {
+    using KV = decltype(kv);
+    constexpr int DP = decltype(dp)::value;
+    const dim3 block(64 * StreamCfg<KV, QT, DP, 4>::kNW);
+    hipLaunchKernelGGL((attn_stream_kernel<false, KV, QT, DP, false, 4, std::is_same<KV, kv4>::value, true>), grid, block, 0,
+                       st, a);
+  };
+  auto by_dim = [&](auto kv) {
+    if (a.head_dim <= 64) go(kv, std::integral_constant<int, 64>());
+    else if (a.head_dim <= 128) go(kv, std::integral_constant<int, 128>());
+    else go(kv, std::integral_constant<int, 256>());
+    return hipGetLastError();
+  };
+  switch (a.kv_dtype) {
+    case kF32: return by_dim(float{});
+    case kBF16: return by_dim(__bf16{});
+    case kF16: return by_dim(_Float16{});
+    case kFP8: return by_dim(fp8e4m3{});
+    case kMXFP4: return by_dim(kv4{});
+    default: return hipErrorInvalidValue;
+  }
 }
 
 // A 4-bit cache: head dims are multiples of 32.

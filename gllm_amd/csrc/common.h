@@ -434,6 +434,59 @@ struct DecodeSeg {
   int32_t ord;
 };
 
+// Keys [k0, k1) that `nrows` query rows (prefix_rows[row0 ..]) of several decode
+// sequences share, for kv head kvh and the wgrp-th 8 x 32 of their (row, head)
+// columns; their blocks stand in the table row of sequence seq.  The rows' states
+// are partial `ord` of their (sequence, kv head).
+struct PrefixItem {
+  int32_t seq, kvh, wgrp;
+  int32_t k0, k1;
+  int32_t row0, nrows;
+  int32_t ord;
+};
+// One such query row: row r of sequence seq, at position pos, row q_row of q.
+struct PrefixRow {
+  int32_t q_row, seq, r, pos;
+};
+
+// A query row of sparse attention: row `row` of q / out / selected, at position pos
+// of sequence seq.
+struct SparseRow {
+  int32_t row, seq, pos, pad;
+};
+// A cache block whose first n keys have bounds to be written: block `block` of
+// sequence seq.
+struct BoundsBlock {
+  int32_t seq, block, n, pad;
+};
+// Up to 16 / (heads of a kv head, rounded up to a power of two) query rows of one
+// sequence whose blocks are scored together: sparse_rows[row0 .. row0 + nrows), of
+// which the last sees nblocks blocks.
+struct ScoreTile {
+  int32_t row0, nrows, seq, nblocks;
+};
+
+// How many entries of a row's selection count: up to the first that is not above
+// the one before it or lies behind the row's own block.  The workgroup's threads
+// take part; tmp: an int of LDS per wave.
+__device__ __forceinline__ int selected_blocks(const int32_t* sel, int width, int own, int nthreads, int* tmp) {
+  int n = width;
+  for (int j = threadIdx.x; j < width; j += nthreads) {
+    const int s = sel[j], before = j > 0 ? sel[j - 1] : -1;
+    if (s <= before || s < 0 || s > own) n = min(n, j);
+  }
+#pragma unroll
+  for (int x = 1; x < 64; x *= 2) n = min(n, __shfl_xor(n, x, 64));
+  if ((threadIdx.x & 63) == 0) tmp[threadIdx.x >> 6] = n;
+  __syncthreads();
+  for (int w = 0; w < nthreads / 64; ++w) n = min(n, tmp[w]);
+  return n;
+}
+// Keys of n > 0 such blocks: whole ones, but the row's own up to its position.
+__device__ __forceinline__ int selected_keys(int n, int last, int own, int pos, int block_size) {
+  return (n - 1) * block_size + (last == own ? pos - own * block_size + 1 : block_size);
+}
+
 // Partials of one (sequence, kv-head group): head i of the group has `count`
 // of them from pbase + i * count on (count <= 1: none, the task wrote the output).
 struct MergeInfo {

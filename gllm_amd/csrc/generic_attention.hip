@@ -2,7 +2,7 @@
 // 256): the fp32 model's kernels and the dispatch between them.  The 16-bit
 // models' instantiations are units of their own (generic_attention_bf16.hip,
 // generic_attention_f16.hip), and so are those with a sliding window
-// (generic_window_*.hip).
+// (generic_window_*.hip) and of sparse attention (generic_sparse_*.hip).
 #ifndef GLLM_GENERIC_QT
 #define GLLM_GENERIC_QT float
 #define GLLM_GENERIC_LAUNCH launch_generic_f32
@@ -10,13 +10,17 @@
 #endif
 
 #include "attention_stream.h"
-#ifndef GLLM_GENERIC_WINDOW
+#if !defined(GLLM_GENERIC_WINDOW) && !defined(GLLM_GENERIC_SPARSE)
 #include "attention_tile.h"
 #endif
 
 namespace gllm {
 
-#ifdef GLLM_GENERIC_WINDOW
+#if defined(GLLM_GENERIC_SPARSE)
+hipError_t GLLM_GENERIC_LAUNCH(const AttnArgs& a, dim3 grid, hipStream_t st) {
+  return launch_stream_sparse<GLLM_GENERIC_QT>(a, grid, st);
+}
+#elif defined(GLLM_GENERIC_WINDOW)
 hipError_t GLLM_GENERIC_LAUNCH(const AttnArgs& a, dim3 grid, hipStream_t st) {
   return launch_stream_t<GLLM_GENERIC_QT, true>(a, false, grid, st);
 }
@@ -33,6 +37,9 @@ hipError_t launch_generic_f16(const AttnArgs& a, bool tile, bool dense, dim3 gri
 hipError_t launch_window_f32(const AttnArgs& a, dim3 grid, hipStream_t st);
 hipError_t launch_window_bf16(const AttnArgs& a, dim3 grid, hipStream_t st);
 hipError_t launch_window_f16(const AttnArgs& a, dim3 grid, hipStream_t st);
+hipError_t launch_sparse_generic_f32(const AttnArgs& a, dim3 grid, hipStream_t st);
+hipError_t launch_sparse_generic_bf16(const AttnArgs& a, dim3 grid, hipStream_t st);
+hipError_t launch_sparse_generic_f16(const AttnArgs& a, dim3 grid, hipStream_t st);
 
 static hipError_t launch_kind(AttnArgs a, bool tile, bool dense, dim3 grid, hipStream_t st) {
   const size_t eq = a.dtype == kF32 ? 4 : 2;
@@ -101,6 +108,23 @@ hipError_t launch_attention_generic(AttnArgs a, bool dense, int B, int max_q, in
   dim3 g = grid(max_stream_q, kStreamCols);
   if (2 * stream_rows < (int64_t)B * max_stream_q) g.x |= 1;
   return launch_kind(a, false, false, g, st);
+}
+
+// Any model dtype over any cache, and groups of more than 16 heads: one workgroup per
+// (row, kv head, 16 heads of the group) over all its selected keys.
+hipError_t launch_sparse_attention_generic(AttnArgs a, hipStream_t st) {
+  if (a.n_sparse_rows == 0) return hipSuccess;
+  const int G = a.num_q_heads / a.num_kv_heads;
+  const dim3 grid(a.n_sparse_rows, a.num_kv_heads, (G + kStreamCols - 1) / kStreamCols);
+  const size_t eq = a.dtype == kF32 ? 4 : 2;
+  a.vec_out = a.out_row_stride % 4 == 0 && ((uintptr_t)a.out & (4 * eq - 1)) == 0;
+  a.window = INT32_MAX;        // the 4-bit kernels take one
+  switch (a.dtype) {
+    case kF32: return launch_sparse_generic_f32(a, grid, st);
+    case kBF16: return launch_sparse_generic_bf16(a, grid, st);
+    case kF16: return launch_sparse_generic_f16(a, grid, st);
+    default: return hipErrorInvalidValue;
+  }
 }
 #endif  // GLLM_GENERIC_DISPATCH
 

@@ -139,6 +139,54 @@ struct AttnArgs {
   int32_t window, sinks;
   int32_t mixed_half;          // windows, 4-bit caches: a mixed launch's items by two 4-wave workgroups each
   int32_t kv4_record;          // 4-bit cache: bytes of one (block, kv head)
+  // shared prefixes (n_prefix_items > 0)
+  const PrefixItem* prefix_items;
+  const PrefixRow* prefix_rows;
+  int32_t n_prefix_items;
+  // sparse attention: the blocks selected for each (query row, kv head)
+  const int32_t* selected;     // [rows, Hkv, sel_width]
+  const SparseRow* sparse_rows;
+  int32_t n_sparse_rows, sel_width, sparse_splits;
+};
+
+// Key bounds, block scores and the selection (sparse_select.hip)
+struct BoundsArgs {
+  const void* k_cache;
+  int64_t cache_slot_stride, num_blocks;
+  const int32_t* block_table;
+  int64_t block_table_stride;
+  const BoundsBlock* blocks;
+  int32_t n_blocks;
+  uint8_t* bounds;
+  int64_t bounds_stride;       // bytes between blocks
+  int32_t block_size, kv4_record, num_kv_heads, head_dim, dtype, kv_dtype;
+};
+struct BoundsValuesArgs {
+  const uint8_t* bounds;
+  int64_t bounds_stride, num_blocks;
+  const int64_t* blocks;
+  int64_t n_blocks;
+  float* out;                  // [n_blocks, Hkv, 2, D]
+  int32_t num_kv_heads, head_dim;
+};
+struct SelectArgs {
+  const void* q;
+  int64_t q_row_stride;
+  const uint8_t* bounds;
+  int64_t bounds_stride, num_blocks;
+  const int32_t* block_table;
+  int64_t block_table_stride;
+  const SparseRow* rows;
+  const ScoreTile* tiles;      // tiles [tile0, tile0 + n_tiles) score the rows [row0, row0 + n_rows)
+  int32_t row0, n_rows, tile0, n_tiles;
+  int32_t max_blocks;          // the most that a row of them sees
+  float* scores;               // [n_rows, Hkv, score_stride]
+  int64_t score_stride;
+  int32_t* selected;           // [rows, Hkv, width]
+  int32_t width, first, recent;
+  uint32_t block_magic;
+  int32_t block_shift;
+  int32_t num_q_heads, num_kv_heads, head_dim, dtype;
 };
 
 struct MetadataArgs {
@@ -242,6 +290,11 @@ hipError_t launch_build_metadata(const MetadataArgs& a, hipStream_t stream);
 // MFMA kernels: bf16 or fp16 model (a.dtype), head dim 64 or 128, cache in
 // the model dtype or fp8 e4m3fn
 hipError_t launch_paged_attention_mfma(const AttnArgs& a, bool has_prefill, bool has_decode, hipStream_t stream);
+hipError_t launch_sparse_attention_mfma(const AttnArgs& a, hipStream_t stream);
+hipError_t launch_sparse_attention_generic(AttnArgs a, hipStream_t stream);
+hipError_t launch_key_bounds(const BoundsArgs& a, hipStream_t stream);
+hipError_t launch_key_bounds_values(const BoundsValuesArgs& a, hipStream_t stream);
+hipError_t launch_select_blocks(const SelectArgs& a, hipStream_t stream);
 hipError_t launch_dense_attention_mfma(const AttnArgs& a, int B, int Tq, hipStream_t stream);
 // Generic kernels: max_q the largest query length, max_stream_q the largest of
 // the sequences on the stream kernel (0: every sequence is tiled)

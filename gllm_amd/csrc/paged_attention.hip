@@ -94,6 +94,7 @@ struct DecodeTask {
   int nseg;     // tasks of this (sequence, head group); 1: normalise and write the output, else a partial for merge_splits_kernel
   int pbase;    // partial of head i of the group: pbase + i * nseg + ord
   int ord;
+  const int32_t* sel = nullptr;   // SEL: the (row, kv head)'s selected blocks, the task's keys counting through them
 };
 
 // New tokens written by the attention launch (a.k_new != null): the task whose
@@ -151,11 +152,14 @@ __device__ __forceinline__ void write_new_keys(const AttnArgs& a, const DecodeTa
 
 // Runs one task with every wave of the workgroup; returns with the workgroup
 // converged (no early exit), so a workgroup can run several tasks in a row.
+// SEL (sparse attention, HW = 1): key v is key v % bs of the block that entry
+// v / bs of tk.sel names, each entry checked by the caller; one query row.
 // WIN: the keys are those of the sequence without the run that its window
 // leaves out (key_skip): tk's range counts them through, key v at v >= from
 // being key v + by.
-template <typename T, int D, int HW, int KW, int KF, bool WIN>
+template <typename T, int D, int HW, int KW, int KF, bool WIN, bool SEL = false>
 __device__ __forceinline__ void decode_task(const AttnArgs& a, const DecodeTask& tk, char* lds) {
+  static_assert(!SEL || HW == 1, "a selection is one kv head's");
   constexpr int NW = HW * KW;
   constexpr int E = KF == kKV16 ? 2 : 1;   // bytes per cached element (4-bit: strides in bytes)
   using Cfg = DecodeCfg<D, NW, KF>;
@@ -208,11 +212,13 @@ __device__ __forceinline__ void decode_task(const AttnArgs& a, const DecodeTask&
   const int nblk_s = both ? (int)div_bs((uint32_t)(sk.from - 1), a.block_magic, a.block_shift) - blk0 + 1 : 0;
   const int bgap = both ? (int)div_bs((uint32_t)(sk.from + sk.by), a.block_magic, a.block_shift) - blk0 - nblk_s : 0;
   const int nblk = (int)div_bs((uint32_t)key_of(kend - 1), a.block_magic, a.block_shift) - (WIN ? blk0 + bgap : blk0) + 1;
-  const int32_t* bt = a.block_table + (int64_t)seq * a.block_table_stride + blk0;
-  const uint32_t bid = tid < nblk ? (uint32_t)bt[WIN && tid >= nblk_s ? tid + bgap : tid] : 0u;
+  const int32_t* bt = a.block_table + (int64_t)seq * a.block_table_stride + (SEL ? 0 : blk0);
+  // the table's column of entry e of the cache
+  const auto column = [&](int e) { return SEL ? tk.sel[blk0 + e] : (WIN && e >= nblk_s ? e + bgap : e); };
+  const uint32_t bid = tid < nblk ? (uint32_t)bt[column(tid)] : 0u;
   const int tid2 = tid + 64 * NW;
   uint32_t bid2 = 0u;
-  if constexpr (kIds2) bid2 = tid2 < nblk ? (uint32_t)bt[WIN && tid2 >= nblk_s ? tid2 + bgap : tid2] : 0u;
+  if constexpr (kIds2) bid2 = tid2 < nblk ? (uint32_t)bt[column(tid2)] : 0u;
   const T* qp = (const T*)a.q + qrow * a.q_row_stride + (int64_t)qh * D;
   u32x4 qraw[NK], praw[kPairInLane ? 1 : NK], craw[NC], sraw[NC];
 #pragma unroll
@@ -823,9 +829,15 @@ __device__ __forceinline__ int pf_swz(int r) {
 // count through the sinks and then the window from its first key; tiles at
 // either edge of a row's window are masked, and a row's reference is chosen at
 // its first tile with a visible key.
-template <typename T, int D, bool DENSE, int NW, int NS, int KF, bool WIN>
-__device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it, int seq, int kvh, int wgrp, char* lds) {
+// PFX (shared prefix): the columns are the (query row, head of the group) pairs of
+// every decode sequence that shares the keys (a.prefix_rows), 32 neighbouring ones a
+// wave; every row sees every key of [px->k0, px->k1), which positions count from k0,
+// and the rows' states go to their partials.
+template <typename T, int D, bool DENSE, int NW, int NS, int KF, bool WIN, bool PFX = false>
+__device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it, int seq, int kvh, int wgrp, char* lds,
+                                           const PrefixItem* px = nullptr) {
   static_assert(!(DENSE && (KF != kKV16 || WIN)), "the dense op has no cache");
+  static_assert(!PFX || (!DENSE && !WIN), "a shared prefix is paged and has no window");
   constexpr bool KREG = KF != kKV16;       // K/V pass through registers (widened) on the way to LDS
   using Cfg = PrefillCfg<D, NS>;
   constexpr int NQ = D / 16;               // Q operand chunks (16 dims)
@@ -845,12 +857,19 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
     qlen = a.dense_Tq;
     TK = a.dense_T;
     qstart = (int64_t)seq * a.dense_Tq;
+  } else if (PFX) {
+    ctx = 0;
+    qlen = px->nrows;
+    TK = px->k1 - px->k0;
+    qstart = 0;
   } else {
     ctx = it.ctx_len;
     qlen = it.q_len;
     TK = ctx + qlen;
     qstart = it.q_row_start;
   }
+  constexpr bool PAIRS = DENSE || PFX;      // columns are neighbouring (row, head) pairs, every key is visible
+  const int k0 = PFX ? px->k0 : 0;          // key that position 0 is
   const int G = a.num_q_heads / a.num_kv_heads;
   // The wave's 32 MFMA columns.  Paged: 32 query rows of one head (the causal
   // edge then cuts few tiles).  Dense: neighbouring (row, head of the group)
@@ -860,20 +879,22 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
   // rows per wave, 73 with this and 8-byte loads a tile ahead).
   const int combo = wgrp * NW + wave;
   const int nrb = (qlen + 31) / 32;
-  const int ncol = qlen * G;                // dense
-  const bool wact = DENSE ? combo * 32 < ncol : combo < G * nrb;
+  const int ncol = qlen * G;                // dense, shared prefix
+  const bool wact = PAIRS ? combo * 32 < ncol : combo < G * nrb;
   const int dcol = min(combo * 32 + n, ncol - 1);
-  const int g = DENSE ? dcol % G : (wact ? combo % G : 0);
-  const int rblk = !DENSE && wact ? combo / G : 0;
+  const int g = PAIRS ? dcol % G : (wact ? combo % G : 0);
+  const int rblk = !PAIRS && wact ? combo / G : 0;
   const int r0 = rblk * 32;
   const int last_combo = min(wgrp * NW + NW - 1, G * nrb - 1);
-  const int kend_wg = DENSE ? TK : ctx + min(qlen - 1, (last_combo / G) * 32 + 31) + 1;
-  const int kend_w = DENSE ? TK : ctx + min(qlen - 1, r0 + 31) + 1;
-  const int r = DENSE ? dcol / G : r0 + n;
-  const bool row_ok = wact && (DENSE ? combo * 32 + n < ncol : r < qlen);
+  const int kend_wg = PAIRS ? TK : ctx + min(qlen - 1, (last_combo / G) * 32 + 31) + 1;
+  const int kend_w = PAIRS ? TK : ctx + min(qlen - 1, r0 + 31) + 1;
+  const int r = PAIRS ? dcol / G : r0 + n;
+  const bool row_ok = wact && (PAIRS ? combo * 32 + n < ncol : r < qlen);
   const int rr = min(r, qlen - 1);
-  const int vis = ctx + rr;
-  const int64_t qrow = qstart + rr;
+  const int vis = PFX ? TK - 1 : ctx + rr;
+  PrefixRow pr{};
+  if constexpr (PFX) pr = a.prefix_rows[px->row0 + rr];
+  const int64_t qrow = PFX ? pr.q_row : qstart + rr;
   const int qh = kvh * G + g;
 
   // WIN: from here on positions count through the keys that are not left out
@@ -890,9 +911,11 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
   // Block ids of keys [0, kend_wg), loaded into registers now and cached in
   // LDS (first kBidCache blocks; any beyond are read from the table
   // directly) after the first tiles' copies are issued.
-  const int32_t* bt = DENSE ? nullptr : a.block_table + (int64_t)seq * a.block_table_stride;
+  // (PFX: those of [k0, k1), the table seen from k0's block on)
+  const int blk0 = PFX ? (int)div_bs((uint32_t)k0, a.block_magic, a.block_shift) : 0;
+  const int32_t* bt = DENSE ? nullptr : a.block_table + (int64_t)seq * a.block_table_stride + blk0;
   constexpr int KB = (Cfg::kBidCache + NT - 1) / NT;
-  const int nbc = DENSE ? 0 : min((int)div_bs((uint32_t)(kend_wg - 1), a.block_magic, a.block_shift) + (WIN ? 1 - bgap : 1), Cfg::kBidCache);
+  const int nbc = DENSE ? 0 : min((int)div_bs((uint32_t)(k0 + kend_wg - 1), a.block_magic, a.block_shift) - blk0 + (WIN ? 1 - bgap : 1), Cfg::kBidCache);
   uint32_t lb[KB];
 #pragma unroll
   for (int k = 0; k < KB; ++k)
@@ -907,7 +930,7 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
 #pragma unroll
     for (int kk = 0; kk < NQ; ++kk) qraw[kk] = ld16(qp + 16 * kk);
     if (q_rope) {
-      const int64_t crow = a.rope_mode == kRopeByPosition ? (int64_t)vis : qrow;
+      const int64_t crow = a.rope_mode == kRopeByPosition ? (int64_t)(PFX ? pr.pos : vis) : qrow;
       const T* cp = (const T*)a.rope_cos + crow * a.rope_row_stride + 8 * h;
       const T* sp = (const T*)a.rope_sin + crow * a.rope_row_stride + 8 * h;
 #pragma unroll
@@ -973,7 +996,7 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
   auto copy_key = [&](int ts, int i) {
     const int row = KF == kKV4 ? (wave & 3) * 16 + (lane & 15) : (i * NW + wave) * RPS + lane / CPR;
     const int v = min(ts + row, nkeys_wg - 1);
-    return WIN && v >= sk.from ? v + by : v;
+    return WIN && v >= sk.from ? v + by : k0 + v;
   };
   auto dma_bids = [&](int ts, Row (&slot)[NB]) {
 #pragma unroll
@@ -983,12 +1006,12 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
       } else {
         const int p = copy_key(ts, i);
         const uint32_t bi = div_bs((uint32_t)p, a.block_magic, a.block_shift);
-        const uint32_t ci = WIN && p >= sk.from + by ? bi - (uint32_t)bgap : bi;
+        const uint32_t ci = WIN && p >= sk.from + by ? bi - (uint32_t)bgap : bi - blk0;
         uint32_t blk;
         if (ci < (uint32_t)Cfg::kBidCache) {
           blk = (uint32_t)lbid[ci];
         } else {
-          blk = (uint32_t)bt[bi];
+          blk = (uint32_t)bt[bi - blk0];
           if (blk >= (uint64_t)a.num_blocks) blk = 0;
         }
         if constexpr (KF == kKV4) slot[i] = Row{blk, (uint32_t)p - bi * (uint32_t)a.block_size};
@@ -1424,7 +1447,7 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
   constexpr int TPB = NS / 2;
   static_assert(NS % 2 == 0 && TPB >= 1, "stage ring must hold two tile groups");
   const int ntiles = (nkeys_wg + BN - 1) / BN;
-  const int full_end = ctx + r0 - by;      // tiles ending at or before key ctx + r0 need no mask
+  const int full_end = PFX ? TK - 1 : ctx + r0 - by;      // tiles ending at or before key ctx + r0 need no mask
   // The first TPB tiles' copies are addressed with block ids read straight
   // from the table (issued together with the loads above), so they need no
   // trip through LDS and a barrier first; every load so far is waited for
@@ -1439,7 +1462,7 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
       if (!DENSE) {
         const int p = copy_key(t * BN, i);
         const uint32_t bi = div_bs((uint32_t)p, a.block_magic, a.block_shift);
-        fbid[t][i] = (uint32_t)bt[bi];
+        fbid[t][i] = (uint32_t)bt[bi - blk0];
         foff[t][i] = (uint32_t)p - bi * (uint32_t)a.block_size;
       }
     }
@@ -1518,6 +1541,24 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
     }
   }
 
+  if constexpr (PFX) {
+    // the row's state: reference (log2 units), sum and unnormalised output
+    const float lt = sum_xor32(lsum);
+    if (row_ok) {
+      const int hg = kvh / a.heads_per_wg;
+      const MergeInfo mi = a.merge[pr.seq * a.head_groups + hg];
+      const int64_t at = ((int64_t)mi.pbase + (int64_t)(kvh - hg * a.heads_per_wg) * mi.count + px->ord) * 16 + pr.r * G + g;
+      float* pa = a.partials + at * D + 4 * h;
+#pragma unroll
+      for (int db = 0; db < NO; ++db)
+#pragma unroll
+        for (int jq = 0; jq < 4; ++jq)
+          *reinterpret_cast<f32x4*>(pa + 32 * db + 8 * jq) =
+              f32x4{o[db][4 * jq], o[db][4 * jq + 1], o[db][4 * jq + 2], o[db][4 * jq + 3]};
+      if (h == 0) *reinterpret_cast<u32x2*>(a.partial_ml + at * 2) = u32x2{__float_as_uint(rref), __float_as_uint(lt)};
+    }
+    return;
+  }
   if (row_ok) {
     const float inv = 1.f / sum_xor32(lsum);
     T* op = (T*)a.out + qrow * a.out_row_stride + (int64_t)qh * D + 4 * h;
@@ -1663,6 +1704,88 @@ prefill_half_kernel(AttnArgs a) {
   prefill_wg<T, D, false, kPrefillHalfWaves, kPrefillHalfStages, KF, true>(a, it, it.seq, it.a, it.kind_b >> 8, lds);
 }
 
+// Shared prefixes: one workgroup per (group, kv head, 8 waves of 32 columns, key
+// range).
+template <typename T, int D, int KF>
+__global__ void __launch_bounds__(64 * kPrefillOnlyWaves) __attribute__((amdgpu_waves_per_eu(2)))
+prefix_kernel(AttnArgs a) {
+  __shared__ __attribute__((aligned(16))) char lds[PrefillCfg<D, kPrefillOnlyStages>::kLdsBytes];
+  const PrefixItem px = a.prefix_items[blockIdx.x];
+  const WorkItem none{};
+  prefill_wg<T, D, false, kPrefillOnlyWaves, kPrefillOnlyStages, KF, false, true>(a, none, px.seq, px.kvh, px.wgrp, lds, &px);
+}
+
+// Sparse attention: one workgroup per (query row, kv head, split of its selected
+// keys), its eight waves taking 16-key sub-tiles in turn (decode_task).  The list
+// ends at the first entry that is not above the one before or lies behind the
+// row's own block, so any list is safe and none counts a key twice.
+template <typename T, int D, int KF>
+__global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D == 64 ? 4 : 2)))
+sparse_attn_kernel(AttnArgs a) {
+  constexpr bool WIN = KF == kKV4;               // the 4-bit kernels always take a window
+  __shared__ __attribute__((aligned(16))) char lds[DecodeCfg<D, kWaves, KF>::kLdsBytes];
+  const int per_row = a.num_kv_heads * a.sparse_splits;
+  const int ri = blockIdx.x / per_row, rest = blockIdx.x - ri * per_row;
+  const int kvh = rest / a.sparse_splits, sp = rest - kvh * a.sparse_splits;
+  const SparseRow sr = a.sparse_rows[ri];
+  const int32_t* sel = a.selected + ((int64_t)sr.row * a.num_kv_heads + kvh) * a.sel_width;
+  const int own = (int)div_bs((uint32_t)sr.pos, a.block_magic, a.block_shift);
+  const int n = selected_blocks(sel, a.sel_width, own, 64 * kWaves, reinterpret_cast<int*>(lds));
+  __syncthreads();                               // the count's LDS is the task's
+  const int keys = n == 0 ? 0 : selected_keys(n, sel[n - 1], own, sr.pos, a.block_size);
+  const int len = split_len_of(keys, a.sparse_splits);
+  DecodeTask tk;
+  tk.seq = sr.seq;
+  tk.hg = kvh;
+  tk.kbeg = min(keys, sp * len);
+  tk.kend = min(keys, tk.kbeg + len);
+  tk.q_row_start = sr.row;
+  tk.ctx_len = keys - 1;
+  tk.q_len = 1;
+  tk.nseg = a.sparse_splits;
+  tk.pbase = (ri * a.num_kv_heads + kvh) * a.sparse_splits;
+  tk.ord = sp;
+  tk.sel = sel;
+  if (tk.kbeg < tk.kend) {
+    decode_task<T, D, 1, kWaves, KF, WIN, true>(a, tk, lds);
+    return;
+  }
+  // no key: an empty partial, or a row of zeros
+  const int G = a.num_q_heads / a.num_kv_heads;
+  if (tk.nseg == 1) {
+    for (int e = threadIdx.x; e < G * D; e += 64 * kWaves)
+      ((T*)a.out)[(int64_t)sr.row * a.out_row_stride + (int64_t)kvh * G * D + e] = (T)0.f;
+  } else if ((int)threadIdx.x < G) {
+    const int64_t at = ((int64_t)tk.pbase + sp) * 16 + threadIdx.x;
+    a.partial_ml[2 * at] = kNegInf;
+    a.partial_ml[2 * at + 1] = 0.f;
+  }
+}
+// Joins the splits of every (query row, kv head): a thread per 4 dims of a head.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) sparse_merge_kernel(AttnArgs a, int total) {
+  const int e = blockIdx.x * 256 + threadIdx.x;
+  if (e >= total) return;
+  constexpr int C = D / 4;
+  const int d = 4 * (e % C), qh = e / C % a.num_q_heads, ri = e / C / a.num_q_heads;
+  const int G = a.num_q_heads / a.num_kv_heads, ns = a.sparse_splits;
+  const int64_t at = ((int64_t)ri * a.num_kv_heads + qh / G) * ns * 16 + qh % G;
+  float M = kNegInf, L = 0.f;
+  for (int s = 0; s < ns; ++s) M = fmaxf(M, a.partial_ml[(at + 16 * s) * 2]);
+  const float mu = M == kNegInf ? 0.f : M;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < ns; ++s) {                 // fixed order
+    const float m = a.partial_ml[(at + 16 * s) * 2];
+    if (m == kNegInf) continue;                  // an empty split wrote no values
+    const float w = fast_exp2(m - mu);
+    L += w * a.partial_ml[(at + 16 * s) * 2 + 1];
+    o += w * *reinterpret_cast<const f32x4*>(a.partials + (at + 16 * s) * D + d);
+  }
+  const float inv = L > 0.f ? 1.f / L : 0.f;     // no key at all: zeros
+  T* op = (T*)a.out + (int64_t)a.sparse_rows[ri].row * a.out_row_stride + (int64_t)qh * D + d;
+  st8(op, u32x2{E16<T>::pack2(o[0] * inv, o[1] * inv), E16<T>::pack2(o[2] * inv, o[3] * inv)});
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(64 * kWaves) dense_attn_kernel(AttnArgs a, int nwg) {
   __shared__ __attribute__((aligned(16))) char lds[PrefillCfg<D, kPrefillStages>::kLdsBytes];
@@ -1783,10 +1906,41 @@ static hipError_t launch_dense_t(const AttnArgs& a, dim3 grid, int nwg, hipStrea
   return hipGetLastError();
 }
 
+template <typename T, int D, int KF>
+static hipError_t launch_sparse_d(const AttnArgs& a, hipStream_t st) {
+  const int64_t wgs = (int64_t)a.n_sparse_rows * a.num_kv_heads * a.sparse_splits;
+  const int64_t total = (int64_t)a.n_sparse_rows * a.num_q_heads * (D / 4);
+  if (wgs > INT32_MAX || total > INT32_MAX - 256) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((sparse_attn_kernel<T, D, KF>), dim3((unsigned)wgs), dim3(64 * kWaves), 0, st, a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || a.sparse_splits == 1) return e;
+  hipLaunchKernelGGL((sparse_merge_kernel<T, D>), dim3((unsigned)((total + 255) / 256)), dim3(256), 0, st, a, (int)total);
+  return hipGetLastError();
+}
+template <typename T, int D>
+static hipError_t launch_sparse_t(const AttnArgs& a, hipStream_t st) {
+  switch (a.kv_dtype) {
+    case kFP8: return launch_sparse_d<T, D, kKV8>(a, st);
+    case kMXFP4: return launch_sparse_d<T, D, kKV4>(a, st);
+    default: return launch_sparse_d<T, D, kKV16>(a, st);
+  }
+}
+template <typename T, int D>
+static hipError_t launch_prefix_t(const AttnArgs& a, hipStream_t st) {
+  const dim3 grid(a.n_prefix_items), block(64 * kPrefillOnlyWaves);
+  switch (a.kv_dtype) {
+    case kFP8: hipLaunchKernelGGL((prefix_kernel<T, D, kKV8>), grid, block, 0, st, a); break;
+    case kMXFP4: hipLaunchKernelGGL((prefix_kernel<T, D, kKV4>), grid, block, 0, st, a); break;
+    default: hipLaunchKernelGGL((prefix_kernel<T, D, kKV16>), grid, block, 0, st, a); break;
+  }
+  return hipGetLastError();
+}
+
 // This file is compiled once per element type and kind, so that they build as
 // separate units in parallel: plain (the dense op and the dispatch beside the
-// bf16 one), GLLM_PAGED_WINDOW (sliding windows) and GLLM_PAGED_KV4 (4-bit
-// cache, with or without a window).
+// bf16 one), GLLM_PAGED_WINDOW (sliding windows), GLLM_PAGED_KV4 (4-bit
+// cache, with or without a window), GLLM_PAGED_SPARSE (selected blocks) and
+// GLLM_PAGED_PREFIX (shared prefixes).
 #ifdef GLLM_PAGED_F16
 using UnitT = _Float16;
 #define GLLM_UNIT(name) name##_f16
@@ -1798,6 +1952,18 @@ using UnitT = __bf16;
 #if defined(GLLM_PAGED_KV4)
 hipError_t GLLM_UNIT(launch_paged_kv4)(const AttnArgs& a, bool pf, bool dc, hipStream_t st) {
   return launch_paged_f<UnitT, kKV4, true>(a, pf, dc, st);
+}
+#elif defined(GLLM_PAGED_SPARSE)
+hipError_t GLLM_UNIT(launch_sparse)(const AttnArgs& a, hipStream_t st) {
+  if (a.head_dim == 64) return launch_sparse_t<UnitT, 64>(a, st);
+  if (a.head_dim == 128) return launch_sparse_t<UnitT, 128>(a, st);
+  return hipErrorInvalidValue;
+}
+#elif defined(GLLM_PAGED_PREFIX)
+hipError_t GLLM_UNIT(launch_prefix)(const AttnArgs& a, hipStream_t st) {
+  if (a.head_dim == 64) return launch_prefix_t<UnitT, 64>(a, st);
+  if (a.head_dim == 128) return launch_prefix_t<UnitT, 128>(a, st);
+  return hipErrorInvalidValue;
 }
 #elif defined(GLLM_PAGED_WINDOW)
 hipError_t GLLM_UNIT(launch_paged_window)(const AttnArgs& a, bool pf, bool dc, hipStream_t st) {
@@ -1814,6 +1980,8 @@ hipError_t GLLM_UNIT(launch_dense)(const AttnArgs& a, dim3 grid, int nwg, hipStr
 using PagedLaunch = hipError_t(const AttnArgs&, bool, bool, hipStream_t);
 PagedLaunch launch_paged_f16, launch_paged_window_bf16, launch_paged_window_f16, launch_paged_kv4_bf16, launch_paged_kv4_f16;
 hipError_t launch_dense_f16(const AttnArgs& a, dim3 grid, int nwg, hipStream_t st);
+using PartLaunch = hipError_t(const AttnArgs&, hipStream_t);
+PartLaunch launch_sparse_bf16, launch_sparse_f16, launch_prefix_bf16, launch_prefix_f16;
 
 hipError_t launch_paged_attention_mfma(const AttnArgs& a, bool has_prefill, bool has_decode, hipStream_t st) {
   if (a.n_items == 0) return hipSuccess;
@@ -1821,6 +1989,8 @@ hipError_t launch_paged_attention_mfma(const AttnArgs& a, bool has_prefill, bool
   if (a.kv_dtype != kFP8 && a.kv_dtype != kMXFP4 && a.kv_dtype != a.dtype) return hipErrorInvalidValue;
   if (a.dtype != kBF16 && a.dtype != kF16) return hipErrorInvalidValue;
   const bool f16 = a.dtype == kF16;
+  if (a.n_prefix_items > 0)    // the shared keys' partials, which the merge behind the decode part takes in
+    if (hipError_t e = (f16 ? launch_prefix_f16 : launch_prefix_bf16)(a, st); e != hipSuccess) return e;
   PagedLaunch* go = f16 ? launch_paged_f16 : launch_paged_bf16;
   if (a.kv_dtype == kMXFP4) go = f16 ? launch_paged_kv4_f16 : launch_paged_kv4_bf16;
   else if (a.window > 0) go = f16 ? launch_paged_window_f16 : launch_paged_window_bf16;
@@ -1830,6 +2000,15 @@ hipError_t launch_paged_attention_mfma(const AttnArgs& a, bool has_prefill, bool
     return go(w, has_prefill, has_decode, st);
   }
   return go(a, has_prefill, has_decode, st);
+}
+
+hipError_t launch_sparse_attention_mfma(const AttnArgs& a, hipStream_t st) {
+  if (a.n_sparse_rows == 0) return hipSuccess;
+  if (a.kv_dtype != kFP8 && a.kv_dtype != kMXFP4 && a.kv_dtype != a.dtype) return hipErrorInvalidValue;
+  if ((a.dtype != kBF16 && a.dtype != kF16) || a.num_q_heads / a.num_kv_heads > 16) return hipErrorInvalidValue;
+  AttnArgs s = a;
+  s.window = INT32_MAX;        // the 4-bit kernel takes one
+  return (a.dtype == kF16 ? launch_sparse_f16 : launch_sparse_bf16)(s, st);
 }
 
 hipError_t launch_dense_attention_mfma(const AttnArgs& a, int B, int Tq, hipStream_t st) {

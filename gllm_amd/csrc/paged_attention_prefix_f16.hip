@@ -1,0 +1,4 @@
+// Shared prefixes, fp16 models (paged_attention.hip).
+#define GLLM_PAGED_F16 1
+#define GLLM_PAGED_PREFIX 1
+#include "paged_attention.hip"

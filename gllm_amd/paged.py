@@ -543,11 +543,19 @@ class AttentionPlan:
     up to its own (t > p - window) and the sequence's first ``sinks`` keys
     (None: every earlier key).  Keys that no row of the batch sees are never
     read, so blocks that hold only such keys may have been given back.
+
+    ``shared_prefixes``: ``[(sequences, tokens), ...]``, sequences of the batch (a
+    sequence in one group at most) that have their first ``tokens`` keys in
+    common: their block-table rows name blocks with the same contents there.  The
+    MFMA kernels read those keys once for all decode sequences of the group
+    (query_len x G <= 16); prompts and the generic kernel read them for each.  Not
+    with a window; the decode share is page-balanced (``split_tokens`` 0 or BALANCED).
     """
 
     def __init__(self, query_lens, seq_lens, *, num_q_heads: int, num_kv_heads: int, head_dim: int,
                  block_size: int, dtype: torch.dtype, device, q_seq_stride: int = 0,
-                 split_tokens: int = 0, heads_per_wg: int = 0, window: int | None = None, sinks: int = 0):
+                 split_tokens: int = 0, heads_per_wg: int = 0, window: int | None = None, sinks: int = 0,
+                 shared_prefixes=()):
         ql = [int(x) for x in query_lens]
         sl = [int(x) for x in seq_lens]
         if len(ql) != len(sl):
@@ -562,10 +570,22 @@ class AttentionPlan:
         self._h = ctypes.c_void_p()
         qa = (ctypes.c_int32 * max(len(ql), 1))(*ql)
         sa = (ctypes.c_int32 * max(len(sl), 1))(*sl)
-        _lib.check(lib.gllm_attn_plan_create_window(ctypes.byref(self._h), qa, sa, len(ql), q_seq_stride,
-                                                    num_q_heads, num_kv_heads, head_dim, block_size,
-                                                    _lib.dtype_code(dtype), split_tokens, heads_per_wg,
-                                                    window or 0, sinks))
+        sizes = (ctypes.byref(self._h), qa, sa, len(ql), q_seq_stride, num_q_heads, num_kv_heads, head_dim, block_size,
+                 _lib.dtype_code(dtype), split_tokens, heads_per_wg)
+        groups = [([operator.index(i) for i in seqs], operator.index(n)) for seqs, n in shared_prefixes]
+        if groups:
+            if window is not None:
+                raise NotImplementedError("shared prefixes with a window, which hides them")
+            members, starts = [i for seqs, _ in groups for i in seqs], [0]
+            for seqs, _ in groups:
+                starts.append(starts[-1] + len(seqs))
+            if not all(-(1 << 31) <= x < 1 << 31 for x in members + [n for _, n in groups]):
+                raise ValueError("shared prefixes: sequence or token count out of range")
+            arrays = [(ctypes.c_int32 * max(len(x), 1))(*x) for x in (starts, members, [n for _, n in groups])]
+            _lib.check(lib.gllm_attn_plan_create_shared(*sizes, len(groups), *arrays))
+        else:
+            _lib.check(lib.gllm_attn_plan_create_window(*sizes, window or 0, sinks))
+        self.shared_prefixes = groups
         self.window, self.sinks = window, sinks
         self.num_q_heads, self.num_kv_heads, self.head_dim = num_q_heads, num_kv_heads, head_dim
         self.block_size, self.dtype = block_size, dtype
@@ -576,10 +596,12 @@ class AttentionPlan:
         self.workspace = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
         _lib.check(lib.gllm_attn_plan_upload(self._h, self.workspace.data_ptr(), nbytes,
                                              _lib.stream_ptr(self.device)))
-        arr = (ctypes.c_int64 * 11)()
-        _lib.check(lib.gllm_attn_plan_info(self._h, arr, 11))
         keys = ("work_items", "split_tokens", "decode_seqs", "prefill_seqs", "partials", "rows", "heads_per_wg",
                 "decode_waves", "prefill_waves", "decode_segments", "mixed_half")
+        if groups:                         # two facts more, the first of which costs a count
+            keys += ("most_task_blocks", "prefix_items")
+        arr = (ctypes.c_int64 * len(keys))()
+        _lib.check(lib.gllm_attn_plan_info(self._h, arr, len(keys)))
         self._info = dict(zip(keys, list(arr)))
         # facts every launch checks, computed once (a plan serves every layer of a step)
         self.rows = self._info["rows"]

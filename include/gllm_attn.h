@@ -26,6 +26,8 @@
  *                         query rows and positions, built on the device from
  *                         the block table and lengths instead of the per-row
  *                         host loop; the paged kernels need no dense bias)
+ *   gllm_sparse_*, gllm_key_bounds_*, gllm_select_blocks
+ *                         no counterpart: attention over selected cache blocks
  *
  * Conventions: every data pointer is a device pointer the caller owns; the
  * library never allocates device memory (the paged path uses a caller-sized
@@ -303,6 +305,26 @@ int gllm_attn_plan_create_window(gllm_attn_plan** plan, const int32_t* query_len
                                  int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
                                  int32_t block_size, int32_t dtype, int32_t split_tokens,
                                  int32_t decode_heads_per_wg, int32_t window, int32_t sinks);
+/*
+ * gllm_attn_plan_create for a batch in which groups of sequences have their first keys
+ * in common.  Group g: the sequences group_seqs[group_ptr[g] .. group_ptr[g + 1]), in any
+ * order, with the same group_tokens[g] first keys (at most what lies before each one's query
+ * rows); a sequence is in one group at most.  Their block-table rows name blocks that
+ * hold the same values there, the same blocks as a rule: which member's are read is
+ * the library's choice.  The MFMA kernels read the shared keys (whole multiples of
+ * 16) once for all decode-path members (query_len x G <= 16; at least two), in a launch
+ * before the others, and join the parts; prompts of a group, and the generic kernel,
+ * read them for each sequence.  Results are those of a plan without groups up to the
+ * order of fp32 sums.  Decode sequences are planned page-balanced: split_tokens 0 or
+ * GLLM_SPLIT_BALANCED.  No counterpart in the reference.
+ */
+int gllm_attn_plan_create_shared(gllm_attn_plan** plan, const int32_t* query_lens,
+                                 const int32_t* seq_lens, int32_t num_seqs, int64_t q_seq_stride,
+                                 int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                                 int32_t block_size, int32_t dtype, int32_t split_tokens,
+                                 int32_t decode_heads_per_wg, int32_t num_groups,
+                                 const int32_t* group_ptr, const int32_t* group_seqs,
+                                 const int32_t* group_tokens);
 /* Device bytes the plan needs (work list, split partials). */
 size_t gllm_attn_plan_workspace_bytes(const gllm_attn_plan* plan);
 /* Stream-ordered upload of the plan into `workspace` (>= workspace_bytes).
@@ -315,8 +337,8 @@ int gllm_attn_plan_upload(gllm_attn_plan* plan, void* workspace, size_t workspac
  * split planner), [10] 1 where a mixed launch over a 4-bit cache or with a window
  * runs each item in two half-size workgroups ([7] and [8] are those of other
  * caches), [11] the most block ids that one decode task of the MFMA kernels looks
- * up (they cache 512; counted when asked for).  [0] counts workgroups for a
- * page-balanced plan.  The first n are written. */
+ * up (they cache 512; counted when asked for), [12] workgroups over shared prefixes.
+ * [0] counts workgroups for a page-balanced plan (without [12]).  The first n are written. */
 int gllm_attn_plan_info(const gllm_attn_plan* plan, int64_t* info, int32_t n);
 int gllm_attn_plan_destroy(gllm_attn_plan* plan);
 
@@ -392,6 +414,80 @@ int gllm_attention_dense(const void* q, int64_t q_row_stride, const void* k, int
                          int64_t bias_row_stride, void* out, int64_t out_row_stride, int32_t batch,
                          int32_t q_len, int32_t kv_len, int32_t num_q_heads, int32_t num_kv_heads,
                          int32_t head_dim, float scale, int32_t dtype, void* stream);
+
+/*
+ * Sparse attention: each (query row, kv head) attends to the keys of at most `blocks`
+ * blocks of the paged cache, chosen by a cheap score over the blocks' key bounds.  No
+ * counterpart in the reference.  Four calls: gllm_key_bounds_write after a step's keys are
+ * in the cache, gllm_select_blocks, gllm_sparse_attention; gllm_key_bounds_values reads
+ * bounds back.  head_dim a multiple of 8, at most 256; any block size, G, model and cache
+ * dtype that gllm_paged_attention takes (4-bit cache: head_dim a multiple of 32).
+ *
+ * Key bounds: one record per block, gllm_key_bounds_record_bytes apart or more (a multiple
+ * of 16; the first 16-byte aligned): for each kv head head_dim int8 codes of the least
+ * value of each dim over the block's keys, rounded down, and head_dim of the largest, rounded
+ * up; then one exponent byte per kv head; padding is not written.  A code stands for
+ * code x 2^(byte - 128), the least power of two from 2^-100 on at which the largest
+ * magnitude is at most 127; past 127 x 2^100, and with an infinity or NaN among the
+ * keys, the byte is 255 and the bounds are -infinity and +infinity.  Keys count as attention reads
+ * them, in the model dtype.
+ *
+ * Scores: q's G heads of a (row, kv head) are rounded to the nearest int8 code, ties to even,
+ * by the same rule with one power of two for all of them (past it, or not finite: all
+ * codes 0).  A block's score is 2^(byte - 128) max over the heads of the sum over the dims
+ * of max(code lo, code hi), +infinity for bounds of infinities: whole numbers times a power
+ * of two, computed exactly.
+ *
+ * Selection of the row at position p, of the blocks 0 .. p / block_size: all of them if
+ * there are at most `blocks`; else the first first_blocks, the last recent_blocks (the row's own
+ * among them) and, of the others, those of the highest scores, the lower block first
+ * among equals.
+ */
+typedef struct gllm_sparse_plan gllm_sparse_plan;
+/* Bytes of one block's record (0 for sizes that have none). */
+size_t gllm_key_bounds_record_bytes(int32_t num_kv_heads, int32_t head_dim);
+/* A batch, from HOST lengths as in gllm_attn_plan_create.  first_blocks >= 0,
+ * recent_blocks >= 1, together at most `blocks`. */
+int gllm_sparse_plan_create(gllm_sparse_plan** plan, const int32_t* query_lens, const int32_t* seq_lens,
+                            int32_t num_seqs, int64_t q_seq_stride, int32_t num_q_heads,
+                            int32_t num_kv_heads, int32_t head_dim, int32_t block_size, int32_t dtype,
+                            int32_t blocks, int32_t first_blocks, int32_t recent_blocks);
+/* Workspace and upload as for gllm_attn_plan: it holds the rows' tables, the scores (at
+ * most 256 MiB, or one tile of rows) and split partials, so a plan's calls must follow each
+ * other in stream order. */
+size_t gllm_sparse_plan_workspace_bytes(const gllm_sparse_plan* plan);
+int gllm_sparse_plan_upload(gllm_sparse_plan* plan, void* workspace, size_t workspace_bytes, void* stream);
+/* Plan facts: [0] rows of q / out / selected that it addresses, [1] query rows, [2] blocks
+ * that the new tokens touch, [3] score tiles, [4] slabs of rows scored at a time, [5]
+ * splits of a row's keys.  The first n are written. */
+int gllm_sparse_plan_info(const gllm_sparse_plan* plan, int64_t* info, int32_t n);
+int gllm_sparse_plan_destroy(gllm_sparse_plan* plan);
+/* Bounds of every block that holds a new token (positions seq_len - query_len ..
+ * seq_len - 1) of a sequence, from all its cached keys: after the step's KV write.  Blocks
+ * that two sequences share are written twice alike. */
+int gllm_key_bounds_write(const gllm_sparse_plan* plan, const void* k_cache, int64_t cache_slot_stride,
+                          int64_t num_blocks, const int32_t* block_table, int64_t block_table_stride,
+                          void* bounds, int64_t bounds_stride, int32_t kv_dtype, void* stream);
+/* Bounds of blocks[0 .. n) as the values they stand for: out [n, num_kv_heads, 2 (least,
+ * largest), head_dim] fp32, 16-byte aligned; zeros for a block outside [0, num_blocks). */
+int gllm_key_bounds_values(const void* bounds, int64_t bounds_stride, int64_t num_blocks, const int64_t* blocks,
+                           int64_t n, int32_t num_kv_heads, int32_t head_dim, float* out, void* stream);
+/* selected: [rows, num_kv_heads, blocks] int32, the selected block numbers (columns of the
+ * sequence's block-table row) in ascending order, then -1; rows past a sequence's query_len
+ * (padded layout) are not written.  q: rotated query rows.  Every block but those that are
+ * always taken needs bounds. */
+int gllm_select_blocks(const gllm_sparse_plan* plan, const void* q, int64_t q_row_stride, const void* bounds,
+                       int64_t bounds_stride, int64_t num_blocks, const int32_t* block_table,
+                       int64_t block_table_stride, int32_t* selected, int32_t dtype, void* stream);
+/* Attention of each row over the keys at or before its position in its selected blocks.
+ * `selected` may come from anywhere: a list ends at the first entry that is negative, not
+ * above the entry before it, or behind the row's own block, and a row without blocks
+ * gives zeros. */
+int gllm_sparse_attention(const gllm_sparse_plan* plan, const void* q, int64_t q_row_stride, void* out,
+                          int64_t out_row_stride, const void* k_cache, const void* v_cache,
+                          int64_t cache_slot_stride, int64_t num_blocks, const int32_t* block_table,
+                          int64_t block_table_stride, const int32_t* selected, float scale, int32_t dtype,
+                          int32_t kv_dtype, void* stream);
 
 #ifdef __cplusplus
 }
