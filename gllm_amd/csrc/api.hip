@@ -200,16 +200,17 @@ struct gllm_sparse_plan {
   int64_t total_rows = 0;                     // rows of q / out / selected that the plan addresses
   std::vector<SparseRow> rows;
   std::vector<BoundsBlock> blocks;
-  std::vector<ScoreTile> tiles;
+  std::vector<ScoreItem> items;
+  int64_t n_tiles = 0;
   // rows are scored and selected a slab at a time, so that the scores' place stays bounded
-  struct Slab { int32_t row0, n_rows, tile0, n_tiles, max_blocks; };
+  struct Slab { int32_t row0, n_rows, item0, n_items, max_blocks; };
   std::vector<Slab> slabs;
   int64_t score_stride = 0;
   int32_t splits = 1;
   void* pinned = nullptr;
   size_t pinned_cap = 0;
   bool pinned_is_host_malloc = false;
-  size_t off_rows = 0, off_blocks = 0, off_tiles = 0, off_scores = 0, off_ml = 0, off_part = 0, ws_bytes = 0, stage_bytes = 0;
+  size_t off_rows = 0, off_blocks = 0, off_items = 0, off_scores = 0, off_ml = 0, off_part = 0, ws_bytes = 0, stage_bytes = 0;
   char* ws = nullptr;
   hipEvent_t upload_done = nullptr;
 };
@@ -1750,21 +1751,38 @@ int sparse_plan_impl(gllm_sparse_plan** out, const int32_t* query_lens, const in
   const int64_t per_row = std::max<int64_t>(1, (int64_t)Hkv * p->score_stride * 4);
   const int64_t slab = std::max<int64_t>(tile_rows, kScoreBytes / per_row);
   int64_t slab_rows = 0;
+  const int hw = score_heads(Hkv), kw = 8 / hw;
   for (int64_t r0 = 0; r0 < (int64_t)p->rows.size(); r0 += slab) {
     const int64_t r1 = std::min<int64_t>((int64_t)p->rows.size(), r0 + slab);
-    gllm_sparse_plan::Slab sb{(int32_t)r0, (int32_t)(r1 - r0), (int32_t)p->tiles.size(), 0, 0};
+    gllm_sparse_plan::Slab sb{(int32_t)r0, (int32_t)(r1 - r0), (int32_t)p->items.size(), 0, 0};
+    std::vector<ScoreItem> tiles;
+    int64_t groups = 0;
     for (int64_t r = r0; r < r1;) {
       int64_t e = r + 1;
       while (e < r1 && e - r < tile_rows && p->rows[e].seq == p->rows[r].seq) ++e;
       const int32_t nb = p->rows[e - 1].pos / bs + 1;
       if (nb > blocks) {
-        p->tiles.push_back({(int32_t)r, (int32_t)(e - r), p->rows[r].seq, nb});
+        tiles.push_back({(int32_t)r, (int32_t)(e - r), p->rows[r].seq, nb, 0, (nb + 15) / 16});
+        groups += (nb + 15) / 16;
         sb.max_blocks = std::max(sb.max_blocks, nb);
       }
       r = e;
     }
-    sb.n_tiles = (int32_t)p->tiles.size() - sb.tile0;
-    if (sb.n_tiles > 0) slab_rows = std::max<int64_t>(slab_rows, sb.n_rows);
+    // a tile's groups in equal items, so many that two a CU take all of them in one go
+    const int64_t slots = 2 * (int64_t)device_cus();
+    const int64_t per_item = std::max<int64_t>(1, (groups * (Hkv / hw) + slots * kw - 1) / (slots * kw)) * kw;
+    for (const ScoreItem& t : tiles) {
+      const int64_t n = (t.groups + per_item - 1) / per_item, len = (t.groups + n - 1) / n;
+      for (int64_t g0 = 0; g0 < t.groups; g0 += len) {
+        ScoreItem it = t;
+        it.group0 = (int32_t)g0;
+        it.groups = (int32_t)std::min<int64_t>(len, t.groups - g0);
+        p->items.push_back(it);
+      }
+    }
+    p->n_tiles += (int64_t)tiles.size();
+    sb.n_items = (int32_t)p->items.size() - sb.item0;
+    if (sb.n_items > 0) slab_rows = std::max<int64_t>(slab_rows, sb.n_rows);
     p->slabs.push_back(sb);
   }
   // Splits of a row's selected keys (MFMA kernel): as many as leave every CU its
@@ -1785,7 +1803,7 @@ int sparse_plan_impl(gllm_sparse_plan** out, const int32_t* query_lens, const in
   size_t o = 0;
   p->off_rows = o; o = align256(o + p->rows.size() * sizeof(SparseRow));
   p->off_blocks = o; o = align256(o + p->blocks.size() * sizeof(BoundsBlock));
-  p->off_tiles = o; o = align256(o + p->tiles.size() * sizeof(ScoreTile));
+  p->off_items = o; o = align256(o + p->items.size() * sizeof(ScoreItem));
   p->stage_bytes = o;
   p->off_scores = o; o = align256(o + (size_t)(slab_rows * per_row));
   p->off_ml = o; o = align256(o + parts * 16 * 2 * sizeof(float));
@@ -1795,7 +1813,7 @@ int sparse_plan_impl(gllm_sparse_plan** out, const int32_t* query_lens, const in
     if (int rc = plan_stage(p)) return rc;
     plan_put(p, p->off_rows, p->rows);
     plan_put(p, p->off_blocks, p->blocks);
-    plan_put(p, p->off_tiles, p->tiles);
+    plan_put(p, p->off_items, p->items);
   }
   *out = owner.release();
   return ok();
@@ -1846,7 +1864,7 @@ int gllm_sparse_plan_upload(gllm_sparse_plan* p, void* workspace, size_t bytes, 
 
 int gllm_sparse_plan_info(const gllm_sparse_plan* p, int64_t* info, int32_t n) {
   if (!p || !info) return fail(GLLM_ATTN_EINVAL, "null plan or info");
-  const int64_t v[6] = {p->total_rows, (int64_t)p->rows.size(), (int64_t)p->blocks.size(), (int64_t)p->tiles.size(),
+  const int64_t v[6] = {p->total_rows, (int64_t)p->rows.size(), (int64_t)p->blocks.size(), p->n_tiles,
                         (int64_t)p->slabs.size(), p->splits};
   for (int i = 0; i < n && i < 6; ++i) info[i] = v[i];
   return ok();
@@ -1901,13 +1919,13 @@ int gllm_select_blocks(const gllm_sparse_plan* p, const void* q, int64_t q_row_s
   a.bounds = (const uint8_t*)bounds; a.bounds_stride = bounds_stride; a.num_blocks = num_blocks;
   a.block_table = block_table; a.block_table_stride = block_table_stride;
   a.rows = (const SparseRow*)(p->ws + p->off_rows);
-  a.tiles = (const ScoreTile*)(p->ws + p->off_tiles);
+  a.items = (const ScoreItem*)(p->ws + p->off_items);
   a.scores = (float*)(p->ws + p->off_scores); a.score_stride = p->score_stride;
   a.selected = selected; a.width = p->width; a.first = p->first; a.recent = p->recent;
   block_div(p->bs, &a.block_magic, &a.block_shift);
   a.num_q_heads = p->Hq; a.num_kv_heads = p->Hkv; a.head_dim = p->D; a.dtype = dtype;
   for (const gllm_sparse_plan::Slab& sb : p->slabs) {
-    a.row0 = sb.row0; a.n_rows = sb.n_rows; a.tile0 = sb.tile0; a.n_tiles = sb.n_tiles; a.max_blocks = sb.max_blocks;
+    a.row0 = sb.row0; a.n_rows = sb.n_rows; a.item0 = sb.item0; a.n_items = sb.n_items; a.max_blocks = sb.max_blocks;
     if (int rc = hip_check(launch_select_blocks(a, (hipStream_t)stream), "block selection launch")) return rc;
   }
   return ok();

@@ -460,11 +460,18 @@ struct BoundsBlock {
   int32_t seq, block, n, pad;
 };
 // Up to 16 / (heads of a kv head, rounded up to a power of two) query rows of one
-// sequence whose blocks are scored together: sparse_rows[row0 .. row0 + nrows), of
-// which the last sees nblocks blocks.
-struct ScoreTile {
-  int32_t row0, nrows, seq, nblocks;
+// sequence, sparse_rows[row0 .. row0 + nrows), scored together against 16-block groups
+// group0 .. group0 + groups - 1 of the nblocks blocks that the last of them sees.
+struct ScoreItem {
+  int32_t row0, nrows, seq, nblocks, group0, groups;
 };
+// kv heads that a workgroup of the score kernel takes: 8 waves, a head each or several
+// waves a head.
+__host__ __device__ inline int score_heads(int num_kv_heads) {
+  int hw = 8;
+  while (num_kv_heads % hw) hw /= 2;
+  return hw;
+}
 
 // How many entries of a row's selection count: up to the first that is not above
 // the one before it or lies behind the row's own block.  The workgroup's threads

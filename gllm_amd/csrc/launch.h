@@ -177,8 +177,8 @@ struct SelectArgs {
   const int32_t* block_table;
   int64_t block_table_stride;
   const SparseRow* rows;
-  const ScoreTile* tiles;      // tiles [tile0, tile0 + n_tiles) score the rows [row0, row0 + n_rows)
-  int32_t row0, n_rows, tile0, n_tiles;
+  const ScoreItem* items;      // items [item0, item0 + n_items) score the rows [row0, row0 + n_rows)
+  int32_t row0, n_rows, item0, n_items;
   int32_t max_blocks;          // the most that a row of them sees
   float* scores;               // [n_rows, Hkv, score_stride]
   int64_t score_stride;
