@@ -241,6 +241,7 @@ struct gllm_attn_plan {
   // each sequence (empty: no sharing) the keys that items cover and their partials
   std::vector<PrefixItem> prefix_items;
   std::vector<PrefixRow> prefix_rows;
+  bool prefix_beside = false;    // in the decode segments' launch
   struct Shared { int32_t keys = 0, parts = 0; };
   std::vector<Shared> shared;
   size_t off_prefix = 0, off_prefix_rows = 0;
@@ -456,7 +457,10 @@ int check_groups(const PrefixGroups& g, const int32_t* query_lens, const int32_t
 // range costs every column a partial.  Prompts in a group keep their keys: they read
 // a key for 32 rows a wave already.  Whole sub-tiles of 16 keys are shared, the rest is
 // the sequences' own.
-void plan_prefixes(gllm_attn_plan* p, const PrefixGroups& g, int cus) {
+//
+// beside: the batch has decode sequences only, whose own keys go in the same launch.
+// Returns the workgroups that it leaves to those (0: a launch of their own).
+int64_t plan_prefixes(gllm_attn_plan* p, const PrefixGroups& g, int cus, int heads_req, bool beside) {
   const int G = p->Hq / p->Hkv;
   constexpr int kCols = 32 * kPrefillOnlyWaves;
   struct Group { int32_t seq, tokens, row0, nrows; };
@@ -480,7 +484,7 @@ void plan_prefixes(gllm_attn_plan* p, const PrefixGroups& g, int cus) {
   }
   if (groups.empty()) {
     p->shared.clear();
-    return;
+    return 0;
   }
   const auto tiles = [&](const Group& gr) { return ((int64_t)gr.nrows * G + kCols - 1) / kCols; };
   const auto items = [&](int64_t len) {
@@ -488,13 +492,48 @@ void plan_prefixes(gllm_attn_plan* p, const PrefixGroups& g, int cus) {
     for (const Group& gr : groups) n += tiles(gr) * p->Hkv * ((gr.tokens + len - 1) / len);
     return n;
   };
-  int64_t lo = 4, hi = 4;                      // in tiles of 64 keys
-  for (const Group& gr : groups) hi = std::max<int64_t>(hi, (gr.tokens + 63) / 64);
-  const int64_t target = (int64_t)cus * (p->D == 64 ? 2 : 1);
-  while (lo < hi) {
-    const int64_t mid = (lo + hi) / 2;
-    if (items(64 * mid) <= target) hi = mid;
-    else lo = mid + 1;
+  int64_t most = 4;                            // in tiles of 64 keys; ranges have at least four
+  for (const Group& gr : groups) most = std::max<int64_t>(most, (gr.tokens + 63) / 64);
+  const auto range_for = [&](int64_t target) { // shortest ranges that make at most `target` items
+    int64_t lo = 4, hi = most;
+    while (lo < hi) {
+      const int64_t mid = (lo + hi) / 2;
+      if (items(64 * mid) <= target) hi = mid;
+      else lo = mid + 1;
+    }
+    return lo;
+  };
+  int64_t lo = range_for((int64_t)cus * (p->D == 64 ? 2 : 1));
+  int64_t decode_wgs = 0;
+  if (beside) {
+    // One launch, a workgroup per CU: k of them stream the sequences' own keys at about
+    // 5.7 (1 - e^(-k / 150)) TB/s and start each segment in 4 us; each of the others takes a
+    // range: 6 us and per 64 keys its columns' flops at 3.5 (head dim 64: 2.6) TFLOP/s or its
+    // K/V at 30 GB/s.  Measured, us at k = 64, 112, 128, 192: 4 x 32 sequences of 128-2,048 own
+    // keys on 16,384-32,768, 64 / 8 heads 306, 217, 225, 427; 64 of the like on 8,192, 32 / 8
+    // heads 158, 103, 97, 77.
+    const BalancedShape sh = balanced_shape(p, cus, heads_req);
+    const double bytes = (double)sh.units * 16 * sh.hw * p->D * 4;
+    double segs = 0;
+    int64_t cols = 0;
+    for (const SeqInfo& s : p->seqs) segs += s.q_len * G <= 16 ? sh.hgroups : 0;
+    for (const Group& gr : groups) cols = std::max<int64_t>(cols, std::min<int64_t>(kCols, (int64_t)gr.nrows * G));
+    const double tile = std::max(64 * 4.0 * p->D * (double)((cols + 31) / 32 * 32) / (p->D == 128 ? 3.5e12 : 2.6e12),
+                                 64 * 4.0 * p->D / 30e9);
+    const int step = cus >= 16 && cus % 8 == 0 ? 8 : 1;
+    double best = 0;
+    for (int64_t k = step; k <= cus - step; k += step) {
+      const int64_t len = range_for(cus - k);
+      const int64_t rounds = (items(64 * len) + cus - k - 1) / (cus - k);
+      const double t = std::max(4e-6 * (1 + segs / (double)k) + bytes / (5.7e12 * (1.0 - std::exp(-(double)k / 150.0))),
+                                (double)rounds * (6e-6 + tile * (double)len));
+      if (decode_wgs == 0 || t < best) {
+        best = t;
+        decode_wgs = k;
+        lo = len;
+      }
+    }
+    p->prefix_beside = true;
   }
   for (const Group& gr : groups) {
     const int64_t n = (gr.tokens + 64 * lo - 1) / (64 * lo);
@@ -509,6 +548,7 @@ void plan_prefixes(gllm_attn_plan* p, const PrefixGroups& g, int cus) {
   }
   std::stable_sort(p->prefix_items.begin(), p->prefix_items.end(),
                    [](const PrefixItem& x, const PrefixItem& y) { return x.k1 - x.k0 > y.k1 - y.k0; });
+  return decode_wgs;
 }
 
 // A prefill work item: 8 waves over the (query head, 32-row block) pairs
@@ -1015,11 +1055,12 @@ static int plan_create_impl(gllm_attn_plan** out, const int32_t* query_lens, con
     p->stream_rows = all_rows;
   }
 
+  int64_t shared_wgs = 0;
   if (groups.n > 0) {
     if (window > 0) return fail(GLLM_ATTN_EUNSUPPORTED, "shared prefixes with a window, which hides them");
     if (split_tokens > 0) return fail(GLLM_ATTN_EINVAL, "shared prefixes: their plans are page-balanced, split_tokens must be 0 or -1");
     if (int rc = check_groups(groups, query_lens, seq_lens, num_seqs)) return rc;
-    if (mfma) plan_prefixes(p, groups, device_cus());
+    if (mfma) shared_wgs = plan_prefixes(p, groups, device_cus(), decode_heads_per_wg, (int64_t)p->max_q * G <= 16);
   }
   if (mfma) {
     const int cus = device_cus();
@@ -1041,6 +1082,7 @@ static int plan_create_impl(gllm_attn_plan** out, const int32_t* query_lens, con
       }
     } else if (split_tokens == GLLM_SPLIT_BALANCED || !p->shared.empty()) {
       balanced = num_seqs > 0;
+      mixed_wgs = shared_wgs;
     } else if (split_tokens == 0 && num_seqs > 0) {
       const BalancedShape bsh = balanced_shape(p, cus, decode_heads_per_wg);
       balanced = bsh.units >= balanced_min_units_per_wg(p->D) * bsh.wgs;
@@ -1608,6 +1650,7 @@ static int paged_attention_impl(const gllm_attn_plan* p, const void* q, int64_t 
     a.prefix_items = (const PrefixItem*)(p->ws + p->off_prefix);
     a.prefix_rows = (const PrefixRow*)(p->ws + p->off_prefix_rows);
     a.n_prefix_items = (int32_t)p->prefix_items.size();
+    a.prefix_beside = p->prefix_beside;
   }
   if (use_mfma)
     return hip_check(launch_paged_attention_mfma(a, p->n_prefill_seqs > 0, p->n_decode_seqs > 0, st),

@@ -143,6 +143,7 @@ struct AttnArgs {
   const PrefixItem* prefix_items;
   const PrefixRow* prefix_rows;
   int32_t n_prefix_items;
+  int32_t prefix_beside;       // decode-only plans: items and segments in one launch
   // sparse attention: the blocks selected for each (query row, kv head)
   const int32_t* selected;     // [rows, Hkv, sel_width]
   const SparseRow* sparse_rows;

@@ -1715,6 +1715,32 @@ prefix_kernel(AttnArgs a) {
   prefill_wg<T, D, false, kPrefillOnlyWaves, kPrefillOnlyStages, KF, false, true>(a, none, px.seq, px.kvh, px.wgrp, lds, &px);
 }
 
+// Shared prefixes beside the decode sequences' own keys, in one launch: workgroups
+// [0, n_seg_wgs) run equal key shares of the sequences (segments, as
+// decode_balanced_kernel), each later one an item of a prefix.  The own keys wait for
+// HBM while the prefixes compute, and one launch less: apart they took, us, 64
+// sequences on 8,192 shared keys 22 + 67, 4 x 32 on 16,384-32,768 (70B heads) 115 + 124.
+template <typename T, int D, int HW, int KF>
+__global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2)))
+prefix_decode_kernel(AttnArgs a) {
+  __shared__ __attribute__((aligned(16))) char lds[MixedLds<D, true, true, kWaves, KF>::kBytes];
+  const int b = blockIdx.x;
+  if (b >= a.n_seg_wgs) {
+    const PrefixItem px = a.prefix_items[b - a.n_seg_wgs];
+    const WorkItem none{};
+    prefill_wg<T, D, false, kWaves, kPrefillStages, KF, false, true>(a, none, px.seq, px.kvh, px.wgrp, lds, &px);
+    return;
+  }
+  const int s0 = a.seg_ptr[b], s1 = a.seg_ptr[b + 1];
+  for (int s = s0; s < s1; ++s) {
+    if (s > s0) __syncthreads();
+    const DecodeSeg sg = a.segs[s];
+    const DecodeTask tk{sg.seq, sg.hg, sg.k0, sg.k1, sg.q_row_start, sg.ctx_len, sg.q_len,
+                        sg.nseg, sg.pbase, sg.ord};
+    decode_task<T, D, HW, kWaves / HW, KF, KF == kKV4>(a, tk, lds);
+  }
+}
+
 // Sparse attention: one workgroup per (query row, kv head, split of its selected
 // keys), its eight waves taking 16-key sub-tiles in turn (decode_task).  The list
 // ends at the first entry that is not above the one before or lies behind the
@@ -1925,15 +1951,31 @@ static hipError_t launch_sparse_t(const AttnArgs& a, hipStream_t st) {
     default: return launch_sparse_d<T, D, kKV16>(a, st);
   }
 }
+template <typename T, int D, int KF>
+static hipError_t launch_prefix_d(const AttnArgs& a, hipStream_t st) {
+  const dim3 block(64 * kWaves), both(a.n_seg_wgs + a.n_prefix_items);
+  if (!a.prefix_beside) {
+    hipLaunchKernelGGL((prefix_kernel<T, D, KF>), dim3(a.n_prefix_items), dim3(64 * kPrefillOnlyWaves), 0, st, a);
+    return hipGetLastError();
+  }
+  switch (a.heads_per_wg) {
+    case 1: hipLaunchKernelGGL((prefix_decode_kernel<T, D, 1, KF>), both, block, 0, st, a); break;
+    case 2: hipLaunchKernelGGL((prefix_decode_kernel<T, D, 2, KF>), both, block, 0, st, a); break;
+    case 4: hipLaunchKernelGGL((prefix_decode_kernel<T, D, 4, KF>), both, block, 0, st, a); break;
+    case 8: hipLaunchKernelGGL((prefix_decode_kernel<T, D, 8, KF>), both, block, 0, st, a); break;
+    default: return hipErrorInvalidValue;
+  }
+  if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  hipLaunchKernelGGL((merge_splits_kernel<T, D>), dim3(a.num_seqs * a.num_kv_heads), dim3(kMergeThreads), 0, st, a);
+  return hipGetLastError();
+}
 template <typename T, int D>
 static hipError_t launch_prefix_t(const AttnArgs& a, hipStream_t st) {
-  const dim3 grid(a.n_prefix_items), block(64 * kPrefillOnlyWaves);
   switch (a.kv_dtype) {
-    case kFP8: hipLaunchKernelGGL((prefix_kernel<T, D, kKV8>), grid, block, 0, st, a); break;
-    case kMXFP4: hipLaunchKernelGGL((prefix_kernel<T, D, kKV4>), grid, block, 0, st, a); break;
-    default: hipLaunchKernelGGL((prefix_kernel<T, D, kKV16>), grid, block, 0, st, a); break;
+    case kFP8: return launch_prefix_d<T, D, kKV8>(a, st);
+    case kMXFP4: return launch_prefix_d<T, D, kKV4>(a, st);
+    default: return launch_prefix_d<T, D, kKV16>(a, st);
   }
-  return hipGetLastError();
 }
 
 // This file is compiled once per element type and kind, so that they build as
@@ -1989,8 +2031,12 @@ hipError_t launch_paged_attention_mfma(const AttnArgs& a, bool has_prefill, bool
   if (a.kv_dtype != kFP8 && a.kv_dtype != kMXFP4 && a.kv_dtype != a.dtype) return hipErrorInvalidValue;
   if (a.dtype != kBF16 && a.dtype != kF16) return hipErrorInvalidValue;
   const bool f16 = a.dtype == kF16;
-  if (a.n_prefix_items > 0)    // the shared keys' partials, which the merge behind the decode part takes in
-    if (hipError_t e = (f16 ? launch_prefix_f16 : launch_prefix_bf16)(a, st); e != hipSuccess) return e;
+  if (a.n_prefix_items > 0) {  // the shared keys' partials, which the merge behind the decode part takes in
+    AttnArgs w = a;
+    w.window = INT32_MAX;      // the 4-bit decode kernel takes one
+    const hipError_t e = (f16 ? launch_prefix_f16 : launch_prefix_bf16)(w, st);
+    if (e != hipSuccess || a.prefix_beside) return e;
+  }
   PagedLaunch* go = f16 ? launch_paged_f16 : launch_paged_bf16;
   if (a.kv_dtype == kMXFP4) go = f16 ? launch_paged_kv4_f16 : launch_paged_kv4_bf16;
   else if (a.window > 0) go = f16 ? launch_paged_window_f16 : launch_paged_window_bf16;
