@@ -206,11 +206,16 @@ struct gllm_sparse_plan {
   struct Slab { int32_t row0, n_rows, item0, n_items, max_blocks; };
   std::vector<Slab> slabs;
   int64_t score_stride = 0;
-  int32_t splits = 1;
+  // MFMA kernels: rows on their own (each in `splits` parts), and prompt rows in tiles
+  // (tile_splits parts each); the generic kernel takes `rows`
+  std::vector<SparseRow> lone, tile_rows;
+  std::vector<SparseTile> tiles;
+  int32_t splits = 1, tile_splits = 1, tile_capacity = 0;
   void* pinned = nullptr;
   size_t pinned_cap = 0;
   bool pinned_is_host_malloc = false;
   size_t off_rows = 0, off_blocks = 0, off_items = 0, off_scores = 0, off_ml = 0, off_part = 0, ws_bytes = 0, stage_bytes = 0;
+  size_t off_lone = 0, off_tile_rows = 0, off_tiles = 0, off_entries = 0, off_keys = 0, off_tile_ml = 0, off_tile_part = 0;
   char* ws = nullptr;
   hipEvent_t upload_done = nullptr;
 };
@@ -1741,6 +1746,66 @@ int bounds_check(const void* bounds, int64_t stride, int64_t num_blocks, int32_t
   return ok();
 }
 
+// Which sequences' rows the MFMA kernels take in tiles of up to 64 (256 columns), which one
+// by one.  A tile reads the blocks that any of its rows selected once and computes all
+// its columns on them; a row alone reads its own blocks.  By the times of a CU, with the
+// blocks that a tile's rows would select between them if they chose independently (rows
+// near each other choose alike, so tiles read fewer): a row 5 us and its K/V at 29 GB/s; a
+// tile 6 us and per 64 keys its columns' flops at 3.2 (head dim 64: 2.4) TFLOP/s or its
+// K/V at 30 GB/s.
+int plan_sparse_tiles(gllm_sparse_plan* p, const int32_t* query_lens, const int32_t* seq_lens) {
+  const int G = p->Hq / p->Hkv, most = std::min(64, 256 / G);
+  const double key = 4.0 * p->D;               // bytes of a 16-bit key and value
+  const auto tile_time = [&](int rows, int32_t nb) {
+    const double share = 1.0 - std::pow(1.0 - std::min(1.0, (double)p->width / nb), rows);
+    const double cols = (rows * G + 31) / 32 * 32;
+    return 64 * std::max(key * cols / (p->D == 128 ? 3.2e12 : 2.4e12), key / 30e9) * (nb * share * p->bs / 64);
+  };
+  double total = 0, longest = 0;
+  int64_t r0 = 0;
+  for (int i = 0; i < p->num_seqs; r0 += query_lens[i++]) {
+    const int32_t ql = query_lens[i], c = seq_lens[i] - ql;
+    const int n = (ql + most - 1) / most;
+    double tiles = 0, rows = 0;
+    for (int t = 0; t < n; ++t) {
+      const int64_t a = (int64_t)ql * t / n, e = (int64_t)ql * (t + 1) / n;
+      tiles += 6e-6 + tile_time((int)(e - a), (int32_t)((c + e - 1) / p->bs + 1));
+      rows += (double)(e - a) * (5e-6 + std::min<double>(p->width, (c + e - 1) / p->bs + 1) * p->bs * key / 29e9);
+    }
+    if (ql < 2 || p->bs % 16 || tiles >= rows) {
+      p->lone.insert(p->lone.end(), p->rows.begin() + r0, p->rows.begin() + r0 + ql);
+      continue;
+    }
+    for (int t = 0; t < n; ++t) {
+      const int64_t a = (int64_t)ql * t / n, e = (int64_t)ql * (t + 1) / n;
+      const int32_t nb = (int32_t)((c + e - 1) / p->bs + 1);
+      p->tiles.push_back({(int32_t)p->tile_rows.size(), (int32_t)(e - a), i, 0});
+      p->tile_rows.insert(p->tile_rows.end(), p->rows.begin() + r0 + a, p->rows.begin() + r0 + e);
+      p->tile_capacity = (int32_t)std::max<int64_t>(p->tile_capacity, std::min<int64_t>(nb, (e - a) * p->width));
+      total += tile_time((int)(e - a), nb);
+      longest = std::max(longest, tile_time((int)(e - a), nb));
+    }
+  }
+  if (p->tiles.empty()) return ok();
+  // Parts of a tile's keys: what ends soonest with a workgroup per CU, a partial's write
+  // and read at 3 TB/s; the ids, rows and numbers of at most 1,022 blocks fit a workgroup.
+  const int64_t cus = device_cus(), units = (int64_t)p->tiles.size() * p->Hkv;
+  const int64_t least = ((int64_t)p->tile_capacity * p->bs + 1022 * (int64_t)p->bs - 65) / (1022 * (int64_t)p->bs - 64);
+  double best = 0;
+  for (int64_t s = least; s <= std::max<int64_t>(least, 16); ++s) {
+    const double round = std::max(total * p->Hkv / (double)units, 0.7 * longest) / (double)s + 6e-6;
+    const double join = s > 1 ? 4e-6 + (double)p->tile_rows.size() * p->Hq * s * p->D * 8 / 3e12 : 0;
+    const double t = (double)((units * s + cus - 1) / cus) * round + join;
+    if (s == least || t < best) {
+      best = t;
+      p->tile_splits = (int32_t)s;
+    }
+  }
+  if (units * p->tile_splits > INT32_MAX || (int64_t)p->tile_rows.size() * p->Hkv * p->tile_splits > INT32_MAX / 16)
+    return fail(GLLM_ATTN_EINVAL, "too many splits");
+  return ok();
+}
+
 int sparse_plan_impl(gllm_sparse_plan** out, const int32_t* query_lens, const int32_t* seq_lens, int32_t num_seqs,
                      int64_t q_seq_stride, int32_t Hq, int32_t Hkv, int32_t D, int32_t bs, int32_t dtype, int32_t blocks,
                      int32_t first, int32_t recent) {
@@ -1828,12 +1893,15 @@ int sparse_plan_impl(gllm_sparse_plan** out, const int32_t* query_lens, const in
     if (sb.n_items > 0) slab_rows = std::max<int64_t>(slab_rows, sb.n_rows);
     p->slabs.push_back(sb);
   }
+  const bool mfma = mfma_dtype(dtype) && (D == 64 || D == 128) && G <= 16;
+  if (mfma) {
+    if (int rc = plan_sparse_tiles(p, query_lens, seq_lens)) return rc;
+  }
   // Splits of a row's selected keys (MFMA kernel): as many as leave every CU its
   // resident workgroups, where the longest sheds enough for the merge's launch, and of
   // at most 510 blocks (the ids that a task caches).
-  const bool mfma = mfma_dtype(dtype) && (D == 64 || D == 128) && G <= 16;
-  if (mfma && !p->rows.empty()) {
-    const int64_t units = (int64_t)p->rows.size() * Hkv;
+  if (!p->lone.empty()) {
+    const int64_t units = (int64_t)p->lone.size() * Hkv;
     const int64_t target = (int64_t)device_cus() * (D == 64 ? 2 : 1);
     int64_t s = std::max<int64_t>(1, std::min(target / units, keys / 128));
     if ((keys - keys / s) * D * 4 < 128 << 10) s = 1;
@@ -1842,12 +1910,21 @@ int sparse_plan_impl(gllm_sparse_plan** out, const int32_t* query_lens, const in
     if (units * s > INT32_MAX / 16) return fail(GLLM_ATTN_EINVAL, "too many splits");
     p->splits = (int32_t)s;
   }
-  const size_t parts = p->splits > 1 ? p->rows.size() * Hkv * p->splits : 0;
+  const size_t parts = p->splits > 1 ? p->lone.size() * Hkv * p->splits : 0;
+  const size_t tile_parts = p->tile_splits > 1 ? p->tile_rows.size() * Hkv * p->tile_splits : 0;
+  const size_t tile_units = p->tiles.size() * (size_t)Hkv;
   size_t o = 0;
   p->off_rows = o; o = align256(o + p->rows.size() * sizeof(SparseRow));
   p->off_blocks = o; o = align256(o + p->blocks.size() * sizeof(BoundsBlock));
   p->off_items = o; o = align256(o + p->items.size() * sizeof(ScoreItem));
+  p->off_lone = o; o = align256(o + p->lone.size() * sizeof(SparseRow));
+  p->off_tile_rows = o; o = align256(o + p->tile_rows.size() * sizeof(SparseRow));
+  p->off_tiles = o; o = align256(o + p->tiles.size() * sizeof(SparseTile));
   p->stage_bytes = o;
+  p->off_entries = o; o = align256(o + tile_units * p->tile_capacity * sizeof(SelectedBlock));
+  p->off_keys = o; o = align256(o + tile_units * sizeof(int32_t));
+  p->off_tile_ml = o; o = align256(o + tile_parts * 16 * 2 * sizeof(float));
+  p->off_tile_part = o; o = align256(o + tile_parts * 16 * D * sizeof(float));
   p->off_scores = o; o = align256(o + (size_t)(slab_rows * per_row));
   p->off_ml = o; o = align256(o + parts * 16 * 2 * sizeof(float));
   p->off_part = o; o = align256(o + parts * 16 * D * sizeof(float));
@@ -1857,6 +1934,9 @@ int sparse_plan_impl(gllm_sparse_plan** out, const int32_t* query_lens, const in
     plan_put(p, p->off_rows, p->rows);
     plan_put(p, p->off_blocks, p->blocks);
     plan_put(p, p->off_items, p->items);
+    plan_put(p, p->off_lone, p->lone);
+    plan_put(p, p->off_tile_rows, p->tile_rows);
+    plan_put(p, p->off_tiles, p->tiles);
   }
   *out = owner.release();
   return ok();
@@ -1907,9 +1987,9 @@ int gllm_sparse_plan_upload(gllm_sparse_plan* p, void* workspace, size_t bytes, 
 
 int gllm_sparse_plan_info(const gllm_sparse_plan* p, int64_t* info, int32_t n) {
   if (!p || !info) return fail(GLLM_ATTN_EINVAL, "null plan or info");
-  const int64_t v[6] = {p->total_rows, (int64_t)p->rows.size(), (int64_t)p->blocks.size(), p->n_tiles,
-                        (int64_t)p->slabs.size(), p->splits};
-  for (int i = 0; i < n && i < 6; ++i) info[i] = v[i];
+  const int64_t v[8] = {p->total_rows, (int64_t)p->rows.size(), (int64_t)p->blocks.size(), p->n_tiles,
+                        (int64_t)p->slabs.size(), p->splits, (int64_t)p->tiles.size(), p->tile_splits};
+  for (int i = 0; i < n && i < 8; ++i) info[i] = v[i];
   return ok();
 }
 
@@ -1996,15 +2076,35 @@ int gllm_sparse_attention(const gllm_sparse_plan* p, const void* q, int64_t q_ro
   block_div(p->bs, &a.block_magic, &a.block_shift);
   if (kv4) a.kv4_record = (int32_t)kv4_record_bytes(p->bs, p->D);
   a.selected = selected; a.sel_width = p->width;
-  a.sparse_rows = (const SparseRow*)(p->ws + p->off_rows);
-  a.n_sparse_rows = (int32_t)p->rows.size();
-  a.sparse_splits = p->splits;
-  a.partial_ml = (float*)(p->ws + p->off_ml);
-  a.partials = (float*)(p->ws + p->off_part);
   const bool mfma = mfma_dtype(dtype) && (p->D == 64 || p->D == 128) && p->Hq / p->Hkv <= 16 &&
                     (kv_dtype == dtype || kv_dtype == GLLM_DTYPE_FP8_E4M3 || kv4);
   hipStream_t st = (hipStream_t)stream;
-  return hip_check(mfma ? launch_sparse_attention_mfma(a, st) : launch_sparse_attention_generic(a, st), "sparse attention launch");
+  if (!mfma) {
+    a.sparse_rows = (const SparseRow*)(p->ws + p->off_rows);
+    a.n_sparse_rows = (int32_t)p->rows.size();
+    return hip_check(launch_sparse_attention_generic(a, st), "sparse attention launch");
+  }
+  if (!p->tiles.empty()) {
+    AttnArgs t = a;
+    t.sparse_rows = t.tile_rows = (const SparseRow*)(p->ws + p->off_tile_rows);
+    t.n_sparse_rows = (int32_t)p->tile_rows.size();
+    t.sparse_tiles = (const SparseTile*)(p->ws + p->off_tiles);
+    t.n_sparse_tiles = (int32_t)p->tiles.size();
+    t.tile_entries = (SelectedBlock*)(p->ws + p->off_entries);
+    t.tile_keys = (int32_t*)(p->ws + p->off_keys);
+    t.tile_capacity = p->tile_capacity;
+    t.tile_splits = t.sparse_splits = p->tile_splits;
+    t.partial_ml = (float*)(p->ws + p->off_tile_ml);
+    t.partials = (float*)(p->ws + p->off_tile_part);
+    if (int rc = hip_check(launch_tile_blocks(t, st), "sparse attention tiles")) return rc;
+    if (int rc = hip_check(launch_sparse_attention_mfma(t, st), "sparse attention launch")) return rc;
+  }
+  a.sparse_rows = (const SparseRow*)(p->ws + p->off_lone);
+  a.n_sparse_rows = (int32_t)p->lone.size();
+  a.sparse_splits = p->splits;
+  a.partial_ml = (float*)(p->ws + p->off_ml);
+  a.partials = (float*)(p->ws + p->off_part);
+  return hip_check(launch_sparse_attention_mfma(a, st), "sparse attention launch");
 }
 
 }  // extern "C"

@@ -454,6 +454,21 @@ struct PrefixRow {
 struct SparseRow {
   int32_t row, seq, pos, pad;
 };
+// Prompt rows of sparse attention that are taken together: nrows (at most 64) of one
+// sequence, tile_rows[row0 ..].
+struct SparseTile {
+  int32_t row0, nrows, seq, pad;
+};
+// A block that rows of a tile selected: bit r of rows is the tile's row r.
+struct SelectedBlock {
+  uint64_t rows;
+  int32_t number, block;        // in the sequence, in the pool
+};
+// One workgroup's part of a tile: keys [k0, k1) of its entries' blocks, one after another.
+struct SelectedTile {
+  const SelectedBlock* entries;
+  int32_t row0, nrows, k0, k1, ord, parts;
+};
 // A cache block whose first n keys have bounds to be written: block `block` of
 // sequence seq.
 struct BoundsBlock {

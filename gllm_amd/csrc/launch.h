@@ -148,6 +148,13 @@ struct AttnArgs {
   const int32_t* selected;     // [rows, Hkv, sel_width]
   const SparseRow* sparse_rows;
   int32_t n_sparse_rows, sel_width, sparse_splits;
+  // prompt rows in tiles: for each (tile, kv head) entries from tile_capacity x it on, and the
+  // keys of their blocks (the last row's own block counts up to its position)
+  const SparseTile* sparse_tiles;
+  const SparseRow* tile_rows;
+  SelectedBlock* tile_entries;
+  int32_t* tile_keys;
+  int32_t n_sparse_tiles, tile_capacity, tile_splits;
 };
 
 // Key bounds, block scores and the selection (sparse_select.hip)
@@ -293,6 +300,7 @@ hipError_t launch_build_metadata(const MetadataArgs& a, hipStream_t stream);
 hipError_t launch_paged_attention_mfma(const AttnArgs& a, bool has_prefill, bool has_decode, hipStream_t stream);
 hipError_t launch_sparse_attention_mfma(const AttnArgs& a, hipStream_t stream);
 hipError_t launch_sparse_attention_generic(AttnArgs a, hipStream_t stream);
+hipError_t launch_tile_blocks(const AttnArgs& a, hipStream_t stream);
 hipError_t launch_key_bounds(const BoundsArgs& a, hipStream_t stream);
 hipError_t launch_key_bounds_values(const BoundsValuesArgs& a, hipStream_t stream);
 hipError_t launch_select_blocks(const SelectArgs& a, hipStream_t stream);

@@ -833,11 +833,18 @@ __device__ __forceinline__ int pf_swz(int r) {
 // every decode sequence that shares the keys (a.prefix_rows), 32 neighbouring ones a
 // wave; every row sees every key of [px->k0, px->k1), which positions count from k0,
 // and the rows' states go to their partials.
-template <typename T, int D, bool DENSE, int NW, int NS, int KF, bool WIN, bool PFX = false>
+// SELT (sparse attention of prompt rows): the columns are those of a tile of one
+// sequence's rows, the keys those of the blocks that some row of it selected (sx's
+// entries, each with a bit per row), positions counting through them from sx->k0 on.
+// A row sees its own blocks' keys up to its position; blocks are multiples of 16
+// keys, so one limit per 16 keys and row masks the scores.
+enum : int { kOwnKeys = 0, kPrefixKeys = 1, kSelectedKeys = 2 };
+template <typename T, int D, bool DENSE, int NW, int NS, int KF, bool WIN, int KIND = kOwnKeys>
 __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it, int seq, int kvh, int wgrp, char* lds,
-                                           const PrefixItem* px = nullptr) {
+                                           const PrefixItem* px = nullptr, const SelectedTile* sx = nullptr) {
+  constexpr bool PFX = KIND == kPrefixKeys, SELT = KIND == kSelectedKeys;
   static_assert(!(DENSE && (KF != kKV16 || WIN)), "the dense op has no cache");
-  static_assert(!PFX || (!DENSE && !WIN), "a shared prefix is paged and has no window");
+  static_assert(KIND == kOwnKeys || (!DENSE && !WIN), "shared prefixes and selected blocks are paged and have no window");
   constexpr bool KREG = KF != kKV16;       // K/V pass through registers (widened) on the way to LDS
   using Cfg = PrefillCfg<D, NS>;
   constexpr int NQ = D / 16;               // Q operand chunks (16 dims)
@@ -862,14 +869,19 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
     qlen = px->nrows;
     TK = px->k1 - px->k0;
     qstart = 0;
+  } else if (SELT) {
+    ctx = 0;
+    qlen = sx->nrows;
+    TK = sx->k1 - sx->k0;
+    qstart = 0;
   } else {
     ctx = it.ctx_len;
     qlen = it.q_len;
     TK = ctx + qlen;
     qstart = it.q_row_start;
   }
-  constexpr bool PAIRS = DENSE || PFX;      // columns are neighbouring (row, head) pairs, every key is visible
-  const int k0 = PFX ? px->k0 : 0;          // key that position 0 is
+  constexpr bool PAIRS = DENSE || KIND != kOwnKeys;     // columns are neighbouring (row, head) pairs
+  const int k0 = PFX ? px->k0 : (SELT ? sx->k0 : 0);    // key that position 0 is
   const int G = a.num_q_heads / a.num_kv_heads;
   // The wave's 32 MFMA columns.  Paged: 32 query rows of one head (the causal
   // edge then cuts few tiles).  Dense: neighbouring (row, head of the group)
@@ -879,7 +891,7 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
   // rows per wave, 73 with this and 8-byte loads a tile ahead).
   const int combo = wgrp * NW + wave;
   const int nrb = (qlen + 31) / 32;
-  const int ncol = qlen * G;                // dense, shared prefix
+  const int ncol = qlen * G;                // where columns are pairs
   const bool wact = PAIRS ? combo * 32 < ncol : combo < G * nrb;
   const int dcol = min(combo * 32 + n, ncol - 1);
   const int g = PAIRS ? dcol % G : (wact ? combo % G : 0);
@@ -891,10 +903,12 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
   const int r = PAIRS ? dcol / G : r0 + n;
   const bool row_ok = wact && (PAIRS ? combo * 32 + n < ncol : r < qlen);
   const int rr = min(r, qlen - 1);
-  const int vis = PFX ? TK - 1 : ctx + rr;
+  const int vis = KIND != kOwnKeys ? TK - 1 : ctx + rr;
   PrefixRow pr{};
+  SparseRow sr{};
   if constexpr (PFX) pr = a.prefix_rows[px->row0 + rr];
-  const int64_t qrow = PFX ? pr.q_row : qstart + rr;
+  if constexpr (SELT) sr = a.tile_rows[sx->row0 + rr];
+  const int64_t qrow = PFX ? pr.q_row : (SELT ? sr.row : qstart + rr);
   const int qh = kvh * G + g;
 
   // WIN: from here on positions count through the keys that are not left out
@@ -912,14 +926,31 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
   // LDS (first kBidCache blocks; any beyond are read from the table
   // directly) after the first tiles' copies are issued.
   // (PFX: those of [k0, k1), the table seen from k0's block on)
-  const int blk0 = PFX ? (int)div_bs((uint32_t)k0, a.block_magic, a.block_shift) : 0;
-  const int32_t* bt = DENSE ? nullptr : a.block_table + (int64_t)seq * a.block_table_stride + blk0;
+  // (SELT: the entries' blocks, at most kBidCache, with their rows and numbers)
+  const int blk0 = KIND != kOwnKeys ? (int)div_bs((uint32_t)k0, a.block_magic, a.block_shift) : 0;
+  const int32_t* bt = DENSE || SELT ? nullptr : a.block_table + (int64_t)seq * a.block_table_stride + blk0;
+  uint64_t* const lrows = reinterpret_cast<uint64_t*>(lds + 2 * Cfg::kStages * Cfg::kTile + Cfg::kBidCache * 4);   // SELT
+  int32_t* const lnum = reinterpret_cast<int32_t*>(lrows + Cfg::kBidCache);
+  const SelectedBlock* const ent = SELT ? sx->entries + blk0 : nullptr;
+  const auto block_at = [&](uint32_t e) { return SELT ? (uint32_t)ent[e].block : (uint32_t)bt[e]; };
   constexpr int KB = (Cfg::kBidCache + NT - 1) / NT;
   const int nbc = DENSE ? 0 : min((int)div_bs((uint32_t)(k0 + kend_wg - 1), a.block_magic, a.block_shift) - blk0 + (WIN ? 1 - bgap : 1), Cfg::kBidCache);
   uint32_t lb[KB];
+  uint64_t le[SELT ? KB : 1];
+  int32_t ln[SELT ? KB : 1];
+  if constexpr (SELT) {
 #pragma unroll
-  for (int k = 0; k < KB; ++k)
-    lb[k] = tid + k * NT < nbc ? (uint32_t)bt[WIN && tid + k * NT >= nblk_s ? tid + k * NT + bgap : tid + k * NT] : 0u;
+    for (int k = 0; k < KB; ++k) {
+      const SelectedBlock x = ent[min(tid + k * NT, nbc - 1)];
+      lb[k] = (uint32_t)x.block;
+      le[k] = x.rows;
+      ln[k] = x.number;
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < KB; ++k)
+      lb[k] = tid + k * NT < nbc ? (uint32_t)bt[WIN && tid + k * NT >= nblk_s ? tid + k * NT + bgap : tid + k * NT] : 0u;
+  }
 
   // Q rows (and their cos/sin rows): loads issued now, used after the first
   // K/V copies are on their way.
@@ -1011,7 +1042,7 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
         if (ci < (uint32_t)Cfg::kBidCache) {
           blk = (uint32_t)lbid[ci];
         } else {
-          blk = (uint32_t)bt[bi - blk0];
+          blk = block_at(bi - blk0);
           if (blk >= (uint64_t)a.num_blocks) blk = 0;
         }
         if constexpr (KF == kKV4) slot[i] = Row{blk, (uint32_t)p - bi * (uint32_t)a.block_size};
@@ -1142,7 +1173,7 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
   constexpr float kT = kF16 ? 15.f : 64.f;
   constexpr float kTwoT = kF16 ? 32768.f : 18446744073709551616.f;   // 2^T
   float rref = 0.f;              // paged mode: the row's reference r (log2 units)
-  bool rset = false;             // WIN: chosen
+  bool rset = false;             // WIN, SELT: chosen
   struct Soft { float alpha, dlt, psum; };
   auto row_max = [&](const f32x16& s) {
     float tmax = kNegInf;
@@ -1155,7 +1186,14 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
   // key k0 + 8(j/4) + 4h + j%4 is hidden iff 8(j/4) + j%4 > vis - k0 - 4h:
   // one per-lane limit against compile-time offsets (nothing to hoist onto the
   // common path)
-  auto apply_mask = [&](f32x16& s, int k0) {
+  int slim[SELT ? 4 : 1];        // SELT: of each 16 keys of the tile the lane's last visible one, less 4 h
+  auto apply_mask = [&](f32x16& s, int k0, int kb) {
+    if constexpr (SELT) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        s[j] = 8 * ((j >> 2) & 1) + (j & 3) > slim[SELT ? 2 * kb + (j >> 3) : 0] ? kNegInf : s[j];
+      return;
+    }
     const int lim = (WIN ? vis - by : vis) - k0 - 4 * h;
     if constexpr (WIN) {               // nor at or before vis - window, unless a sink
       const int lo = before_window(lim, a.window), sink = a.sinks - k0 - 4 * h;
@@ -1171,12 +1209,13 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
   };
   // paged mode, piece 0: scale and reference (one FMA), the causal mask, and
   // on the row's first half-tile the choice of r
-  auto fs_prep = [&](f32x16& s, int k0, bool mask, bool first) {
+  constexpr bool LATE = WIN || SELT;      // rows may meet their first visible key in any tile
+  auto fs_prep = [&](f32x16& s, int k0, int kb, bool mask, bool first) {
     const float nr = -rref;
 #pragma unroll
     for (int j = 0; j < 16; ++j) s[j] = __builtin_fmaf(s[j], sl2, nr);
-    if (mask) apply_mask(s, k0);
-    if constexpr (WIN) {
+    if (mask) apply_mask(s, k0, kb);
+    if constexpr (LATE) {
       // rows that have met no visible key yet (l and O are 0 there)
       if (__builtin_amdgcn_ballot_w64(!rset)) {
         const float m1 = row_max(s);
@@ -1239,7 +1278,7 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
       for (int j = 0; j < 16; ++j)   // bias in natural-log units: to log2 units like the scaled scores
         s[j] = __builtin_fmaf(s[j], sl2, __builtin_fmaf(bv[j], kLog2e, sbase));
     } else if (mask) {
-      apply_mask(s, k0);
+      apply_mask(s, k0, 0);
     }
     const float tmax = row_max(s) - sbase;
     const float mn = tmax > m + 8.f ? tmax : m;
@@ -1281,7 +1320,7 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
   // 4 x exp, convert, sum.
   auto sm_piece = [&](int p, f32x16& s, int kb, int k0, bool mask, Soft& q, u32x4* pb, bool first) {
     if (p == 0) {
-      if (kFast) fs_prep(s, k0, mask, first);
+      if (kFast) fs_prep(s, k0, kb, mask, first);
       else sm_max(s, k0, mask, q, bcur[DENSE ? kb : 0]);
     }
     else if (p <= 4) sm_exp(s, 4 * (p - 1));
@@ -1309,7 +1348,7 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
       const float nr = -rref;
 #pragma unroll
       for (int j = 0; j < 16; ++j) t[j] = __builtin_fmaf(t[j], sl2, nr);
-      if (mask) apply_mask(t, k0);
+      if (mask) apply_mask(t, k0, kb);
       const float tmax = row_max(t);
       const float d = tmax > kT ? tmax : 0.f;          // rows whose p passed 2^T move up to their max
       const float alpha = fast_exp2(-d);
@@ -1462,7 +1501,7 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
       if (!DENSE) {
         const int p = copy_key(t * BN, i);
         const uint32_t bi = div_bs((uint32_t)p, a.block_magic, a.block_shift);
-        fbid[t][i] = (uint32_t)bt[bi - blk0];
+        fbid[t][i] = block_at(bi - blk0);
         foff[t][i] = (uint32_t)p - bi * (uint32_t)a.block_size;
       }
     }
@@ -1482,7 +1521,13 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
   if (!DENSE) {
 #pragma unroll
     for (int k = 0; k < KB; ++k)
-      if (tid + k * NT < nbc) lbid[tid + k * NT] = lb[k] < (uint64_t)a.num_blocks ? (int32_t)lb[k] : 0;
+      if (tid + k * NT < nbc) {
+        lbid[tid + k * NT] = lb[k] < (uint64_t)a.num_blocks ? (int32_t)lb[k] : 0;
+        if constexpr (SELT) {
+          lrows[tid + k * NT] = le[k];
+          lnum[tid + k * NT] = ln[k];
+        }
+      }
   }
   Row nbid[NB];
   if (DENSE && kBiasAhead && wact) bias_load(0);
@@ -1526,11 +1571,28 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
             const bool dma = t + TPB < ntiles;
             const int dts = (t + TPB) * BN, dstage = (stage + TPB) % NS;
             // keys of the wave's rows in the tile (WIN: not all before its windows and past the sinks)
-            const bool live = wact && ts < nkeys_w && !(WIN && ts + BN <= lo_w && ts >= a.sinks);
+            bool live = wact && ts < nkeys_w && !(WIN && ts + BN <= lo_w && ts >= a.sinks);
+            if constexpr (SELT) {
+              // the tile's four times 16 keys, each in one block: none for rows that did not
+              // select it, else up to the row's position; tiles that no row of the wave sees
+              // are passed over
+              uint64_t any = 0;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int p = k0 + min(ts + 16 * i, (nkeys_wg - 1) & ~15);
+                const uint32_t bi = div_bs((uint32_t)p, a.block_magic, a.block_shift);
+                const uint64_t rows = lrows[bi - blk0];
+                const int from = lnum[bi - blk0] * a.block_size + (p - (int)bi * a.block_size);
+                const bool in = ts + 16 * i < nkeys_wg && ((rr & 32 ? (uint32_t)(rows >> 32) : (uint32_t)rows) >> (rr & 31)) & 1u;
+                slim[i] = in ? sr.pos - from - 4 * h : -16;
+                any |= __builtin_amdgcn_ballot_w64(in);
+              }
+              live = live && any != 0;
+            }
             if (KREG && dma && live) reg_fetch(dts, nbid);   // written in the tile's last region
             if (live)
               compute(lds + stage * Cfg::kTile, ts,
-                      DENSE || ts + BN - 1 > full_end || (WIN && ts <= hid_w && ts + BN > a.sinks), dma, dts, dstage, nbid,
+                      DENSE || SELT || ts + BN - 1 > full_end || (WIN && ts <= hid_w && ts + BN > a.sinks), dma, dts, dstage, nbid,
                       t == 0);
             else if (dma)
               dma_issue(dts, dstage, nbid);
@@ -1541,13 +1603,18 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
     }
   }
 
-  if constexpr (PFX) {
+  if (PFX || (SELT && sx->parts > 1)) {
     // the row's state: reference (log2 units), sum and unnormalised output
     const float lt = sum_xor32(lsum);
     if (row_ok) {
-      const int hg = kvh / a.heads_per_wg;
-      const MergeInfo mi = a.merge[pr.seq * a.head_groups + hg];
-      const int64_t at = ((int64_t)mi.pbase + (int64_t)(kvh - hg * a.heads_per_wg) * mi.count + px->ord) * 16 + pr.r * G + g;
+      int64_t at;
+      if constexpr (PFX) {
+        const int hg = kvh / a.heads_per_wg;
+        const MergeInfo mi = a.merge[pr.seq * a.head_groups + hg];
+        at = ((int64_t)mi.pbase + (int64_t)(kvh - hg * a.heads_per_wg) * mi.count + px->ord) * 16 + pr.r * G + g;
+      } else {
+        at = (((int64_t)(sx->row0 + rr) * a.num_kv_heads + kvh) * sx->parts + sx->ord) * 16 + g;
+      }
       float* pa = a.partials + at * D + 4 * h;
 #pragma unroll
       for (int db = 0; db < NO; ++db)
@@ -1555,12 +1622,15 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
         for (int jq = 0; jq < 4; ++jq)
           *reinterpret_cast<f32x4*>(pa + 32 * db + 8 * jq) =
               f32x4{o[db][4 * jq], o[db][4 * jq + 1], o[db][4 * jq + 2], o[db][4 * jq + 3]};
-      if (h == 0) *reinterpret_cast<u32x2*>(a.partial_ml + at * 2) = u32x2{__float_as_uint(rref), __float_as_uint(lt)};
+      // SELT: a row that saw no key has no reference
+      const float ref = SELT && !rset ? kNegInf : rref;
+      if (h == 0) *reinterpret_cast<u32x2*>(a.partial_ml + at * 2) = u32x2{__float_as_uint(ref), __float_as_uint(lt)};
     }
     return;
   }
   if (row_ok) {
-    const float inv = 1.f / sum_xor32(lsum);
+    const float lt = sum_xor32(lsum);
+    const float inv = SELT && lt == 0.f ? 0.f : 1.f / lt;        // SELT: no key at all: zeros
     T* op = (T*)a.out + qrow * a.out_row_stride + (int64_t)qh * D + 4 * h;
 #pragma unroll
     for (int db = 0; db < NO; ++db)
@@ -1712,7 +1782,7 @@ prefix_kernel(AttnArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[PrefillCfg<D, kPrefillOnlyStages>::kLdsBytes];
   const PrefixItem px = a.prefix_items[blockIdx.x];
   const WorkItem none{};
-  prefill_wg<T, D, false, kPrefillOnlyWaves, kPrefillOnlyStages, KF, false, true>(a, none, px.seq, px.kvh, px.wgrp, lds, &px);
+  prefill_wg<T, D, false, kPrefillOnlyWaves, kPrefillOnlyStages, KF, false, kPrefixKeys>(a, none, px.seq, px.kvh, px.wgrp, lds, &px);
 }
 
 // Shared prefixes beside the decode sequences' own keys, in one launch: workgroups
@@ -1728,7 +1798,7 @@ prefix_decode_kernel(AttnArgs a) {
   if (b >= a.n_seg_wgs) {
     const PrefixItem px = a.prefix_items[b - a.n_seg_wgs];
     const WorkItem none{};
-    prefill_wg<T, D, false, kWaves, kPrefillStages, KF, false, true>(a, none, px.seq, px.kvh, px.wgrp, lds, &px);
+    prefill_wg<T, D, false, kWaves, kPrefillStages, KF, false, kPrefixKeys>(a, none, px.seq, px.kvh, px.wgrp, lds, &px);
     return;
   }
   const int s0 = a.seg_ptr[b], s1 = a.seg_ptr[b + 1];
@@ -1787,6 +1857,47 @@ sparse_attn_kernel(AttnArgs a) {
     a.partial_ml[2 * at + 1] = 0.f;
   }
 }
+// Sparse attention of prompt rows: one workgroup per (tile of a sequence's rows, kv
+// head, part of the keys that the tile's rows selected).  A tile's rows share each K/V
+// tile, and MFMAs have all their columns; the row form above reads a key again for
+// each row.  Against it, 771 rows on 8,192-16,384 keys, 2,048 selected at random:
+// 874 -> @@ us.
+template <typename T, int D, int KF>
+__global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2)))
+sparse_tile_kernel(AttnArgs a) {
+  using Cfg = PrefillCfg<D, kPrefillStages>;
+  __shared__ __attribute__((aligned(16))) char lds[Cfg::kLdsBytes + Cfg::kBidCache * 12];
+  const int Hkv = a.num_kv_heads, per_tile = Hkv * a.tile_splits;
+  const int ti = blockIdx.x / per_tile, rest = blockIdx.x - ti * per_tile;
+  const int sp = rest / Hkv, kvh = rest - sp * Hkv;
+  const SparseTile st = a.sparse_tiles[ti];
+  const int unit = ti * Hkv + kvh;
+  const int keys = a.tile_keys[unit];
+  const int len = ((keys + a.tile_splits - 1) / a.tile_splits + 63) / 64 * 64;
+  const SelectedTile sx{a.tile_entries + (int64_t)unit * a.tile_capacity, st.row0, st.nrows, min(keys, sp * len),
+                        min(keys, (sp + 1) * len), sp, a.tile_splits};
+  if (sx.k0 < sx.k1) {
+    const WorkItem none{};
+    prefill_wg<T, D, false, kWaves, kPrefillStages, KF, false, kSelectedKeys>(a, none, st.seq, kvh, 0, lds, nullptr, &sx);
+    return;
+  }
+  // no key: empty partials, or rows of zeros
+  const int G = a.num_q_heads / Hkv;
+  if (a.tile_splits == 1) {
+    for (int e = threadIdx.x; e < st.nrows * G * D; e += 64 * kWaves) {
+      const int r = e / (G * D);
+      ((T*)a.out)[(int64_t)a.tile_rows[st.row0 + r].row * a.out_row_stride + (int64_t)kvh * G * D + (e - r * G * D)] = (T)0.f;
+    }
+  } else {
+    for (int c = threadIdx.x; c < st.nrows * G; c += 64 * kWaves) {
+      const int r = c / G;
+      const int64_t at = (((int64_t)(st.row0 + r) * Hkv + kvh) * a.tile_splits + sp) * 16 + c - r * G;
+      a.partial_ml[2 * at] = kNegInf;
+      a.partial_ml[2 * at + 1] = 0.f;
+    }
+  }
+}
+
 // Joins the splits of every (query row, kv head): a thread per 4 dims of a head.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) sparse_merge_kernel(AttnArgs a, int total) {
@@ -1932,16 +2043,28 @@ static hipError_t launch_dense_t(const AttnArgs& a, dim3 grid, int nwg, hipStrea
   return hipGetLastError();
 }
 
-template <typename T, int D, int KF>
-static hipError_t launch_sparse_d(const AttnArgs& a, hipStream_t st) {
-  const int64_t wgs = (int64_t)a.n_sparse_rows * a.num_kv_heads * a.sparse_splits;
+template <typename T, int D>
+static hipError_t launch_sparse_merge(const AttnArgs& a, hipStream_t st) {
   const int64_t total = (int64_t)a.n_sparse_rows * a.num_q_heads * (D / 4);
-  if (wgs > INT32_MAX || total > INT32_MAX - 256) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((sparse_attn_kernel<T, D, KF>), dim3((unsigned)wgs), dim3(64 * kWaves), 0, st, a);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess || a.sparse_splits == 1) return e;
+  if (total > INT32_MAX - 256) return hipErrorInvalidValue;
   hipLaunchKernelGGL((sparse_merge_kernel<T, D>), dim3((unsigned)((total + 255) / 256)), dim3(256), 0, st, a, (int)total);
   return hipGetLastError();
+}
+// Tiles (n_sparse_tiles > 0: their rows are n_sparse_rows of them) or single rows.
+template <typename T, int D, int KF>
+static hipError_t launch_sparse_d(const AttnArgs& a, hipStream_t st) {
+  if (a.n_sparse_tiles > 0) {
+    const int64_t wgs = (int64_t)a.n_sparse_tiles * a.num_kv_heads * a.tile_splits;
+    if (wgs > INT32_MAX) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((sparse_tile_kernel<T, D, KF>), dim3((unsigned)wgs), dim3(64 * kWaves), 0, st, a);
+    hipError_t e = hipGetLastError();
+    return e != hipSuccess || a.tile_splits == 1 ? e : launch_sparse_merge<T, D>(a, st);
+  }
+  const int64_t wgs = (int64_t)a.n_sparse_rows * a.num_kv_heads * a.sparse_splits;
+  if (wgs > INT32_MAX) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((sparse_attn_kernel<T, D, KF>), dim3((unsigned)wgs), dim3(64 * kWaves), 0, st, a);
+  hipError_t e = hipGetLastError();
+  return e != hipSuccess || a.sparse_splits == 1 ? e : launch_sparse_merge<T, D>(a, st);
 }
 template <typename T, int D>
 static hipError_t launch_sparse_t(const AttnArgs& a, hipStream_t st) {

@@ -648,4 +648,100 @@ hipError_t launch_select_blocks(const SelectArgs& a, hipStream_t st) {
   return hipGetLastError();
 }
 
+// ---------------------------------------------------------------- tiles of prompt rows
+// For each (tile, kv head) the blocks that one of its rows selected, in order, each with
+// a bit per row: a workgroup marks them in LDS, kTileWindow blocks of the sequence at a
+// time, and writes the marked ones one after another.  A row's list counts up to its
+// first entry out of order (selected_blocks).
+constexpr int kTileThreads = 512;
+constexpr int kTileWindow = 4096;
+__global__ void __launch_bounds__(kTileThreads) tile_blocks_kernel(AttnArgs a) {
+  constexpr int NW = kTileThreads / 64, PER = kTileWindow / kTileThreads;
+  __shared__ unsigned long long mark[kTileWindow];
+  __shared__ int len[64], own[64], sums[2][NW];
+  const int ti = blockIdx.x / a.num_kv_heads, kvh = blockIdx.x - ti * a.num_kv_heads;
+  const SparseTile st = a.sparse_tiles[ti];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int K = a.sel_width;
+  if (tid < st.nrows) {
+    len[tid] = K;
+    own[tid] = (int)div_bs((uint32_t)a.tile_rows[st.row0 + tid].pos, a.block_magic, a.block_shift);
+  }
+  const auto list = [&](int r) { return a.selected + ((int64_t)a.tile_rows[st.row0 + r].row * a.num_kv_heads + kvh) * K; };
+  __syncthreads();
+  // a wave a row
+  for (int r = wave; r < st.nrows; r += NW) {
+    const int32_t* sel = list(r);
+    int n = K;
+    for (int j = lane; j < K; j += 64) {
+      const int x = sel[j], before = j > 0 ? sel[j - 1] : -1;
+      if (x <= before || x < 0 || x > own[r]) n = min(n, j);
+    }
+#pragma unroll
+    for (int s = 1; s < 64; s *= 2) n = min(n, __shfl_xor(n, s, 64));
+    if (lane == 0) len[r] = n;
+  }
+  const int last = own[st.nrows - 1];                    // rows are in the order of their positions
+  SelectedBlock* out = a.tile_entries + (int64_t)blockIdx.x * a.tile_capacity;
+  int at = 0, flip = 0;
+  for (int w0 = 0; w0 <= last; w0 += kTileWindow) {
+    for (int j = tid; j < kTileWindow; j += kTileThreads) mark[j] = 0ull;
+    __syncthreads();
+    for (int r = wave; r < st.nrows; r += NW) {
+      const int32_t* sel = list(r);
+      for (int j = lane; j < len[r]; j += 64) {
+        const int x = sel[j] - w0;
+        if (x >= 0 && x < kTileWindow) atomicOr(&mark[x], 1ull << r);
+      }
+    }
+    __syncthreads();
+    // a thread's neighbouring blocks; their places from the threads before
+    unsigned long long m[PER];
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      m[i] = mark[tid * PER + i];
+      n += m[i] != 0;
+    }
+    int upto = n;
+#pragma unroll
+    for (int s = 1; s < 64; s *= 2) {
+      const int y = __shfl_up(upto, s, 64);
+      upto += lane >= s ? y : 0;
+    }
+    if (lane == 63) sums[flip][wave] = upto;
+    __syncthreads();
+    int place = at + upto - n;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      place += w < wave ? sums[flip][w] : 0;
+      at += sums[flip][w];
+    }
+    flip ^= 1;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (m[i] == 0) continue;
+      const int b = w0 + tid * PER + i;
+      const uint32_t blk = (uint32_t)a.block_table[(int64_t)st.seq * a.block_table_stride + b];
+      if (place < a.tile_capacity)
+        out[place] = SelectedBlock{m[i], b, blk < (uint64_t)a.num_blocks ? (int32_t)blk : 0};   // never outside the pool
+      ++place;
+    }
+  }
+  // the last row's own block, if any row selected it, ends at that row's key: nothing
+  // behind it is read
+  if (tid == 0) {
+    const int keys = min(at, a.tile_capacity) * a.block_size, pos = a.tile_rows[st.row0 + st.nrows - 1].pos;
+    const bool ends = mark[last % kTileWindow] != 0;
+    a.tile_keys[blockIdx.x] = keys - (ends ? (last + 1) * a.block_size - 1 - pos : 0);
+  }
+}
+hipError_t launch_tile_blocks(const AttnArgs& a, hipStream_t st) {
+  const int64_t units = (int64_t)a.n_sparse_tiles * a.num_kv_heads;
+  if (units > INT32_MAX) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(tile_blocks_kernel, dim3((unsigned)units), dim3(kTileThreads), 0, st, a);
+  return hipGetLastError();
+}
+
 }  // namespace gllm

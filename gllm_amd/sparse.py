@@ -74,9 +74,10 @@ class SparsePlan:
         self.query_lens, self.seq_lens, self.q_seq_stride = ql, sl, q_seq_stride
         self.table_width = -(-max(sl, default=0) // block_size)
         self.record_bytes = key_bounds_bytes(num_kv_heads, head_dim)
-        arr = (ctypes.c_int64 * 6)()
-        _lib.check(lib.gllm_sparse_plan_info(self._h, arr, 6))
-        self._info = dict(zip(("rows", "query_rows", "touched_blocks", "score_tiles", "slabs", "splits"), list(arr)))
+        keys = ("rows", "query_rows", "touched_blocks", "score_tiles", "slabs", "splits", "tiles", "tile_splits")
+        arr = (ctypes.c_int64 * len(keys))()
+        _lib.check(lib.gllm_sparse_plan_info(self._h, arr, len(keys)))
+        self._info = dict(zip(keys, list(arr)))
         self.rows = self._info["rows"]
         nbytes = lib.gllm_sparse_plan_workspace_bytes(self._h)
         self.workspace = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
@@ -236,7 +237,8 @@ def sparse_attention(plan: SparsePlan, q: torch.Tensor, k_cache: torch.Tensor, v
     q and out as in :func:`gllm_amd.paged_attention` (q rotated), ``selected`` int32
     ``[rows, Hkv, blocks]`` from :func:`select_blocks` or any other choice: a list ends
     at the first entry that is negative, not above the entry before it, or behind
-    the row's own block.  A row without blocks gives zeros.  Returns ``out``.
+    the row's own block.  A row without blocks gives zeros.  Keys that some row of
+    a sequence sees must be finite.  Returns ``out``.
     """
     index = q.get_device()
     if index >= 0 and index != torch.cuda.current_device() and index == plan.device.index:

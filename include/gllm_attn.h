@@ -459,7 +459,8 @@ size_t gllm_sparse_plan_workspace_bytes(const gllm_sparse_plan* plan);
 int gllm_sparse_plan_upload(gllm_sparse_plan* plan, void* workspace, size_t workspace_bytes, void* stream);
 /* Plan facts: [0] rows of q / out / selected that it addresses, [1] query rows, [2] blocks
  * that the new tokens touch, [3] score tiles, [4] slabs of rows scored at a time, [5]
- * splits of a row's keys.  The first n are written. */
+ * splits of a row's keys, [6] tiles of prompt rows that attend together, [7] splits of a
+ * tile's keys ([5] to [7]: on the MFMA kernels).  The first n are written. */
 int gllm_sparse_plan_info(const gllm_sparse_plan* plan, int64_t* info, int32_t n);
 int gllm_sparse_plan_destroy(gllm_sparse_plan* plan);
 /* Bounds of every block that holds a new token (positions seq_len - query_len ..
@@ -482,7 +483,7 @@ int gllm_select_blocks(const gllm_sparse_plan* plan, const void* q, int64_t q_ro
 /* Attention of each row over the keys at or before its position in its selected blocks.
  * `selected` may come from anywhere: a list ends at the first entry that is negative, not
  * above the entry before it, or behind the row's own block, and a row without blocks
- * gives zeros. */
+ * gives zeros.  Every key that some row of a sequence sees has to hold finite values. */
 int gllm_sparse_attention(const gllm_sparse_plan* plan, const void* q, int64_t q_row_stride, void* out,
                           int64_t out_row_stride, const void* k_cache, const void* v_cache,
                           int64_t cache_slot_stride, int64_t num_blocks, const int32_t* block_table,

@@ -273,6 +273,65 @@ def test_attention_over_any_lists(Hq, Hkv, D, dtype, kv, bs, blocks):
     check_attention(b, out, {(row, h): sel[row, h].tolist() for _, row, _ in rows_of(b) for h in range(Hkv)})
 
 
+@pytest.mark.parametrize("Hq,Hkv,D,dtype,kv,bs", [
+    (8, 2, 64, BF, BF, 16), (8, 2, 128, BF, BF, 32), (16, 2, 128, F16, F16, 16), (4, 1, 64, F16, F8, 48), (6, 2, 128, BF, F8, 16),
+    (8, 1, 128, BF, "4", 16), (32, 2, 64, BF, "4", 32), (2, 2, 64, BF, BF, 16), (12, 1, 128, F16, F16, 112)])
+def test_prompt_rows_in_tiles(Hq, Hkv, D, dtype, kv, bs):
+    """Chunks whose rows attend in tiles, beside rows on their own: any lists, whole ones
+    and rows that all miss some tiles of keys."""
+    b = Batch([500, 0, 900, 333], [70, 40, 1, 3], Hq=Hq, Hkv=Hkv, D=D, dtype=dtype, kv=kv, bs=bs, seed=Hq + bs)
+    plan = plan_of(b, 9, 0)
+    assert plan.info["tiles"] >= 2
+    for seed, whole in ((1, False), (2, True)):
+        sel = random_lists(b, 9, seed, whole)
+        if whole:
+            sel[5:40, 0] = torch.where(sel[5:40, 0] > 3, -1, sel[5:40, 0])     # only early blocks
+            sel[45:60] = -1
+        out = sparse.sparse_attention(plan, b.q.cuda(), b.kc.cuda(), b.vc.cuda(), b.bt.cuda(), sel.cuda())
+        check_attention(b, out, {(row, h): sel[row, h].tolist() for _, row, _ in rows_of(b) for h in range(Hkv)}, f"seed {seed}")
+
+
+@pytest.mark.parametrize("ctx,rows,blocks", [(40000, 64, 20), (70000, 20, 12), (3000, 200, 3)])
+@pytest.mark.parametrize("kv", [BF, F8])
+def test_tiles_of_many_blocks(ctx, rows, blocks, kv):
+    """More blocks than a workgroup caches (the keys in parts) and than are marked at a
+    time; no row of a tile left out of the parts' joining."""
+    b = Batch([ctx], [rows], Hq=4, Hkv=1, D=64, kv=kv, bs=16, seed=ctx)
+    plan = plan_of(b, blocks, 0)
+    assert plan.info["tiles"] >= 1 and (ctx < 10000 or plan.info["tile_splits"] > 1)
+    sel = random_lists(b, blocks, 7, whole=True)
+    sel[rows // 2] = -1
+    args = (b.q.cuda(), b.kc.cuda(), b.vc.cuda(), b.bt.cuda(), sel.cuda())
+    out = sparse.sparse_attention(plan, *args)
+    check_attention(b, out, {(r, 0): sel[r, 0].tolist() for r in range(rows)})
+    assert torch.equal(out, sparse.sparse_attention(plan, *args))
+
+
+def test_tiles_do_not_read_behind_the_last_row():
+    """NaN behind the sequence's end, and in every block that no row selected."""
+    b = Batch([700], [50], Hq=8, Hkv=2, D=128, bs=32)
+    plan = plan_of(b, 6, 0)
+    assert plan.info["tiles"] >= 1
+    sel = random_lists(b, 6, 1, whole=True) % 14
+    sel = torch.where(sel < 0, -1, sel).sort(-1).values
+    sel[..., -1] = torch.tensor([p // 32 for _, _, p in rows_of(b)], dtype=torch.int32)[:, None]
+    args = (b.q.cuda(), b.bt.cuda(), sel.cuda())
+    out = sparse.sparse_attention(plan, args[0], b.kc.cuda(), b.vc.cuda(), args[1], args[2])
+    check_attention(b, out, {(r, h): sel[r, h].tolist() for r in range(50) for h in range(2)})
+    kc, vc, bt = b.kc.clone(), b.vc.clone(), b.bt.clone()
+    used = {int(x) for x in sel.flatten()} | {p // 32 for _, _, p in rows_of(b)}
+    seen = torch.zeros(b.nb * 32, dtype=torch.bool)
+    for j in range(-(-750 // 32)):
+        if j in used:
+            n = min(32, 750 - 32 * j)
+            seen[int(bt[0, j]) * 32:int(bt[0, j]) * 32 + n] = True
+        else:
+            bt[0, j] = (-1, 1 << 30)[j % 2]
+    assert not seen.all()
+    kc[~seen], vc[~seen] = math.nan, math.nan
+    assert torch.equal(out, sparse.sparse_attention(plan, args[0], kc.cuda(), vc.cuda(), bt.cuda(), args[2]))
+
+
 @pytest.mark.parametrize("D,kv", [(64, BF), (128, BF), (64, F8), (128, "4")])
 def test_attention_in_splits(D, kv):
     """One long row: its keys are split over workgroups; short and empty lists leave
