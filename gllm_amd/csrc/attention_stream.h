@@ -204,12 +204,12 @@ __global__ void __launch_bounds__((64 * StreamCfg<KV, QT, DP, V>::kNW)) attn_str
     const SparseRow sr = a.sparse_rows[b];
     sel = a.selected + ((int64_t)sr.row * a.num_kv_heads + kvh) * a.sel_width;
     const int own = (int)div_bs((uint32_t)sr.pos, a.block_magic, a.block_shift);
-    const int ns = selected_blocks(sel, a.sel_width, own, 64 * NW, reinterpret_cast<int*>(lds));
+    const Selection ns = selected_blocks(sel, a.sel_width, own, 64 * NW, reinterpret_cast<int*>(lds), [](int, int) {});
     __syncthreads();
     seq = sr.seq;
     row0 = sr.row;
     qlen = 1;
-    L = ns == 0 ? 0 : selected_keys(ns, sel[ns - 1], own, sr.pos, a.block_size);
+    L = selected_keys(ns, own, sr.pos, a.block_size);
     ctx = L - 1;
     if (L == 0) {                                // no key: zeros
       const int c1 = min(16 * wgrp + 16, G);

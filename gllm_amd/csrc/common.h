@@ -488,25 +488,39 @@ __host__ __device__ inline int score_heads(int num_kv_heads) {
   return hw;
 }
 
-// How many entries of a row's selection count: up to the first that is not above
-// the one before it or lies behind the row's own block.  The workgroup's threads
-// take part; tmp: an int of LDS per wave.
-__device__ __forceinline__ int selected_blocks(const int32_t* sel, int width, int own, int nthreads, int* tmp) {
-  int n = width;
+// How many entries of a row's selection count: up to the first that is not above the
+// one before it or lies behind the row's own block; and whether the last of them is the
+// own one.  The workgroup's threads take part; tmp: two ints of LDS per wave.  each(j, s):
+// called for every entry by one thread, before it is known which count.
+struct Selection { int n; bool own; };
+template <typename F>
+__device__ __forceinline__ Selection selected_blocks(const int32_t* sel, int width, int own, int nthreads, int* tmp, F each) {
+  int n = width, at = width;
   for (int j = threadIdx.x; j < width; j += nthreads) {
     const int s = sel[j], before = j > 0 ? sel[j - 1] : -1;
     if (s <= before || s < 0 || s > own) n = min(n, j);
+    if (s == own) at = min(at, j);
+    each(j, s);
   }
 #pragma unroll
-  for (int x = 1; x < 64; x *= 2) n = min(n, __shfl_xor(n, x, 64));
-  if ((threadIdx.x & 63) == 0) tmp[threadIdx.x >> 6] = n;
+  for (int x = 1; x < 64; x *= 2) {
+    n = min(n, __shfl_xor(n, x, 64));
+    at = min(at, __shfl_xor(at, x, 64));
+  }
+  if ((threadIdx.x & 63) == 0) {
+    tmp[2 * (threadIdx.x >> 6)] = n;
+    tmp[2 * (threadIdx.x >> 6) + 1] = at;
+  }
   __syncthreads();
-  for (int w = 0; w < nthreads / 64; ++w) n = min(n, tmp[w]);
-  return n;
+  for (int w = 0; w < nthreads / 64; ++w) {
+    n = min(n, tmp[2 * w]);
+    at = min(at, tmp[2 * w + 1]);
+  }
+  return {n, at == n - 1};
 }
-// Keys of n > 0 such blocks: whole ones, but the row's own up to its position.
-__device__ __forceinline__ int selected_keys(int n, int last, int own, int pos, int block_size) {
-  return (n - 1) * block_size + (last == own ? pos - own * block_size + 1 : block_size);
+// Keys of such blocks: whole ones, but the row's own up to its position.
+__device__ __forceinline__ int selected_keys(Selection s, int own, int pos, int block_size) {
+  return s.n * block_size - (s.own ? (own + 1) * block_size - 1 - pos : 0);
 }
 
 // Partials of one (sequence, kv-head group): head i of the group has `count`

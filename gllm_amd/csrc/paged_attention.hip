@@ -95,6 +95,7 @@ struct DecodeTask {
   int pbase;    // partial of head i of the group: pbase + i * nseg + ord
   int ord;
   const int32_t* sel = nullptr;   // SEL: the (row, kv head)'s selected blocks, the task's keys counting through them
+  bool ids = false;               // SEL: the id cache holds those of all entries already
 };
 
 // New tokens written by the attention launch (a.k_new != null): the task whose
@@ -208,17 +209,18 @@ __device__ __forceinline__ void decode_task(const AttnArgs& a, const DecodeTask&
   const KeySkip sk = WIN ? key_skip(tk.ctx_len, a.window, a.sinks, 16) : KeySkip{0, 0, 0};
   const bool both = WIN && kbeg < sk.from && kend > sk.from && sk.by > 0;
   const auto key_of = [&](int v) { return WIN && v >= sk.from ? v + sk.by : v; };
-  const int blk0 = (int)div_bs((uint32_t)key_of(kbeg), a.block_magic, a.block_shift);
+  const bool ids = SEL && tk.ids;
+  const int blk0 = ids ? 0 : (int)div_bs((uint32_t)key_of(kbeg), a.block_magic, a.block_shift);
   const int nblk_s = both ? (int)div_bs((uint32_t)(sk.from - 1), a.block_magic, a.block_shift) - blk0 + 1 : 0;
   const int bgap = both ? (int)div_bs((uint32_t)(sk.from + sk.by), a.block_magic, a.block_shift) - blk0 - nblk_s : 0;
   const int nblk = (int)div_bs((uint32_t)key_of(kend - 1), a.block_magic, a.block_shift) - (WIN ? blk0 + bgap : blk0) + 1;
   const int32_t* bt = a.block_table + (int64_t)seq * a.block_table_stride + (SEL ? 0 : blk0);
   // the table's column of entry e of the cache
   const auto column = [&](int e) { return SEL ? tk.sel[blk0 + e] : (WIN && e >= nblk_s ? e + bgap : e); };
-  const uint32_t bid = tid < nblk ? (uint32_t)bt[column(tid)] : 0u;
+  const uint32_t bid = tid < nblk && !ids ? (uint32_t)bt[column(tid)] : 0u;
   const int tid2 = tid + 64 * NW;
   uint32_t bid2 = 0u;
-  if constexpr (kIds2) bid2 = tid2 < nblk ? (uint32_t)bt[column(tid2)] : 0u;
+  if constexpr (kIds2) bid2 = tid2 < nblk && !ids ? (uint32_t)bt[column(tid2)] : 0u;
   const T* qp = (const T*)a.q + qrow * a.q_row_stride + (int64_t)qh * D;
   u32x4 qraw[NK], praw[kPairInLane ? 1 : NK], craw[NC], sraw[NC];
 #pragma unroll
@@ -239,9 +241,9 @@ __device__ __forceinline__ void decode_task(const AttnArgs& a, const DecodeTask&
       for (int kk = 0; kk < NK; ++kk) praw[kk] = ld16(qp + (chunk_dim<D, KF>(kk, grp) ^ (D / 2)));
     }
   }
-  if (tid < nblk) lbid[tid] = bid < (uint64_t)a.num_blocks ? (int32_t)bid : 0;  // never address outside the pool
+  if (tid < nblk && !ids) lbid[tid] = bid < (uint64_t)a.num_blocks ? (int32_t)bid : 0;  // never address outside the pool
   if constexpr (kIds2) {
-    if (tid2 < nblk) lbid[tid2] = bid2 < (uint64_t)a.num_blocks ? (int32_t)bid2 : 0;
+    if (tid2 < nblk && !ids) lbid[tid2] = bid2 < (uint64_t)a.num_blocks ? (int32_t)bid2 : 0;
   }
   if constexpr (KF != kKV4) {
     if (a.k_new) write_new_keys<T, D, HW, KF, WIN>(a, tk, tid, 64 * NW);
@@ -1826,9 +1828,19 @@ sparse_attn_kernel(AttnArgs a) {
   const SparseRow sr = a.sparse_rows[ri];
   const int32_t* sel = a.selected + ((int64_t)sr.row * a.num_kv_heads + kvh) * a.sel_width;
   const int own = (int)div_bs((uint32_t)sr.pos, a.block_magic, a.block_shift);
-  const int n = selected_blocks(sel, a.sel_width, own, 64 * kWaves, reinterpret_cast<int*>(lds));
+  // lists that fit the task's id cache are looked up while they are counted
+  using Cfg = DecodeCfg<D, kWaves, KF>;
+  int32_t* const ids = reinterpret_cast<int32_t*>(lds + kWaves * Cfg::kVBytes);
+  const bool all = a.sel_width <= Cfg::kMaxBlocks;
+  const int32_t* bt = a.block_table + (int64_t)sr.seq * a.block_table_stride;
+  const Selection n = selected_blocks(sel, a.sel_width, own, 64 * kWaves, reinterpret_cast<int*>(lds), [&](int j, int s) {
+    if (all) {
+      const uint32_t blk = (uint32_t)bt[min(max(s, 0), own)];
+      ids[j] = blk < (uint64_t)a.num_blocks ? (int32_t)blk : 0;     // never address outside the pool
+    }
+  });
   __syncthreads();                               // the count's LDS is the task's
-  const int keys = n == 0 ? 0 : selected_keys(n, sel[n - 1], own, sr.pos, a.block_size);
+  const int keys = selected_keys(n, own, sr.pos, a.block_size);
   const int len = split_len_of(keys, a.sparse_splits);
   DecodeTask tk;
   tk.seq = sr.seq;
@@ -1842,6 +1854,7 @@ sparse_attn_kernel(AttnArgs a) {
   tk.pbase = (ri * a.num_kv_heads + kvh) * a.sparse_splits;
   tk.ord = sp;
   tk.sel = sel;
+  tk.ids = all;
   if (tk.kbeg < tk.kend) {
     decode_task<T, D, 1, kWaves, KF, WIN, true>(a, tk, lds);
     return;
@@ -1900,23 +1913,41 @@ sparse_tile_kernel(AttnArgs a) {
 
 // Joins the splits of every (query row, kv head): a thread per 4 dims of a head.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) sparse_merge_kernel(AttnArgs a, int total) {
-  const int e = blockIdx.x * 256 + threadIdx.x;
+__global__ void __launch_bounds__(64) sparse_merge_kernel(AttnArgs a, int total) {
+  const int e = blockIdx.x * 64 + threadIdx.x;
   if (e >= total) return;
   constexpr int C = D / 4;
   const int d = 4 * (e % C), qh = e / C % a.num_q_heads, ri = e / C / a.num_q_heads;
   const int G = a.num_q_heads / a.num_kv_heads, ns = a.sparse_splits;
   const int64_t at = ((int64_t)ri * a.num_kv_heads + qh / G) * ns * 16 + qh % G;
+  constexpr int CH = 8;                          // splits' loads in flight
   float M = kNegInf, L = 0.f;
-  for (int s = 0; s < ns; ++s) M = fmaxf(M, a.partial_ml[(at + 16 * s) * 2]);
-  const float mu = M == kNegInf ? 0.f : M;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < ns; ++s) {                 // fixed order
-    const float m = a.partial_ml[(at + 16 * s) * 2];
-    if (m == kNegInf) continue;                  // an empty split wrote no values
-    const float w = fast_exp2(m - mu);
-    L += w * a.partial_ml[(at + 16 * s) * 2 + 1];
-    o += w * *reinterpret_cast<const f32x4*>(a.partials + (at + 16 * s) * D + d);
+  for (int s0 = 0; s0 < ns; s0 += CH) {
+    u32x2 x[CH];
+    f32x4 v[CH];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {               // splits past the last one re-read it, with weight 0
+      const int64_t p = at + 16 * min(s0 + c, ns - 1);
+      x[c] = *reinterpret_cast<const u32x2*>(a.partial_ml + p * 2);
+      v[c] = *reinterpret_cast<const f32x4*>(a.partials + p * D + d);
+    }
+    float Mn = M;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) Mn = fmaxf(Mn, __uint_as_float(x[c][0]));
+    const float mu = Mn == kNegInf ? 0.f : Mn, al = fast_exp2(M - mu);
+    L *= al;
+    o *= al;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {               // fixed order: deterministic sums
+      const float m = __uint_as_float(x[c][0]);
+      const bool none = m == kNegInf || s0 + c >= ns;      // an empty split wrote no values
+      const float w = none ? 0.f : fast_exp2(m - mu);
+      L += w * __uint_as_float(x[c][1]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] += none ? 0.f : w * v[c][i];
+    }
+    M = Mn;
   }
   const float inv = L > 0.f ? 1.f / L : 0.f;     // no key at all: zeros
   T* op = (T*)a.out + (int64_t)a.sparse_rows[ri].row * a.out_row_stride + (int64_t)qh * D + d;
@@ -2047,7 +2078,7 @@ template <typename T, int D>
 static hipError_t launch_sparse_merge(const AttnArgs& a, hipStream_t st) {
   const int64_t total = (int64_t)a.n_sparse_rows * a.num_q_heads * (D / 4);
   if (total > INT32_MAX - 256) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((sparse_merge_kernel<T, D>), dim3((unsigned)((total + 255) / 256)), dim3(256), 0, st, a, (int)total);
+  hipLaunchKernelGGL((sparse_merge_kernel<T, D>), dim3((unsigned)((total + 63) / 64)), dim3(64), 0, st, a, (int)total);
   return hipGetLastError();
 }
 // Tiles (n_sparse_tiles > 0: their rows are n_sparse_rows of them) or single rows.

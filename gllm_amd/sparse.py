@@ -21,17 +21,16 @@ import operator
 import torch
 
 from . import _lib
-from .paged import KV4, _cache_rows, _index_rows, _kv4_blocks, _kv_code, _row_stride, _same_device
+from .paged import KV4, _index_rows, _kv4_blocks, _row_stride, _same_device
 
 
 def key_bounds_bytes(num_kv_heads: int, head_dim: int) -> int:
     """Bytes of one block's key bounds: for each KV head ``head_dim`` int8 codes of
     the least key values and ``head_dim`` of the largest, then one exponent byte
     per head (a code stands for code x 2^(byte - 128); 255: unbounded), padded to 16."""
-    n = _lib.load().gllm_key_bounds_record_bytes(num_kv_heads, head_dim)
-    if not n:
+    if num_kv_heads <= 0 or not 0 < head_dim <= 256 or head_dim % 8:
         raise ValueError(f"key bounds: {num_kv_heads} KV heads of head_dim {head_dim} (a multiple of 8, at most 256)")
-    return n
+    return -(-num_kv_heads * (2 * head_dim + 1) // 16) * 16
 
 
 def new_key_bounds(num_blocks: int, num_kv_heads: int, head_dim: int, device) -> torch.Tensor:
@@ -78,7 +77,11 @@ class SparsePlan:
         arr = (ctypes.c_int64 * len(keys))()
         _lib.check(lib.gllm_sparse_plan_info(self._h, arr, len(keys)))
         self._info = dict(zip(keys, list(arr)))
+        # facts that every call looks at
         self.rows = self._info["rows"]
+        self.row_elements = self.rows * num_q_heads * head_dim
+        self.index = self.device.index if self.device.type == "cuda" else -1
+        self.code, self.scale = _lib.dtype_code(dtype), 1.0 / math.sqrt(head_dim)
         nbytes = lib.gllm_sparse_plan_workspace_bytes(self._h)
         self.workspace = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
         if self.device.type == "cuda":
@@ -100,38 +103,51 @@ class SparsePlan:
             self._h = None
 
 
-def _on_device(plan: SparsePlan, call, *args, **kw):
-    """`call` with the plan's device as the current one, where another is."""
+# The calls look at each tensor's dtype, shape, strides and device once: on a decode
+# step the host's part of a call is as long as the kernels'.
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+
+
+def _on_device(plan: SparsePlan, call, *args):
+    """`call` with the plan's device as the current one."""
     with torch.cuda.device(plan.device):
-        return call(*args, **kw)
+        return call(*args)
 
 
-def _on_gpu(index: int, **tensors) -> None:
-    """Refuses tensors of several devices, and of none."""
-    _same_device(index, **tensors)
-    if index < 0:
-        raise ValueError("tensors on the CPU: the kernels need a GPU")
+def _elsewhere(plan: SparsePlan, **tensors) -> None:
+    """Refuses tensors that are not all on the plan's GPU."""
+    if plan.device.type != "cuda":
+        raise ValueError("the plan is for the CPU: the kernels need a GPU")
+    _same_device(plan.index, **tensors)
 
 
-def _table(plan: SparsePlan, block_table: torch.Tensor) -> None:
-    shape = block_table.shape
-    if block_table.dtype != torch.int32 or len(shape) != 2 or block_table.stride(1) != 1:
+def _table(plan: SparsePlan, block_table: torch.Tensor) -> int:
+    """The row stride of the block table, after a check of it."""
+    shape, stride = block_table.shape, block_table.stride()
+    if block_table.dtype != torch.int32 or len(shape) != 2 or stride[1] != 1:
         raise ValueError("block_table must be int32 [B, W] with contiguous rows")
     if shape[0] < len(plan.query_lens) or shape[1] < plan.table_width:
         raise ValueError(f"block_table {tuple(shape)}: {len(plan.query_lens)} rows of {plan.table_width} blocks needed")
+    return stride[0]
 
 
-def _bounds(bounds: torch.Tensor, record: int) -> None:
-    if bounds.dtype != torch.uint8 or bounds.dim() != 2 or bounds.shape[1] < record or bounds.stride(1) != 1:
-        raise ValueError(f"bounds: expected uint8 [num_blocks, {record}] records, got {bounds.dtype} {tuple(bounds.shape)}")
+def _bounds(bounds: torch.Tensor, record: int):
+    """(blocks, bytes between records) of a bounds pool, after a check of it."""
+    shape, stride = bounds.shape, bounds.stride()
+    if bounds.dtype != torch.uint8 or len(shape) != 2 or shape[1] < record or stride[1] != 1:
+        raise ValueError(f"bounds: expected uint8 [num_blocks, {record}] records, got {bounds.dtype} {tuple(shape)}")
+    return shape[0], stride[0]
 
 
-def _cache_blocks(plan: SparsePlan, k_cache: torch.Tensor, v_cache: torch.Tensor) -> int:
+def _key_cache(plan: SparsePlan, k_cache: torch.Tensor):
+    """(blocks, slot or block stride, dtype code) of a cache, after a check of it."""
+    dtype, shape, stride = k_cache.dtype, k_cache.shape, k_cache.stride()
     Hkv, D = plan.num_kv_heads, plan.head_dim
-    if k_cache.dtype == KV4:
-        return _kv4_blocks(k_cache, v_cache, Hkv, D, plan.block_size)
-    _cache_rows(k_cache, v_cache, Hkv, D)
-    return k_cache.shape[0] // plan.block_size
+    if dtype == KV4:
+        return _kv4_blocks(k_cache, k_cache, Hkv, D, plan.block_size), stride[0], _lib.DTYPE_MXFP4
+    if len(shape) != 3 or shape[1] != Hkv or shape[2] != D or stride[1] != D or stride[2] != 1:
+        raise ValueError(f"k_cache: expected [num_slots, {Hkv}, {D}] with contiguous rows")
+    return shape[0] // plan.block_size, stride[0], _lib.dtype_code(dtype)
 
 
 def _query_rows(plan: SparsePlan, t: torch.Tensor, name: str) -> int:
@@ -139,9 +155,19 @@ def _query_rows(plan: SparsePlan, t: torch.Tensor, name: str) -> int:
     if t.dtype != plan.dtype:
         raise ValueError(f"{name} is {t.dtype}, the plan's model dtype {plan.dtype}")
     stride = _row_stride(t, t.shape, plan.num_q_heads, plan.head_dim, name)
-    if t.numel() < plan.rows * plan.num_q_heads * plan.head_dim:
+    if t.numel() < plan.row_elements:
         raise ValueError(f"{name} has {t.numel() // (plan.num_q_heads * plan.head_dim)} rows, the plan addresses {plan.rows}")
     return stride
+
+
+def _selection(plan: SparsePlan, t: torch.Tensor, name: str) -> None:
+    shape = t.shape
+    if t.dtype != torch.int32 or len(shape) != 3 or shape[1] != plan.num_kv_heads or shape[2] != plan.blocks \
+            or not t.is_contiguous():
+        raise ValueError(f"{name}: expected contiguous int32 [rows, {plan.num_kv_heads}, {plan.blocks}], got {t.dtype} "
+                         f"{tuple(shape)}")
+    if shape[0] < plan.rows:
+        raise ValueError(f"{name} has {shape[0]} rows, the plan addresses {plan.rows}")
 
 
 def write_key_bounds(plan: SparsePlan, k_cache: torch.Tensor, bounds: torch.Tensor, block_table: torch.Tensor) -> None:
@@ -151,18 +177,19 @@ def write_key_bounds(plan: SparsePlan, k_cache: torch.Tensor, bounds: torch.Tens
     ``k_cache`` ``[num_slots, Hkv, D]`` (or a 4-bit one), ``bounds`` uint8
     ``[num_blocks, >= key_bounds_bytes]``, block_table int32 ``[B, W]``.
     """
-    index = k_cache.get_device()
-    if index >= 0 and index != torch.cuda.current_device() and index == plan.device.index:
+    index = plan.index
+    if index >= 0 and _current_device() != index:
         return _on_device(plan, write_key_bounds, plan, k_cache, bounds, block_table)
-    _table(plan, block_table)
-    _bounds(bounds, plan.record_bytes)
-    nb = _cache_blocks(plan, k_cache, k_cache)
-    if bounds.shape[0] < nb:
-        raise ValueError(f"bounds of {bounds.shape[0]} blocks for a cache of {nb}")
-    _on_gpu(index, plan=plan.workspace, bounds=bounds, block_table=block_table)
+    bt_stride = _table(plan, block_table)
+    pool, stride = _bounds(bounds, plan.record_bytes)
+    nb, slot, code = _key_cache(plan, k_cache)
+    if pool < nb:
+        raise ValueError(f"bounds of {pool} blocks for a cache of {nb}")
+    if index < 0 or k_cache.get_device() != index or bounds.get_device() != index or block_table.get_device() != index:
+        _elsewhere(plan, k_cache=k_cache, bounds=bounds, block_table=block_table)
     _lib.check(plan._lib.gllm_key_bounds_write(
-        plan._h, k_cache.data_ptr(), k_cache.stride(0), nb, block_table.data_ptr(), block_table.stride(0),
-        bounds.data_ptr(), bounds.stride(0), _kv_code(k_cache), _lib.raw_stream(index)))
+        plan._h, k_cache.data_ptr(), slot, nb, block_table.data_ptr(), bt_stride, bounds.data_ptr(), stride, code,
+        _lib.raw_stream(index)))
 
 
 def key_bounds_values(bounds: torch.Tensor, blocks: torch.Tensor, num_kv_heads: int, head_dim: int,
@@ -171,23 +198,28 @@ def key_bounds_values(bounds: torch.Tensor, blocks: torch.Tensor, num_kv_heads: 
     them: float32 ``[N, Hkv, 2, D]`` (least, largest; infinities where a block is
     unbounded) for int64 ``blocks [N]`` (zeros for a block outside the pool)."""
     index = bounds.get_device()
-    if index >= 0 and index != torch.cuda.current_device():
+    if index >= 0 and _current_device() != index:
         with torch.cuda.device(index):
             return key_bounds_values(bounds, blocks, num_kv_heads, head_dim, out)
-    _bounds(bounds, key_bounds_bytes(num_kv_heads, head_dim))
-    if blocks.dtype.is_floating_point or blocks.dtype == torch.bool:
-        raise ValueError("blocks must be integers")
-    b = _index_rows(blocks)
-    shape = (b.numel(), num_kv_heads, 2, head_dim)
+    pool, stride = _bounds(bounds, key_bounds_bytes(num_kv_heads, head_dim))
+    b = blocks
+    if b.dtype != torch.int64 or b.dim() != 1 or not b.is_contiguous():
+        if b.dtype.is_floating_point or b.dtype == torch.bool:
+            raise ValueError("blocks must be integers")
+        b = _index_rows(b)
+    n = b.shape[0]
     if out is None:
-        out = torch.empty(shape, dtype=torch.float32, device=bounds.device)
-    elif out.dtype != torch.float32 or out.shape != shape or not out.is_contiguous():
-        raise ValueError(f"out must be contiguous float32 {shape}")
-    _on_gpu(index, blocks=b, out=out)
-    if b.numel():
-        _lib.check(_lib.load().gllm_key_bounds_values(bounds.data_ptr(), bounds.stride(0), bounds.shape[0], b.data_ptr(),
-                                                      b.numel(), num_kv_heads, head_dim, out.data_ptr(),
-                                                      _lib.raw_stream(index)))
+        out = torch.empty((n, num_kv_heads, 2, head_dim), dtype=torch.float32, device=bounds.device)
+    elif out.dtype != torch.float32 or out.shape != (n, num_kv_heads, 2, head_dim) or not out.is_contiguous():
+        raise ValueError(f"out must be contiguous float32 {(n, num_kv_heads, 2, head_dim)}")
+    if b.get_device() != index or out.get_device() != index:
+        _same_device(index, blocks=b, out=out)
+    if index < 0:
+        raise ValueError("tensors on the CPU: the kernels need a GPU")
+    if n:
+        lib = _lib._lib or _lib.load()
+        _lib.check(lib.gllm_key_bounds_values(bounds.data_ptr(), stride, pool, b.data_ptr(), n, num_kv_heads, head_dim,
+                                              out.data_ptr(), _lib.raw_stream(index)))
     return out
 
 
@@ -201,31 +233,23 @@ def select_blocks(plan: SparsePlan, q: torch.Tensor, bounds: torch.Tensor, block
     rounded to int8 steps of one power of two, so no key of the block scores
     higher (but for q's rounding); equal scores go to the lower block.
     """
-    index = q.get_device()
-    if index >= 0 and index != torch.cuda.current_device() and index == plan.device.index:
+    index = plan.index
+    if index >= 0 and _current_device() != index:
         return _on_device(plan, select_blocks, plan, q, bounds, block_table, out)
-    stride = _query_rows(plan, q, "q")
-    _table(plan, block_table)
-    _bounds(bounds, plan.record_bytes)
-    if out is None:
-        out = torch.empty((plan.rows, plan.num_kv_heads, plan.blocks), dtype=torch.int32, device=q.device)
-    else:
+    q_stride = _query_rows(plan, q, "q")
+    bt_stride = _table(plan, block_table)
+    pool, stride = _bounds(bounds, plan.record_bytes)
+    if out is not None:
         _selection(plan, out, "out")
-    _on_gpu(index, plan=plan.workspace, bounds=bounds, block_table=block_table, out=out)
+    if index < 0 or q.get_device() != index or bounds.get_device() != index or block_table.get_device() != index \
+            or (out is not None and out.get_device() != index):
+        _elsewhere(plan, q=q, bounds=bounds, block_table=block_table, out=out)
+    if out is None:
+        out = torch.empty((plan.rows, plan.num_kv_heads, plan.blocks), dtype=torch.int32, device=plan.device)
     _lib.check(plan._lib.gllm_select_blocks(
-        plan._h, q.data_ptr(), stride, bounds.data_ptr(), bounds.stride(0), bounds.shape[0], block_table.data_ptr(),
-        block_table.stride(0), out.data_ptr(), _lib.dtype_code(q.dtype), _lib.raw_stream(index)))
+        plan._h, q.data_ptr(), q_stride, bounds.data_ptr(), stride, pool, block_table.data_ptr(), bt_stride,
+        out.data_ptr(), plan.code, _lib.raw_stream(index)))
     return out
-
-
-def _selection(plan: SparsePlan, t: torch.Tensor, name: str) -> None:
-    shape = t.shape
-    if t.dtype != torch.int32 or len(shape) != 3 or shape[1] != plan.num_kv_heads or shape[2] != plan.blocks \
-            or not t.is_contiguous():
-        raise ValueError(f"{name}: expected contiguous int32 [rows, {plan.num_kv_heads}, {plan.blocks}], got {t.dtype} "
-                         f"{tuple(shape)}")
-    if shape[0] < plan.rows:
-        raise ValueError(f"{name} has {shape[0]} rows, the plan addresses {plan.rows}")
 
 
 def sparse_attention(plan: SparsePlan, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -240,25 +264,24 @@ def sparse_attention(plan: SparsePlan, q: torch.Tensor, k_cache: torch.Tensor, v
     the row's own block.  A row without blocks gives zeros.  Keys that some row of
     a sequence sees must be finite.  Returns ``out``.
     """
-    index = q.get_device()
-    if index >= 0 and index != torch.cuda.current_device() and index == plan.device.index:
+    index = plan.index
+    if index >= 0 and _current_device() != index:
         return _on_device(plan, sparse_attention, plan, q, k_cache, v_cache, block_table, selected, out, scale)
-    Hq, D = plan.num_q_heads, plan.head_dim
-    stride = _query_rows(plan, q, "q")
-    if out is None:
-        out, out_stride = torch.empty_like(q, memory_format=torch.contiguous_format), Hq * D
-    else:
-        out_stride = _query_rows(plan, out, "out")
-    _table(plan, block_table)
+    q_stride = _query_rows(plan, q, "q")
+    out_stride = plan.num_q_heads * plan.head_dim if out is None else _query_rows(plan, out, "out")
+    bt_stride = _table(plan, block_table)
     _selection(plan, selected, "selected")
-    nb = _cache_blocks(plan, k_cache, v_cache)
-    if k_cache.stride(0) != v_cache.stride(0):
-        raise ValueError("k_cache and v_cache slot strides differ")
-    _on_gpu(index, plan=plan.workspace, out=out, k_cache=k_cache, v_cache=v_cache, block_table=block_table,
-                 selected=selected)
-    sc = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    nb, slot, code = _key_cache(plan, k_cache)
+    if v_cache.shape != k_cache.shape or v_cache.stride() != k_cache.stride() or v_cache.dtype != k_cache.dtype:
+        raise ValueError("k_cache and v_cache must have the same shape, strides and dtype")
+    if index < 0 or q.get_device() != index or k_cache.get_device() != index or v_cache.get_device() != index \
+            or block_table.get_device() != index or selected.get_device() != index \
+            or (out is not None and out.get_device() != index):
+        _elsewhere(plan, q=q, out=out, k_cache=k_cache, v_cache=v_cache, block_table=block_table, selected=selected)
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     _lib.check(plan._lib.gllm_sparse_attention(
-        plan._h, q.data_ptr(), stride, out.data_ptr(), out_stride, k_cache.data_ptr(), v_cache.data_ptr(),
-        k_cache.stride(0), nb, block_table.data_ptr(), block_table.stride(0), selected.data_ptr(), sc,
-        _lib.dtype_code(q.dtype), _kv_code(k_cache), _lib.raw_stream(index)))
+        plan._h, q.data_ptr(), q_stride, out.data_ptr(), out_stride, k_cache.data_ptr(), v_cache.data_ptr(), slot, nb,
+        block_table.data_ptr(), bt_stride, selected.data_ptr(), plan.scale if scale is None else float(scale), plan.code,
+        code, _lib.raw_stream(index)))
     return out

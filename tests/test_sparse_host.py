@@ -130,8 +130,9 @@ def test_sparse_plan_refuses_lengths():
 
 def test_record_bytes():
     for Hkv, D in ((1, 8), (3, 16), (8, 128), (20, 96), (1, 256)):
-        assert sparse.key_bounds_bytes(Hkv, D) == osp.record_bytes(Hkv, D)
+        assert sparse.key_bounds_bytes(Hkv, D) == osp.record_bytes(Hkv, D) == _lib.load().gllm_key_bounds_record_bytes(Hkv, D)
     for Hkv, D in ((0, 64), (8, 60), (8, 264), (8, 0)):
+        assert _lib.load().gllm_key_bounds_record_bytes(Hkv, D) == 0
         with pytest.raises(ValueError):
             sparse.key_bounds_bytes(Hkv, D)
     b = sparse.new_key_bounds(3, 2, 64, "cpu")
