@@ -1864,21 +1864,31 @@ int sparse_plan_impl(gllm_sparse_plan** out, const int32_t* query_lens, const in
     const int64_t r1 = std::min<int64_t>((int64_t)p->rows.size(), r0 + slab);
     gllm_sparse_plan::Slab sb{(int32_t)r0, (int32_t)(r1 - r0), (int32_t)p->items.size(), 0, 0};
     std::vector<ScoreItem> tiles;
-    int64_t groups = 0;
     for (int64_t r = r0; r < r1;) {
       int64_t e = r + 1;
       while (e < r1 && e - r < tile_rows && p->rows[e].seq == p->rows[r].seq) ++e;
       const int32_t nb = p->rows[e - 1].pos / bs + 1;
       if (nb > blocks) {
         tiles.push_back({(int32_t)r, (int32_t)(e - r), p->rows[r].seq, nb, 0, (nb + 15) / 16});
-        groups += (nb + 15) / 16;
         sb.max_blocks = std::max(sb.max_blocks, nb);
       }
       r = e;
     }
-    // a tile's groups in equal items, so many that two a CU take all of them in one go
-    const int64_t slots = 2 * (int64_t)device_cus();
-    const int64_t per_item = std::max<int64_t>(1, (groups * (Hkv / hw) + slots * kw - 1) / (slots * kw)) * kw;
+    // a tile's groups in equal items: as many items as run at once, two a CU (more tiles
+    // than that: as many as fill the rounds that the tiles need)
+    const int64_t slots = 2 * (int64_t)device_cus() * hw / Hkv;
+    const int64_t room = std::max<int64_t>(1, slots) * std::max<int64_t>(1, ((int64_t)tiles.size() + slots) / std::max<int64_t>(1, slots));
+    const auto count = [&](int64_t len) {
+      int64_t n = 0;
+      for (const ScoreItem& t : tiles) n += (t.groups + len - 1) / len;
+      return n;
+    };
+    int64_t per_item = kw, hi = std::max<int64_t>(kw, (sb.max_blocks + 15) / 16);
+    while (per_item < hi) {
+      const int64_t mid = (per_item + hi) / 2;
+      if (count(mid) <= room) hi = mid;
+      else per_item = mid + 1;
+    }
     for (const ScoreItem& t : tiles) {
       const int64_t n = (t.groups + per_item - 1) / per_item, len = (t.groups + n - 1) / n;
       for (int64_t g0 = 0; g0 < t.groups; g0 += len) {
@@ -1897,13 +1907,15 @@ int sparse_plan_impl(gllm_sparse_plan** out, const int32_t* query_lens, const in
   if (mfma) {
     if (int rc = plan_sparse_tiles(p, query_lens, seq_lens)) return rc;
   }
-  // Splits of a row's selected keys (MFMA kernel): as many as leave every CU its
-  // resident workgroups, where the longest sheds enough for the merge's launch, and of
-  // at most 510 blocks (the ids that a task caches).
+  // Splits of a row's selected keys (MFMA kernel): as many as leave every CU one 4-wave
+  // workgroup, where the longest sheds enough for the merge's launch, and of at most 510
+  // blocks (the ids that a task caches).  Two or three a CU, us at one / two / three, bf16
+  // and fp8 cache: 32 rows of 4,096 keys, 64 / 8 heads of 128 105 / 110 / 110, 64 / 70 / 63; 16 rows,
+  // 32 / 8 heads 60 / 62 / 61, 39 / 40 / 37; 4 rows 22 / 22 / 27, 17 / 18 / 20; the other side, 16 rows
+  // of 4,096, heads of 64 40 / 40 / 35, 32 / 33 / 31.
   if (!p->lone.empty()) {
     const int64_t units = (int64_t)p->lone.size() * Hkv;
-    const int64_t target = (int64_t)device_cus() * (D == 64 ? 2 : 1);
-    int64_t s = std::max<int64_t>(1, std::min(target / units, keys / 128));
+    int64_t s = std::max<int64_t>(1, std::min((int64_t)device_cus() / units, keys / 128));
     if ((keys - keys / s) * D * 4 < 128 << 10) s = 1;
     const int64_t cap = std::max<int64_t>(16, (int64_t)(510 * (int64_t)bs) / 16 * 16 - 16);   // split_len_of rounds up to 16
     s = std::max<int64_t>(s, (keys + cap - 1) / cap);

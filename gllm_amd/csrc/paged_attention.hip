@@ -1814,14 +1814,17 @@ prefix_decode_kernel(AttnArgs a) {
 }
 
 // Sparse attention: one workgroup per (query row, kv head, split of its selected
-// keys), its eight waves taking 16-key sub-tiles in turn (decode_task).  The list
+// keys), its four waves taking 16-key sub-tiles in turn (decode_task).  The list
 // ends at the first entry that is not above the one before or lies behind the
 // row's own block, so any list is safe and none counts a key twice.
+// Four waves, not eight: a CU that holds two such workgroups starts one under the other's
+// keys (us, eight -> four: 64 rows of 2,048 keys 113 -> 105, eight 1B rows of 1,024 13.9 -> 11.8).
+constexpr int kSparseWaves = 4;
 template <typename T, int D, int KF>
-__global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D == 64 ? 4 : 2)))
+__global__ void __launch_bounds__(64 * kSparseWaves) __attribute__((amdgpu_waves_per_eu(D == 64 ? 4 : KF == kKV8 ? 3 : 2)))
 sparse_attn_kernel(AttnArgs a) {
   constexpr bool WIN = KF == kKV4;               // the 4-bit kernels always take a window
-  __shared__ __attribute__((aligned(16))) char lds[DecodeCfg<D, kWaves, KF>::kLdsBytes];
+  __shared__ __attribute__((aligned(16))) char lds[DecodeCfg<D, kSparseWaves, KF>::kLdsBytes];
   const int per_row = a.num_kv_heads * a.sparse_splits;
   const int ri = blockIdx.x / per_row, rest = blockIdx.x - ri * per_row;
   const int kvh = rest / a.sparse_splits, sp = rest - kvh * a.sparse_splits;
@@ -1829,11 +1832,11 @@ sparse_attn_kernel(AttnArgs a) {
   const int32_t* sel = a.selected + ((int64_t)sr.row * a.num_kv_heads + kvh) * a.sel_width;
   const int own = (int)div_bs((uint32_t)sr.pos, a.block_magic, a.block_shift);
   // lists that fit the task's id cache are looked up while they are counted
-  using Cfg = DecodeCfg<D, kWaves, KF>;
-  int32_t* const ids = reinterpret_cast<int32_t*>(lds + kWaves * Cfg::kVBytes);
+  using Cfg = DecodeCfg<D, kSparseWaves, KF>;
+  int32_t* const ids = reinterpret_cast<int32_t*>(lds + kSparseWaves * Cfg::kVBytes);
   const bool all = a.sel_width <= Cfg::kMaxBlocks;
   const int32_t* bt = a.block_table + (int64_t)sr.seq * a.block_table_stride;
-  const Selection n = selected_blocks(sel, a.sel_width, own, 64 * kWaves, reinterpret_cast<int*>(lds), [&](int j, int s) {
+  const Selection n = selected_blocks(sel, a.sel_width, own, 64 * kSparseWaves, reinterpret_cast<int*>(lds), [&](int j, int s) {
     if (all) {
       const uint32_t blk = (uint32_t)bt[min(max(s, 0), own)];
       ids[j] = blk < (uint64_t)a.num_blocks ? (int32_t)blk : 0;     // never address outside the pool
@@ -1856,13 +1859,13 @@ sparse_attn_kernel(AttnArgs a) {
   tk.sel = sel;
   tk.ids = all;
   if (tk.kbeg < tk.kend) {
-    decode_task<T, D, 1, kWaves, KF, WIN, true>(a, tk, lds);
+    decode_task<T, D, 1, kSparseWaves, KF, WIN, true>(a, tk, lds);
     return;
   }
   // no key: an empty partial, or a row of zeros
   const int G = a.num_q_heads / a.num_kv_heads;
   if (tk.nseg == 1) {
-    for (int e = threadIdx.x; e < G * D; e += 64 * kWaves)
+    for (int e = threadIdx.x; e < G * D; e += 64 * kSparseWaves)
       ((T*)a.out)[(int64_t)sr.row * a.out_row_stride + (int64_t)kvh * G * D + e] = (T)0.f;
   } else if ((int)threadIdx.x < G) {
     const int64_t at = ((int64_t)tk.pbase + sp) * 16 + threadIdx.x;
@@ -2093,7 +2096,7 @@ static hipError_t launch_sparse_d(const AttnArgs& a, hipStream_t st) {
   }
   const int64_t wgs = (int64_t)a.n_sparse_rows * a.num_kv_heads * a.sparse_splits;
   if (wgs > INT32_MAX) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((sparse_attn_kernel<T, D, KF>), dim3((unsigned)wgs), dim3(64 * kWaves), 0, st, a);
+  hipLaunchKernelGGL((sparse_attn_kernel<T, D, KF>), dim3((unsigned)wgs), dim3(64 * kSparseWaves), 0, st, a);
   hipError_t e = hipGetLastError();
   return e != hipSuccess || a.sparse_splits == 1 ? e : launch_sparse_merge<T, D>(a, st);
 }

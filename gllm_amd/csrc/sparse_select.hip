@@ -290,13 +290,19 @@ __global__ void __launch_bounds__(64 * kScoreWaves) block_scores_kernel(SelectAr
   };
   uint32_t m = 0u;
   float x[2 * NH][8];
-  for (int p = 0; p < passes; ++p) {
+  const auto load_half = [&](int p, int half) {
     const QT* qp = q_at(p);
-    for (int half = 0; half < (folded ? 1 : 2); ++half) {
 #pragma unroll
-      for (int s = 0; s < 2 * NH; ++s) {
-        load8<QT>(qp + dim_at(s + half * 2 * NH), x[s]);
-      }
+    for (int s = 0; s < 2 * NH; ++s) load8<QT>(qp + dim_at(s + half * 2 * NH), x[s]);
+  };
+  load_half(0, 0);
+  __builtin_amdgcn_sched_barrier(0);                     // q first: its codes are made while bounds are on their way
+#pragma unroll
+  for (int u = 0; u < kScorePF; ++u) issue(blk[u], ring[u]);
+  __builtin_amdgcn_sched_barrier(0);
+  for (int p = 0; p < passes; ++p) {
+    for (int half = 0; half < (folded ? 1 : 2); ++half) {
+      if (p + half > 0) load_half(p, half);
 #pragma unroll
       for (int s = 0; s < 2 * NH; ++s)
 #pragma unroll
@@ -333,8 +339,6 @@ __global__ void __launch_bounds__(64 * kScoreWaves) block_scores_kernel(SelectAr
       qb[s / 2][2 * (s % 2) + 1] = none || k >= 2 * D ? 0u : w[1] ^ 0x80808080u;
     }
   };
-#pragma unroll
-  for (int u = 0; u < kScorePF; ++u) issue(blk[u], ring[u]);
   codes(0);
   float* const sp = a.scores + ((int64_t)(tl.row0 + ri - a.row0) * Hkv + h) * a.score_stride;
   const auto score = [&](int u, const Group& x) {
