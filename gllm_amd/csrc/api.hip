@@ -463,6 +463,14 @@ int check_groups(const PrefixGroups& g, const int32_t* query_lens, const int32_t
 // a key for 32 rows a wave already.  Whole sub-tiles of 16 keys are shared, the rest is
 // the sequences' own.
 //
+// Prefixes from 256 keys on (head dim 64: 512) are shared: below that, the partials and
+// their join cost what the keys save.  Measured, us without / with sharing, 32 / 8 heads,
+// bf16, 64 own keys each: head dim 128, 64 sequences on 128, 512, 2,048, 8,192 shared keys 17.6 /
+// 21.9, 28.9 / 23.5, 71.7 / 26.5, 246 / 34.7; two on 512, 2,048, 8,192 17.8 / 17.0, 19.0 / 17.3, 24.9 /
+// 19.9; 64 with 1,000 own keys on 128, 512 54.6 / 56.4, 61.3 / 56.7; head dim 64, 64 on 128, 512, 2,048
+// 14.8 / 17.9, 19.9 / 18.0, 41.2 / 20.4, with 1,000 own keys on 128, 512, 2,048 30.3 / 34.0, 33.8 / 33.8,
+// 54.5 / 37.7.
+//
 // beside: the batch has decode sequences only, whose own keys go in the same launch.
 // Returns the workgroups that it leaves to those (0: a launch of their own).
 int64_t plan_prefixes(gllm_attn_plan* p, const PrefixGroups& g, int cus, int heads_req, bool beside) {
@@ -475,7 +483,7 @@ int64_t plan_prefixes(gllm_attn_plan* p, const PrefixGroups& g, int cus, int hea
     Group gr{0, g.tokens[k] / 16 * 16, (int32_t)p->prefix_rows.size(), 0};
     int members = 0;
     for (int32_t j = g.ptr[k]; j < g.ptr[k + 1]; ++j) members += p->seqs[g.seqs[j]].q_len * G <= 16;
-    if (gr.tokens == 0 || members < 2) continue;
+    if (gr.tokens < (p->D == 64 ? 512 : 256) || members < 2) continue;
     for (int32_t j = g.ptr[k]; j < g.ptr[k + 1]; ++j) {
       const int32_t i = g.seqs[j];
       const SeqInfo& s = p->seqs[i];

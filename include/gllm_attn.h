@@ -312,9 +312,9 @@ int gllm_attn_plan_create_window(gllm_attn_plan** plan, const int32_t* query_len
  * rows); a sequence is in one group at most.  Their block-table rows name blocks that
  * hold the same values there, the same blocks as a rule: which member's are read is
  * the library's choice.  The MFMA kernels read the shared keys (whole multiples of
- * 16) once for all decode-path members (query_len x G <= 16; at least two), in a launch
- * before the others, and join the parts; prompts of a group, and the generic kernel,
- * read them for each sequence.  Results are those of a plan without groups up to the
+ * 16) once for all decode-path members (query_len x G <= 16; at least two; at least 256
+ * tokens, at head_dim 64 512) and join the parts; prompts of a group, and the generic
+ * kernel, read them for each sequence.  Results are those of a plan without groups up to the
  * order of fp32 sums.  Decode sequences are planned page-balanced: split_tokens 0 or
  * GLLM_SPLIT_BALANCED.  No counterpart in the reference.
  */

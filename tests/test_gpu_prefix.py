@@ -47,8 +47,8 @@ def run(b, groups, plan=None, **kw):
 def test_groups(Hq, Hkv, dtype, kv, bs, D):
     """Two groups in no order, a sequence alone, prefixes that end inside a block or
     a sub-tile, one own key and many."""
-    b = Batch([330, 411, 300, 55, 333, 900, 410], [1] * 7, Hq=Hq, Hkv=Hkv, D=D, dtype=dtype, kv=kv, bs=bs, seed=D + Hq)
-    groups = [([4, 0, 2], 300), ([6, 1], 203)]
+    b = Batch([630, 711, 600, 55, 633, 900, 610], [1] * 7, Hq=Hq, Hkv=Hkv, D=D, dtype=dtype, kv=kv, bs=bs, seed=D + Hq)
+    groups = [([4, 0, 2], 600), ([6, 1], 523)]
     share(b, groups)
     plan = plan_of(b, groups)
     assert plan.info["prefix_items"] > 0
@@ -57,21 +57,23 @@ def test_groups(Hq, Hkv, dtype, kv, bs, D):
     assert torch.equal(out, run(b, groups, plan))
 
 
-@pytest.mark.parametrize("P", [1, 15, 16, 17, 63, 64, 65, 1000, 4097])
+@pytest.mark.parametrize("P", [1, 255, 256, 273, 511, 512, 527, 575, 576, 577, 1000, 4097])
 @pytest.mark.parametrize("D", [64, 128])
 def test_prefix_lengths(P, D):
     b = share(Batch([P + 3, P, P + 40], [1, 1, 1], Hq=8, Hkv=2, D=D), [([0, 1, 2], P)])
     plan = plan_of(b, [([0, 1, 2], P)])
-    assert (plan.info["prefix_items"] > 0) == (P >= 16)
+    assert (plan.info["prefix_items"] > 0) == (P >= (512 if D == 64 else 256))
     b.check(run(b, None, plan), None, 0)
 
 
 @pytest.mark.parametrize("Hq,Hkv", [(8, 2), (12, 4), (8, 1)])
 def test_more_columns_than_a_workgroup_takes(Hq, Hkv):
     n = 70
-    b = Batch([200 + i for i in range(n)], [1] * n, Hq=Hq, Hkv=Hkv, D=64, seed=2)
-    groups = [(range(n), 190)]
-    b.check(run(share(b, groups), groups), None, 0)
+    b = Batch([530 + i for i in range(n)], [1] * n, Hq=Hq, Hkv=Hkv, D=64, seed=2)
+    groups = [(range(n), 520)]
+    plan = plan_of(share(b, groups), groups)
+    assert plan.info["prefix_items"] > 0
+    b.check(run(b, groups, plan), None, 0)
 
 
 def test_several_query_rows_and_prompts():
@@ -109,11 +111,12 @@ def test_long_prefix_of_many_blocks():
 def test_rotation_and_the_write_inside_the_launch(mode, kv):
     """q rotated on load in both parts and the new keys written by the launch: bit for bit
     the cache, and the attention, of the calls apart."""
-    b = share(Batch([100, 130, 97], [1, 1, 2], Hq=8, Hkv=2, D=64, kv=kv, seed=3), [([0, 1, 2], 96)])
-    groups = [([0, 1, 2], 96)]
+    groups = [([0, 1, 2], 528)]
+    b = share(Batch([540, 570, 529], [1, 1, 2], Hq=8, Hkv=2, D=64, kv=kv, seed=3), groups)
     plan, plain = plan_of(b, groups), plan_of(b, ())
-    cos, sin = (x.cuda() for x in orope.rope_cache(200, 64, 10000.0, BF))
-    pos = torch.tensor([100, 130, 97, 98]).cuda()
+    assert plan.info["prefix_items"] > 0
+    cos, sin = (x.cuda() for x in orope.rope_cache(600, 64, 10000.0, BF))
+    pos = torch.tensor([540, 570, 529, 530]).cuda()
     rope = (cos, sin, mode) if mode == "position" else (cos[pos], sin[pos], mode)
     k, v = (torch.randn(4, 2, 64, generator=torch.Generator().manual_seed(i)).to(BF).cuda() for i in (1, 2))
     kc, vc, bt, q = b.kc.cuda(), b.vc.cuda(), b.bt.cuda(), b.q.cuda()
@@ -144,16 +147,16 @@ def test_other_kernels_take_the_plan(D, dtype, kv):
 def test_shared_blocks_are_read_from_one_row():
     """The other members' entries for whole shared sub-tiles are not followed outside the
     pool; entries outside it are never addresses."""
-    b = share(Batch([330, 300], [1, 1], Hq=8, Hkv=2, D=64), [([0, 1], 288)])
-    groups = [([0, 1], 288)]
+    groups = [([0, 1], 528)]
+    b = share(Batch([570, 540], [1, 1], Hq=8, Hkv=2, D=64), groups)
     want = run(b, groups)
-    b.bt[1, :18] = 1 << 30
+    b.bt[1, :33] = 1 << 30
     assert torch.equal(want, run(b, groups))
 
 
 def test_rows_past_the_batch_stay():
-    b = share(Batch([330, 300], [1, 2], Hq=8, Hkv=2, D=64, stride=3), [([0, 1], 288)])
-    out = torch.full((7, 8, 64), 7.0, dtype=BF, device="cuda")
+    b = share(Batch([330, 300], [1, 2], Hq=8, Hkv=2, D=128, stride=3), [([0, 1], 288)])
+    out = torch.full((7, 8, 128), 7.0, dtype=BF, device="cuda")
     run(b, [([0, 1], 288)], out=out)
     b.check(out, None, 0)
     assert (out[[1, 2, 5, 6]] == 7.0).all()

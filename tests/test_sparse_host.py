@@ -237,9 +237,12 @@ def test_prefix_plans():
     assert i["parts"] >= 64 * 8 * (i["prefix"] // 8 + 1)
     # 65 sequences: a second workgroup of columns
     assert _shared([(1, 9000)] * 65, [(range(65), 8192)])["prefix"] % 16 == 0
-    # a group of one, fewer than 16 keys, no group: nothing shared
-    for groups in ([([0], 8192)], [([0, 1], 15)], [([], 3)], [], [([0, 1], 0)]):
+    # a group of one, too few keys, no group: nothing shared
+    for groups in ([([0], 8192)], [([0, 1], 15)], [([], 3)], [], [([0, 1], 0)], [([0, 1], 255)]):
         assert _shared([(1, 9000)] * 4, groups)["prefix"] == 0
+    assert _shared([(1, 9000)] * 4, [([0, 1], 256)])["prefix"] > 0
+    assert _shared([(1, 9000)] * 4, [([0, 1], 511)], D=64)["prefix"] == 0
+    assert _shared([(1, 9000)] * 4, [([0, 1], 512)], D=64)["prefix"] > 0
     # prompts (query_len x G > 16) keep their keys; two decodes beside them share
     i = _shared([(1, 9000), (300, 9000), (4, 9000)], [(range(3), 4000)])
     assert i["pre"] == 1 and i["dec"] == 2 and i["prefix"] > 0
@@ -251,9 +254,9 @@ def test_prefix_plans():
 @pytest.mark.parametrize("bs", [1, 3, 16, 100])
 @pytest.mark.parametrize("own", [1, 40, 9000])
 def test_prefix_segments_cache_their_blocks(own, bs):
-    for P in (16, 100, 5000):
+    for P in (16, 257, 5000):
         i = _shared([(1, P + own)] * 5, [((3, 0, 4), P)], bs=bs)
-        assert i["ids"] <= 512 and i["prefix"] > 0
+        assert i["ids"] <= 512 and (i["prefix"] > 0) == (P > 16)
 
 
 @pytest.mark.parametrize("groups", [[([0, 1], 49)], [([0, 2], 10)], [([0, -1], 10)], [([0, 1], 10), ([1], 5)], [([0, 0], 10)],
