@@ -25,7 +25,8 @@ from . import paged
 @dataclass
 class AttentionMetadata:
     """Field-for-field ``attention.py:12-26`` plus the pool's ``block_size``
-    (the reference keeps it in ``GeneratorParams``, ``generator_params.py``).
+    (the reference keeps it in ``GeneratorParams``, ``generator_params.py``) and
+    what the engine knows of shared prefixes.
     ``block_size=None`` (and the reference's own metadata object, which has
     no such field) makes :func:`plan_for` derive it from the slot mapping."""
 
@@ -37,6 +38,9 @@ class AttentionMetadata:
     query_slot_mapping: torch.Tensor    # [B, T_q] int64
     bias: torch.Tensor | None           # [B, T_q, T] (unused by the kernels)
     block_size: int | None = None
+    # [(sequences of the batch, tokens), ...]: their first keys in common (paged.AttentionPlan);
+    # layers with a sliding window take no notice
+    shared_prefixes: list | None = None
 
 
 def _block_size(meta, ql: list[int], sl: list[int], hint: int | None = None) -> int:
@@ -102,7 +106,8 @@ def plan_for(meta, *, num_q_heads: int, num_kv_heads: int, head_dim: int,
         plan = paged.AttentionPlan(ql, sl, num_q_heads=num_q_heads, num_kv_heads=num_kv_heads,
                                    head_dim=head_dim, block_size=bs, dtype=dtype,
                                    device=device, q_seq_stride=meta.query_slot_mapping.shape[1], window=window,
-                                   sinks=sinks)
+                                   sinks=sinks,
+                                   shared_prefixes=(getattr(meta, "shared_prefixes", None) or ()) if window is None else ())
         if window is None:
             object.__setattr__(meta, "_gllm_plan", plan)
         else:

@@ -3,8 +3,10 @@ knows nothing of sharing (error bound of oracle/window.py)."""
 import pytest
 import torch
 
+import gllm_amd
 from gllm_amd import paged
 from oracle import rope as orope
+from tests.gpu_helpers import assert_close_bf16
 from tests.window_helpers import BF, F8, F16, F32, Batch
 
 pytestmark = pytest.mark.gpu
@@ -196,3 +198,46 @@ def test_pool_past_4_gib():
     kc[shift * bs:], vc[shift * bs:] = b.kc.cuda(), b.vc.cuda()
     out = paged.paged_attention(plan_of(b, [([0, 1], 288)]), b.q.cuda(), kc, vc, (b.bt + shift).cuda())
     b.check(out, None, 0)
+
+
+@pytest.mark.parametrize("kv", [BF, F8])
+def test_attention_layer_shares_what_the_metadata_says(kv):
+    """Attention.attention and forward with AttentionMetadata.shared_prefixes; a layer
+    with a window takes no notice."""
+    Hq, Hkv, D, hid = 8, 2, 128, 1024
+    groups = [([0, 2, 1], 288)]
+    b = share(Batch([330, 300, 420, 50], [1] * 4, Hq=Hq, Hkv=Hkv, D=D, kv=kv), groups)
+    pos = torch.tensor(b.ctx)
+    slots = b.bt[torch.arange(4), pos // 16].long() * 16 + pos % 16
+    lens = torch.tensor(b.L, dtype=torch.int32, device="cuda")
+
+    def meta(groups):
+        return gllm_amd.AttentionMetadata(torch.ones(4, dtype=torch.int32, device="cuda"), lens, max(b.L), b.bt.cuda(), None,
+                                          slots[:, None].cuda(), None, 16, groups)
+
+    class Cfg:
+        num_attn_heads, num_kv_heads, head_dim, hidden_size, dtype = Hq, Hkv, D, hid, BF
+
+    g = torch.Generator().manual_seed(4)
+    w = {f"model.layers.0.self_attn.{n}_proj.weight": (torch.randn(r, hid, generator=g) / 32).to(BF).cuda()
+         for n, r in (("q", hid), ("k", Hkv * D), ("v", Hkv * D), ("o", hid))}
+    att, win = gllm_amd.Attention(0, Cfg, w), gllm_amd.Attention(0, Cfg, w, window=64)
+    cos, sin = (x[pos][:, None].cuda() for x in orope.rope_cache(500, D, 10000.0, BF))
+    k, v = (torch.randn(4, 1, Hkv, D, generator=g).to(BF).cuda() for _ in range(2))
+    pool = torch.stack([b.kc.view(torch.uint8) if kv == F8 else b.kc, b.vc.view(torch.uint8) if kv == F8 else b.vc]).cuda()
+    pool = pool.view(F8) if kv == F8 else pool
+    m = meta(groups)
+    out = att.attention(b.q[:, None].cuda(), k, v, cos, sin, pool, m)
+    assert m._gllm_plan.info["prefix_items"] > 0
+    b.q = paged.rope_rotate(b.q.cuda(), cos[:, 0], sin[:, 0]).cpu()
+    b.kc, b.vc = pool[0].cpu(), pool[1].cpu()
+    b.check(out.view(4, Hq, D), None, 0)
+    # the whole layer, on its fused route too: up to roundings of the 16-bit steps, whose
+    # errors are those of the plan without groups
+    x = torch.randn(4, 1, hid, generator=g).to(BF).cuda()
+    m = meta(groups)
+    got, want = att.forward(x, cos, sin, pool.clone(), m), att.forward(x, cos, sin, pool.clone(), meta(None))
+    assert m._gllm_plan.info["prefix_items"] > 0
+    assert_close_bf16(got, want, "forward")
+    m = meta(groups)
+    assert torch.equal(win.forward(x, cos, sin, pool.clone(), m), win.forward(x, cos, sin, pool.clone(), meta(None)))

@@ -277,3 +277,28 @@ def test_prefix_plans_refuse_splits_and_windows():
         paged.AttentionPlan([1, 1], [50, 60], shared_prefixes=[([0, 1], 32.0)], **args)
     with pytest.raises(ValueError):
         paged.AttentionPlan([1, 1], [50, 60], shared_prefixes=[([0, 1], 1 << 40)], **args)
+
+
+def test_metadata_passes_prefixes_to_the_plan(monkeypatch):
+    """plan_for: what the engine knows of prefixes reaches the plan, but not windowed ones;
+    metadata without the field (the reference's own) shares nothing."""
+    import types
+    from gllm_amd import attention
+    seen = []
+
+    def plan(ql, sl, **kw):
+        seen.append((kw["shared_prefixes"], kw["window"]))
+        return types.SimpleNamespace()
+    monkeypatch.setattr(attention.paged, "AttentionPlan", plan)
+
+    def meta(**kw):
+        return types.SimpleNamespace(query_lens=torch.tensor([1, 1]), seq_lens=torch.tensor([40, 50]), block_size=16,
+                                     block_table=torch.tensor([[1, 2, 3, 0], [1, 2, 4, 5]]),
+                                     query_slot_mapping=torch.tensor([[3 * 16 + 7], [5 * 16 + 1]]), **kw)
+    args = dict(num_q_heads=8, num_kv_heads=2, head_dim=64, dtype=torch.bfloat16, device="cpu")
+    groups = [([0, 1], 32)]
+    attention.plan_for(meta(shared_prefixes=groups), **args)
+    attention.plan_for(meta(shared_prefixes=groups), window=16, **args)
+    attention.plan_for(meta(shared_prefixes=None), **args)
+    attention.plan_for(meta(), **args)
+    assert seen == [(groups, None), ((), 16), ((), None), ((), None)]
