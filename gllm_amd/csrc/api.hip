@@ -1882,6 +1882,7 @@ int sparse_plan_impl(gllm_sparse_plan** out, const int32_t* query_lens, const in
       }
       r = e;
     }
+    p->n_tiles += (int64_t)tiles.size();
     // a tile's groups in equal items: as many items as run at once, two a CU (more tiles
     // than that: as many as fill the rounds that the tiles need)
     const int64_t slots = 2 * (int64_t)device_cus() * hw / Hkv;
@@ -1906,7 +1907,6 @@ int sparse_plan_impl(gllm_sparse_plan** out, const int32_t* query_lens, const in
         p->items.push_back(it);
       }
     }
-    p->n_tiles += (int64_t)tiles.size();
     sb.n_items = (int32_t)p->items.size() - sb.item0;
     if (sb.n_items > 0) slab_rows = std::max<int64_t>(slab_rows, sb.n_rows);
     p->slabs.push_back(sb);

@@ -224,7 +224,7 @@ hipError_t launch_key_bounds_values(const BoundsValuesArgs& a, hipStream_t st) {
 // ---------------------------------------------------------------- scores
 // One 8-wave workgroup per (item: a tile of query rows and a run of 16-block groups; HW
 // kv heads); a wave takes one of the heads and its share of the groups, two groups'
-// loads ahead.  The plan cuts tiles into items that end together, two a CU.  A column of the
+// loads ahead.  The plan cuts tiles into items that end together, two a CU.   A column of the
 // MFMA is a (row of the tile, head of the group) pair, n = row x Gp + g with Gp = G
 // rounded up to a power of two, so a tile's rows share the bounds they load; more than 16
 // heads go by in passes.  Lane (n, grp) loads bytes 64 s + 16 grp .. + 15 of block n's
@@ -232,7 +232,8 @@ hipError_t launch_key_bounds_values(const BoundsValuesArgs& a, hipStream_t st) {
 // sequences.
 constexpr int kScoreWaves = 8;
 // The maximum over the lane's aligned run of gp = 1, 2, 4, 8 or 16 lanes.
-__device__ __forceinline__ int columns_max(int v, int gp) {
+template <int gp>
+__device__ __forceinline__ int columns_max(int v) {
   if (gp > 1) v = max(v, __builtin_amdgcn_mov_dpp(v, 0xb1, 0xf, 0xf, true));     // quad_perm 1 0 3 2
   if (gp > 2) v = max(v, __builtin_amdgcn_mov_dpp(v, 0x4e, 0xf, 0xf, true));     // quad_perm 2 3 0 1
   if (gp > 4) v = max(v, __builtin_amdgcn_mov_dpp(v, 0x141, 0xf, 0xf, true));    // the other half of 8
@@ -240,42 +241,51 @@ __device__ __forceinline__ int columns_max(int v, int gp) {
   return v;
 }
 constexpr int kScorePF = 2;
-struct ScoreShape { int32_t gp_log, hw; };
-template <typename QT, int NK, bool PASSES>
-__global__ void __launch_bounds__(64 * kScoreWaves) block_scores_kernel(SelectArgs a, ScoreShape sh) {
+template <typename QT, int NK, int GP, bool PASSES>
+__global__ void __launch_bounds__(64 * kScoreWaves) block_scores_kernel(SelectArgs a, int hw) {
   const int lane = threadIdx.x & 63, n = lane & 15, grp = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int D = a.head_dim, G = a.num_q_heads / a.num_kv_heads, Hkv = a.num_kv_heads;
-  const int hgs = Hkv / sh.hw;
+  const int hgs = Hkv / hw;
   const ScoreItem tl = a.items[a.item0 + blockIdx.x / hgs];
-  const int h = blockIdx.x % hgs * sh.hw + wave % sh.hw;
-  const int kw = kScoreWaves / sh.hw;                    // waves of a head, their groups one after another
-  const int share = (tl.groups + kw - 1) / kw, first = wave / sh.hw * share;
+  const int h = blockIdx.x % hgs * hw + wave % hw;
+  const int kw = kScoreWaves / hw;                       // waves of a head, their groups one after another
+  const int share = (tl.groups + kw - 1) / kw, first = wave / hw * share;
   const int b0 = (tl.group0 + first) * 16;
   const int ng = min(share, tl.groups - first);
   if (ng <= 0) return;
-  const int gp = 1 << sh.gp_log, ri = n >> sh.gp_log, g0 = n & (gp - 1);
+  const int ri = n / GP, g0 = n % GP;
   const bool row_ok = ri < tl.nrows;
   const int row = a.rows[tl.row0 + (row_ok ? ri : 0)].row;
   const int passes = PASSES ? (G + 15) / 16 : 1;
-  struct Group { u32x4 box[NK]; int e; };
+  // a byte of the word that is loaded (a byte load's value is widened where the loop ends,
+  // which waits for every load in flight)
+  struct Group { u32x4 box[NK]; uint32_t e; };
   const int32_t* bt = a.block_table + (int64_t)tl.seq * a.block_table_stride;
-  const auto block_of = [&](int u) {                     // the lane's block n of group u (past the last: the last)
-    const uint32_t blk = (uint32_t)bt[min(b0 + 16 * u + n, tl.nblocks - 1)];
-    return blk < (uint64_t)a.num_blocks ? blk : 0u;      // never address outside the pool
+  // the pool's blocks of 16 groups, 64 a register, so that no load waits in the loop for
+  // the older ones, which loads return in order
+  constexpr int NI = 4;
+  uint32_t ids[NI];
+  const auto load_ids = [&](int u0) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const uint32_t blk = (uint32_t)bt[min(b0 + 16 * u0 + 64 * i + lane, tl.nblocks - 1)];   // past the last: the last
+      ids[i] = blk < (uint64_t)a.num_blocks ? blk : 0u;  // never address outside the pool
+    }
   };
-  const auto issue = [&](uint32_t blk, Group& x) {
+  const auto issue = [&](int u, Group& x) {              // group u of the 16
+    const int i = u >> 2;
+    const uint32_t src = i == 0 ? ids[0] : i == 1 ? ids[1] : i == 2 ? ids[2] : ids[3];
+    const uint32_t blk = (uint32_t)__shfl((int)src, 16 * (u & 3) + n, 64);
     const uint8_t* rec = a.bounds + (int64_t)blk * a.bounds_stride;
     const uint8_t* box = rec + h * 2 * D + 16 * grp;
 #pragma unroll
     for (int s = 0; s < NK; ++s)
       x.box[s] = 64 * s + 64 <= 2 * D ? ld16(box + 64 * s) : ld16(rec + h * 2 * D + min(64 * s + 16 * grp, 2 * D - 16));
-    x.e = rec[Hkv * 2 * D + h];
+    x.e = *reinterpret_cast<const uint32_t*>(rec + Hkv * 2 * D + (h & ~3));
   };
   Group ring[kScorePF + 1];
-  uint32_t blk[kScorePF + 1];
-#pragma unroll
-  for (int u = 0; u <= kScorePF; ++u) blk[u] = block_of(u);
+  load_ids(0);
 
   // q's codes: one power of two for all heads of the group, then each half's sign.  A
   // lane's dims of the lo half are those of its hi half where 64 divides D.
@@ -298,7 +308,7 @@ __global__ void __launch_bounds__(64 * kScoreWaves) block_scores_kernel(SelectAr
   load_half(0, 0);
   __builtin_amdgcn_sched_barrier(0);                     // q first: its codes are made while bounds are on their way
 #pragma unroll
-  for (int u = 0; u < kScorePF; ++u) issue(blk[u], ring[u]);
+  for (int u = 0; u < kScorePF; ++u) issue(u, ring[u]);
   __builtin_amdgcn_sched_barrier(0);
   for (int p = 0; p < passes; ++p) {
     for (int half = 0; half < (folded ? 1 : 2); ++half) {
@@ -311,7 +321,8 @@ __global__ void __launch_bounds__(64 * kScoreWaves) block_scores_kernel(SelectAr
   }
   m = max(m, (uint32_t)__shfl_xor((int)m, 16, 64));
   m = max(m, (uint32_t)__shfl_xor((int)m, 32, 64));
-  for (int s = 1; s < gp; s *= 2) m = max(m, (uint32_t)__shfl_xor((int)m, s, 64));
+#pragma unroll
+  for (int s = 1; s < GP; s *= 2) m = max(m, (uint32_t)__shfl_xor((int)m, s, 64));
   const bool none = !row_ok || m > kCodeMax;
   const float inv = m > kCodeMax ? 0.f : pow2f(-code_exponent(m));
   u32x4 qb[NK];
@@ -356,27 +367,33 @@ __global__ void __launch_bounds__(64 * kScoreWaves) block_scores_kernel(SelectAr
     f32x4 sc;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int v = columns_max(best[j], gp);
-      const int e = __shfl(x.e, 4 * grp + j, 64);        // lane 4 grp + j holds block 4 grp + j's
+      const int v = columns_max<GP>(best[j]);
+      const int e = __shfl((int)(x.e >> (8 * (h & 3)) & 255u), 4 * grp + j, 64);   // lane 4 grp + j holds block 4 grp + j's
       // bytes that no writer leaves are limited, so that the score stays a number
       sc[j] = e == kOpen ? -kNegInf : (float)v * pow2f(min(max(e - 128, -100), 100));
     }
     const int b = b0 + 16 * u + 4 * grp;
     if (row_ok && g0 == 0 && b < a.score_stride) *reinterpret_cast<f32x4*>(sp + b) = sc;   // rows are padded to 4
   };
-  int u0 = 0;
-  for (; u0 + kScorePF < ng; u0 += kScorePF + 1) {
+  for (int c0 = 0; c0 < ng; c0 += 4 * NI) {
+    const int nc = min(4 * NI, ng - c0);
+    if (c0 > 0) {
+      load_ids(c0);
 #pragma unroll
-    for (int u = 0; u <= kScorePF; ++u) {
-      const int w = (u + kScorePF) % (kScorePF + 1);
-      issue(blk[w], ring[w]);
-      blk[u] = block_of(u0 + u + kScorePF + 1);
-      score(u0 + u, ring[u]);
+      for (int u = 0; u < kScorePF; ++u) issue(u, ring[u]);
     }
-  }
+    int u0 = 0;
+    for (; u0 + kScorePF < nc; u0 += kScorePF + 1) {
 #pragma unroll
-  for (int u = 0; u < kScorePF; ++u)
-    if (u0 + u < ng) score(u0 + u, ring[u]);
+      for (int u = 0; u <= kScorePF; ++u) {
+        issue(min(u0 + u + kScorePF, 4 * NI - 1), ring[(u + kScorePF) % (kScorePF + 1)]);
+        score(c0 + u0 + u, ring[u]);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kScorePF; ++u)
+      if (u0 + u < nc) score(c0 + u0 + u, ring[u]);
+  }
 }
 
 // ---------------------------------------------------------------- selection
@@ -608,18 +625,25 @@ __global__ void __launch_bounds__(NT) select_kernel(SelectArgs a) {
 }
 
 template <typename QT>
-static hipError_t launch_scores_t(const SelectArgs& a, const ScoreShape& sh, dim3 grid, hipStream_t st) {
+static hipError_t launch_scores_t(const SelectArgs& a, int hw, dim3 grid, hipStream_t st) {
   const dim3 block(64 * kScoreWaves);
   const int nk = (2 * a.head_dim + 63) / 64;
-  const bool passes = a.num_q_heads / a.num_kv_heads > 16;
-  const auto go = [&](auto n) {
-    constexpr int NK = decltype(n)::value;
-    if (passes) hipLaunchKernelGGL((block_scores_kernel<QT, NK, true>), grid, block, 0, st, a, sh);
-    else hipLaunchKernelGGL((block_scores_kernel<QT, NK, false>), grid, block, 0, st, a, sh);
+  const auto go = [&](auto n, auto gp, auto pass) {
+    constexpr int NK = decltype(n)::value, GP = decltype(gp)::value;
+    hipLaunchKernelGGL((block_scores_kernel<QT, NK, GP, decltype(pass)::value>), grid, block, 0, st, a, hw);
   };
-  if (nk <= 2) go(std::integral_constant<int, 2>());
-  else if (nk <= 4) go(std::integral_constant<int, 4>());
-  else go(std::integral_constant<int, 8>());
+  const auto by_group = [&](auto n) {
+    const int G = a.num_q_heads / a.num_kv_heads;
+    if (G == 1) go(n, std::integral_constant<int, 1>(), std::false_type());
+    else if (G == 2) go(n, std::integral_constant<int, 2>(), std::false_type());
+    else if (G <= 4) go(n, std::integral_constant<int, 4>(), std::false_type());
+    else if (G <= 8) go(n, std::integral_constant<int, 8>(), std::false_type());
+    else if (G <= 16) go(n, std::integral_constant<int, 16>(), std::false_type());
+    else go(n, std::integral_constant<int, 16>(), std::true_type());
+  };
+  if (nk <= 2) by_group(std::integral_constant<int, 2>());
+  else if (nk <= 4) by_group(std::integral_constant<int, 4>());
+  else by_group(std::integral_constant<int, 8>());
   return hipGetLastError();
 }
 
@@ -628,17 +652,15 @@ hipError_t launch_select_blocks(const SelectArgs& a, hipStream_t st) {
   const int64_t units = (int64_t)a.n_rows * a.num_kv_heads;
   if (units > INT32_MAX) return hipErrorInvalidValue;
   if (a.n_items > 0) {
-    const int G = a.num_q_heads / a.num_kv_heads;
-    ScoreShape sh{0, score_heads(a.num_kv_heads)};
-    while ((1 << sh.gp_log) < G && sh.gp_log < 4) ++sh.gp_log;
-    const int64_t wgs = (int64_t)a.n_items * (a.num_kv_heads / sh.hw);
+    const int hw = score_heads(a.num_kv_heads);
+    const int64_t wgs = (int64_t)a.n_items * (a.num_kv_heads / hw);
     if (wgs > INT32_MAX) return hipErrorInvalidValue;
     hipError_t e = hipErrorInvalidValue;
     const dim3 grid((unsigned)wgs);
     switch (a.dtype) {
-      case kF32: e = launch_scores_t<float>(a, sh, grid, st); break;
-      case kBF16: e = launch_scores_t<__bf16>(a, sh, grid, st); break;
-      case kF16: e = launch_scores_t<_Float16>(a, sh, grid, st); break;
+      case kF32: e = launch_scores_t<float>(a, hw, grid, st); break;
+      case kBF16: e = launch_scores_t<__bf16>(a, hw, grid, st); break;
+      case kF16: e = launch_scores_t<_Float16>(a, hw, grid, st); break;
       default: break;
     }
     if (e != hipSuccess) return e;

@@ -499,6 +499,31 @@ def test_slabs_of_rows():
         assert torch.equal(sparse.select_blocks(part, q[r0:r1], rec, bt), got[r0:r1])
 
 
+def test_many_blocks_a_wave():
+    """So many rows of many blocks that a wave takes more than 16 groups of blocks: each
+    row as in a plan of its own."""
+    D, L, n, Hkv = 8, 2100, 80, 8
+    g = torch.Generator().manual_seed(6)
+    k = torch.randn(L, Hkv, D, generator=g).cuda()
+    q = torch.randn(n, Hkv, D, generator=g).cuda()
+    bt = torch.randperm(L, generator=g).to(torch.int32)[None].expand(n, -1).contiguous().cuda()
+    args = dict(num_q_heads=Hkv, num_kv_heads=Hkv, head_dim=D, block_size=1, dtype=F32, device="cuda", blocks=40)
+    rec = sparse.new_key_bounds(L, Hkv, D, "cuda")
+    sparse.write_key_bounds(sparse.SparsePlan([L], [L], **args), k, rec, bt)
+    lens = [L - i for i in range(n)]
+    got = sparse.select_blocks(sparse.SparsePlan([1] * n, lens, **args), q, rec, bt)
+    for r in (0, 1, 33, 79):
+        assert torch.equal(sparse.select_blocks(sparse.SparsePlan([1], lens[r:r + 1], **args), q[r:r + 1], rec, bt)[0], got[r])
+    # against the definition: one key a block, its codes the same at both ends
+    c = osp.query_codes(q[5, 3:4].cpu())
+    keys = k[bt[0, :lens[5]].long(), 3].cpu()
+    sc = []
+    for x in keys:
+        codes, byte = osp.key_bounds(x[None, None])
+        sc.append(torch.maximum(c * codes[0, 0], c * codes[0, 1]).sum() * 2.0 ** (int(byte) - 128))
+    assert got[5, 3].tolist() == osp.select(torch.stack(sc), 40, 1, 1)
+
+
 def test_blocks_past_4_gib():
     """Places past 2^32 bytes in the cache and in the bounds."""
     bs, Hkv, D = 16, 8, 128
