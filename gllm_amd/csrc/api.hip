@@ -1761,7 +1761,7 @@ int bounds_check(const void* bounds, int64_t stride, int64_t num_blocks, int32_t
 // near each other choose alike, so tiles read fewer): a row 5 us and its K/V at 29 GB/s; a
 // tile 6 us and per 64 keys its columns' flops at 3.2 (head dim 64: 2.4) TFLOP/s or its
 // K/V at 30 GB/s.
-int plan_sparse_tiles(gllm_sparse_plan* p, const int32_t* query_lens, const int32_t* seq_lens) {
+void plan_sparse_tiles(gllm_sparse_plan* p, const int32_t* query_lens, const int32_t* seq_lens) {
   const int G = p->Hq / p->Hkv, most = std::min(64, 256 / G);
   const double key = 4.0 * p->D;               // bytes of a 16-bit key and value
   const auto tile_time = [&](int rows, int32_t nb) {
@@ -1794,7 +1794,7 @@ int plan_sparse_tiles(gllm_sparse_plan* p, const int32_t* query_lens, const int3
       longest = std::max(longest, tile_time((int)(e - a), nb));
     }
   }
-  if (p->tiles.empty()) return ok();
+  if (p->tiles.empty()) return;
   // Parts of a tile's keys: what ends soonest with a workgroup per CU, a partial's write
   // and read at 3 TB/s; the ids, rows and numbers of at most 1,022 blocks fit a workgroup.
   const int64_t cus = device_cus(), units = (int64_t)p->tiles.size() * p->Hkv;
@@ -1809,9 +1809,15 @@ int plan_sparse_tiles(gllm_sparse_plan* p, const int32_t* query_lens, const int3
       p->tile_splits = (int32_t)s;
     }
   }
-  if (units * p->tile_splits > INT32_MAX || (int64_t)p->tile_rows.size() * p->Hkv * p->tile_splits > INT32_MAX / 16)
-    return fail(GLLM_ATTN_EINVAL, "too many splits");
-  return ok();
+  // partials past 1 GiB, or too many workgroups: rows on their own
+  if (units * p->tile_splits > INT32_MAX ||
+      (p->tile_splits > 1 && (int64_t)p->tile_rows.size() * p->Hq * p->tile_splits * p->D * 4 > int64_t(1) << 30)) {
+    p->lone = p->rows;
+    p->tiles.clear();
+    p->tile_rows.clear();
+    p->tile_capacity = 0;
+    p->tile_splits = 1;
+  }
 }
 
 int sparse_plan_impl(gllm_sparse_plan** out, const int32_t* query_lens, const int32_t* seq_lens, int32_t num_seqs,
@@ -1912,9 +1918,7 @@ int sparse_plan_impl(gllm_sparse_plan** out, const int32_t* query_lens, const in
     p->slabs.push_back(sb);
   }
   const bool mfma = mfma_dtype(dtype) && (D == 64 || D == 128) && G <= 16;
-  if (mfma) {
-    if (int rc = plan_sparse_tiles(p, query_lens, seq_lens)) return rc;
-  }
+  if (mfma) plan_sparse_tiles(p, query_lens, seq_lens);
   // Splits of a row's selected keys (MFMA kernel): as many as leave every CU one 4-wave
   // workgroup, where the longest sheds enough for the merge's launch, and of at most 510
   // blocks (the ids that a task caches).  Two or three a CU, us at one / two / three, bf16
@@ -1943,8 +1947,8 @@ int sparse_plan_impl(gllm_sparse_plan** out, const int32_t* query_lens, const in
   p->stage_bytes = o;
   p->off_entries = o; o = align256(o + tile_units * p->tile_capacity * sizeof(SelectedBlock));
   p->off_keys = o; o = align256(o + tile_units * sizeof(int32_t));
-  p->off_tile_ml = o; o = align256(o + tile_parts * 16 * 2 * sizeof(float));
-  p->off_tile_part = o; o = align256(o + tile_parts * 16 * D * sizeof(float));
+  p->off_tile_ml = o; o = align256(o + tile_parts * G * 2 * sizeof(float));
+  p->off_tile_part = o; o = align256(o + tile_parts * G * D * sizeof(float));
   p->off_scores = o; o = align256(o + (size_t)(slab_rows * per_row));
   p->off_ml = o; o = align256(o + parts * 16 * 2 * sizeof(float));
   p->off_part = o; o = align256(o + parts * 16 * D * sizeof(float));

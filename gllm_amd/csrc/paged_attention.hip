@@ -1615,7 +1615,7 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
         const MergeInfo mi = a.merge[pr.seq * a.head_groups + hg];
         at = ((int64_t)mi.pbase + (int64_t)(kvh - hg * a.heads_per_wg) * mi.count + px->ord) * 16 + pr.r * G + g;
       } else {
-        at = (((int64_t)(sx->row0 + rr) * a.num_kv_heads + kvh) * sx->parts + sx->ord) * 16 + g;
+        at = (((int64_t)(sx->row0 + rr) * a.num_kv_heads + kvh) * sx->parts + sx->ord) * G + g;
       }
       float* pa = a.partials + at * D + 4 * h;
 #pragma unroll
@@ -1908,7 +1908,7 @@ sparse_tile_kernel(AttnArgs a) {
   } else {
     for (int c = threadIdx.x; c < st.nrows * G; c += 64 * kWaves) {
       const int r = c / G;
-      const int64_t at = (((int64_t)(st.row0 + r) * Hkv + kvh) * a.tile_splits + sp) * 16 + c - r * G;
+      const int64_t at = (((int64_t)(st.row0 + r) * Hkv + kvh) * a.tile_splits + sp) * G + c - r * G;
       a.partial_ml[2 * at] = kNegInf;
       a.partial_ml[2 * at + 1] = 0.f;
     }
@@ -1923,7 +1923,8 @@ __global__ void __launch_bounds__(64) sparse_merge_kernel(AttnArgs a, int total)
   constexpr int C = D / 4;
   const int d = 4 * (e % C), qh = e / C % a.num_q_heads, ri = e / C / a.num_q_heads;
   const int G = a.num_q_heads / a.num_kv_heads, ns = a.sparse_splits;
-  const int64_t at = ((int64_t)ri * a.num_kv_heads + qh / G) * ns * 16 + qh % G;
+  const int slots = a.n_sparse_tiles > 0 ? G : 16;     // of a partial: a tile's rows have theirs side by side
+  const int64_t at = ((int64_t)ri * a.num_kv_heads + qh / G) * ns * slots + qh % G;
   constexpr int CH = 8;                          // splits' loads in flight
   float M = kNegInf, L = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
@@ -1932,7 +1933,7 @@ __global__ void __launch_bounds__(64) sparse_merge_kernel(AttnArgs a, int total)
     f32x4 v[CH];
 #pragma unroll
     for (int c = 0; c < CH; ++c) {               // splits past the last one re-read it, with weight 0
-      const int64_t p = at + 16 * min(s0 + c, ns - 1);
+      const int64_t p = at + slots * min(s0 + c, ns - 1);
       x[c] = *reinterpret_cast<const u32x2*>(a.partial_ml + p * 2);
       v[c] = *reinterpret_cast<const f32x4*>(a.partials + p * D + d);
     }

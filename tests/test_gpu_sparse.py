@@ -348,6 +348,18 @@ def test_attention_in_splits(D, kv):
     assert torch.equal(out, sparse.sparse_attention(plan, *args))
 
 
+@pytest.mark.parametrize("rows", [1, 40])
+def test_lists_longer_than_a_task_caches(rows):
+    """More than 512 entries a list: looked up part by part."""
+    b = Batch([9000] * rows, [1] * rows, Hq=4, Hkv=2, D=64, bs=8, seed=rows)
+    sel = random_lists(b, 700, 5, whole=True)
+    sel[0, 1, 600:] = -1
+    out = sparse.sparse_attention(plan_of(b, 700, 0), b.q.cuda(), b.kc.cuda(), b.vc.cuda(), b.bt.cuda(), sel.cuda())
+    part = Batch.__new__(Batch)
+    part.__dict__.update(b.__dict__, ql=b.ql[:2], ctx=b.ctx[:2], L=b.L[:2])
+    check_attention(part, out, {(r, h): sel[r, h].tolist() for r in range(rows) for h in range(2)})
+
+
 def test_all_blocks_are_all_keys():
     """Where a row selects every block, the result is paged attention's."""
     b = Batch([200, 0, 77], [3, 1, 1], Hq=8, Hkv=2, D=64, bs=16)

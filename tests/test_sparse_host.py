@@ -95,6 +95,24 @@ def test_plan_facts():
     assert i["slabs"] == 4 and i["bytes"] < (256 << 20) + (2 << 20)
 
 
+def _tiles(ql, sl, **kw):
+    p = _plan(ql, sl, num_q_heads=32, num_kv_heads=8, head_dim=128, **kw)
+    return p.info["tiles"], p.info["tile_splits"], p.workspace.numel()
+
+
+def test_prompt_rows_go_in_tiles_where_that_reads_less():
+    # 64 rows a tile at G = 4; decode rows and other block sizes go alone
+    assert _tiles([386, 1], [12000, 12000], blocks=64, block_size=32)[0] == 7
+    assert _tiles([386], [12000], blocks=64, block_size=24)[0] == 0
+    assert _tiles([1] * 9, [12000] * 9, blocks=64, block_size=32)[0] == 0
+    # choices spread over very many blocks have little in common
+    assert _tiles([64], [1 << 20], blocks=64, block_size=16)[0] == 0
+    # parts of at most 1,022 blocks; partials stay below 1 GiB
+    n, parts, size = _tiles([512], [16384 * 4], blocks=256, block_size=16)
+    assert n == 8 and parts >= 5 and size < 1 << 30
+    assert _tiles([16384], [65536], blocks=256, block_size=16)[2] < 3 << 30
+
+
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("bs", [1, 3, 16, 100])
 @pytest.mark.parametrize("rows", [1, 3, 64, 600])
