@@ -1970,7 +1970,8 @@ int sparse_plan_impl(gllm_sparse_plan** out, const int32_t* query_lens, const in
 int sparse_check(const gllm_sparse_plan* p, int64_t num_blocks, const int32_t* block_table, int64_t block_table_stride) {
   if (!p) return fail(GLLM_ATTN_EINVAL, "null plan");
   if (!p->ws) return fail(GLLM_ATTN_EINVAL, "plan was not uploaded (gllm_sparse_plan_upload)");
-  if (!block_table || block_table_stride <= 0) return fail(GLLM_ATTN_EINVAL, "null block table, or block_table_stride <= 0");
+  if (!p->rows.empty() && (!block_table || block_table_stride <= 0))   // an empty table has no address
+    return fail(GLLM_ATTN_EINVAL, "null block table, or block_table_stride <= 0");
   if (num_blocks <= 0) return fail(GLLM_ATTN_EINVAL, "num_blocks must be > 0");
   if ((uint64_t)num_blocks * (uint64_t)p->bs >= (1ull << 32))
     return fail(GLLM_ATTN_EUNSUPPORTED, "pool of %lld blocks x %d slots exceeds 2^32 slots", (long long)num_blocks, p->bs);

@@ -231,14 +231,14 @@ hipError_t launch_key_bounds_values(const BoundsValuesArgs& a, hipStream_t st) {
 // [lo | hi]; the codes of q lie in the same order.  HBM- or L2-bound by the bounds of long
 // sequences.
 constexpr int kScoreWaves = 8;
-// The maximum over the lane's aligned run of gp = 1, 2, 4, 8 or 16 lanes.
-template <int gp>
-__device__ __forceinline__ int columns_max(int v) {
-  if (gp > 1) v = max(v, __builtin_amdgcn_mov_dpp(v, 0xb1, 0xf, 0xf, true));     // quad_perm 1 0 3 2
-  if (gp > 2) v = max(v, __builtin_amdgcn_mov_dpp(v, 0x4e, 0xf, 0xf, true));     // quad_perm 2 3 0 1
-  if (gp > 4) v = max(v, __builtin_amdgcn_mov_dpp(v, 0x141, 0xf, 0xf, true));    // the other half of 8
-  if (gp > 8) v = max(v, __builtin_amdgcn_mov_dpp(v, 0x140, 0xf, 0xf, true));    // and of 16
-  return v;
+// The maximum over lanes {l, l ^ 16} and {l, l ^ 32}.
+__device__ __forceinline__ int columns_max16(int v) {
+  const auto r = __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false);
+  return max((int)r[0], (int)r[1]);
+}
+__device__ __forceinline__ int columns_max32(int v) {
+  const auto r = __builtin_amdgcn_permlane32_swap((uint32_t)v, (uint32_t)v, false, false);
+  return max((int)r[0], (int)r[1]);
 }
 constexpr int kScorePF = 2;
 template <typename QT, int NK, int GP, bool PASSES>
@@ -351,7 +351,11 @@ __global__ void __launch_bounds__(64 * kScoreWaves) block_scores_kernel(SelectAr
     }
   };
   codes(0);
-  float* const sp = a.scores + ((int64_t)(tl.row0 + ri - a.row0) * Hkv + h) * a.score_stride;
+  // lane (n, grp) holds block n's sums with columns 4 grp .. + 3: NS rows of the tile from
+  // sr on, whose heads are in the lane (GP > 4: in it and its neighbours of the same n)
+  constexpr int NS = GP < 4 ? 4 / GP : 1;
+  const int sr = 4 * grp / GP;
+  float* const sp = a.scores + ((int64_t)(tl.row0 + sr - a.row0) * Hkv + h) * a.score_stride;
   const auto score = [&](int u, const Group& x) {
     int best[4] = {INT32_MIN, INT32_MIN, INT32_MIN, INT32_MIN};
     for (int p = 0; p < passes; ++p) {
@@ -359,21 +363,24 @@ __global__ void __launch_bounds__(64 * kScoreWaves) block_scores_kernel(SelectAr
       i32x4 acc = {0, 0, 0, 0};
 #pragma unroll
       for (int s = 0; s < NK; ++s)
-        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, x.box[s]), __builtin_bit_cast(i32x4, qb[s]), acc, 0, 0, 0);
-      const bool real = 16 * p + g0 < G;
+        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, qb[s]), __builtin_bit_cast(i32x4, x.box[s]), acc, 0, 0, 0);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) best[j] = max(best[j], real ? acc[j] : INT32_MIN);
+      for (int j = 0; j < 4; ++j) best[j] = PASSES ? max(best[j], acc[j]) : acc[j];   // columns past G repeat the last head
     }
-    f32x4 sc;
+    const int e = (int)(x.e >> (8 * (h & 3)) & 255u);
+    // bytes that no writer leaves are limited, so that the score stays a number
+    const float scale = pow2f(min(max(e - 128, -100), 100));
+    const int b = b0 + 16 * u + n;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int v = columns_max<GP>(best[j]);
-      const int e = __shfl((int)(x.e >> (8 * (h & 3)) & 255u), 4 * grp + j, 64);   // lane 4 grp + j holds block 4 grp + j's
-      // bytes that no writer leaves are limited, so that the score stays a number
-      sc[j] = e == kOpen ? -kNegInf : (float)v * pow2f(min(max(e - 128, -100), 100));
+    for (int i = 0; i < NS; ++i) {
+      int v = best[GP < 4 ? GP * i : 0];
+#pragma unroll
+      for (int j = 1; j < (GP < 4 ? GP : 4); ++j) v = max(v, best[(GP < 4 ? GP * i : 0) + j]);
+      if (GP > 4) v = columns_max16(v);
+      if (GP > 8) v = columns_max32(v);
+      if (sr + i < tl.nrows && (GP <= 4 || 4 * grp % GP == 0) && b < a.score_stride)
+        sp[(int64_t)i * Hkv * a.score_stride + b] = e == kOpen ? -kNegInf : (float)v * scale;
     }
-    const int b = b0 + 16 * u + 4 * grp;
-    if (row_ok && g0 == 0 && b < a.score_stride) *reinterpret_cast<f32x4*>(sp + b) = sc;   // rows are padded to 4
   };
   for (int c0 = 0; c0 < ng; c0 += 4 * NI) {
     const int nc = min(4 * NI, ng - c0);

@@ -261,8 +261,9 @@ def sparse_attention(plan: SparsePlan, q: torch.Tensor, k_cache: torch.Tensor, v
     q and out as in :func:`gllm_amd.paged_attention` (q rotated), ``selected`` int32
     ``[rows, Hkv, blocks]`` from :func:`select_blocks` or any other choice: a list ends
     at the first entry that is negative, not above the entry before it, or behind
-    the row's own block.  A row without blocks gives zeros.  Keys that some row of
-    a sequence sees must be finite.  Returns ``out``.
+    the row's own block.  A row without blocks gives zeros.  A selected block's keys
+    and values up to the position of the sequence's last row must be finite, those that
+    rows before it do not see too.  Returns ``out``.
     """
     index = plan.index
     if index >= 0 and _current_device() != index:

@@ -136,6 +136,29 @@ def test_bounds_of_special_values():
         assert torch.equal(rec[blk[j] // bs, :len(x)].cpu(), x), f"block {j}"
 
 
+@pytest.mark.parametrize("dtype,kv", [(BF, BF), (F16, F16), (BF, F8), (F16, F32), (BF, "4")])
+def test_one_nan_opens_its_block_and_head(dtype, kv):
+    """In every type of cache: bounds of the other blocks and heads stay as they were.  F16
+    over a float32 cache: a key that fp16 holds as infinity."""
+    bs, Hkv, D = 16, 4, 64
+    b = Batch([0, 5], [bs * 4, 40], Hq=Hkv, Hkv=Hkv, D=D, dtype=dtype, bs=bs, kv=kv)
+    plan, kc, bt = plan_of(b, 4), b.kc.cuda(), b.bt.cuda()
+    before, after = sparse.new_key_bounds(b.nb, Hkv, D, "cuda"), sparse.new_key_bounds(b.nb, Hkv, D, "cuda")
+    sparse.write_key_bounds(plan, kc, before, bt)
+    blk = int(b.bt[0, 2])
+    if kv == "4":
+        kc[blk, 1, bs * D // 2 + 7 * D // 32 + 1] = 255      # the scale of dims 32-63 of key 7
+    elif kv == F8:
+        kc.view(torch.uint8)[blk * bs + 7, 1, 33] = 0x7F
+    else:
+        kc[blk * bs + 7, 1, 33] = 1e6 if kv == F32 else math.nan
+    sparse.write_key_bounds(plan, kc, after, bt)
+    want = before.clone()
+    want[blk, 1 * 2 * D:2 * 2 * D] = 0
+    want[blk, Hkv * 2 * D + 1] = 255
+    assert torch.equal(after, want)
+
+
 # ---------------------------------------------------------------- selection
 def check_selection(b, rec, bounds, blocks, first, recent, padded=True):
     plan = plan_of(b, blocks, first, recent)
@@ -566,4 +589,8 @@ def test_empty_batch():
     sparse.write_key_bounds(plan, kc, bounds, bt)
     sel = sparse.select_blocks(plan, q, bounds, bt)
     assert sel.shape == (0, 2, 3) and sparse.sparse_attention(plan, q, kc, kc, bt, sel).shape == q.shape
+    for none in (bt[:0], bt[:0, :0]):
+        sparse.write_key_bounds(plan, kc, bounds, none)
+        sel = sparse.select_blocks(plan, q, bounds, none)
+        assert sel.shape == (0, 2, 3) and sparse.sparse_attention(plan, q, kc, kc, none, sel).shape == q.shape
     assert sparse.key_bounds_values(bounds, torch.zeros(0, dtype=torch.int64, device="cuda"), 2, 64).shape == (0, 2, 2, 64)
