@@ -202,6 +202,7 @@ struct gllm_sparse_plan {
   std::vector<BoundsBlock> blocks;
   std::vector<ScoreItem> items;
   int64_t n_tiles = 0;
+  int32_t row_tiles = 1;                      // 16-column tiles of rows that one item takes
   // rows are scored and selected a slab at a time, so that the scores' place stays bounded
   struct Slab { int32_t row0, n_rows, item0, n_items, max_blocks; };
   std::vector<Slab> slabs;
@@ -1842,7 +1843,9 @@ int sparse_plan_impl(gllm_sparse_plan** out, const int32_t* query_lens, const in
   const int G = Hq / Hkv;
   int gp = 1;
   while (gp < G && gp < 16) gp *= 2;
-  const int tile_rows = 16 / gp;
+  // (larger heads have no registers for a second tile, larger groups take them in passes)
+  if (num_seqs > 0 && G <= 16 && D <= 128 && *std::max_element(query_lens, query_lens + num_seqs) > 16 / gp) p->row_tiles = kScoreRowTiles;
+  const int tile_rows = p->row_tiles * (16 / gp);
   int64_t row = 0, keys = 0, scored = 0;
   for (int i = 0; i < num_seqs; ++i) {
     const int32_t ql = query_lens[i], sl = seq_lens[i];
@@ -1889,9 +1892,9 @@ int sparse_plan_impl(gllm_sparse_plan** out, const int32_t* query_lens, const in
       r = e;
     }
     p->n_tiles += (int64_t)tiles.size();
-    // a tile's groups in equal items: as many items as run at once, two a CU (more tiles
-    // than that: as many as fill the rounds that the tiles need)
-    const int64_t slots = 2 * (int64_t)device_cus() * hw / Hkv;
+    // a tile's groups in equal items: as many items as run at once, two a CU (one where row
+    // tiles take the registers; more tiles than that: as many as fill the rounds that they need)
+    const int64_t slots = (p->row_tiles > 1 && D > 64 ? 1 : 2) * (int64_t)device_cus() * hw / Hkv;
     const int64_t room = std::max<int64_t>(1, slots) * std::max<int64_t>(1, ((int64_t)tiles.size() + slots) / std::max<int64_t>(1, slots));
     const auto count = [&](int64_t len) {
       int64_t n = 0;
@@ -2072,6 +2075,7 @@ int gllm_select_blocks(const gllm_sparse_plan* p, const void* q, int64_t q_row_s
   a.selected = selected; a.width = p->width; a.first = p->first; a.recent = p->recent;
   block_div(p->bs, &a.block_magic, &a.block_shift);
   a.num_q_heads = p->Hq; a.num_kv_heads = p->Hkv; a.head_dim = p->D; a.dtype = dtype;
+  a.row_tiles = p->row_tiles;
   for (const gllm_sparse_plan::Slab& sb : p->slabs) {
     a.row0 = sb.row0; a.n_rows = sb.n_rows; a.item0 = sb.item0; a.n_items = sb.n_items; a.max_blocks = sb.max_blocks;
     if (int rc = hip_check(launch_select_blocks(a, (hipStream_t)stream), "block selection launch")) return rc;

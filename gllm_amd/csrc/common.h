@@ -475,11 +475,12 @@ struct BoundsBlock {
   int32_t seq, block, n, pad;
 };
 // Up to 16 / (heads of a kv head, rounded up to a power of two) query rows of one
-// sequence, sparse_rows[row0 .. row0 + nrows), scored together against 16-block groups
+// sequence (prompts: kScoreRowTiles times as many), sparse_rows[row0 .. row0 + nrows), scored together against 16-block groups
 // group0 .. group0 + groups - 1 of the nblocks blocks that the last of them sees.
 struct ScoreItem {
   int32_t row0, nrows, seq, nblocks, group0, groups;
 };
+constexpr int kScoreRowTiles = 2;
 // kv heads that a workgroup of the score kernel takes: 8 waves, a head each or several
 // waves a head.
 __host__ __device__ inline int score_heads(int num_kv_heads) {

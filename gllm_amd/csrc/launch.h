@@ -188,6 +188,7 @@ struct SelectArgs {
   const ScoreItem* items;      // items [item0, item0 + n_items) score the rows [row0, row0 + n_rows)
   int32_t row0, n_rows, item0, n_items;
   int32_t max_blocks;          // the most that a row of them sees
+  int32_t row_tiles;           // 1, or kScoreRowTiles if an item may have so many times 16 / GP rows
   float* scores;               // [n_rows, Hkv, score_stride]
   int64_t score_stride;
   int32_t* selected;           // [rows, Hkv, width]

@@ -224,12 +224,17 @@ hipError_t launch_key_bounds_values(const BoundsValuesArgs& a, hipStream_t st) {
 // ---------------------------------------------------------------- scores
 // One 8-wave workgroup per (item: a tile of query rows and a run of 16-block groups; HW
 // kv heads); a wave takes one of the heads and its share of the groups, two groups'
-// loads ahead.  The plan cuts tiles into items that end together, two a CU.   A column of the
-// MFMA is a (row of the tile, head of the group) pair, n = row x Gp + g with Gp = G
-// rounded up to a power of two, so a tile's rows share the bounds they load; more than 16
-// heads go by in passes.  Lane (n, grp) loads bytes 64 s + 16 grp .. + 15 of block n's
-// [lo | hi]; the codes of q lie in the same order.  HBM- or L2-bound by the bounds of long
-// sequences.
+// loads ahead.  A column of the MFMA is a (row of the tile, head of the group) pair, n = row x
+// GP + g with GP = G rounded up to a power of two (columns past G repeat the last head), so
+// a tile's rows share the bounds they load; more than 16 heads go by in passes.  Lane (n, grp)
+// loads bytes 64 s + 16 grp .. + 15 of block n's [lo | hi]; the codes of q lie in the same
+// order.  Blocks are the product's columns, so a lane has one block's scale and up to four
+// heads of a row to reduce.
+// Decode rows are HBM-bound (64 rows on 8,192-32,768 keys, blocks of 16: 170 MB in 33 us
+// from cache, ~44 from HBM).  Prompt rows are bound by the CU's loads, which take the 16
+// records of an instruction one by one; RT = 2 tiles of 16 columns on the same loads, one
+// workgroup a CU for its registers, cut 840 rows on 8,192-16,384 keys, blocks of 32, from 28.2
+// to 19.9 us (four: 20.2).
 constexpr int kScoreWaves = 8;
 // The maximum over lanes {l, l ^ 16} and {l, l ^ 32}.
 __device__ __forceinline__ int columns_max16(int v) {
@@ -241,8 +246,8 @@ __device__ __forceinline__ int columns_max32(int v) {
   return max((int)r[0], (int)r[1]);
 }
 constexpr int kScorePF = 2;
-template <typename QT, int NK, int GP, bool PASSES>
-__global__ void __launch_bounds__(64 * kScoreWaves) block_scores_kernel(SelectArgs a, int hw) {
+template <typename QT, int NK, int GP, int RT, bool PASSES>
+__global__ void __launch_bounds__(64 * kScoreWaves) __attribute__((amdgpu_waves_per_eu(NK == 8 || RT > 1 || PASSES ? 2 : 4))) block_scores_kernel(SelectArgs a, int hw) {
   const int lane = threadIdx.x & 63, n = lane & 15, grp = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int D = a.head_dim, G = a.num_q_heads / a.num_kv_heads, Hkv = a.num_kv_heads;
@@ -254,9 +259,21 @@ __global__ void __launch_bounds__(64 * kScoreWaves) block_scores_kernel(SelectAr
   const int b0 = (tl.group0 + first) * 16;
   const int ng = min(share, tl.groups - first);
   if (ng <= 0) return;
-  const int ri = n / GP, g0 = n % GP;
-  const bool row_ok = ri < tl.nrows;
-  const int row = a.rows[tl.row0 + (row_ok ? ri : 0)].row;
+  static_assert(RT == 1 || !PASSES, "heads or rows fill the columns");
+  constexpr int TR = 16 / GP;                            // rows of 16 columns
+  const int g0 = n % GP, nt = RT == 1 ? 1 : (tl.nrows + TR - 1) / TR;
+  static_assert(RT <= 2, "tile indexes are compile-time constants");
+  const auto each_tile = [&](auto f) {
+    f(std::integral_constant<int, 0>());
+    if constexpr (RT > 1) f(std::integral_constant<int, 1>());
+  };
+  bool row_ok[RT];
+  int row[RT];
+  each_tile([&](auto t) {
+    const int ri = t * TR + n / GP;
+    row_ok[t] = ri < tl.nrows;
+    row[t] = a.rows[tl.row0 + (row_ok[t] ? ri : 0)].row;
+  });
   const int passes = PASSES ? (G + 15) / 16 : 1;
   // a byte of the word that is loaded (a byte load's value is widened where the loop ends,
   // which waits for every load in flight)
@@ -291,43 +308,29 @@ __global__ void __launch_bounds__(64 * kScoreWaves) block_scores_kernel(SelectAr
   // lane's dims of the lo half are those of its hi half where 64 divides D.
   constexpr int NH = NK / 2;
   const bool folded = D == 32 * NK && D % 64 == 0;
-  const auto q_at = [&](int p) {
-    return (const QT*)a.q + (int64_t)row * a.q_row_stride + (int64_t)(h * G + min(16 * p + g0, G - 1)) * D;
+  const auto q_at = [&](auto t, int p) {
+    return (const QT*)a.q + (int64_t)row[t] * a.q_row_stride + (int64_t)(h * G + min(16 * p + g0, G - 1)) * D;
   };
   const auto dim_at = [&](int s) {                       // first dim of the lane's s-th 8 bytes
     const int k = 64 * (s / 2) + 16 * grp + 8 * (s % 2);
     return min(k < D ? k : k - D, D - 8);
   };
-  uint32_t m = 0u;
   float x[2 * NH][8];
-  const auto load_half = [&](int p, int half) {
-    const QT* qp = q_at(p);
+  const auto load_half = [&](auto t, int p, int half) {
+    const QT* qp = q_at(t, p);
 #pragma unroll
     for (int s = 0; s < 2 * NH; ++s) load8<QT>(qp + dim_at(s + half * 2 * NH), x[s]);
   };
-  load_half(0, 0);
+  load_half(std::integral_constant<int, 0>(), 0, 0);
   __builtin_amdgcn_sched_barrier(0);                     // q first: its codes are made while bounds are on their way
 #pragma unroll
   for (int u = 0; u < kScorePF; ++u) issue(u, ring[u]);
   __builtin_amdgcn_sched_barrier(0);
-  for (int p = 0; p < passes; ++p) {
-    for (int half = 0; half < (folded ? 1 : 2); ++half) {
-      if (p + half > 0) load_half(p, half);
-#pragma unroll
-      for (int s = 0; s < 2 * NH; ++s)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) m = max(m, magnitude(x[s][i]));
-    }
-  }
-  m = max(m, (uint32_t)__shfl_xor((int)m, 16, 64));
-  m = max(m, (uint32_t)__shfl_xor((int)m, 32, 64));
-#pragma unroll
-  for (int s = 1; s < GP; s *= 2) m = max(m, (uint32_t)__shfl_xor((int)m, s, 64));
-  const bool none = !row_ok || m > kCodeMax;
-  const float inv = m > kCodeMax ? 0.f : pow2f(-code_exponent(m));
-  u32x4 qb[NK];
-  const auto codes = [&](int p) {
-    const QT* qp = q_at(p);
+  bool none[RT];
+  float inv[RT];
+  u32x4 qb[RT][NK];
+  const auto codes = [&](auto t, int p) {
+    const QT* qp = q_at(t, p);
 #pragma unroll
     for (int s = 0; s < 2 * NK; ++s) {
       const int k = 64 * (s / 2) + 16 * grp + 8 * (s % 2);
@@ -342,45 +345,66 @@ __global__ void __launch_bounds__(64 * kScoreWaves) block_scores_kernel(SelectAr
       uint32_t w[2] = {0u, 0u};
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float c = __builtin_rintf(v[i] * inv), c1 = lo ? fminf(c, 0.f) : fmaxf(c, 0.f);
+        const float c = __builtin_rintf(v[i] * inv[t]), c1 = lo ? fminf(c, 0.f) : fmaxf(c, 0.f);
         w[i / 4] = __builtin_amdgcn_cvt_pk_u8_f32(c1 + 128.f, i % 4, w[i / 4]);
       }
       // code + 128 as a byte is the code's with the top bit turned
-      qb[s / 2][2 * (s % 2)] = none || k >= 2 * D ? 0u : w[0] ^ 0x80808080u;
-      qb[s / 2][2 * (s % 2) + 1] = none || k >= 2 * D ? 0u : w[1] ^ 0x80808080u;
+      qb[t][s / 2][2 * (s % 2)] = none[t] || k >= 2 * D ? 0u : w[0] ^ 0x80808080u;
+      qb[t][s / 2][2 * (s % 2) + 1] = none[t] || k >= 2 * D ? 0u : w[1] ^ 0x80808080u;
     }
   };
-  codes(0);
+  each_tile([&](auto t) {
+    uint32_t m = 0u;
+    for (int p = 0; p < passes; ++p) {
+      for (int half = 0; half < (folded ? 1 : 2); ++half) {
+        if (t + p + half > 0) load_half(t, p, half);
+#pragma unroll
+        for (int s = 0; s < 2 * NH; ++s)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) m = max(m, magnitude(x[s][i]));
+      }
+    }
+    m = max(m, (uint32_t)__shfl_xor((int)m, 16, 64));
+    m = max(m, (uint32_t)__shfl_xor((int)m, 32, 64));
+#pragma unroll
+    for (int s = 1; s < GP; s *= 2) m = max(m, (uint32_t)__shfl_xor((int)m, s, 64));
+    none[t] = !row_ok[t] || m > kCodeMax;
+    inv[t] = m > kCodeMax ? 0.f : pow2f(-code_exponent(m));
+    codes(t, 0);
+  });
   // lane (n, grp) holds block n's sums with columns 4 grp .. + 3: NS rows of the tile from
   // sr on, whose heads are in the lane (GP > 4: in it and its neighbours of the same n)
   constexpr int NS = GP < 4 ? 4 / GP : 1;
   const int sr = 4 * grp / GP;
   float* const sp = a.scores + ((int64_t)(tl.row0 + sr - a.row0) * Hkv + h) * a.score_stride;
   const auto score = [&](int u, const Group& x) {
-    int best[4] = {INT32_MIN, INT32_MIN, INT32_MIN, INT32_MIN};
-    for (int p = 0; p < passes; ++p) {
-      if (PASSES) codes(p);
-      i32x4 acc = {0, 0, 0, 0};
-#pragma unroll
-      for (int s = 0; s < NK; ++s)
-        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, qb[s]), __builtin_bit_cast(i32x4, x.box[s]), acc, 0, 0, 0);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) best[j] = PASSES ? max(best[j], acc[j]) : acc[j];   // columns past G repeat the last head
-    }
     const int e = (int)(x.e >> (8 * (h & 3)) & 255u);
     // bytes that no writer leaves are limited, so that the score stays a number
     const float scale = pow2f(min(max(e - 128, -100), 100));
     const int b = b0 + 16 * u + n;
+    each_tile([&](auto t) {
+      if (t > 0 && t >= nt) return;
+      int best[4] = {INT32_MIN, INT32_MIN, INT32_MIN, INT32_MIN};
+      for (int p = 0; p < passes; ++p) {
+        if (PASSES) codes(t, p);
+        i32x4 acc = {0, 0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < NS; ++i) {
-      int v = best[GP < 4 ? GP * i : 0];
+        for (int s = 0; s < NK; ++s)
+          acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, qb[t][s]), __builtin_bit_cast(i32x4, x.box[s]), acc, 0, 0, 0);
 #pragma unroll
-      for (int j = 1; j < (GP < 4 ? GP : 4); ++j) v = max(v, best[(GP < 4 ? GP * i : 0) + j]);
-      if (GP > 4) v = columns_max16(v);
-      if (GP > 8) v = columns_max32(v);
-      if (sr + i < tl.nrows && (GP <= 4 || 4 * grp % GP == 0) && b < a.score_stride)
-        sp[(int64_t)i * Hkv * a.score_stride + b] = e == kOpen ? -kNegInf : (float)v * scale;
-    }
+        for (int j = 0; j < 4; ++j) best[j] = PASSES ? max(best[j], acc[j]) : acc[j];   // columns past G repeat the last head
+      }
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        int v = best[GP < 4 ? GP * i : 0];
+#pragma unroll
+        for (int j = 1; j < (GP < 4 ? GP : 4); ++j) v = max(v, best[(GP < 4 ? GP * i : 0) + j]);
+        if (GP > 4) v = columns_max16(v);
+        if (GP > 8) v = columns_max32(v);
+        if (t * TR + sr + i < tl.nrows && (GP <= 4 || 4 * grp % GP == 0) && b < a.score_stride)
+          sp[(int64_t)(t * TR + i) * Hkv * a.score_stride + b] = e == kOpen ? -kNegInf : (float)v * scale;
+      }
+    });
   };
   for (int c0 = 0; c0 < ng; c0 += 4 * NI) {
     const int nc = min(4 * NI, ng - c0);
@@ -637,7 +661,10 @@ static hipError_t launch_scores_t(const SelectArgs& a, int hw, dim3 grid, hipStr
   const int nk = (2 * a.head_dim + 63) / 64;
   const auto go = [&](auto n, auto gp, auto pass) {
     constexpr int NK = decltype(n)::value, GP = decltype(gp)::value;
-    hipLaunchKernelGGL((block_scores_kernel<QT, NK, GP, decltype(pass)::value>), grid, block, 0, st, a, hw);
+    constexpr bool PASSES = decltype(pass)::value;
+    constexpr int RT = PASSES || NK == 8 ? 1 : kScoreRowTiles;
+    if (RT == 1 || a.row_tiles == 1) hipLaunchKernelGGL((block_scores_kernel<QT, NK, GP, 1, PASSES>), grid, block, 0, st, a, hw);
+    else hipLaunchKernelGGL((block_scores_kernel<QT, NK, GP, RT, PASSES>), grid, block, 0, st, a, hw);
   };
   const auto by_group = [&](auto n) {
     const int G = a.num_q_heads / a.num_kv_heads;

@@ -185,6 +185,15 @@ def test_selection_is_the_oracles(Hq, Hkv, D, dtype, bs, blocks, first, recent):
     check_selection(b, *all_bounds(b), blocks, first, recent)
 
 
+@pytest.mark.parametrize("Hq,Hkv,D,dtype", [(4, 4, 64, BF), (4, 2, 128, F16), (12, 4, 128, BF), (8, 2, 64, BF), (8, 1, 128, F32),
+                                            (20, 2, 40, F16), (16, 1, 96, BF), (20, 1, 64, BF), (8, 2, 256, BF)])
+def test_selection_of_prompt_rows_in_tiles(Hq, Hkv, D, dtype):
+    """Prompts of every remainder of a tile's rows beside single rows, in one plan."""
+    b = Batch([400, 300, 250, 500, 260, 333, 290], [1, 31, 5, 1, 17, 3, 66], Hq=Hq, Hkv=Hkv, D=D, dtype=dtype, bs=4, seed=Hq + D)
+    rec, bounds = all_bounds(b)
+    check_selection(b, rec, bounds, 9, 1, 2)
+
+
 def test_selection_of_padded_rows_and_strided_tensors():
     b = Batch([300, 0, 500], [2, 1, 4], Hq=8, Hkv=2, D=64, bs=16, stride=5)
     rec, bounds = all_bounds(b, extra=48)
