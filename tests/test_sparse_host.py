@@ -83,9 +83,12 @@ def test_plan_facts():
     assert i["rows"] == i["query_rows"] == 44 and i["slabs"] == 1
     # the last key's block; keys 4997 .. 4999 (block 312); 4056 .. 4095 (blocks 253 .. 255)
     assert i["blocks"] == 1 + 1 + 3
-    # 4 rows a tile at G = 4; the first sequence has 7 blocks, all selected
-    assert i["tiles"] == 1 + 10
-    assert _info([1, 3, 40], [100, 5000, 4096], Hq=8)["tiles"] == 1 + 3       # 16 rows a tile
+    # 4 rows a tile at G = 4, twice as many where a sequence has more; the first has 7 blocks,
+    # all selected
+    assert i["tiles"] == 1 + 5
+    assert _info([1, 3, 4], [100, 5000, 4096])["tiles"] == 1 + 1
+    assert _info([1, 3, 40], [100, 5000, 4096], Hq=8)["tiles"] == 1 + 2       # 16 rows
+    assert _info([1, 3, 40], [100, 5000, 4096], D=192)["tiles"] == 1 + 10
     assert _info([1, 3, 40], [100, 5000, 4096], Hq=256)["tiles"] == 3 + 40
     assert _info([1, 3, 40], [100, 5000, 4096], blocks=400)["tiles"] == 0
     assert _info([3, 1], [10, 20], stride=5) | {"bytes": 0} == dict(rows=10, query_rows=4, blocks=2, tiles=0, slabs=1, splits=1, bytes=0)
