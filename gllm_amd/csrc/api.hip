@@ -208,15 +208,17 @@ struct gllm_sparse_plan {
   std::vector<Slab> slabs;
   int64_t score_stride = 0;
   // MFMA kernels: rows on their own (each in `splits` parts), and prompt rows in tiles
-  // (tile_splits parts each); the generic kernel takes `rows`
+  // (their keys dealt to tile_wgs workgroups); the generic kernel takes `rows`
   std::vector<SparseRow> lone, tile_rows;
   std::vector<SparseTile> tiles;
-  int32_t splits = 1, tile_splits = 1, tile_capacity = 0;
+  int32_t splits = 1, tile_wgs = 0, tile_round = 1, tile_capacity = 0;
+  int64_t tile_slots = 0;                     // partials of tile_cols columns
+  int32_t tile_cols = 0;
   void* pinned = nullptr;
   size_t pinned_cap = 0;
   bool pinned_is_host_malloc = false;
   size_t off_rows = 0, off_blocks = 0, off_items = 0, off_scores = 0, off_ml = 0, off_part = 0, ws_bytes = 0, stage_bytes = 0;
-  size_t off_lone = 0, off_tile_rows = 0, off_tiles = 0, off_entries = 0, off_keys = 0, off_tile_ml = 0, off_tile_part = 0;
+  size_t off_lone = 0, off_tile_rows = 0, off_tiles = 0, off_entries = 0, off_keys = 0, off_parts = 0, off_tile_ml = 0, off_tile_part = 0;
   char* ws = nullptr;
   hipEvent_t upload_done = nullptr;
 };
@@ -1770,8 +1772,7 @@ void plan_sparse_tiles(gllm_sparse_plan* p, const int32_t* query_lens, const int
     const double cols = (rows * G + 31) / 32 * 32;
     return 64 * std::max(key * cols / (p->D == 128 ? 3.2e12 : 2.4e12), key / 30e9) * (nb * share * p->bs / 64);
   };
-  double total = 0, longest = 0;
-  int64_t r0 = 0;
+  int64_t all = 0, r0 = 0;                     // 64-key tiles at most
   for (int i = 0; i < p->num_seqs; r0 += query_lens[i++]) {
     const int32_t ql = query_lens[i], c = seq_lens[i] - ql;
     const int n = (ql + most - 1) / most;
@@ -1789,35 +1790,33 @@ void plan_sparse_tiles(gllm_sparse_plan* p, const int32_t* query_lens, const int
       const int64_t a = (int64_t)ql * t / n, e = (int64_t)ql * (t + 1) / n;
       const int32_t nb = (int32_t)((c + e - 1) / p->bs + 1);
       p->tiles.push_back({(int32_t)p->tile_rows.size(), (int32_t)(e - a), i, 0});
-      p->tile_rows.insert(p->tile_rows.end(), p->rows.begin() + r0 + a, p->rows.begin() + r0 + e);
-      p->tile_capacity = (int32_t)std::max<int64_t>(p->tile_capacity, std::min<int64_t>(nb, (e - a) * p->width));
-      total += tile_time((int)(e - a), nb);
-      longest = std::max(longest, tile_time((int)(e - a), nb));
+      for (int64_t r = a; r < e; ++r) {
+        p->tile_rows.push_back(p->rows[(size_t)(r0 + r)]);
+        p->tile_rows.back().pad = (int32_t)p->tiles.size() - 1;
+      }
+      const int64_t most_blocks = std::min<int64_t>(nb, (e - a) * p->width);
+      p->tile_capacity = (int32_t)std::max<int64_t>(p->tile_capacity, most_blocks);
+      all += p->Hkv * ((most_blocks * p->bs + 63) / 64);
     }
   }
   if (p->tiles.empty()) return;
-  // Parts of a tile's keys: what ends soonest with a workgroup per CU, a partial's write
-  // and read at 3 TB/s; the ids, rows and numbers of at most 1,022 blocks fit a workgroup.
-  const int64_t cus = device_cus(), units = (int64_t)p->tiles.size() * p->Hkv;
-  const int64_t least = ((int64_t)p->tile_capacity * p->bs + 1022 * (int64_t)p->bs - 65) / (1022 * (int64_t)p->bs - 64);
-  double best = 0;
-  for (int64_t s = least; s <= std::max<int64_t>(least, 16); ++s) {
-    const double round = std::max(total * p->Hkv / (double)units, 0.7 * longest) / (double)s + 6e-6;
-    const double join = s > 1 ? 4e-6 + (double)p->tile_rows.size() * p->Hq * s * p->D * 8 / 3e12 : 0;
-    const double t = (double)((units * s + cus - 1) / cus) * round + join;
-    if (s == least || t < best) {
-      best = t;
-      p->tile_splits = (int32_t)s;
-    }
-  }
-  // partials past 1 GiB, or too many workgroups: rows on their own
-  if (units * p->tile_splits > INT32_MAX ||
-      (p->tile_splits > 1 && (int64_t)p->tile_rows.size() * p->Hq * p->tile_splits * p->D * 4 > int64_t(1) << 30)) {
+  // Equal runs of the units' keys, one a CU, or as many more as leave a run the ids, rows
+  // and numbers of 1,022 blocks that a workgroup holds.  A run's first and last unit may be
+  // parts: a slot for each (fewer units than runs: one a run and one a unit).
+  const int64_t cus = device_cus(), units = (int64_t)p->tiles.size() * p->Hkv, most_tiles = 1022 * (int64_t)p->bs / 64;
+  const int64_t wgs = std::min(std::max<int64_t>(1, all / 4),   // of four tiles at least
+                               cus * std::max<int64_t>(1, (all + cus * most_tiles - 1) / (cus * most_tiles)));
+  p->tile_cols = most * G;
+  p->tile_slots = wgs + std::min(wgs, units);
+  p->tile_wgs = (int32_t)std::min<int64_t>(wgs, INT32_MAX);
+  p->tile_round = (int32_t)cus;
+  // partials past 1 GiB, or too many tiles to count: rows on their own
+  if (all > INT32_MAX || units > INT32_MAX || p->tile_slots > (int64_t(1) << 30) / ((int64_t)p->tile_cols * p->D * 4)) {
     p->lone = p->rows;
     p->tiles.clear();
     p->tile_rows.clear();
-    p->tile_capacity = 0;
-    p->tile_splits = 1;
+    p->tile_capacity = p->tile_wgs = 0;
+    p->tile_slots = 0;
   }
 }
 
@@ -1938,7 +1937,7 @@ int sparse_plan_impl(gllm_sparse_plan** out, const int32_t* query_lens, const in
     p->splits = (int32_t)s;
   }
   const size_t parts = p->splits > 1 ? p->lone.size() * Hkv * p->splits : 0;
-  const size_t tile_parts = p->tile_splits > 1 ? p->tile_rows.size() * Hkv * p->tile_splits : 0;
+  const size_t tile_parts = (size_t)p->tile_slots * p->tile_cols;
   const size_t tile_units = p->tiles.size() * (size_t)Hkv;
   size_t o = 0;
   p->off_rows = o; o = align256(o + p->rows.size() * sizeof(SparseRow));
@@ -1950,8 +1949,9 @@ int sparse_plan_impl(gllm_sparse_plan** out, const int32_t* query_lens, const in
   p->stage_bytes = o;
   p->off_entries = o; o = align256(o + tile_units * p->tile_capacity * sizeof(SelectedBlock));
   p->off_keys = o; o = align256(o + tile_units * sizeof(int32_t));
-  p->off_tile_ml = o; o = align256(o + tile_parts * G * 2 * sizeof(float));
-  p->off_tile_part = o; o = align256(o + tile_parts * G * D * sizeof(float));
+  p->off_parts = o; o = align256(o + tile_units * sizeof(TileParts));
+  p->off_tile_ml = o; o = align256(o + tile_parts * 2 * sizeof(float));
+  p->off_tile_part = o; o = align256(o + tile_parts * D * sizeof(float));
   p->off_scores = o; o = align256(o + (size_t)(slab_rows * per_row));
   p->off_ml = o; o = align256(o + parts * 16 * 2 * sizeof(float));
   p->off_part = o; o = align256(o + parts * 16 * D * sizeof(float));
@@ -2016,7 +2016,7 @@ int gllm_sparse_plan_upload(gllm_sparse_plan* p, void* workspace, size_t bytes, 
 int gllm_sparse_plan_info(const gllm_sparse_plan* p, int64_t* info, int32_t n) {
   if (!p || !info) return fail(GLLM_ATTN_EINVAL, "null plan or info");
   const int64_t v[8] = {p->total_rows, (int64_t)p->rows.size(), (int64_t)p->blocks.size(), p->n_tiles,
-                        (int64_t)p->slabs.size(), p->splits, (int64_t)p->tiles.size(), p->tile_splits};
+                        (int64_t)p->slabs.size(), p->splits, (int64_t)p->tiles.size(), p->tile_wgs};
   for (int i = 0; i < n && i < 8; ++i) info[i] = v[i];
   return ok();
 }
@@ -2122,7 +2122,8 @@ int gllm_sparse_attention(const gllm_sparse_plan* p, const void* q, int64_t q_ro
     t.tile_entries = (SelectedBlock*)(p->ws + p->off_entries);
     t.tile_keys = (int32_t*)(p->ws + p->off_keys);
     t.tile_capacity = p->tile_capacity;
-    t.tile_splits = t.sparse_splits = p->tile_splits;
+    t.tile_parts = (TileParts*)(p->ws + p->off_parts);
+    t.tile_wgs = p->tile_wgs; t.tile_round = p->tile_round; t.tile_cols = p->tile_cols;
     t.partial_ml = (float*)(p->ws + p->off_tile_ml);
     t.partials = (float*)(p->ws + p->off_tile_part);
     if (int rc = hip_check(launch_tile_blocks(t, st), "sparse attention tiles")) return rc;

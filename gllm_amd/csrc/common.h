@@ -455,7 +455,7 @@ struct SparseRow {
   int32_t row, seq, pos, pad;
 };
 // Prompt rows of sparse attention that are taken together: nrows (at most 64) of one
-// sequence, tile_rows[row0 ..].
+// sequence, tile_rows[row0 ..], whose pad is the tile's index.
 struct SparseTile {
   int32_t row0, nrows, seq, pad;
 };
@@ -464,10 +464,16 @@ struct SelectedBlock {
   uint64_t rows;
   int32_t number, block;        // in the sequence, in the pool
 };
-// One workgroup's part of a tile: keys [k0, k1) of its entries' blocks, one after another.
+// One workgroup's part of a tile: keys [k0, k1) of its entries' blocks, one after another;
+// slot: of its partials (-1: it has all of the tile's keys).
 struct SelectedTile {
   const SelectedBlock* entries;
-  int32_t row0, nrows, k0, k1, ord, parts;
+  int32_t row0, nrows, k0, k1, slot;
+};
+// The partials of a (kv head, tile): slot first, then rest, rest + step, ... (count in all;
+// 1: none, the output is written).
+struct TileParts {
+  int32_t first, rest, step, count;
 };
 // A cache block whose first n keys have bounds to be written: block `block` of
 // sequence seq.

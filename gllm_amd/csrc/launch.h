@@ -154,7 +154,9 @@ struct AttnArgs {
   const SparseRow* tile_rows;
   SelectedBlock* tile_entries;
   int32_t* tile_keys;
-  int32_t n_sparse_tiles, tile_capacity, tile_splits;
+  TileParts* tile_parts;       // [Hkv][tiles]
+  int32_t n_sparse_tiles, tile_capacity;
+  int32_t tile_wgs, tile_round, tile_cols;   // workgroups that share the tiles' keys (a CU each a round), columns of a partial
 };
 
 // Key bounds, block scores and the selection (sparse_select.hip)

@@ -856,7 +856,10 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
   constexpr int CPR = D / 8;               // 16-byte chunks per key row
   constexpr int NT = 64 * NW;              // threads per workgroup
   int32_t* const lbid = reinterpret_cast<int32_t*>(lds + 2 * Cfg::kStages * Cfg::kTile);
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  int tid = threadIdx.x;
+  // SELT runs in a loop: what depends on the lane is made anew, not kept across it
+  if constexpr (SELT) asm volatile("v_mov_b32 %0, %1" : "=v"(tid) : "v"((int)threadIdx.x));
+  const int wave = tid >> 6, lane = tid & 63;
   const int n = lane & 31, h = lane >> 5;
 
   int ctx, qlen, TK;
@@ -1605,7 +1608,7 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
     }
   }
 
-  if (PFX || (SELT && sx->parts > 1)) {
+  if (PFX || (SELT && sx->slot >= 0)) {
     // the row's state: reference (log2 units), sum and unnormalised output
     const float lt = sum_xor32(lsum);
     if (row_ok) {
@@ -1615,7 +1618,7 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
         const MergeInfo mi = a.merge[pr.seq * a.head_groups + hg];
         at = ((int64_t)mi.pbase + (int64_t)(kvh - hg * a.heads_per_wg) * mi.count + px->ord) * 16 + pr.r * G + g;
       } else {
-        at = (((int64_t)(sx->row0 + rr) * a.num_kv_heads + kvh) * sx->parts + sx->ord) * G + g;
+        at = (int64_t)sx->slot * a.tile_cols + rr * G + g;
       }
       float* pa = a.partials + at * D + 4 * h;
 #pragma unroll
@@ -1873,67 +1876,120 @@ sparse_attn_kernel(AttnArgs a) {
     a.partial_ml[2 * at + 1] = 0.f;
   }
 }
-// Sparse attention of prompt rows: one workgroup per (tile of a sequence's rows, kv
-// head, part of the keys that the tile's rows selected).  A tile's rows share each K/V
-// tile, and MFMAs have all their columns; the row form above reads a key again for
-// each row.  Against it, 771 rows on 8,192-16,384 keys, 2,048 selected at random:
-// 874 -> 250 us: 600 TFLOP/s of the computed pairs (plain prompts 770), as its 208
-// workgroups leave 48 CUs idle.
+// Sparse attention of prompt rows: the (kv head, tile of a sequence's rows) units' 64-key
+// tiles, one unit after another, in equal runs for the workgroups (a CU each); a unit
+// that a run's end cuts leaves partials.  A tile's rows share each K/V tile, and MFMAs have
+// all their columns; the row form above reads a key again for each row.  771 rows on
+// 8,192-16,384 keys, 2,048 selected at random, with lists and join: 874 us by rows, 252 by
+// tiles cut in equal parts (208 workgroups), 221 by equal runs (224 of this kernel's 670
+// TFLOP/s of the computed pairs; plain prompts 770).
 template <typename T, int D, int KF>
 __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2)))
 sparse_tile_kernel(AttnArgs a) {
   using Cfg = PrefillCfg<D, kPrefillStages>;
   __shared__ __attribute__((aligned(16))) char lds[Cfg::kLdsBytes + Cfg::kBidCache * 12];
-  const int Hkv = a.num_kv_heads, per_tile = Hkv * a.tile_splits;
-  const int ti = blockIdx.x / per_tile, rest = blockIdx.x - ti * per_tile;
-  const int sp = rest / Hkv, kvh = rest - sp * Hkv;
-  const SparseTile st = a.sparse_tiles[ti];
-  const int unit = ti * Hkv + kvh;
-  const int keys = a.tile_keys[unit];
-  const int len = ((keys + a.tile_splits - 1) / a.tile_splits + 63) / 64 * 64;
-  const SelectedTile sx{a.tile_entries + (int64_t)unit * a.tile_capacity, st.row0, st.nrows, min(keys, sp * len),
-                        min(keys, (sp + 1) * len), sp, a.tile_splits};
-  if (sx.k0 < sx.k1) {
-    const WorkItem none{};
-    prefill_wg<T, D, false, kWaves, kPrefillStages, KF, false, kSelectedKeys>(a, none, st.seq, kvh, 0, lds, nullptr, &sx);
-    return;
-  }
-  // no key: empty partials, or rows of zeros
-  const int G = a.num_q_heads / Hkv;
-  if (a.tile_splits == 1) {
-    for (int e = threadIdx.x; e < st.nrows * G * D; e += 64 * kWaves) {
-      const int r = e / (G * D);
-      ((T*)a.out)[(int64_t)a.tile_rows[st.row0 + r].row * a.out_row_stride + (int64_t)kvh * G * D + (e - r * G * D)] = (T)0.f;
+  __shared__ int sums[2][kWaves], next[6];        // next: see below
+  const int nt = a.n_sparse_tiles, Hkv = a.num_kv_heads, units = nt * Hkv, W = gridDim.x;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // neighbouring runs on one XCD: they share keys
+  const int b = W % 8 ? blockIdx.x : blockIdx.x % 8 * (W / 8) + blockIdx.x / 8;
+  const auto keys_of = [&](int u) { return a.tile_keys[u % nt * Hkv + u / nt]; };
+  const auto tiles_of = [&](int keys) { return max(1, (keys + 63) / 64); };
+  // all units' tiles, and the runs that they make: one a CU, of at least four tiles and at
+  // most as many as the ids, rows and numbers of 1,022 blocks allow (the plan's W counts every
+  // block that the tiles could have)
+  int mine = 0;
+  for (int u = tid; u < units; u += 64 * kWaves) mine += tiles_of(keys_of(u));
+#pragma unroll
+  for (int x = 1; x < 64; x *= 2) mine += __shfl_xor(mine, x, 64);
+  if (lane == 0) sums[1][wave] = mine;
+  __syncthreads();
+  int64_t C = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) C += sums[1][w];
+  const int64_t round = (int64_t)a.tile_round * (1022 * (int64_t)a.block_size / 64);
+  const int64_t runs = min((int64_t)W, min(max((int64_t)1, C / 4), (C + round - 1) / round * a.tile_round));
+  if (b >= runs) return;
+  const int lo = (int)(C * b / runs), hi = (int)(C * (b + 1) / runs);
+  // the unit of the run's first tile; run 0 writes down where every unit's partials are
+  int base = 0, flip = 0;
+  for (int u1 = 0; u1 < units && (b == 0 || base <= lo); u1 += 64 * kWaves, flip ^= 1) {
+    const int u = u1 + tid, c = u < units ? tiles_of(keys_of(u)) : 0;
+    int upto = c;
+#pragma unroll
+    for (int x = 1; x < 64; x *= 2) {
+      const int y = __shfl_up(upto, x, 64);
+      upto += lane >= x ? y : 0;
     }
-  } else {
-    for (int c = threadIdx.x; c < st.nrows * G; c += 64 * kWaves) {
-      const int r = c / G;
-      const int64_t at = (((int64_t)(st.row0 + r) * Hkv + kvh) * a.tile_splits + sp) * G + c - r * G;
-      a.partial_ml[2 * at] = kNegInf;
-      a.partial_ml[2 * at + 1] = 0.f;
+    if (lane == 63) sums[flip][wave] = upto;
+    __syncthreads();
+    int s0 = base + upto - c;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      s0 += w < wave ? sums[flip][w] : 0;
+      base += sums[flip][w];
+    }
+    if (c > 0 && s0 <= lo && lo < s0 + c) {
+      next[0] = u;
+      next[1] = s0;
+      next[2] = lo;
+      next[3] = units < runs ? b + u : 2 * b;
+      next[4] = units < runs;
+      next[5] = hi;
+    }
+    if (b == 0 && c > 0) {
+      // run r has tile s iff floor(C r / runs) <= s, r the last such
+      const int r0 = (int)(((s0 + (int64_t)1) * runs - 1) / C), r1 = (int)(((s0 + (int64_t)c) * runs - 1) / C);
+      const bool cut = (int)(C * r0 / runs) < s0;
+      a.tile_parts[u] = units < runs ? TileParts{r0 + u, r0 + u + 1, 1, r1 - r0 + 1}
+                                     : TileParts{2 * r0 + cut, 2 * (r0 + 1), 2, r1 - r0 + 1};
+    }
+  }
+  // the walk's state is in LDS, so that no register holds it through a unit: the unit, its
+  // first tile, the run's next tile, the slot of its partials and how they count, the run's end
+  for (;;) {
+    __syncthreads();
+    const int u = __builtin_amdgcn_readfirstlane(next[0]), s0 = __builtin_amdgcn_readfirstlane(next[1]);
+    const int s = __builtin_amdgcn_readfirstlane(next[2]), slot = __builtin_amdgcn_readfirstlane(next[3]);
+    const int stop = __builtin_amdgcn_readfirstlane(next[5]);
+    if (s >= stop) return;
+    __syncthreads();
+    const int kvh = u / nt, ti = u - kvh * nt, keys = keys_of(u), c = tiles_of(keys);
+    const SparseTile st = a.sparse_tiles[ti];
+    const int end = min(stop, s0 + c);
+    const SelectedTile sx{a.tile_entries + ((int64_t)ti * Hkv + kvh) * a.tile_capacity, st.row0, st.nrows, 64 * (s - s0),
+                          min(keys, 64 * (end - s0)), s == s0 && end == s0 + c ? -1 : slot};
+    if (threadIdx.x == 0) {
+      next[0] = u + 1;
+      next[1] = s0 + c;
+      next[2] = end;
+      next[3] = next[4] ? slot + 1 : slot | 1;   // b + u, or 2 b and then 2 b + 1
+    }
+    if (keys > 0) {
+      const WorkItem none{};
+      prefill_wg<T, D, false, kWaves, kPrefillStages, KF, false, kSelectedKeys>(a, none, st.seq, kvh, 0, lds, nullptr, &sx);
+    } else {                                     // no key: rows of zeros
+      const int G = a.num_q_heads / Hkv;
+      for (int e = threadIdx.x; e < st.nrows * G * D; e += 64 * kWaves) {
+        const int r = e / (G * D);
+        ((T*)a.out)[(int64_t)a.tile_rows[st.row0 + r].row * a.out_row_stride + (int64_t)kvh * G * D + (e - r * G * D)] = (T)0.f;
+      }
     }
   }
 }
 
-// Joins the splits of every (query row, kv head): a thread per 4 dims of a head.
-template <typename T, int D>
-__global__ void __launch_bounds__(64) sparse_merge_kernel(AttnArgs a, int total) {
-  const int e = blockIdx.x * 64 + threadIdx.x;
-  if (e >= total) return;
-  constexpr int C = D / 4;
-  const int d = 4 * (e % C), qh = e / C % a.num_q_heads, ri = e / C / a.num_q_heads;
-  const int G = a.num_q_heads / a.num_kv_heads, ns = a.sparse_splits;
-  const int slots = a.n_sparse_tiles > 0 ? G : 16;     // of a partial: a tile's rows have theirs side by side
-  const int64_t at = ((int64_t)ri * a.num_kv_heads + qh / G) * ns * slots + qh % G;
-  constexpr int CH = 8;                          // splits' loads in flight
+// Joins ns partials of 4 dims of a head from d on, those at place(0 .. ns - 1), into row op.
+template <typename T, int D, typename F>
+__device__ __forceinline__ void join_partials(const AttnArgs& a, int ns, int d, T* op, F place) {
+  constexpr int CH = 8;                          // partials' loads in flight
   float M = kNegInf, L = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
   for (int s0 = 0; s0 < ns; s0 += CH) {
     u32x2 x[CH];
     f32x4 v[CH];
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {               // splits past the last one re-read it, with weight 0
-      const int64_t p = at + slots * min(s0 + c, ns - 1);
+    for (int c = 0; c < CH; ++c) {               // those past the last one re-read it, with weight 0
+      const int64_t p = place(min(s0 + c, ns - 1));
       x[c] = *reinterpret_cast<const u32x2*>(a.partial_ml + p * 2);
       v[c] = *reinterpret_cast<const f32x4*>(a.partials + p * D + d);
     }
@@ -1946,7 +2002,7 @@ __global__ void __launch_bounds__(64) sparse_merge_kernel(AttnArgs a, int total)
 #pragma unroll
     for (int c = 0; c < CH; ++c) {               // fixed order: deterministic sums
       const float m = __uint_as_float(x[c][0]);
-      const bool none = m == kNegInf || s0 + c >= ns;      // an empty split wrote no values
+      const bool none = m == kNegInf || s0 + c >= ns;      // an empty one wrote no values
       const float w = none ? 0.f : fast_exp2(m - mu);
       L += w * __uint_as_float(x[c][1]);
 #pragma unroll
@@ -1955,8 +2011,30 @@ __global__ void __launch_bounds__(64) sparse_merge_kernel(AttnArgs a, int total)
     M = Mn;
   }
   const float inv = L > 0.f ? 1.f / L : 0.f;     // no key at all: zeros
-  T* op = (T*)a.out + (int64_t)a.sparse_rows[ri].row * a.out_row_stride + (int64_t)qh * D + d;
   st8(op, u32x2{E16<T>::pack2(o[0] * inv, o[1] * inv), E16<T>::pack2(o[2] * inv, o[3] * inv)});
+}
+// Joins the splits of every (query row, kv head), or the parts of a tile's rows where
+// there are several: a thread per 4 dims of a head.
+template <typename T, int D, bool TILES>
+__global__ void __launch_bounds__(64) sparse_merge_kernel(AttnArgs a, int total) {
+  const int e = blockIdx.x * 64 + threadIdx.x;
+  if (e >= total) return;
+  constexpr int C = D / 4;
+  const int d = 4 * (e % C), qh = e / C % a.num_q_heads, ri = e / C / a.num_q_heads;
+  const int G = a.num_q_heads / a.num_kv_heads, kvh = qh / G;
+  const SparseRow sr = a.sparse_rows[ri];
+  T* op = (T*)a.out + (int64_t)sr.row * a.out_row_stride + (int64_t)qh * D + d;
+  if constexpr (TILES) {
+    const TileParts tp = a.tile_parts[kvh * a.n_sparse_tiles + sr.pad];
+    if (tp.count == 1) return;
+    const int col = (ri - a.sparse_tiles[sr.pad].row0) * G + qh % G;
+    join_partials<T, D>(a, tp.count, d, op, [&](int s) {
+      return (int64_t)(s == 0 ? tp.first : tp.rest + (s - 1) * tp.step) * a.tile_cols + col;
+    });
+  } else {
+    const int64_t at = ((int64_t)ri * a.num_kv_heads + kvh) * a.sparse_splits * 16 + qh % G;
+    join_partials<T, D>(a, a.sparse_splits, d, op, [&](int s) { return at + 16 * s; });
+  }
 }
 
 template <typename T, int D>
@@ -2079,28 +2157,26 @@ static hipError_t launch_dense_t(const AttnArgs& a, dim3 grid, int nwg, hipStrea
   return hipGetLastError();
 }
 
-template <typename T, int D>
+template <typename T, int D, bool TILES>
 static hipError_t launch_sparse_merge(const AttnArgs& a, hipStream_t st) {
   const int64_t total = (int64_t)a.n_sparse_rows * a.num_q_heads * (D / 4);
   if (total > INT32_MAX - 256) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((sparse_merge_kernel<T, D>), dim3((unsigned)((total + 63) / 64)), dim3(64), 0, st, a, (int)total);
+  hipLaunchKernelGGL((sparse_merge_kernel<T, D, TILES>), dim3((unsigned)((total + 63) / 64)), dim3(64), 0, st, a, (int)total);
   return hipGetLastError();
 }
 // Tiles (n_sparse_tiles > 0: their rows are n_sparse_rows of them) or single rows.
 template <typename T, int D, int KF>
 static hipError_t launch_sparse_d(const AttnArgs& a, hipStream_t st) {
   if (a.n_sparse_tiles > 0) {
-    const int64_t wgs = (int64_t)a.n_sparse_tiles * a.num_kv_heads * a.tile_splits;
-    if (wgs > INT32_MAX) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((sparse_tile_kernel<T, D, KF>), dim3((unsigned)wgs), dim3(64 * kWaves), 0, st, a);
-    hipError_t e = hipGetLastError();
-    return e != hipSuccess || a.tile_splits == 1 ? e : launch_sparse_merge<T, D>(a, st);
+    hipLaunchKernelGGL((sparse_tile_kernel<T, D, KF>), dim3(a.tile_wgs), dim3(64 * kWaves), 0, st, a);
+    const hipError_t e = hipGetLastError();
+    return e != hipSuccess ? e : launch_sparse_merge<T, D, true>(a, st);
   }
   const int64_t wgs = (int64_t)a.n_sparse_rows * a.num_kv_heads * a.sparse_splits;
   if (wgs > INT32_MAX) return hipErrorInvalidValue;
   hipLaunchKernelGGL((sparse_attn_kernel<T, D, KF>), dim3((unsigned)wgs), dim3(64 * kSparseWaves), 0, st, a);
   hipError_t e = hipGetLastError();
-  return e != hipSuccess || a.sparse_splits == 1 ? e : launch_sparse_merge<T, D>(a, st);
+  return e != hipSuccess || a.sparse_splits == 1 ? e : launch_sparse_merge<T, D, false>(a, st);
 }
 template <typename T, int D>
 static hipError_t launch_sparse_t(const AttnArgs& a, hipStream_t st) {

@@ -330,13 +330,26 @@ def test_tiles_of_many_blocks(ctx, rows, blocks, kv):
     time; no row of a tile left out of the parts' joining."""
     b = Batch([ctx], [rows], Hq=4, Hkv=1, D=64, kv=kv, bs=16, seed=ctx)
     plan = plan_of(b, blocks, 0)
-    assert plan.info["tiles"] >= 1 and (ctx < 10000 or plan.info["tile_splits"] > 1)
+    assert plan.info["tiles"] >= 1 and (ctx < 10000 or plan.info["tile_workgroups"] > 1)
     sel = random_lists(b, blocks, 7, whole=True)
     sel[rows // 2] = -1
     args = (b.q.cuda(), b.kc.cuda(), b.vc.cuda(), b.bt.cuda(), sel.cuda())
     out = sparse.sparse_attention(plan, *args)
     check_attention(b, out, {(r, 0): sel[r, 0].tolist() for r in range(rows)})
     assert torch.equal(out, sparse.sparse_attention(plan, *args))
+
+
+@pytest.mark.parametrize("ql,Hkv,blocks", [([300] * 3, 2, 8), ([64] * 70, 8, 6), ([20] * 160, 2, 8), ([100, 1, 1000], 4, 3)])
+def test_runs_that_cut_and_span_tiles(ql, Hkv, blocks):
+    """Fewer (tile, KV head) units than runs of keys and more; units without keys between
+    others; rows of every part."""
+    b = Batch([700 + 37 * (i % 5) for i in range(len(ql))], ql, Hq=2 * Hkv, Hkv=Hkv, D=64, bs=16, seed=sum(ql))
+    plan = plan_of(b, blocks, 0)
+    assert plan.info["tiles"] >= 2
+    sel = random_lists(b, blocks, 3, whole=True)
+    sel[b.start[1]:b.start[1] + b.ql[1], 0] = -1
+    out = sparse.sparse_attention(plan, b.q.cuda(), b.kc.cuda(), b.vc.cuda(), b.bt.cuda(), sel.cuda())
+    check_attention(b, out, {(row, h): sel[row, h].tolist() for _, row, _ in rows_of(b) for h in range(Hkv)})
 
 
 def test_tiles_do_not_read_behind_the_last_row():

@@ -100,7 +100,7 @@ def test_plan_facts():
 
 def _tiles(ql, sl, **kw):
     p = _plan(ql, sl, num_q_heads=32, num_kv_heads=8, head_dim=128, **kw)
-    return p.info["tiles"], p.info["tile_splits"], p.workspace.numel()
+    return p.info["tiles"], p.info["tile_workgroups"], p.workspace.numel()
 
 
 def test_prompt_rows_go_in_tiles_where_that_reads_less():
@@ -110,10 +110,12 @@ def test_prompt_rows_go_in_tiles_where_that_reads_less():
     assert _tiles([1] * 9, [12000] * 9, blocks=64, block_size=32)[0] == 0
     # choices spread over very many blocks have little in common
     assert _tiles([64], [1 << 20], blocks=64, block_size=16)[0] == 0
-    # parts of at most 1,022 blocks; partials stay below 1 GiB
-    n, parts, size = _tiles([512], [16384 * 4], blocks=256, block_size=16)
-    assert n == 8 and parts >= 5 and size < 1 << 30
-    assert _tiles([16384], [65536], blocks=256, block_size=16)[2] < 3 << 30
+    # a run of keys per CU, of at most 1,022 blocks; partials stay below 1 GiB
+    n, wgs, size = _tiles([512], [16384 * 4], blocks=256, block_size=16)
+    assert n == 8 and wgs % 256 == 0 and wgs * 1022 * 16 >= 8 * 8 * 65536 and size < 1 << 30
+    n, wgs, size = _tiles([2000], [16384 * 8], blocks=512, block_size=16)
+    assert n == 32 and wgs * 1022 * 16 >= 32 * 8 * 16384 * 8 * 0.98 and wgs % 256 == 0 and size < 3 << 30
+    assert _tiles([16384], [65536], blocks=256, block_size=16)[2] < 4 << 30
 
 
 @pytest.mark.parametrize("D", [64, 128])
