@@ -459,8 +459,8 @@ size_t gllm_sparse_plan_workspace_bytes(const gllm_sparse_plan* plan);
 int gllm_sparse_plan_upload(gllm_sparse_plan* plan, void* workspace, size_t workspace_bytes, void* stream);
 /* Plan facts: [0] rows of q / out / selected that it addresses, [1] query rows, [2] blocks
  * that the new tokens touch, [3] score tiles, [4] slabs of rows scored at a time, [5]
- * splits of a row's keys, [6] tiles of prompt rows that attend together, [7] splits of a
- * tile's keys ([5] to [7]: on the MFMA kernels).  The first n are written. */
+ * splits of a row's keys, [6] tiles of prompt rows that attend together, [7] workgroups
+ * that share those tiles' keys ([5] to [7]: on the MFMA kernels).  The first n are written. */
 int gllm_sparse_plan_info(const gllm_sparse_plan* plan, int64_t* info, int32_t n);
 int gllm_sparse_plan_destroy(gllm_sparse_plan* plan);
 /* Bounds of every block that holds a new token (positions seq_len - query_len ..
