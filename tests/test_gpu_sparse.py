@@ -519,6 +519,36 @@ def test_replays_of_a_captured_step():
         assert torch.equal(replayed[0], want) and torch.equal(replayed[1], sel), f"replay {i}"
 
 
+def test_replays_of_captured_prompt_tiles():
+    """Lists that change between replays move the runs of keys and the tiles that they
+    cut: each replay is the eager call's, bit for bit."""
+    b = Batch([1500, 300, 700], [130, 1, 70], Hq=8, Hkv=2, D=128, bs=16)
+    plan = plan_of(b, 8, 0)
+    assert plan.info["tiles"] >= 3
+    q, kc, vc, bt = b.q.cuda(), b.kc.cuda(), b.vc.cuda(), b.bt.cuda()
+    lists = [random_lists(b, 8, seed, seed % 2 == 0).cuda() for seed in range(4)]
+    lists += [torch.full_like(lists[0], -1), torch.where(lists[0] > 5, -1, lists[0])]
+    sel, out = lists[0].clone(), torch.empty_like(q)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        sparse.sparse_attention(plan, q, kc, vc, bt, sel, out=out)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        sparse.sparse_attention(plan, q, kc, vc, bt, sel, out=out)
+    for k, x in enumerate(lists + lists[::-1]):
+        sel.copy_(x)
+        out.fill_(math.nan)
+        graph.replay()
+        torch.cuda.synchronize()
+        replayed = out.clone()
+        want = sparse.sparse_attention(plan, q, kc, vc, bt, x)
+        assert torch.equal(replayed, want), f"replay {k}"
+        if k < len(lists):
+            check_attention(b, want, {(row, h): x[row, h].tolist() for _, row, _ in rows_of(b) for h in range(2)}, f"lists {k}")
+
+
 def test_calls_on_another_stream():
     b = Batch([900, 500], [1, 1], Hq=8, Hkv=2, D=64, bs=16)
     q, kc, vc, bt = b.q.cuda(), b.kc.cuda(), b.vc.cuda(), b.bt.cuda()
