@@ -1609,8 +1609,13 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
   }
 
   if (PFX || (SELT && sx->slot >= 0)) {
-    // the row's state: reference (log2 units), sum and unnormalised output
+    // the row's state: reference (log2 units), sum and unnormalised output.  The reference may
+    // lie 2^64 off the row's largest weight either way, where a join's weights 2^(m - M) pass
+    // under fp32's least exponent for the part that carries the row: the sum's exponent goes
+    // to the reference (powers of two, exact), so that m is the part's weight to a factor of 2
     const float lt = sum_xor32(lsum);
+    const int up = __builtin_amdgcn_frexp_expf(lt);      // 0 for 0, infinities and NaN
+    const float unit = __builtin_amdgcn_ldexpf(1.f, -up);
     if (row_ok) {
       int64_t at;
       if constexpr (PFX) {
@@ -1626,10 +1631,10 @@ __device__ __forceinline__ void prefill_wg(const AttnArgs& a, const WorkItem& it
 #pragma unroll
         for (int jq = 0; jq < 4; ++jq)
           *reinterpret_cast<f32x4*>(pa + 32 * db + 8 * jq) =
-              f32x4{o[db][4 * jq], o[db][4 * jq + 1], o[db][4 * jq + 2], o[db][4 * jq + 3]};
+              f32x4{o[db][4 * jq], o[db][4 * jq + 1], o[db][4 * jq + 2], o[db][4 * jq + 3]} * unit;
       // SELT: a row that saw no key has no reference
-      const float ref = SELT && !rset ? kNegInf : rref;
-      if (h == 0) *reinterpret_cast<u32x2*>(a.partial_ml + at * 2) = u32x2{__float_as_uint(ref), __float_as_uint(lt)};
+      const float ref = SELT && !rset ? kNegInf : rref + (float)up;
+      if (h == 0) *reinterpret_cast<u32x2*>(a.partial_ml + at * 2) = u32x2{__float_as_uint(ref), __float_as_uint(lt * unit)};
     }
     return;
   }
