@@ -1800,14 +1800,10 @@ void plan_sparse_tiles(gllm_sparse_plan* p, const int32_t* query_lens, const int
     }
   }
   if (p->tiles.empty()) return;
-  // Equal runs of the units' keys, one a CU, or as many more as leave a run the ids, rows
-  // and numbers of 1,022 blocks that a workgroup holds.  A run's first and last unit may be
-  // parts: a slot for each (fewer units than runs: one a run and one a unit).
-  const int64_t cus = device_cus(), units = (int64_t)p->tiles.size() * p->Hkv, most_tiles = 1022 * (int64_t)p->bs / 64;
-  const int64_t wgs = std::min(std::max<int64_t>(1, all / 4),   // of four tiles at least
-                               cus * std::max<int64_t>(1, (all + cus * most_tiles - 1) / (cus * most_tiles)));
+  // Equal runs of the units' keys (tile_runs.h)
+  const int64_t cus = device_cus(), units = (int64_t)p->tiles.size() * p->Hkv, wgs = tile_runs(all, cus, p->bs);
   p->tile_cols = most * G;
-  p->tile_slots = wgs + std::min(wgs, units);
+  p->tile_slots = run_slots(wgs, units);
   p->tile_wgs = (int32_t)std::min<int64_t>(wgs, INT32_MAX);
   p->tile_round = (int32_t)cus;
   // partials past 1 GiB, or too many tiles to count: rows on their own

@@ -13,6 +13,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "tile_runs.h"
+
 namespace gllm {
 
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
@@ -469,11 +471,6 @@ struct SelectedBlock {
 struct SelectedTile {
   const SelectedBlock* entries;
   int32_t row0, nrows, k0, k1, slot;
-};
-// The partials of a (kv head, tile): slot first, then rest, rest + step, ... (count in all;
-// 1: none, the output is written).
-struct TileParts {
-  int32_t first, rest, step, count;
 };
 // A cache block whose first n keys have bounds to be written: block `block` of
 // sequence seq.

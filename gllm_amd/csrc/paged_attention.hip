@@ -795,7 +795,7 @@ template <int D, int NS> struct PrefillCfg {
   static constexpr int kTile = kBN * kRow;         // bytes per K (or V) tile
   static constexpr int kStages = NS;               // LDS ring: tiles t+1 .. t+NS-1 in flight while t is computed
   static constexpr int kVBase = NS * kTile;        // start of the V tiles
-  static constexpr int kBidCache = 1024;           // block ids cached per workgroup
+  static constexpr int kBidCache = kRunCache;      // block ids cached per workgroup
   static constexpr int kLdsBytes = 2 * NS * kTile + kBidCache * 4;
   static_assert((NS - 1) * kTile + (kBN - 16) * kRow < 65536, "stage offsets must fit a DS immediate");
 };
@@ -1900,9 +1900,8 @@ sparse_tile_kernel(AttnArgs a) {
   const int b = W % 8 ? blockIdx.x : blockIdx.x % 8 * (W / 8) + blockIdx.x / 8;
   const auto keys_of = [&](int u) { return a.tile_keys[u % nt * Hkv + u / nt]; };
   const auto tiles_of = [&](int keys) { return max(1, (keys + 63) / 64); };
-  // all units' tiles, and the runs that they make: one a CU, of at least four tiles and at
-  // most as many as the ids, rows and numbers of 1,022 blocks allow (the plan's W counts every
-  // block that the tiles could have)
+  // all units' tiles, and the runs that they make (the plan's W counts every block that the
+  // tiles could have)
   int mine = 0;
   for (int u = tid; u < units; u += 64 * kWaves) mine += tiles_of(keys_of(u));
 #pragma unroll
@@ -1912,10 +1911,9 @@ sparse_tile_kernel(AttnArgs a) {
   int64_t C = 0;
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) C += sums[1][w];
-  const int64_t round = (int64_t)a.tile_round * (1022 * (int64_t)a.block_size / 64);
-  const int64_t runs = min((int64_t)W, min(max((int64_t)1, C / 4), (C + round - 1) / round * a.tile_round));
+  const int64_t runs = min((int64_t)W, tile_runs(C, a.tile_round, a.block_size));
   if (b >= runs) return;
-  const int lo = (int)(C * b / runs), hi = (int)(C * (b + 1) / runs);
+  const int lo = (int)run_start(C, runs, b), hi = (int)run_start(C, runs, b + 1);
   // the unit of the run's first tile; run 0 writes down where every unit's partials are
   int base = 0, flip = 0;
   for (int u1 = 0; u1 < units && (b == 0 || base <= lo); u1 += 64 * kWaves, flip ^= 1) {
@@ -1938,17 +1936,11 @@ sparse_tile_kernel(AttnArgs a) {
       next[0] = u;
       next[1] = s0;
       next[2] = lo;
-      next[3] = units < runs ? b + u : 2 * b;
+      next[3] = part_slot(runs, units, b, u, true);
       next[4] = units < runs;
       next[5] = hi;
     }
-    if (b == 0 && c > 0) {
-      // run r has tile s iff floor(C r / runs) <= s, r the last such
-      const int r0 = (int)(((s0 + (int64_t)1) * runs - 1) / C), r1 = (int)(((s0 + (int64_t)c) * runs - 1) / C);
-      const bool cut = (int)(C * r0 / runs) < s0;
-      a.tile_parts[u] = units < runs ? TileParts{r0 + u, r0 + u + 1, 1, r1 - r0 + 1}
-                                     : TileParts{2 * r0 + cut, 2 * (r0 + 1), 2, r1 - r0 + 1};
-    }
+    if (b == 0 && c > 0) a.tile_parts[u] = unit_parts(C, runs, units, u, s0, c);
   }
   // the walk's state is in LDS, so that no register holds it through a unit: the unit, its
   // first tile, the run's next tile, the slot of its partials and how they count, the run's end
@@ -1968,7 +1960,7 @@ sparse_tile_kernel(AttnArgs a) {
       next[0] = u + 1;
       next[1] = s0 + c;
       next[2] = end;
-      next[3] = next[4] ? slot + 1 : slot | 1;   // b + u, or 2 b and then 2 b + 1
+      next[3] = next[4] ? slot + 1 : slot | 1;   // part_slot of the next unit
     }
     if (keys > 0) {
       const WorkItem none{};
