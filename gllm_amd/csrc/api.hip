@@ -208,12 +208,14 @@ struct gllm_sparse_plan {
   std::vector<Slab> slabs;
   int64_t score_stride = 0;
   // MFMA kernels: rows on their own (each in `splits` parts), and prompt rows in tiles
-  // (their keys dealt to tile_wgs workgroups); the generic kernel takes `rows`
+  // (their keys dealt to wgs workgroups); the generic kernel takes `rows`
   std::vector<SparseRow> lone, tile_rows;
   std::vector<SparseTile> tiles;
-  int32_t splits = 1, tile_wgs = 0, tile_round = 1, tile_capacity = 0;
-  int64_t tile_slots = 0;                     // partials of tile_cols columns
-  int32_t tile_cols = 0;
+  int32_t splits = 1, tile_round = 1, tile_cols = 0;
+  // tiles attend a slab at a time, so that their blocks and partials stay bounded: n_tiles
+  // from tile0 on and their rows (each counted from the slab's first), of `capacity` blocks at most
+  struct TileSlab { int32_t tile0, n_tiles, row0, n_rows, wgs, capacity; };
+  std::vector<TileSlab> tile_slabs;
   void* pinned = nullptr;
   size_t pinned_cap = 0;
   bool pinned_is_host_malloc = false;
@@ -1745,6 +1747,8 @@ int gllm_attention_dense(const void* q, int64_t q_row_stride, const void* k, int
 namespace {
 // Scores of a slab of rows: at most this many bytes (or one tile's).
 constexpr int64_t kScoreBytes = int64_t(256) << 20;
+// The blocks, and the partials, of a slab of prompt tiles.
+constexpr int64_t kTileBytes = int64_t(256) << 20;
 
 int64_t bounds_record(int64_t Hkv, int64_t D) { return (Hkv * (2 * D + 1) + 15) / 16 * 16; }
 
@@ -1772,47 +1776,55 @@ void plan_sparse_tiles(gllm_sparse_plan* p, const int32_t* query_lens, const int
     const double cols = (rows * G + 31) / 32 * 32;
     return 64 * std::max(key * cols / (p->D == 128 ? 3.2e12 : 2.4e12), key / 30e9) * (nb * share * p->bs / 64);
   };
-  int64_t all = 0, r0 = 0;                     // 64-key tiles at most
+  const int64_t cus = device_cus();
+  p->tile_round = (int32_t)cus;
+  p->tile_cols = most * G;
+  // The most blocks that a tile of n rows on nb blocks selects, and 64-key tiles of its units
+  const auto blocks_of = [&](int64_t n, int64_t nb) { return std::min<int64_t>(nb, n * p->width); };
+  const auto tiles_of = [&](int64_t blocks) { return p->Hkv * ((blocks * p->bs + 63) / 64); };
+  // A slab of `n` tiles, `all` 64-key tiles at most: its blocks and its partials, each bounded
+  const auto fits = [&](int64_t n, int64_t blocks, int64_t all) {
+    const int64_t slots = run_slots(tile_runs(all, cus, p->bs), n * p->Hkv);
+    return all <= INT32_MAX && n * p->Hkv * blocks <= kTileBytes / (int64_t)sizeof(SelectedBlock) &&
+           slots <= kTileBytes / ((int64_t)p->tile_cols * (p->D + 2) * 4);
+  };
+  int64_t all = 0, r0 = 0;                     // of the last slab
   for (int i = 0; i < p->num_seqs; r0 += query_lens[i++]) {
     const int32_t ql = query_lens[i], c = seq_lens[i] - ql;
     const int n = (ql + most - 1) / most;
+    const auto first_row = [&](int t) { return (int64_t)ql * t / n; };
+    const auto seen = [&](int t) { return (c + first_row(t + 1) - 1) / p->bs + 1; };   // blocks
     double tiles = 0, rows = 0;
-    for (int t = 0; t < n; ++t) {
-      const int64_t a = (int64_t)ql * t / n, e = (int64_t)ql * (t + 1) / n;
-      tiles += 6e-6 + tile_time((int)(e - a), (int32_t)((c + e - 1) / p->bs + 1));
-      rows += (double)(e - a) * (5e-6 + std::min<double>(p->width, (c + e - 1) / p->bs + 1) * p->bs * key / 29e9);
+    bool alone = ql < 2 || p->bs % 16 != 0;
+    for (int t = 0; t < n && !alone; ++t) {
+      const int64_t nr = first_row(t + 1) - first_row(t), nb = seen(t), blocks = blocks_of(nr, nb);
+      tiles += 6e-6 + tile_time((int)nr, (int32_t)nb);
+      rows += (double)nr * (5e-6 + std::min<double>(p->width, (double)nb) * p->bs * key / 29e9);
+      alone = !fits(1, blocks, tiles_of(blocks));        // one tile is too much for a slab
     }
-    if (ql < 2 || p->bs % 16 || tiles >= rows) {
+    if (alone || tiles >= rows) {
       p->lone.insert(p->lone.end(), p->rows.begin() + r0, p->rows.begin() + r0 + ql);
       continue;
     }
     for (int t = 0; t < n; ++t) {
-      const int64_t a = (int64_t)ql * t / n, e = (int64_t)ql * (t + 1) / n;
-      const int32_t nb = (int32_t)((c + e - 1) / p->bs + 1);
-      p->tiles.push_back({(int32_t)p->tile_rows.size(), (int32_t)(e - a), i, 0});
+      const int64_t a = first_row(t), e = first_row(t + 1), blocks = blocks_of(e - a, seen(t));
+      gllm_sparse_plan::TileSlab* sb = p->tile_slabs.empty() ? nullptr : &p->tile_slabs.back();
+      if (!sb || !fits(sb->n_tiles + 1, std::max<int64_t>(sb->capacity, blocks), all + tiles_of(blocks))) {
+        p->tile_slabs.push_back({(int32_t)p->tiles.size(), 0, (int32_t)p->tile_rows.size(), 0, 0, 0});
+        sb = &p->tile_slabs.back();
+        all = 0;
+      }
+      all += tiles_of(blocks);
+      p->tiles.push_back({sb->n_rows, (int32_t)(e - a), i, 0});
       for (int64_t r = a; r < e; ++r) {
         p->tile_rows.push_back(p->rows[(size_t)(r0 + r)]);
-        p->tile_rows.back().pad = (int32_t)p->tiles.size() - 1;
+        p->tile_rows.back().pad = sb->n_tiles;
       }
-      const int64_t most_blocks = std::min<int64_t>(nb, (e - a) * p->width);
-      p->tile_capacity = (int32_t)std::max<int64_t>(p->tile_capacity, most_blocks);
-      all += p->Hkv * ((most_blocks * p->bs + 63) / 64);
+      ++sb->n_tiles;
+      sb->n_rows += (int32_t)(e - a);
+      sb->capacity = std::max(sb->capacity, (int32_t)blocks);
+      sb->wgs = (int32_t)tile_runs(all, cus, p->bs);     // equal runs of its units' keys
     }
-  }
-  if (p->tiles.empty()) return;
-  // Equal runs of the units' keys (tile_runs.h)
-  const int64_t cus = device_cus(), units = (int64_t)p->tiles.size() * p->Hkv, wgs = tile_runs(all, cus, p->bs);
-  p->tile_cols = most * G;
-  p->tile_slots = run_slots(wgs, units);
-  p->tile_wgs = (int32_t)std::min<int64_t>(wgs, INT32_MAX);
-  p->tile_round = (int32_t)cus;
-  // partials past 1 GiB, or too many tiles to count: rows on their own
-  if (all > INT32_MAX || units > INT32_MAX || p->tile_slots > (int64_t(1) << 30) / ((int64_t)p->tile_cols * p->D * 4)) {
-    p->lone = p->rows;
-    p->tiles.clear();
-    p->tile_rows.clear();
-    p->tile_capacity = p->tile_wgs = 0;
-    p->tile_slots = 0;
   }
 }
 
@@ -1933,8 +1945,13 @@ int sparse_plan_impl(gllm_sparse_plan** out, const int32_t* query_lens, const in
     p->splits = (int32_t)s;
   }
   const size_t parts = p->splits > 1 ? p->lone.size() * Hkv * p->splits : 0;
-  const size_t tile_parts = (size_t)p->tile_slots * p->tile_cols;
-  const size_t tile_units = p->tiles.size() * (size_t)Hkv;
+  size_t tile_parts = 0, tile_units = 0, tile_entries = 0;       // of the largest slab each
+  for (const gllm_sparse_plan::TileSlab& sb : p->tile_slabs) {
+    const size_t units = (size_t)sb.n_tiles * Hkv;
+    tile_units = std::max(tile_units, units);
+    tile_entries = std::max(tile_entries, units * sb.capacity);
+    tile_parts = std::max(tile_parts, (size_t)run_slots(sb.wgs, (int64_t)units) * p->tile_cols);
+  }
   size_t o = 0;
   p->off_rows = o; o = align256(o + p->rows.size() * sizeof(SparseRow));
   p->off_blocks = o; o = align256(o + p->blocks.size() * sizeof(BoundsBlock));
@@ -1943,7 +1960,7 @@ int sparse_plan_impl(gllm_sparse_plan** out, const int32_t* query_lens, const in
   p->off_tile_rows = o; o = align256(o + p->tile_rows.size() * sizeof(SparseRow));
   p->off_tiles = o; o = align256(o + p->tiles.size() * sizeof(SparseTile));
   p->stage_bytes = o;
-  p->off_entries = o; o = align256(o + tile_units * p->tile_capacity * sizeof(SelectedBlock));
+  p->off_entries = o; o = align256(o + tile_entries * sizeof(SelectedBlock));
   p->off_keys = o; o = align256(o + tile_units * sizeof(int32_t));
   p->off_parts = o; o = align256(o + tile_units * sizeof(TileParts));
   p->off_tile_ml = o; o = align256(o + tile_parts * 2 * sizeof(float));
@@ -2011,9 +2028,11 @@ int gllm_sparse_plan_upload(gllm_sparse_plan* p, void* workspace, size_t bytes, 
 
 int gllm_sparse_plan_info(const gllm_sparse_plan* p, int64_t* info, int32_t n) {
   if (!p || !info) return fail(GLLM_ATTN_EINVAL, "null plan or info");
-  const int64_t v[8] = {p->total_rows, (int64_t)p->rows.size(), (int64_t)p->blocks.size(), p->n_tiles,
-                        (int64_t)p->slabs.size(), p->splits, (int64_t)p->tiles.size(), p->tile_wgs};
-  for (int i = 0; i < n && i < 8; ++i) info[i] = v[i];
+  int64_t wgs = 0;
+  for (const gllm_sparse_plan::TileSlab& sb : p->tile_slabs) wgs += sb.wgs;
+  const int64_t v[9] = {p->total_rows, (int64_t)p->rows.size(), (int64_t)p->blocks.size(), p->n_tiles,
+                         (int64_t)p->slabs.size(), p->splits, (int64_t)p->tiles.size(), wgs, (int64_t)p->tile_slabs.size()};
+  for (int i = 0; i < n && i < 9; ++i) info[i] = v[i];
   return ok();
 }
 
@@ -2109,27 +2128,27 @@ int gllm_sparse_attention(const gllm_sparse_plan* p, const void* q, int64_t q_ro
     a.n_sparse_rows = (int32_t)p->rows.size();
     return hip_check(launch_sparse_attention_generic(a, st), "sparse attention launch");
   }
-  if (!p->tiles.empty()) {
+  for (const gllm_sparse_plan::TileSlab& sb : p->tile_slabs) {
     AttnArgs t = a;
-    t.sparse_rows = t.tile_rows = (const SparseRow*)(p->ws + p->off_tile_rows);
-    t.n_sparse_rows = (int32_t)p->tile_rows.size();
-    t.sparse_tiles = (const SparseTile*)(p->ws + p->off_tiles);
-    t.n_sparse_tiles = (int32_t)p->tiles.size();
+    t.sparse_rows = t.tile_rows = (const SparseRow*)(p->ws + p->off_tile_rows) + sb.row0;
+    t.n_sparse_rows = sb.n_rows;
+    t.sparse_tiles = (const SparseTile*)(p->ws + p->off_tiles) + sb.tile0;
+    t.n_sparse_tiles = sb.n_tiles;
     t.tile_entries = (SelectedBlock*)(p->ws + p->off_entries);
     t.tile_keys = (int32_t*)(p->ws + p->off_keys);
-    t.tile_capacity = p->tile_capacity;
+    t.tile_capacity = sb.capacity;
     t.tile_parts = (TileParts*)(p->ws + p->off_parts);
-    t.tile_wgs = p->tile_wgs; t.tile_round = p->tile_round; t.tile_cols = p->tile_cols;
+    t.tile_wgs = sb.wgs; t.tile_round = p->tile_round; t.tile_cols = p->tile_cols;
     t.partial_ml = (float*)(p->ws + p->off_tile_ml);
     t.partials = (float*)(p->ws + p->off_tile_part);
     if (int rc = hip_check(launch_tile_blocks(t, st), "sparse attention tiles")) return rc;
     if (int rc = hip_check(launch_sparse_attention_mfma(t, st), "sparse attention launch")) return rc;
   }
-  a.sparse_rows = (const SparseRow*)(p->ws + p->off_lone);
-  a.n_sparse_rows = (int32_t)p->lone.size();
   a.sparse_splits = p->splits;
   a.partial_ml = (float*)(p->ws + p->off_ml);
   a.partials = (float*)(p->ws + p->off_part);
+  a.sparse_rows = (const SparseRow*)(p->ws + p->off_lone);
+  a.n_sparse_rows = (int32_t)p->lone.size();
   return hip_check(launch_sparse_attention_mfma(a, st), "sparse attention launch");
 }
 
