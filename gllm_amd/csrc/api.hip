@@ -216,6 +216,7 @@ struct gllm_sparse_plan {
   // from tile0 on and their rows (each counted from the slab's first), of `capacity` blocks at most
   struct TileSlab { int32_t tile0, n_tiles, row0, n_rows, wgs, capacity; };
   std::vector<TileSlab> tile_slabs;
+  int64_t lone_slab = 0;                      // and so do rows on their own, this many
   void* pinned = nullptr;
   size_t pinned_cap = 0;
   bool pinned_is_host_malloc = false;
@@ -1747,8 +1748,9 @@ int gllm_attention_dense(const void* q, int64_t q_row_stride, const void* k, int
 namespace {
 // Scores of a slab of rows: at most this many bytes (or one tile's).
 constexpr int64_t kScoreBytes = int64_t(256) << 20;
-// The blocks, and the partials, of a slab of prompt tiles.
-constexpr int64_t kTileBytes = int64_t(256) << 20;
+// The blocks, and the partials, of a slab of prompt tiles; the partials of a slab of rows on
+// their own (or one row's).
+constexpr int64_t kTileBytes = int64_t(256) << 20, kPartBytes = int64_t(256) << 20;
 
 int64_t bounds_record(int64_t Hkv, int64_t D) { return (Hkv * (2 * D + 1) + 15) / 16 * 16; }
 
@@ -1941,10 +1943,13 @@ int sparse_plan_impl(gllm_sparse_plan** out, const int32_t* query_lens, const in
     if ((keys - keys / s) * D * 4 < 128 << 10) s = 1;
     const int64_t cap = std::max<int64_t>(16, (int64_t)(510 * (int64_t)bs) / 16 * 16 - 16);   // split_len_of rounds up to 16
     s = std::max<int64_t>(s, (keys + cap - 1) / cap);
-    if (units * s > INT32_MAX / 16) return fail(GLLM_ATTN_EINVAL, "too many splits");
+    if (Hkv * s > INT32_MAX / 16) return fail(GLLM_ATTN_EINVAL, "too many splits");
     p->splits = (int32_t)s;
+    // partials of 16 columns; without any, as many rows as a launch takes
+    const int64_t row = s > 1 ? kPartBytes / (Hkv * s * 16 * (D + 2) * 4) : INT32_MAX / Hkv;
+    p->lone_slab = std::min<int64_t>((int64_t)p->lone.size(), std::max<int64_t>(1, row));
   }
-  const size_t parts = p->splits > 1 ? p->lone.size() * Hkv * p->splits : 0;
+  const size_t parts = p->splits > 1 ? (size_t)p->lone_slab * Hkv * p->splits : 0;
   size_t tile_parts = 0, tile_units = 0, tile_entries = 0;       // of the largest slab each
   for (const gllm_sparse_plan::TileSlab& sb : p->tile_slabs) {
     const size_t units = (size_t)sb.n_tiles * Hkv;
@@ -2030,9 +2035,10 @@ int gllm_sparse_plan_info(const gllm_sparse_plan* p, int64_t* info, int32_t n) {
   if (!p || !info) return fail(GLLM_ATTN_EINVAL, "null plan or info");
   int64_t wgs = 0;
   for (const gllm_sparse_plan::TileSlab& sb : p->tile_slabs) wgs += sb.wgs;
-  const int64_t v[9] = {p->total_rows, (int64_t)p->rows.size(), (int64_t)p->blocks.size(), p->n_tiles,
-                         (int64_t)p->slabs.size(), p->splits, (int64_t)p->tiles.size(), wgs, (int64_t)p->tile_slabs.size()};
-  for (int i = 0; i < n && i < 9; ++i) info[i] = v[i];
+  const int64_t v[10] = {p->total_rows, (int64_t)p->rows.size(), (int64_t)p->blocks.size(), p->n_tiles,
+                         (int64_t)p->slabs.size(), p->splits, (int64_t)p->tiles.size(), wgs, (int64_t)p->tile_slabs.size(),
+                         p->lone.empty() ? 0 : ((int64_t)p->lone.size() + p->lone_slab - 1) / p->lone_slab};
+  for (int i = 0; i < n && i < 10; ++i) info[i] = v[i];
   return ok();
 }
 
@@ -2147,9 +2153,12 @@ int gllm_sparse_attention(const gllm_sparse_plan* p, const void* q, int64_t q_ro
   a.sparse_splits = p->splits;
   a.partial_ml = (float*)(p->ws + p->off_ml);
   a.partials = (float*)(p->ws + p->off_part);
-  a.sparse_rows = (const SparseRow*)(p->ws + p->off_lone);
-  a.n_sparse_rows = (int32_t)p->lone.size();
-  return hip_check(launch_sparse_attention_mfma(a, st), "sparse attention launch");
+  for (int64_t r0 = 0; r0 < (int64_t)p->lone.size(); r0 += p->lone_slab) {
+    a.sparse_rows = (const SparseRow*)(p->ws + p->off_lone) + r0;
+    a.n_sparse_rows = (int32_t)std::min<int64_t>(p->lone_slab, (int64_t)p->lone.size() - r0);
+    if (int rc = hip_check(launch_sparse_attention_mfma(a, st), "sparse attention launch")) return rc;
+  }
+  return ok();
 }
 
 }  // extern "C"

@@ -73,7 +73,8 @@ class SparsePlan:
         self.query_lens, self.seq_lens, self.q_seq_stride = ql, sl, q_seq_stride
         self.table_width = -(-max(sl, default=0) // block_size)
         self.record_bytes = key_bounds_bytes(num_kv_heads, head_dim)
-        keys = ("rows", "query_rows", "touched_blocks", "score_tiles", "slabs", "splits", "tiles", "tile_workgroups", "tile_slabs")
+        keys = ("rows", "query_rows", "touched_blocks", "score_tiles", "slabs", "splits", "tiles", "tile_workgroups", "tile_slabs",
+                "row_slabs")
         arr = (ctypes.c_int64 * len(keys))()
         _lib.check(lib.gllm_sparse_plan_info(self._h, arr, len(keys)))
         self._info = dict(zip(keys, list(arr)))

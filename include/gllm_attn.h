@@ -454,14 +454,15 @@ int gllm_sparse_plan_create(gllm_sparse_plan** plan, const int32_t* query_lens, 
                             int32_t blocks, int32_t first_blocks, int32_t recent_blocks);
 /* Workspace and upload as for gllm_attn_plan: it holds the rows' tables, the scores (at
  * most 256 MiB, or one tile of rows), prompt tiles' blocks and partials (at most 256 MiB
- * each; longer batches go through them in slabs) and split partials of single rows, so a
- * plan's calls must follow each other in stream order. */
+ * each) and split partials of single rows (at most 256 MiB, or one row's): longer batches go
+ * through them in slabs.  So a plan's calls must follow each other in stream order. */
 size_t gllm_sparse_plan_workspace_bytes(const gllm_sparse_plan* plan);
 int gllm_sparse_plan_upload(gllm_sparse_plan* plan, void* workspace, size_t workspace_bytes, void* stream);
 /* Plan facts: [0] rows of q / out / selected that it addresses, [1] query rows, [2] blocks
  * that the new tokens touch, [3] score tiles, [4] slabs of rows scored at a time, [5]
  * splits of a row's keys, [6] tiles of prompt rows that attend together, [7] workgroups
- * that share those tiles' keys, [8] slabs of tiles ([5] to [8]: on the MFMA kernels).  The first n are written. */
+ * that share those tiles' keys, [8] slabs of tiles, [9] slabs of single rows ([5] to [9]: on the
+ * MFMA kernels).  The first n are written. */
 int gllm_sparse_plan_info(const gllm_sparse_plan* plan, int64_t* info, int32_t n);
 int gllm_sparse_plan_destroy(gllm_sparse_plan* plan);
 /* Bounds of every block that holds a new token (positions seq_len - query_len ..

@@ -1,4 +1,4 @@
-"""Sparse attention of prompts in several slabs of tiles."""
+"""Sparse attention of prompts in several slabs, of tiles and of single rows."""
 import pytest
 import torch
 
@@ -70,3 +70,23 @@ def test_many_short_tiles_in_slabs():
     out = sparse.sparse_attention(plan, b.q.cuda(), b.kc.cuda(), b.vc.cuda(), b.bt.cuda(), sel)
     assert torch.isfinite(out).all()
     check_rows(b, out, sel.cpu(), [256 * i + (37 * i) % 256 for i in range(n)] + [256 * n - 1])
+
+
+def test_slabs_of_single_rows():
+    """Rows in two splits, more than fit at a time: bit for bit those of plans of their own."""
+    b = Batch([6000], [4100], Hq=16, Hkv=8, D=64, bs=8, seed=3)
+    plan = gs.plan_of(b, 600, 0)
+    assert plan.info["tiles"] == 0 and plan.info["splits"] == 2 and plan.info["row_slabs"] == 2
+    sel = lists(b, 600, 5)
+    sel[7] = -1
+    sel[4000, 3, 5:] = -1
+    args = (b.kc.cuda(), b.vc.cuda(), b.bt.cuda())
+    q = b.q.cuda()
+    out = sparse.sparse_attention(plan, q, *args, sel)
+    for r0, r1 in ((0, 90), (3900, 4100)):
+        part = sparse.SparsePlan([r1 - r0], [6000 + r1], num_q_heads=16, num_kv_heads=8, head_dim=64, block_size=8, dtype=BF,
+                                 device="cuda", blocks=600, first_blocks=0)
+        assert part.info["row_slabs"] == 1 and part.info["splits"] == 2
+        assert torch.equal(out[r0:r1], sparse.sparse_attention(part, q[r0:r1], *args, sel[r0:r1].contiguous()))
+    assert (out[7] == 0).all()
+    check_rows(b, out, sel.cpu(), [0, 1, 3970, 3971, 3972, 4099])

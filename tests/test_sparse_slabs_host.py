@@ -7,7 +7,8 @@ import pytest
 from gllm_amd import _lib
 
 MIB = 1 << 20
-KEYS = ("rows", "query_rows", "touched_blocks", "score_tiles", "slabs", "splits", "tiles", "tile_workgroups", "tile_slabs")
+KEYS = ("rows", "query_rows", "touched_blocks", "score_tiles", "slabs", "splits", "tiles", "tile_workgroups", "tile_slabs",
+        "row_slabs")
 
 
 def info(ql, sl, Hq=32, Hkv=8, D=128, bs=16, blocks=128, dtype=_lib.DTYPE_BF16):
@@ -47,4 +48,13 @@ def test_tiles_beside_a_long_prompt():
 def test_a_tile_too_large_for_a_slab_goes_by_rows():
     """Rows that select 300,000 blocks each of 134 million: that sequence alone."""
     i = info([64, 128], [(1 << 31) - 20000, 8192], Hkv=4, Hq=16, blocks=300000)
-    assert i["tiles"] == 2 and i["splits"] > 1
+    assert i["tiles"] == 2 and i["row_slabs"] >= 1 and i["splits"] > 1
+
+
+@pytest.mark.parametrize("rows,ctx,bs", [(8192, 65536, 8), (8192, 65536, 24), (32768, 65536, 8), (20000, 40000, 1)])
+def test_partials_of_single_rows_stay_bounded(rows, ctx, bs):
+    """Lists longer than a task caches are split whatever the number of rows."""
+    i = info([rows], [ctx], bs=bs, blocks=600)
+    assert i["tiles"] == 0 and i["splits"] == 2 and i["row_slabs"] == -(-rows // (256 * MIB // (8 * 2 * 16 * 130 * 4)))
+    assert i["bytes"] <= 2 * 256 * MIB + tables(i)
+    assert info([rows], [ctx], bs=bs, blocks=64)["row_slabs"] == 1
