@@ -1896,8 +1896,6 @@ sparse_tile_kernel(AttnArgs a) {
   __shared__ int sums[2][kWaves], next[6];        // next: see below
   const int nt = a.n_sparse_tiles, Hkv = a.num_kv_heads, units = nt * Hkv, W = gridDim.x;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  // neighbouring runs on one XCD: they share keys
-  const int b = W % 8 ? blockIdx.x : blockIdx.x % 8 * (W / 8) + blockIdx.x / 8;
   const auto keys_of = [&](int u) { return a.tile_keys[u % nt * Hkv + u / nt]; };
   const auto tiles_of = [&](int keys) { return max(1, (keys + 63) / 64); };
   // all units' tiles, and the runs that they make (the plan's W counts every block that the
@@ -1912,6 +1910,7 @@ sparse_tile_kernel(AttnArgs a) {
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) C += sums[1][w];
   const int64_t runs = min((int64_t)W, tile_runs(C, a.tile_round, a.block_size));
+  const int b = (int)run_of_group(blockIdx.x, runs);
   if (b >= runs) return;
   const int lo = (int)run_start(C, runs, b), hi = (int)run_start(C, runs, b + 1);
   // the unit of the run's first tile; run 0 writes down where every unit's partials are

@@ -28,6 +28,13 @@ GLLM_RUNS int64_t tile_runs(int64_t C, int64_t round, int32_t block_size) {
 GLLM_RUNS int64_t run_start(int64_t C, int64_t runs, int64_t r) { return C * r / runs; }
 GLLM_RUNS int64_t run_of(int64_t C, int64_t runs, int64_t s) { return ((s + 1) * runs - 1) / C; }
 
+// The run of a workgroup (past the last run: none).  Workgroups go to the 8 XCDs in turn:
+// neighbouring runs, which share keys, on one XCD, and every XCD has its share of the runs
+// that there are, however many the plan launches workgroups for.
+GLLM_RUNS int64_t run_of_group(int64_t group, int64_t runs) {
+  return group < runs && runs % 8 == 0 ? group % 8 * (runs / 8) + group / 8 : group;
+}
+
 // Slots of partials.  Only a run's first and last unit can be parts: two slots a run, of
 // which the first unit takes the even one; where there are fewer units than runs one a run
 // and one a unit are less.

@@ -63,6 +63,7 @@ extern "C" int walk(int64_t round, int32_t bs, int32_t units, const int32_t* til
   }
   return 0;
 }
+extern "C" int64_t group_run(int64_t group, int64_t runs) { return run_of_group(group, runs); }
 extern "C" int64_t most_tiles(int32_t bs) { return most_run_tiles(bs); }
 extern "C" int64_t runs_of(int64_t C, int64_t round, int32_t bs) { return tile_runs(C, round, bs); }
 """
@@ -76,6 +77,7 @@ def lib(tmp_path_factory):
                     str(d / "walk.so")], check=True)
     so = ctypes.CDLL(str(d / "walk.so"))
     so.most_tiles.restype = so.runs_of.restype = ctypes.c_int64
+    so.group_run.restype, so.group_run.argtypes = ctypes.c_int64, [ctypes.c_int64, ctypes.c_int64]
     so.runs_of.argtypes = [ctypes.c_int64, ctypes.c_int64, ctypes.c_int32]
     so.walk.argtypes = [ctypes.c_int64, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]
     return so
@@ -132,3 +134,17 @@ def test_runs_grow_with_the_tiles(lib):
                 n = lib.runs_of(C, round_, bs)
                 assert n >= last
                 last = n
+
+
+@pytest.mark.parametrize("runs", [1, 7, 8, 9, 250, 256, 1024, 1280])
+@pytest.mark.parametrize("planned", [1, 2, 5])
+def test_every_xcd_has_its_share_of_runs(lib, runs, planned):
+    """Workgroups go to the 8 XCDs in turn.  A plan counts the most runs that there can be; the
+    ones that there are must not leave XCDs idle."""
+    groups = [lib.group_run(g, runs) for g in range(runs * planned)]
+    assert sorted(r for r in groups if r < runs) == list(range(runs))
+    share = [sum(r < runs for r in groups[x::8]) for x in range(8)]
+    assert max(share) - min(share) <= 1
+    if runs % 8 == 0:                                   # neighbours together
+        for x in range(8):
+            assert sorted(r for r in groups[x::8] if r < runs) == list(range(x * runs // 8, (x + 1) * runs // 8))
