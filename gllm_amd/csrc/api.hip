@@ -465,9 +465,10 @@ int check_groups(const PrefixGroups& g, const int32_t* query_lens, const int32_t
 // Items over the keys that decode sequences share.  All (query row, head) columns of
 // a group, 256 a workgroup, take a range of the shared keys together; the ranges are
 // as long as leaves every CU its resident workgroups (of at least 256 keys), since a
-// range costs every column a partial.  Prompts in a group keep their keys: they read
-// a key for 32 rows a wave already.  Whole sub-tiles of 16 keys are shared, the rest is
-// the sequences' own.
+// range costs every column a partial.  Members of more than 16 columns (query_len x G) keep
+// their keys, as partials have 16: long prompts read a key for 32 rows a wave already, short
+// ones, of 5 to 31 rows at G = 4, would gain.  Whole sub-tiles of 16 keys are shared, the rest
+// is the sequences' own.
 //
 // Prefixes from 256 keys on (head dim 64: 512) are shared: below that, the partials and
 // their join cost what the keys save.  Measured, us without / with sharing, 32 / 8 heads,
@@ -475,7 +476,11 @@ int check_groups(const PrefixGroups& g, const int32_t* query_lens, const int32_t
 // 21.9, 28.9 / 23.5, 71.7 / 26.5, 246 / 34.7; two on 512, 2,048, 8,192 17.8 / 17.0, 19.0 / 17.3, 24.9 /
 // 19.9; 64 with 1,000 own keys on 128, 512 54.6 / 56.4, 61.3 / 56.7; head dim 64, 64 on 128, 512, 2,048
 // 14.8 / 17.9, 19.9 / 18.0, 41.2 / 20.4, with 1,000 own keys on 128, 512, 2,048 30.3 / 34.0, 33.8 / 33.8,
-// 54.5 / 37.7.
+// 54.5 / 37.7.  A batch that holds prompts too becomes page-balanced with its first group and
+// has a launch more, which few shared keys do not make up for: beside 4 prompts of 512 rows, 256
+// decodes of 500-2,000 keys, a group of 2 on 256 263 / 289, all on 256 240 / 261, on 480 228 / 221, 64 of
+// them on 4,096 379 / 314; 64 of 500-4,000, 2 on 256 153 / 163, 16 on 4,096 181 / 170, all on 4,096 246 /
+// 182: sharing gains from about a third of the decode sequences' keys on.
 //
 // beside: the batch has decode sequences only, whose own keys go in the same launch.
 // Returns the workgroups that it leaves to those (0: a launch of their own).

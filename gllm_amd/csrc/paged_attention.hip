@@ -1886,8 +1886,9 @@ sparse_attn_kernel(AttnArgs a) {
 // that a run's end cuts leaves partials.  A tile's rows share each K/V tile, and MFMAs have
 // all their columns; the row form above reads a key again for each row.  771 rows on
 // 8,192-16,384 keys, 2,048 selected at random, with lists and join: 874 us by rows, 252 by
-// tiles cut in equal parts (208 workgroups), 221 by equal runs: 670 TFLOP/s of the computed
-// pairs or more (traced), plain prompts 770.
+// tiles cut in equal parts (208 workgroups), 221 by equal runs.  Of those this kernel 191
+// (traced, at the clock of a lasting load): 146 GFLOP by the count of MFMAs, 5.6 times the
+// selected pairs', at 760 TFLOP/s; plain prompts 770.
 template <typename T, int D, int KF>
 __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2)))
 sparse_tile_kernel(AttnArgs a) {

@@ -46,6 +46,8 @@ class SparsePlan:
     0 .. p // block_size (all, if there are no more): the first ``first_blocks``, the last
     ``recent_blocks`` (at least 1: the row's own) and those of the highest scores.
     The calls of one plan share its workspace and follow each other on one stream.
+    Beside tables of the rows the workspace holds four areas of at most 256 MiB each (or what
+    one tile or row takes), through which longer batches go in slabs.
     """
 
     def __init__(self, query_lens, seq_lens, *, num_q_heads: int, num_kv_heads: int, head_dim: int, block_size: int,

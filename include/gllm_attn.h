@@ -485,7 +485,8 @@ int gllm_select_blocks(const gllm_sparse_plan* plan, const void* q, int64_t q_ro
 /* Attention of each row over the keys at or before its position in its selected blocks.
  * `selected` may come from anywhere: a list ends at the first entry that is negative, not
  * above the entry before it, or behind the row's own block, and a row without blocks
- * gives zeros.  Every key that some row of a sequence sees has to hold finite values. */
+ * gives zeros.  Keys and values of a block that some row selected have to be finite up to the
+ * position of the sequence's last row, those that the row itself does not see too. */
 int gllm_sparse_attention(const gllm_sparse_plan* plan, const void* q, int64_t q_row_stride, void* out,
                           int64_t out_row_stride, const void* k_cache, const void* v_cache,
                           int64_t cache_slot_stride, int64_t num_blocks, const int32_t* block_table,
